@@ -407,6 +407,40 @@ int na_linear_wgrad(int32_t dtype, int64_t rows, int64_t n, int64_t k,
                     const void *g, const void *x, void *dw, void *db,
                     void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- layer norm ------------------------------------------------------------ */
+#define NA_NORM_MAX_CHANNELS 16384
+
+/*
+ * y = (x - mean) / sqrt(var + eps) * w + b over the last dimension, for a layer's
+ * input or its queries and keys.  No counterpart in the reference, whose models
+ * take their framework's.  Row r of x starts at element
+ * (r / inner) * x_stride[0] + (r % inner) * x_stride[1] (a head of a packed
+ * projection is read in place; contiguous rows: inner 1, x_stride[0] = channels),
+ * dy likewise; y and dx are contiguous.  Any alignment of the types.
+ */
+typedef struct na_norm_params {
+  int64_t rows;         /* below 2^30 */
+  int32_t channels;     /* 1 .. NA_NORM_MAX_CHANNELS */
+  int32_t dtype;        /* x, y, dy, dx */
+  int32_t weight_dtype; /* w, b, dw, db: dtype or NA_F32 */
+  float eps;
+  int64_t inner;        /* 1 .. 2^31 - 1 */
+  int64_t x_stride[2];
+  int64_t dy_stride[2];
+} na_norm_params;
+
+/* w, b and stats may be NULL (ones, zeros, not kept); stats [rows, 2] float32:
+ * each row's mean and 1 / sqrt(var + eps). */
+int na_norm_fwd(const na_norm_params *p, const void *x, const void *w,
+                const void *b, void *y, float *stats, void *stream);
+/* Bytes that na_norm_bwd needs when dw or db is wanted. */
+size_t na_norm_bwd_workspace_bytes(const na_norm_params *p);
+/* Gradients of na_norm_fwd; dx, dw and db may each be NULL (not wanted).
+ * Deterministic: no atomics. */
+int na_norm_bwd(const na_norm_params *p, const void *x, const void *w,
+                const void *dy, const float *stats, void *dx, void *dw, void *db,
+                void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

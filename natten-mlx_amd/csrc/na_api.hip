@@ -820,4 +820,65 @@ int na_merge_bwd(const na_merge_params *p, const void *const *outs,
   return launch_status("na_merge_bwd");
 }
 
+namespace {
+
+int check_norm(const na_norm_params *p, na::NormArgs *A) {
+  if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
+  if (p->rows < 0 || p->rows >= na::kNormMaxRows)
+    return fail(NA_ERR_UNSUPPORTED, "layer norm takes up to 2^30 - 1 rows, got %lld",
+                (long long)p->rows);
+  if (p->channels < 1 || p->channels > na::kNormMaxChannels)
+    return fail(NA_ERR_UNSUPPORTED, "layer norm takes 1 to %d channels, got %d",
+                na::kNormMaxChannels, p->channels);
+  if (p->dtype != NA_F32 && p->dtype != NA_F16 && p->dtype != NA_BF16)
+    return fail(NA_ERR_INVALID, "unknown dtype %d", p->dtype);
+  if (p->weight_dtype != p->dtype && p->weight_dtype != NA_F32)
+    return fail(NA_ERR_INVALID, "weight dtype %d is neither the rows' (%d) nor float32",
+                p->weight_dtype, p->dtype);
+  if (!(p->eps >= 0.f))
+    return fail(NA_ERR_INVALID, "eps must be >= 0, got %g", (double)p->eps);
+  if (p->inner < 1 || p->inner >= ((int64_t)1 << 31))
+    return fail(NA_ERR_INVALID, "inner must be in [1, 2^31), got %lld", (long long)p->inner);
+  *A = {p->dtype, p->weight_dtype, p->rows, p->channels, p->eps, p->inner, p->x_stride[0],
+        p->x_stride[1], p->dy_stride[0], p->dy_stride[1]};
+  return NA_OK;
+}
+
+}  // namespace
+
+int na_norm_fwd(const na_norm_params *p, const void *x, const void *w, const void *b, void *y,
+                float *stats, void *stream) {
+  na::NormArgs A;
+  const int rc = check_norm(p, &A);
+  if (rc != NA_OK) return rc;
+  if (A.rows == 0) return NA_OK;
+  if (x == nullptr || y == nullptr) return fail(NA_ERR_INVALID, "x/y must be non-NULL");
+  na::norm_fwd(A, x, w, b, y, stats, as_stream(stream));
+  return launch_status("na_norm_fwd");
+}
+
+size_t na_norm_bwd_workspace_bytes(const na_norm_params *p) {
+  na::NormArgs A;
+  if (check_norm(p, &A) != NA_OK) return 0;
+  return align256(na::norm_workspace(A.dtype, A.rows, A.C));
+}
+
+int na_norm_bwd(const na_norm_params *p, const void *x, const void *w, const void *dy,
+                const float *stats, void *dx, void *dw, void *db, void *workspace,
+                size_t workspace_bytes, void *stream) {
+  na::NormArgs A;
+  const int rc = check_norm(p, &A);
+  if (rc != NA_OK) return rc;
+  if (dx == nullptr && dw == nullptr && db == nullptr) return NA_OK;
+  if (A.rows > 0 && (x == nullptr || dy == nullptr || stats == nullptr))
+    return fail(NA_ERR_INVALID, "x/dy/stats must be non-NULL");
+  const size_t need = align256(na::norm_workspace(A.dtype, A.rows, A.C));
+  if ((dw != nullptr || db != nullptr) && need > 0 &&
+      (workspace == nullptr || workspace_bytes < need))
+    return fail(NA_ERR_WORKSPACE, "na_norm_bwd needs a %zu-byte workspace (got %zu)", need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  na::norm_bwd(A, x, w, dy, stats, dx, dw, db, workspace, as_stream(stream));
+  return launch_status("na_norm_bwd");
+}
+
 }  // extern "C"

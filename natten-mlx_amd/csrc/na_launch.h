@@ -217,6 +217,29 @@ size_t linear_wgrad_workspace(int64_t M, int64_t N, int64_t K);
 void linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *g, const void *x,
                   void *dw, void *db, void *workspace, hipStream_t st);
 
+// Layer norm over the last dimension (na_norm.hip).  Row r of x is at
+// (r / inner) * x_outer + (r % inner) * x_inner (dy likewise); y and dx are
+// contiguous.  stats [rows][2]: mean and 1 / std.  Channels up to
+// kNormMaxChannels, rows below 2^30 (a group's next row stays in 32 bits).
+constexpr int kNormMaxChannels = 16384;
+constexpr int64_t kNormMaxRows = (int64_t)1 << 30;
+constexpr int kNormFewRows = 2048;
+constexpr int kNormFwdBlocks = 2048, kNormBwdBlocks = 512;
+struct NormArgs {
+  int dtype, wdtype;  // wdtype: dtype or NA_F32
+  int64_t rows;
+  int C;
+  float eps;
+  int64_t inner, x_outer, x_inner, g_outer, g_inner;
+};
+size_t norm_workspace(int dtype, int64_t rows, int C);
+void norm_fwd(const NormArgs &A, const void *x, const void *w, const void *b, void *y, float *stats,
+              hipStream_t st);
+// dx may be null (not wanted); dw and db may be null, or both are written from
+// the partial sums in `workspace`.
+void norm_bwd(const NormArgs &A, const void *x, const void *w, const void *dy, const float *stats,
+              void *dx, void *dw, void *db, void *workspace, hipStream_t st);
+
 // Generic pieces reused around the MFMA backward.
 void valu_delta(const Prob &P, int dtype, const void *out, const void *dout,
                 const float *dlse, float *delta, hipStream_t st);

@@ -1,7 +1,7 @@
 // The differentiable ops as torch custom operators with their autograd nodes
 // in C++ over the C ABI of libnatten_amd.so: the fused op (natten_amd::na_fused),
-// the split ops (na_split_qk, na_split_av), the DiNAT ops (na_rpb_qk, na_rpb_av)
-// and a layer's projections (na_linear).
+// the split ops (na_split_qk, na_split_av), the DiNAT ops (na_rpb_qk, na_rpb_av),
+// a layer's projections (na_linear) and the layer norm (na_layer_norm).
 //
 // The reference's autograd layer (autograd/na1d.py:34-53, na2d.py:34-64,
 // na3d.py) wraps the fused forward / backward in an mx.custom_function; the
@@ -21,6 +21,7 @@
 // on the stream of its forward).
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -642,6 +643,168 @@ at::Tensor na_rpb_av(const at::Tensor &attn, const at::Tensor &v, at::IntArrayRe
   return RpbAV::apply(attn, v, kernel, dilation, heads_first, out_f32, stream);
 }
 
+// ---- layer norm (norm.py) ---------------------------------------------------
+
+// t's rows (its last dimension, dense) as two levels of strides: row r starts at
+// (r / inner) * outer + (r % inner) * step.  False where it takes more levels.
+struct RowView {
+  int64_t inner = 1, outer = 0, step = 0;
+};
+bool row_view(const at::Tensor &t, RowView *v) {
+  const int64_t nd = t.dim();
+  *v = RowView{};
+  if (t.numel() == 0) return true;
+  if (t.size(nd - 1) > 1 && t.stride(nd - 1) != 1) return false;
+  int64_t size[2] = {1, 1}, stride[2] = {0, 0};
+  int level = -1;
+  for (int64_t d = nd - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (level >= 0 && t.stride(d) == size[level] * stride[level]) {
+      size[level] *= t.size(d);
+    } else {
+      if (++level > 1) return false;
+      size[level] = t.size(d);
+      stride[level] = t.stride(d);
+    }
+  }
+  if (level < 1) {  // one level of rows, or a single row
+    v->inner = 1;
+    v->outer = stride[0];
+    v->step = 0;
+  } else {
+    v->inner = size[0];
+    v->step = stride[0];
+    v->outer = stride[1];
+  }
+  return v->inner < ((int64_t)1 << 31);
+}
+
+// `t`, or a contiguous copy, with its row view.
+at::Tensor viewed(const at::Tensor &t, RowView *v) {
+  if (row_view(t, v)) return t;
+  const at::Tensor c = t.contiguous();
+  row_view(c, v);
+  return c;
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor *t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+na_norm_params norm_params(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, double eps,
+                           const RowView &v) {
+  na_norm_params p{};
+  p.channels = (int32_t)std::min<int64_t>(x.size(-1), INT32_MAX);
+  p.rows = x.size(-1) > 0 ? x.numel() / x.size(-1) : 0;
+  p.dtype = dtype_code(x.scalar_type());
+  p.weight_dtype = w.defined()   ? dtype_code(w.scalar_type())
+                   : b.defined() ? dtype_code(b.scalar_type())
+                                 : p.dtype;
+  p.eps = (float)eps;
+  p.inner = v.inner;
+  p.x_stride[0] = v.outer;
+  p.x_stride[1] = v.step;
+  return p;
+}
+
+// y, and the rows' statistics where a backward will want them.  x as the kernels
+// read it comes back in `xs`.
+at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, double eps,
+                        int64_t stream, at::Tensor *xs, at::Tensor *stats, na_norm_params *out) {
+  TORCH_CHECK(x.dim() >= 1 && (!w.defined() || (w.dim() == 1 && w.size(0) == x.size(-1))) &&
+                  (!b.defined() || (b.dim() == 1 && b.size(0) == x.size(-1))) &&
+                  (!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type()),
+              "natten_amd na_layer_norm: x [..., C], weight and bias [C] of one dtype, got ",
+              x.sizes());
+  check_devices(x, {&w, &b});
+  const c10::DeviceGuard guard(x.device());
+  RowView v;
+  *xs = viewed(x, &v);
+  const na_norm_params p = norm_params(x, w, b, eps, v);
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  if (stats != nullptr) *stats = at::empty({p.rows, 2}, x.options().dtype(at::kFloat));
+  const at::Tensor wc = contig(w), bc = contig(b);
+  check_rc(na_norm_fwd(&p, xs->data_ptr(), cptr(wc), cptr(bc), y.data_ptr(),
+                       stats != nullptr ? static_cast<float *>(stats->data_ptr()) : nullptr,
+                       as_stream(stream)),
+           "na_norm_fwd");
+  *out = p;
+  return y;
+}
+
+struct LayerNorm : public torch::autograd::Function<LayerNorm> {
+  static at::Tensor forward(AutogradContext *ctx, at::Tensor x, std::optional<at::Tensor> w_opt,
+                            std::optional<at::Tensor> b_opt, double eps, int64_t stream) {
+    const at::Tensor w = w_opt.value_or(at::Tensor()), b = b_opt.value_or(at::Tensor());
+    at::Tensor xs, stats;
+    na_norm_params p;
+    const at::Tensor y = norm_forward(x, w, b, eps, stream, &xs, &stats, &p);
+    ctx->save_for_backward({x, w, stats});
+    ctx->saved_data["p"] =
+        std::vector<int64_t>{stream, b.defined() ? (int64_t)b.scalar_type() : (int64_t)-1};
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "natten_amd layer_norm: the backward is not differentiable");
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &w = s[1], &stats = s[2];
+    const std::vector<int64_t> m = ctx->saved_data["p"].toIntVector();
+    const c10::DeviceGuard guard(s[0].device());
+    RowView xv, gv;
+    const at::Tensor x = viewed(s[0], &xv);
+    at::Tensor g = viewed(to_type(grads[0], x.scalar_type()), &gv);
+    na_norm_params p = norm_params(x, w, at::Tensor(), ctx->saved_data["eps"].toDouble(), xv);
+    if (gv.inner != xv.inner) {  // both views as contiguous rows, or one of them read in its order
+      if (xv.inner > 1 && gv.inner == 1) {
+        gv.step = gv.outer;
+        gv.outer *= xv.inner;
+      } else if (gv.inner > 1 && xv.inner == 1) {
+        p.inner = gv.inner;
+        p.x_stride[1] = xv.outer;
+        p.x_stride[0] = xv.outer * gv.inner;
+      } else {
+        g = g.contiguous();
+        gv.step = x.size(-1);
+        gv.outer = x.size(-1) * xv.inner;
+      }
+    }
+    p.dy_stride[0] = gv.outer;
+    p.dy_stride[1] = gv.step;
+    at::Tensor dx, dw, db, ws;
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
+    if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty(w.sizes(), w.options());
+    if (m[1] >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1)) {  // counts present tensors
+      db = at::empty({x.size(-1)}, x.options().dtype((at::ScalarType)m[1]));
+      if (!w.defined()) p.weight_dtype = dtype_code((at::ScalarType)m[1]);
+    }
+    size_t bytes = 0;
+    if (dw.defined() || db.defined()) {
+      bytes = na_norm_bwd_workspace_bytes(&p);
+      if (bytes) ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    }
+    const at::Tensor wc = contig(w);
+    check_rc(na_norm_bwd(&p, x.data_ptr(), cptr(wc), g.data_ptr(),
+                         static_cast<const float *>(stats.data_ptr()), mptr(dx), mptr(dw), mptr(db),
+                         mptr(ws), bytes, as_stream(m[0])),
+             "na_norm_bwd");
+    return {dx, dw, db, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor na_layer_norm(const at::Tensor &x, const std::optional<at::Tensor> &w,
+                         const std::optional<at::Tensor> &b, double eps, int64_t stream) {
+  const at::Tensor wt = w.value_or(at::Tensor()), bt = b.value_or(at::Tensor());
+  if (wants_grad({&x, &wt, &bt})) return LayerNorm::apply(x, w, b, eps, stream);
+  at::Tensor xs;
+  na_norm_params p;
+  return norm_forward(x, wt, bt, eps, stream, &xs, nullptr, &p);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(natten_amd, m) {
@@ -665,6 +828,8 @@ TORCH_LIBRARY(natten_amd, m) {
       "na_fused_qkv(Tensor qkv, int[] kernel, int[] stride, int[] dilation, int[] causal, "
       "float scale, int flags, int stream) -> Tensor");
   m.def("na_linear(Tensor x, Tensor weight, Tensor? bias, int stream) -> Tensor");
+  m.def(
+      "na_layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int stream) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
@@ -675,4 +840,5 @@ TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
   m.impl("na_rpb_av", na_rpb_av);
   m.impl("na_linear", na_linear);
   m.impl("na_fused_qkv", na_fused_qkv);
+  m.impl("na_layer_norm", na_layer_norm);
 }

@@ -123,9 +123,28 @@ class NaMergeParams(ctypes.Structure):
 
 MERGE_MAX_PARTS = 8
 
+
+class NaNormParams(ctypes.Structure):
+    """Mirror of ``na_norm_params`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("inner", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64 * 2),
+        ("dy_stride", ctypes.c_int64 * 2),
+    ]
+
+
+NORM_MAX_CHANNELS = 16384
+
 _P = ctypes.POINTER(NaParams)
 _R = ctypes.POINTER(NaRpbParams)
 _M = ctypes.POINTER(NaMergeParams)
+_N = ctypes.POINTER(NaNormParams)
 _PP = ctypes.POINTER(ctypes.c_void_p)  # host array of device pointers
 _V = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -164,6 +183,9 @@ SIGNATURES = {
                         + [ctypes.c_size_t, _V]),
     "na_merge_fwd": (ctypes.c_int, [_M, _PP, _PP, _V, _V, _V]),
     "na_merge_bwd": (ctypes.c_int, [_M, _PP, _PP, _V, _V, _PP, _PP, _V]),
+    "na_norm_fwd": (ctypes.c_int, [_N] + [_V] * 6),
+    "na_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_N]),
+    "na_norm_bwd": (ctypes.c_int, [_N] + [_V] * 8 + [ctypes.c_size_t, _V]),
 }
 
 _lib = None
@@ -209,7 +231,8 @@ def _load_fused_op() -> None:
     _fused_op = ns.na_fused.default
     _node_ops = {"qk": ns.na_split_qk.default, "av": ns.na_split_av.default,
                  "rpb_qk": ns.na_rpb_qk.default, "rpb_av": ns.na_rpb_av.default,
-                 "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default}
+                 "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default,
+                 "norm": ns.na_layer_norm.default}
 
 
 def fused_op():
@@ -226,8 +249,8 @@ _OP_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 def node_op(name: str, a: torch.Tensor, b: torch.Tensor):
     """The C++ operator of a split ("qk", "av") or DiNAT ("rpb_qk", "rpb_av")
-    op, or a layer's projection ("linear") and packed attention
-    ("fused_qkv"), where it takes these tensors: built, and both of a supported dtype on
+    op, of a layer's projection ("linear") and packed attention
+    ("fused_qkv"), or of the layer norm ("norm"), where it takes these tensors: built, and both of a supported dtype on
     one HIP device.  None otherwise (the Python autograd Function then runs
     the same kernels, or raises): under compilation, which can leave a Python
     Function to eager execution but not an operator without a fake kernel, while

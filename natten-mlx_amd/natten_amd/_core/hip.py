@@ -609,3 +609,49 @@ def merge_backward(outs, lses, d_out, d_lse, need_outs, need_lses):
                                 _lib.ptr(dl), _lib.ptr_array(d_outs), _lib.ptr_array(d_lses),
                                 _lib.stream_of(do)), "na_merge_bwd")
     return d_outs, d_lses
+
+
+# ---------------------------------------------------------------------------
+# layer norm (C ABI na_norm_fwd / na_norm_bwd)
+
+def _norm_params(x, w, eps):
+    p = _lib.NaNormParams()
+    c = int(x.shape[-1])
+    p.rows, p.channels = x.numel() // max(c, 1), c
+    p.dtype = _lib.dtype_code(x.dtype)
+    p.weight_dtype = p.dtype if w is None else _lib.dtype_code(w.dtype)
+    p.eps, p.inner = float(eps), 1
+    p.x_stride[0] = p.dy_stride[0] = c
+    return p
+
+
+def norm_forward(x, w, b, eps):
+    """``(y, stats)``: stats float32 ``[*lead, 2]``, each row's mean and
+    1 / sqrt(var + eps)."""
+    dev = _require_device(x, w, b)
+    x, w, b = map(_c, (x, w, b))
+    p = _norm_params(x, b if w is None else w, eps)
+    y = torch.empty_like(x)
+    stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().na_norm_fwd(p, _lib.ptr(x), _lib.ptr(w), _lib.ptr(b), _lib.ptr(y),
+                                           _lib.ptr(stats), _lib.stream_of(x)), "na_norm_fwd")
+    return y, stats
+
+
+def norm_backward(x, w, b, dy, stats, eps, need):
+    """``(dx, dw, db)`` of ``norm_forward``; those not needed come back as None."""
+    dev = _require_device(x, w, b, dy, stats)
+    x, w, stats, dy = map(_c, (x, w, stats, dy.to(x.dtype)))
+    p = _norm_params(x, b if w is None else w, eps)
+    dx = torch.empty_like(x) if need[0] else None
+    dw = torch.empty_like(w) if need[1] and w is not None else None
+    db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need[2] and b is not None else None
+    lib = _lib.load()
+    nbytes = 0 if dw is None and db is None else int(lib.na_norm_bwd_workspace_bytes(p))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.na_norm_bwd(p, _lib.ptr(x), _lib.ptr(w), _lib.ptr(dy), _lib.ptr(stats),
+                                   _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes,
+                                   _lib.stream_of(x)), "na_norm_bwd")
+    return dx, dw, db

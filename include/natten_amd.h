@@ -441,6 +441,52 @@ int na_norm_bwd(const na_norm_params *p, const void *x, const void *w,
                 const void *dy, const float *stats, void *dx, void *dw, void *db,
                 void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- rotary positions by axis ----------------------------------------------- */
+#define NA_ROTARY_MAX_AXES 4
+#define NA_ROTARY_MAX_CHANNELS 512 /* rotated channels of a head */
+
+enum na_position_t {
+  NA_POS_GRID = 0, /* the token's own coordinates on extent[] */
+  NA_POS_F32 = 1,  /* a tensor of n_axes coordinates per token */
+  NA_POS_F64 = 2,
+  NA_POS_I32 = 3,
+  NA_POS_I64 = 4
+};
+
+/*
+ * Queries [B, *extent, heads, D] and keys [B, *extent, kv_heads, D] rotated by
+ * their tokens' positions: axis a owns axis_dim[a] channels (the axes' channels
+ * follow each other from 0, the rest of a row passes through) and turns its
+ * pair i by position_a * theta^(-2 i / axis_dim[a]), by the negated angle where
+ * `inverse` (the gradient's map).  Pairs lie half an axis apart, or side by side
+ * where `interleaved`.  Angles are formed in float64.  No counterpart in the
+ * reference.
+ */
+typedef struct na_rotary_params {
+  int64_t batch;
+  int32_t extent[3];   /* spatial sizes, leading 1s for fewer axes */
+  int32_t heads;       /* of q; 0: no q */
+  int32_t kv_heads;    /* of k; 0: no k */
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t n_axes;      /* 1 .. NA_ROTARY_MAX_AXES; NA_POS_GRID: the last n_axes
+                          of extent (at most 3) */
+  int32_t axis_dim[NA_ROTARY_MAX_AXES]; /* even, their sum at most head_dim and
+                                           NA_ROTARY_MAX_CHANNELS */
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t pos_type;    /* enum na_position_t */
+  int32_t pos_batched; /* positions [B, *extent, n_axes], else [*extent, n_axes] */
+  double theta;        /* positive and finite */
+  int64_t q_stride[3]; /* elements from sample to sample, token to token and
+                          head to head; channels are adjacent */
+  int64_t k_stride[3];
+} na_rotary_params;
+
+/* Writes oq and ok, contiguous, in the types of q and k. */
+int na_rotary(const na_rotary_params *p, const void *q, const void *k,
+              const void *positions, void *oq, void *ok, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -881,4 +881,48 @@ int na_norm_bwd(const na_norm_params *p, const void *x, const void *w, const voi
   return launch_status("na_norm_bwd");
 }
 
+int na_rotary(const na_rotary_params *p, const void *q, const void *k, const void *positions,
+              void *oq, void *ok, void *stream) {
+  if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
+  if (p->dtype != NA_F32 && p->dtype != NA_F16 && p->dtype != NA_BF16)
+    return fail(NA_ERR_INVALID, "unknown dtype %d", p->dtype);
+  if (p->batch < 0 || p->heads < 0 || p->kv_heads < 0 || p->head_dim < 1)
+    return fail(NA_ERR_INVALID, "batch/heads/kv_heads/head_dim out of range (got %lld/%d/%d/%d)",
+                (long long)p->batch, p->heads, p->kv_heads, p->head_dim);
+  int64_t tokens = p->batch;
+  for (int a = 0; a < 3; ++a) {
+    if (p->extent[a] < 0) return fail(NA_ERR_INVALID, "extent[%d] is negative", a);
+    if (p->extent[a] > 0 && tokens > (((int64_t)1 << 31) - 1) / p->extent[a])
+      return fail(NA_ERR_UNSUPPORTED, "rotary takes fewer than 2^31 tokens");
+    tokens *= p->extent[a];
+  }
+  if (p->n_axes < 1 || p->n_axes > NA_ROTARY_MAX_AXES)
+    return fail(NA_ERR_INVALID, "n_axes must be 1 .. %d, got %d", NA_ROTARY_MAX_AXES, p->n_axes);
+  int64_t rotated = 0;
+  for (int a = 0; a < p->n_axes; ++a) {
+    if (p->axis_dim[a] < 2 || p->axis_dim[a] % 2 != 0)
+      return fail(NA_ERR_INVALID, "axis_dim[%d] must be positive and even, got %d", a,
+                  p->axis_dim[a]);
+    rotated += p->axis_dim[a];
+  }
+  if (rotated > p->head_dim || rotated > NA_ROTARY_MAX_CHANNELS)
+    return fail(NA_ERR_UNSUPPORTED, "%lld rotated channels of %d (at most %d)", (long long)rotated,
+                p->head_dim, NA_ROTARY_MAX_CHANNELS);
+  if (!(p->theta > 0.0) || p->theta > 1e300)
+    return fail(NA_ERR_INVALID, "theta must be positive and finite, got %g", p->theta);
+  if (p->pos_type < NA_POS_GRID || p->pos_type > NA_POS_I64)
+    return fail(NA_ERR_INVALID, "unknown position type %d", p->pos_type);
+  if (p->pos_type == NA_POS_GRID && p->n_axes > 3)
+    return fail(NA_ERR_INVALID, "a grid has at most 3 axes, got %d", p->n_axes);
+  if (((int64_t)p->heads + p->kv_heads) * p->head_dim >= ((int64_t)1 << 24))
+    return fail(NA_ERR_UNSUPPORTED, "rotary takes fewer than 2^24 channels per token");
+  if (tokens == 0 || p->heads + p->kv_heads == 0) return NA_OK;
+  if ((p->heads > 0 && (q == nullptr || oq == nullptr)) ||
+      (p->kv_heads > 0 && (k == nullptr || ok == nullptr)) ||
+      (p->pos_type != NA_POS_GRID && positions == nullptr))
+    return fail(NA_ERR_INVALID, "q/k/positions and their outputs must be non-NULL");
+  na::rotary(p, q, k, positions, oq, ok, as_stream(stream));
+  return launch_status("na_rotary");
+}
+
 }  // extern "C"

@@ -1,0 +1,234 @@
+// na_rotary.hip — rotary positions by axis, of queries and keys in one launch.
+//
+// A token at (p_0, p_1, ...) rotates each pair (u, v) of axis a's channels:
+//   angle = p_a theta^(-2 i / d_a), i the pair's place among the axis's d_a / 2,
+//   (u, v) -> (u cos - v sin, u sin + v cos).
+// The pairs of an axis whose channels start at c are (c + i, c + d_a / 2 + i), or
+// (c + 2 i, c + 2 i + 1) interleaved; channels behind the last axis pass through.
+// The backward is the same kernel with the angle negated.
+//
+// The angle is formed in float64, in turns, and reduced to half a turn before it
+// is rounded: a float32 product of position and frequency is off by half a
+// radian at a million tokens.  A workgroup takes a run of tokens: its threads
+// first fill a table of (cos, sin) per token and pair in LDS, once for all heads,
+// then stream the rows of all heads of q and k past it in 16-byte chunks.
+#include "na_chunk.h"
+#include "na_launch.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace na {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTable = 4096;  // (cos, sin) entries of a workgroup, 32 KB
+
+// How a row splits into the units that threads take: two chunks half an axis
+// apart, a chunk of adjacent pairs, or single pairs where no chunk fits.
+enum RotMode { kRotHalves, kRotAdjacent, kRotPairs };
+
+struct RotProb {
+  int32_t tokens, per_block;    // tokens, tokens per workgroup
+  int32_t H, Hk, D, heads_per;  // query heads, key heads, channels, heads per workgroup
+  int32_t pairs, upr;           // rotated pairs, units per row
+  int32_t axes, interleaved, pos_type, pos_batched;
+  int32_t first[kRotaryMaxAxes + 1];  // first pair of each axis, then `pairs`
+  double scale[kRotaryMaxAxes];       // -2 log2(theta) / d_a
+  float sign;                         // of the sines
+  FastDiv fS, fE1, fE2, fupr, fheads, fpairs;
+  int64_t qs[3], ks[3];               // element strides: sample, token, head
+};
+
+// Position of token s (of sample b) on axis a.
+__device__ __forceinline__ double rot_position(const RotProb &P, const void *pos, uint32_t b,
+                                               uint32_t s, int a) {
+  if (P.pos_type == NA_POS_GRID) {
+    const uint32_t r = fdiv(s, P.fE2), x2 = s - r * P.fE2.d;
+    const uint32_t x0 = fdiv(r, P.fE1), x1 = r - x0 * P.fE1.d;
+    const int k = a + 3 - P.axes;  // the last axis is the innermost
+    return (double)(k == 2 ? x2 : k == 1 ? x1 : x0);
+  }
+  const int64_t i = ((P.pos_batched ? (int64_t)b * P.fS.d : 0) + s) * P.axes + a;
+  switch (P.pos_type) {
+    case NA_POS_I32:
+      return (double)static_cast<const int32_t *>(pos)[i];
+    case NA_POS_I64:
+      return (double)static_cast<const int64_t *>(pos)[i];
+    case NA_POS_F64:
+      return static_cast<const double *>(pos)[i];
+    default:
+      return (double)static_cast<const float *>(pos)[i];
+  }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRotThreads)
+    k_rotary(RotProb P, const T *__restrict__ q, const T *__restrict__ k,
+             const void *__restrict__ pos, T *__restrict__ oq, T *__restrict__ ok) {
+  typedef Chunk<T> K;
+  constexpr int N = K::N;
+  extern __shared__ __align__(16) char smem[];
+  float2 *const cs = reinterpret_cast<float2 *>(smem);            // [per_block][pairs]
+  double *const rate = reinterpret_cast<double *>(cs + P.per_block * P.pairs);  // [pairs]
+  const int tid = threadIdx.x;
+  const int t0 = blockIdx.x * P.per_block, nt = min(P.per_block, P.tokens - t0);
+  const int h0 = blockIdx.y * P.heads_per, nh = min(P.heads_per, P.H + P.Hk - h0);
+
+  for (int i = tid; i < P.pairs; i += kRotThreads) {
+    int a = 0;
+#pragma unroll
+    for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && i >= P.first[x] ? 1 : 0;
+    rate[i] = exp2((double)(i - P.first[a]) * P.scale[a]) * 0.15915494309189533577;
+  }
+  __syncthreads();
+  for (int i = tid; i < nt * P.pairs; i += kRotThreads) {
+    const uint32_t t = fdiv((uint32_t)i, P.fpairs), p = (uint32_t)i - t * P.fpairs.d;
+    int a = 0;
+#pragma unroll
+    for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && (int)p >= P.first[x] ? 1 : 0;
+    const uint32_t tok = (uint32_t)t0 + t, b = fdiv(tok, P.fS);
+    const double turns = rot_position(P, pos, b, tok - b * P.fS.d, a) * rate[p];
+    float sn, cn;
+    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
+    cs[i] = make_float2(cn, P.sign * sn);
+  }
+  __syncthreads();
+
+  const int units = nt * nh * P.upr;
+#pragma unroll 2
+  for (int i = tid; i < units; i += kRotThreads) {
+    const uint32_t row = fdiv((uint32_t)i, P.fupr);
+    const int j = i - (int)(row * P.fupr.d);
+    const uint32_t t = fdiv(row, P.fheads);
+    const int h = h0 + (int)(row - t * P.fheads.d);
+    const uint32_t tok = (uint32_t)t0 + t, b = fdiv(tok, P.fS), s = tok - b * P.fS.d;
+    const bool isq = h < P.H;
+    const int64_t *st = isq ? P.qs : P.ks;
+    const int hh = isq ? h : h - P.H;
+    const T *src = (isq ? q : k) + b * st[0] + s * st[1] + hh * st[2];
+    T *dst = isq ? oq + ((int64_t)tok * P.H + hh) * P.D : ok + ((int64_t)tok * P.Hk + hh) * P.D;
+    const float2 *c = cs + t * P.pairs;
+    if (MODE == kRotHalves) {
+      const int p0 = j * N;
+      if (p0 < P.pairs) {
+        int a = 0;
+#pragma unroll
+        for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && p0 >= P.first[x] ? 1 : 0;
+        const int c0 = p0 + P.first[a], c1 = c0 + P.first[a + 1] - P.first[a];
+        const typename K::raw ru = K::load(src + c0, N), rv = K::load(src + c1, N);
+        float xu[N], xv[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float2 z = c[p0 + e];
+          const float u = K::get(ru, e), v = K::get(rv, e);
+          xu[e] = u * z.x - v * z.y;
+          xv[e] = fmaf(v, z.x, u * z.y);
+        }
+        K::store(dst + c0, xu, N);
+        K::store(dst + c1, xv, N);
+      } else {  // channels that pass through
+        const int c0 = P.pairs + p0, n = P.D - c0;
+        const typename K::raw r = K::load(src + c0, n);
+        float x[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = K::get(r, e);
+        K::store(dst + c0, x, n);
+      }
+    } else if (MODE == kRotAdjacent) {
+      const int c0 = j * N, n = P.D - c0;
+      const typename K::raw r = K::load(src + c0, n);
+      float x[N];
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const float u = K::get(r, e), v = K::get(r, e + 1);
+        const int p = (c0 + e) / 2;
+        const float2 z = p < P.pairs ? c[p] : make_float2(1.f, 0.f);
+        x[e] = p < P.pairs ? u * z.x - v * z.y : u;
+        x[e + 1] = p < P.pairs ? fmaf(v, z.x, u * z.y) : v;
+      }
+      K::store(dst + c0, x, n);
+    } else if (j < P.pairs) {
+      int a = 0;
+#pragma unroll
+      for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && j >= P.first[x] ? 1 : 0;
+      const int c0 = j + P.first[a], c1 = c0 + P.first[a + 1] - P.first[a];
+      const float u = to_f32(src[c0]), v = to_f32(src[c1]);
+      const float2 z = c[j];
+      dst[c0] = from_f32<T>(u * z.x - v * z.y);
+      dst[c1] = from_f32<T>(fmaf(v, z.x, u * z.y));
+    } else {
+      dst[P.pairs + j] = src[P.pairs + j];
+    }
+  }
+}
+
+}  // namespace
+
+void rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
+            void *ok, hipStream_t st) {
+  RotProb P{};
+  const int n = p->dtype == NA_F32 ? 4 : 8;
+  int64_t per_sample = 1;
+  for (int a = 0; a < 3; ++a) per_sample *= p->extent[a];
+  P.tokens = (int32_t)(p->batch * per_sample);
+  P.H = p->heads;
+  P.Hk = p->kv_heads;
+  P.D = p->head_dim;
+  P.axes = p->n_axes;
+  P.interleaved = p->interleaved;
+  P.pos_type = p->pos_type;
+  P.pos_batched = p->pos_batched;
+  P.sign = p->inverse ? -1.f : 1.f;
+  bool whole = true;  // every half axis is a number of chunks
+  for (int a = 0; a < p->n_axes; ++a) {
+    P.first[a] = P.pairs;
+    P.pairs += p->axis_dim[a] / 2;
+    P.scale[a] = -2.0 * std::log2(p->theta) / p->axis_dim[a];
+    whole = whole && p->axis_dim[a] / 2 % n == 0;
+  }
+  for (int a = p->n_axes; a <= kRotaryMaxAxes; ++a) P.first[a] = P.pairs;
+  const int mode = p->interleaved ? kRotAdjacent : whole ? kRotHalves : kRotPairs;
+  const int rest = P.D - 2 * P.pairs;
+  P.upr = mode == kRotAdjacent ? (P.D + n - 1) / n
+          : mode == kRotHalves ? P.pairs / n + (rest + n - 1) / n
+                               : P.pairs + rest;
+  for (int i = 0; i < 3; ++i) {
+    P.qs[i] = p->q_stride[i];
+    P.ks[i] = p->k_stride[i];
+  }
+  // about four units per thread; fewer where the launch would not fill the chip
+  const int heads = P.H + P.Hk;
+  const int64_t row_units = (int64_t)heads * P.upr;
+  int64_t per = std::max<int64_t>(1, kRotUnits * kRotThreads / row_units);
+  per = std::min<int64_t>(per, std::max(1, kRotTable / P.pairs));
+  per = std::min<int64_t>(per, std::max<int64_t>(1, P.tokens / kRotBlocks));
+  P.per_block = (int32_t)per;
+  P.heads_per = heads;
+  if (per == 1 && row_units > kRotThreads && P.tokens < kRotBlocks)
+    P.heads_per = std::max(1, kRotThreads / P.upr);
+  P.fS = make_fastdiv((uint32_t)per_sample);
+  P.fE1 = make_fastdiv((uint32_t)p->extent[1]);
+  P.fE2 = make_fastdiv((uint32_t)p->extent[2]);
+  P.fupr = make_fastdiv((uint32_t)P.upr);
+  P.fheads = make_fastdiv((uint32_t)std::min(P.heads_per, heads));
+  P.fpairs = make_fastdiv((uint32_t)P.pairs);
+  const dim3 grid((unsigned)((P.tokens + per - 1) / per),
+                  (unsigned)((heads + P.heads_per - 1) / P.heads_per));
+  const size_t lds = sizeof(float2) * per * P.pairs + sizeof(double) * P.pairs;
+  auto run = [&](auto tag) {
+    using T = decltype(tag);
+#define R_(M)                                                                                   \
+  hipLaunchKernelGGL((k_rotary<T, M>), grid, dim3(kRotThreads), lds, st, P, (const T *)q,       \
+                     (const T *)k, pos, (T *)oq, (T *)ok)
+    if (mode == kRotHalves) R_(kRotHalves);
+    else if (mode == kRotAdjacent) R_(kRotAdjacent);
+    else R_(kRotPairs);
+#undef R_
+  };
+  if (p->dtype == NA_F32) run(float{});
+  else if (p->dtype == NA_F16) run(f16_t{});
+  else run(bf16_t{});
+}
+
+}  // namespace na

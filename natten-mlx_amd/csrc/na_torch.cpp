@@ -1,7 +1,8 @@
 // The differentiable ops as torch custom operators with their autograd nodes
 // in C++ over the C ABI of libnatten_amd.so: the fused op (natten_amd::na_fused),
 // the split ops (na_split_qk, na_split_av), the DiNAT ops (na_rpb_qk, na_rpb_av),
-// a layer's projections (na_linear) and the layer norm (na_layer_norm).
+// a layer's projections (na_linear), the layer norm (na_layer_norm) and rotary
+// positions (na_rotary).
 //
 // The reference's autograd layer (autograd/na1d.py:34-53, na2d.py:34-64,
 // na3d.py) wraps the fused forward / backward in an mx.custom_function; the
@@ -805,6 +806,161 @@ at::Tensor na_layer_norm(const at::Tensor &x, const std::optional<at::Tensor> &w
   return norm_forward(x, wt, bt, eps, stream, &xs, nullptr, &p);
 }
 
+// ---- rotary positions (rotary.py) -------------------------------------------
+
+// Element strides of t [B, *spatial, H, D] from sample to sample, token to token
+// and head to head; a contiguous copy where its tokens have no single stride.
+at::Tensor token_view(const at::Tensor &t, int64_t *stride) {
+  const int64_t nd = t.dim();
+  bool ok = t.size(nd - 1) == 1 || t.stride(nd - 1) == 1;
+  int64_t step = 0, count = 1;
+  for (int64_t d = nd - 3; d >= 1 && ok; --d) {
+    if (t.size(d) == 1) continue;
+    if (count == 1) step = t.stride(d);
+    else ok = t.stride(d) == count * step;
+    count *= t.size(d);
+  }
+  if (!ok || t.numel() == 0) {  // (an empty tensor of any strides counts as contiguous)
+    stride[2] = t.size(nd - 1);
+    stride[1] = t.size(nd - 2) * stride[2];
+    stride[0] = t.size(0) > 0 ? t.numel() / t.size(0) : 0;
+    return t.contiguous();
+  }
+  stride[0] = t.stride(0);
+  stride[1] = step;
+  stride[2] = t.stride(nd - 2);
+  return t;
+}
+
+// q or k may be undefined; the shape rules restate the functional layer's for
+// direct callers of the operator.
+variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &pos,
+                             at::IntArrayRef dims, double theta, bool interleaved, bool inverse,
+                             int64_t stream) {
+  const at::Tensor &x = q.defined() ? q : k;
+  const int64_t nd = x.dim();
+  TORCH_CHECK(nd >= 4 && nd <= 6 &&
+                  (!q.defined() || !k.defined() ||
+                   (k.dim() == nd && k.sizes().slice(0, nd - 2) == q.sizes().slice(0, nd - 2) &&
+                    k.size(-1) == q.size(-1) && k.scalar_type() == q.scalar_type())),
+              "natten_amd na_rotary: q and k [B, *spatial, heads, D] of one dtype, got ", x.sizes());
+  TORCH_CHECK((int64_t)dims.size() >= 1 && dims.size() <= NA_ROTARY_MAX_AXES,
+              "natten_amd na_rotary: 1 to 4 axes, got ", dims.size());
+  na_rotary_params p{};
+  p.batch = x.size(0);
+  for (int a = 0; a < 3; ++a) p.extent[a] = 1;
+  for (int64_t d = 1; d < nd - 2; ++d) {
+    TORCH_CHECK(x.size(d) <= INT32_MAX, "natten_amd na_rotary: axis too long");
+    p.extent[3 - (nd - 3) + d - 1] = (int32_t)x.size(d);
+  }
+  p.heads = q.defined() ? (int32_t)q.size(-2) : 0;
+  p.kv_heads = k.defined() ? (int32_t)k.size(-2) : 0;
+  p.head_dim = (int32_t)x.size(-1);
+  p.dtype = dtype_code(x.scalar_type());
+  p.n_axes = (int32_t)dims.size();
+  for (size_t a = 0; a < dims.size(); ++a)
+    p.axis_dim[a] = (int32_t)std::min<int64_t>(std::max<int64_t>(dims[a], 0), INT32_MAX);
+  p.interleaved = interleaved ? 1 : 0;
+  p.inverse = inverse ? 1 : 0;
+  p.theta = theta;
+  at::Tensor pc;
+  if (pos.defined()) {
+    const at::IntArrayRef lead = pos.sizes().slice(0, pos.dim() > 0 ? pos.dim() - 1 : 0);
+    p.pos_batched = pos.dim() == nd - 1 ? 1 : 0;
+    TORCH_CHECK(pos.dim() >= 1 && pos.size(-1) == p.n_axes &&
+                    lead == x.sizes().slice(p.pos_batched ? 0 : 1, nd - 2 - (p.pos_batched ? 0 : 1)),
+                "natten_amd na_rotary: positions [*spatial, axes] or [B, *spatial, axes], got ",
+                pos.sizes());
+    switch (pos.scalar_type()) {
+      case at::kFloat: p.pos_type = NA_POS_F32; break;
+      case at::kDouble: p.pos_type = NA_POS_F64; break;
+      case at::kInt: p.pos_type = NA_POS_I32; break;
+      case at::kLong: p.pos_type = NA_POS_I64; break;
+      default:
+        TORCH_CHECK(false, "natten_amd na_rotary: positions are int32, int64, float32 or float64");
+    }
+    pc = pos.contiguous();
+  } else {
+    TORCH_CHECK(p.n_axes == nd - 3, "natten_amd na_rotary: one axis_dims entry per spatial axis");
+    p.pos_type = NA_POS_GRID;
+  }
+  check_devices(x, {&k, &pos});
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor qc, kc, oq, ok;
+  if (q.defined()) {
+    qc = token_view(q, p.q_stride);
+    oq = at::empty(q.sizes(), q.options());
+  }
+  if (k.defined()) {
+    kc = token_view(k, p.k_stride);
+    ok = at::empty(k.sizes(), k.options());
+  }
+  check_rc(na_rotary(&p, cptr(qc), cptr(kc), cptr(pc), mptr(oq), mptr(ok), as_stream(stream)),
+           "na_rotary");
+  return {oq, ok};
+}
+
+struct Rotary : public torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext *ctx, std::optional<at::Tensor> q,
+                               std::optional<at::Tensor> k, std::optional<at::Tensor> pos,
+                               std::vector<int64_t> dims, double theta, bool interleaved,
+                               bool inverse, int64_t stream) {
+    ctx->save_for_backward({pos.value_or(at::Tensor())});
+    std::vector<int64_t> m{stream, interleaved ? 1 : 0, inverse ? 1 : 0, q.has_value() ? 1 : 0,
+                           k.has_value() ? 1 : 0};
+    m.insert(m.end(), dims.begin(), dims.end());
+    ctx->saved_data["p"] = m;
+    ctx->saved_data["theta"] = theta;
+    ctx->set_materialize_grads(false);
+    variable_list out = rotary_forward(q.value_or(at::Tensor()), k.value_or(at::Tensor()),
+                                       pos.value_or(at::Tensor()), dims, theta, interleaved,
+                                       inverse, stream);
+    variable_list have;
+    for (at::Tensor &t : out)
+      if (t.defined()) have.push_back(t);
+    return have;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const at::Tensor pos = ctx->get_saved_variables()[0];
+    const std::vector<int64_t> m = ctx->saved_data["p"].toIntVector();
+    const std::vector<int64_t> dims(m.begin() + 5, m.end());
+    const double theta = ctx->saved_data["theta"].toDouble();
+    at::Tensor gq, gk;
+    if (m[3] && ctx->needs_input_grad(0)) gq = grads[0];
+    if (m[4] && ctx->needs_input_grad(m[3] ? 1 : 0)) gk = grads[m[3] ? 1 : 0];
+    variable_list d(2);
+    if (gq.defined() || gk.defined()) d = apply_rotary(gq, gk, pos, dims, theta, m[1] != 0, m[2] == 0, m[0]);
+    const at::Tensor none;
+    return {d[0], d[1], none, none, none, none, none, none};
+  }
+  // {q, k} rotated, undefined where the input is; recorded where a gradient may follow
+  static variable_list apply_rotary(const at::Tensor &q, const at::Tensor &k, const at::Tensor &pos,
+                                    const std::vector<int64_t> &dims, double theta,
+                                    bool interleaved, bool inverse, int64_t stream) {
+    if (!wants_grad({&q, &k}))
+      return rotary_forward(q, k, pos, dims, theta, interleaved, inverse, stream);
+    auto opt = [](const at::Tensor &t) {
+      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    };
+    variable_list r = apply(opt(q), opt(k), opt(pos), dims, theta, interleaved, inverse, stream);
+    if (!q.defined()) r.insert(r.begin(), at::Tensor());
+    if (!k.defined()) r.push_back(at::Tensor());
+    return r;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> na_rotary_op(const at::Tensor &q,
+                                                const std::optional<at::Tensor> &k,
+                                                const std::optional<at::Tensor> &positions,
+                                                at::IntArrayRef axis_dims, double theta,
+                                                bool interleaved, bool inverse, int64_t stream) {
+  variable_list r =
+      Rotary::apply_rotary(q, k.value_or(at::Tensor()), positions.value_or(at::Tensor()),
+                           axis_dims.vec(), theta, interleaved, inverse, stream);
+  if (!r[1].defined()) r[1] = at::empty({0}, q.options());  // no key: an empty tensor
+  return {r[0], r[1]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(natten_amd, m) {
@@ -830,6 +986,9 @@ TORCH_LIBRARY(natten_amd, m) {
   m.def("na_linear(Tensor x, Tensor weight, Tensor? bias, int stream) -> Tensor");
   m.def(
       "na_layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int stream) -> Tensor");
+  m.def(
+      "na_rotary(Tensor q, Tensor? k, Tensor? positions, int[] axis_dims, float theta, "
+      "bool interleaved, bool inverse, int stream) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
@@ -841,4 +1000,5 @@ TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
   m.impl("na_linear", na_linear);
   m.impl("na_fused_qkv", na_fused_qkv);
   m.impl("na_layer_norm", na_layer_norm);
+  m.impl("na_rotary", na_rotary_op);
 }

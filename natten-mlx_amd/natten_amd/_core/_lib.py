@@ -141,10 +141,39 @@ class NaNormParams(ctypes.Structure):
 
 NORM_MAX_CHANNELS = 16384
 
+
+class NaRotaryParams(ctypes.Structure):
+    """Mirror of ``na_rotary_params`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("extent", _I32x3),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("n_axes", ctypes.c_int32),
+        ("axis_dim", ctypes.c_int32 * 4),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("pos_type", ctypes.c_int32),
+        ("pos_batched", ctypes.c_int32),
+        ("theta", ctypes.c_double),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+    ]
+
+
+ROTARY_MAX_AXES = 4
+ROTARY_MAX_CHANNELS = 512
+# na_position_t by the positions' dtype
+POSITIONS = {None: 0, torch.float32: 1, torch.float64: 2, torch.int32: 3, torch.int64: 4}
+
 _P = ctypes.POINTER(NaParams)
 _R = ctypes.POINTER(NaRpbParams)
 _M = ctypes.POINTER(NaMergeParams)
 _N = ctypes.POINTER(NaNormParams)
+_RO = ctypes.POINTER(NaRotaryParams)
 _PP = ctypes.POINTER(ctypes.c_void_p)  # host array of device pointers
 _V = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -186,6 +215,7 @@ SIGNATURES = {
     "na_norm_fwd": (ctypes.c_int, [_N] + [_V] * 6),
     "na_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_N]),
     "na_norm_bwd": (ctypes.c_int, [_N] + [_V] * 8 + [ctypes.c_size_t, _V]),
+    "na_rotary": (ctypes.c_int, [_RO] + [_V] * 6),
 }
 
 _lib = None
@@ -232,7 +262,7 @@ def _load_fused_op() -> None:
     _node_ops = {"qk": ns.na_split_qk.default, "av": ns.na_split_av.default,
                  "rpb_qk": ns.na_rpb_qk.default, "rpb_av": ns.na_rpb_av.default,
                  "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default,
-                 "norm": ns.na_layer_norm.default}
+                 "norm": ns.na_layer_norm.default, "rotary": ns.na_rotary.default}
 
 
 def fused_op():
@@ -250,7 +280,7 @@ _OP_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 def node_op(name: str, a: torch.Tensor, b: torch.Tensor):
     """The C++ operator of a split ("qk", "av") or DiNAT ("rpb_qk", "rpb_av")
     op, of a layer's projection ("linear") and packed attention
-    ("fused_qkv"), or of the layer norm ("norm"), where it takes these tensors: built, and both of a supported dtype on
+    ("fused_qkv"), of the layer norm ("norm") or of rotary positions ("rotary"), where it takes these tensors: built, and both of a supported dtype on
     one HIP device.  None otherwise (the Python autograd Function then runs
     the same kernels, or raises): under compilation, which can leave a Python
     Function to eager execution but not an operator without a fake kernel, while

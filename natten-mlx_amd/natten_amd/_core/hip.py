@@ -655,3 +655,34 @@ def norm_backward(x, w, b, dy, stats, eps, need):
                                    _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes,
                                    _lib.stream_of(x)), "na_norm_bwd")
     return dx, dw, db
+
+
+# ---------------------------------------------------------------------------
+# rotary positions (C ABI na_rotary)
+
+def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
+    """``(q, k)`` rotated by their tokens' positions; either may be None."""
+    dev = _require_device(q, k, positions)
+    q, k, positions = map(_c, (q, k, positions))
+    x = k if q is None else q
+    p = _lib.NaRotaryParams()
+    spatial = tuple(x.shape[1:-2])
+    p.batch, p.head_dim, p.dtype = x.shape[0], x.shape[-1], _lib.dtype_code(x.dtype)
+    p.heads, p.kv_heads = (0 if t is None else t.shape[-2] for t in (q, k))
+    for i, e in enumerate((1,) * (3 - len(spatial)) + spatial):
+        p.extent[i] = e
+    p.n_axes = len(axis_dims)
+    for i, d in enumerate(axis_dims):
+        p.axis_dim[i] = d
+    p.interleaved, p.inverse, p.theta = int(interleaved), int(inverse), float(theta)
+    p.pos_type = _lib.POSITIONS[None if positions is None else positions.dtype]
+    p.pos_batched = int(positions is not None and positions.dim() == x.dim() - 1)
+    for st, t in ((p.q_stride, q), (p.k_stride, k)):
+        if t is not None:
+            st[0], st[1], st[2] = t.numel() // max(t.shape[0], 1), t.shape[-2] * t.shape[-1], t.shape[-1]
+    oq, ok = (None if t is None else torch.empty_like(t) for t in (q, k))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().na_rotary(p, _lib.ptr(q), _lib.ptr(k), _lib.ptr(positions),
+                                         _lib.ptr(oq), _lib.ptr(ok), _lib.stream_of(x)),
+                   "na_rotary")
+    return oq, ok

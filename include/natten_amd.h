@@ -467,7 +467,7 @@ typedef struct na_rotary_params {
   int32_t extent[3];   /* spatial sizes, leading 1s for fewer axes */
   int32_t heads;       /* of q; 0: no q */
   int32_t kv_heads;    /* of k; 0: no k */
-  int32_t head_dim;
+  int32_t head_dim;    /* up to 1024 */
   int32_t dtype;
   int32_t n_axes;      /* 1 .. NA_ROTARY_MAX_AXES; NA_POS_GRID: the last n_axes
                           of extent (at most 3) */

@@ -914,8 +914,9 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
     return fail(NA_ERR_INVALID, "unknown position type %d", p->pos_type);
   if (p->pos_type == NA_POS_GRID && p->n_axes > 3)
     return fail(NA_ERR_INVALID, "a grid has at most 3 axes, got %d", p->n_axes);
-  if (((int64_t)p->heads + p->kv_heads) * p->head_dim >= ((int64_t)1 << 24))
-    return fail(NA_ERR_UNSUPPORTED, "rotary takes fewer than 2^24 channels per token");
+  if (p->head_dim > kMaxHeadDim || (int64_t)p->heads + p->kv_heads >= ((int64_t)1 << 20))
+    return fail(NA_ERR_UNSUPPORTED, "rotary takes up to %d channels and 2^20 heads, got %d and %lld",
+                kMaxHeadDim, p->head_dim, (long long)p->heads + p->kv_heads);
   if (tokens == 0 || p->heads + p->kv_heads == 0) return NA_OK;
   if ((p->heads > 0 && (q == nullptr || oq == nullptr)) ||
       (p->kv_heads > 0 && (k == nullptr || ok == nullptr)) ||

@@ -242,7 +242,6 @@ void norm_bwd(const NormArgs &A, const void *x, const void *w, const void *dy, c
 
 // Rotary positions of q and k in one launch (na_rotary.hip).
 constexpr int kRotaryMaxAxes = NA_ROTARY_MAX_AXES;
-constexpr int kRotUnits = 4;      // units per thread of a full launch
 constexpr int kRotBlocks = 1024;  // workgroups that fill the chip
 void rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
             void *ok, hipStream_t st);

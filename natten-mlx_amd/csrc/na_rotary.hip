@@ -23,10 +23,13 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotTable = 4096;  // (cos, sin) entries of a workgroup, 32 KB
+constexpr int kRotUnits = 4;     // units per thread of a full launch
 
 // How a row splits into the units that threads take: two chunks half an axis
-// apart, a chunk of adjacent pairs, or single pairs where no chunk fits.
-enum RotMode { kRotHalves, kRotAdjacent, kRotPairs };
+// apart; a chunk of adjacent pairs; or, where half an axis is no number of
+// chunks, any chunk, whose channels find their partners in a copy of the rows
+// in LDS (the table then holds an entry per channel).
+enum RotMode { kRotHalves, kRotAdjacent, kRotStaged };
 
 struct RotProb {
   int32_t tokens, per_block;    // tokens, tokens per workgroup
@@ -62,6 +65,82 @@ __device__ __forceinline__ double rot_position(const RotProb &P, const void *pos
   }
 }
 
+// Places for the pairs' rates in LDS, a multiple of 16 bytes.
+__host__ __device__ constexpr int rot_rates(int pairs) { return (pairs + 1) & ~1; }
+
+// Rows of head h (of q, then of k) of a token.
+template <typename T>
+struct RotRow {
+  const T *src;
+  T *dst;
+  __device__ __forceinline__ RotRow(const RotProb &P, const T *q, const T *k, T *oq, T *ok,
+                                    uint32_t tok, int h) {
+    const uint32_t b = fdiv(tok, P.fS), s = tok - b * P.fS.d;
+    const bool isq = h < P.H;
+    const int64_t *st = isq ? P.qs : P.ks;
+    const int hh = isq ? h : h - P.H;
+    src = (isq ? q : k) + b * st[0] + s * st[1] + hh * st[2];
+    dst = isq ? oq + ((int64_t)tok * P.H + hh) * P.D : ok + ((int64_t)tok * P.Hk + hh) * P.D;
+  }
+};
+
+// The rows of a workgroup, kRotUnits chunks per thread: kept in registers and
+// copied to LDS, from where each channel takes its partner.
+template <typename T>
+__device__ __forceinline__ void rotate_staged(const RotProb &P, char *smem, const T *q, const T *k,
+                                              T *oq, T *ok, int t0, int nt, int h0, int nh) {
+  typedef Chunk<T> K;
+  constexpr int N = K::N;
+  const int width = 2 * P.pairs;
+  const float2 *const cs = reinterpret_cast<const float2 *>(smem);
+  // behind the rates: partner channel of each rotated one, then the rows, each
+  // region from a 16-byte boundary
+  uint16_t *const partner = reinterpret_cast<uint16_t *>(
+      smem + sizeof(float2) * P.per_block * width + sizeof(double) * rot_rates(P.pairs));
+  T *const rows = reinterpret_cast<T *>(partner + (width + 7) / 8 * 8);
+  for (int c = threadIdx.x; c < width; c += kRotThreads) {
+    int a = 0;
+#pragma unroll
+    for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && c >= 2 * P.first[x] ? 1 : 0;
+    const int half = P.first[a + 1] - P.first[a];
+    partner[c] = (uint16_t)(c - 2 * P.first[a] < half ? c + half : c - half);
+  }
+  const int units = nt * nh * P.upr;
+  typename K::raw raw[kRotUnits];
+  int tok[kRotUnits], c0[kRotUnits];
+  T *dst[kRotUnits];
+#pragma unroll
+  for (int u = 0; u < kRotUnits; ++u) {
+    const int i = threadIdx.x + u * kRotThreads;
+    if (i >= units) break;
+    const uint32_t row = fdiv((uint32_t)i, P.fupr), t = fdiv(row, P.fheads);
+    const RotRow<T> r(P, q, k, oq, ok, (uint32_t)t0 + t, h0 + (int)(row - t * P.fheads.d));
+    tok[u] = (int)t;
+    c0[u] = (i - (int)(row * P.fupr.d)) * N;
+    dst[u] = r.dst + c0[u];
+    raw[u] = K::load(r.src + c0[u], P.D - c0[u]);
+    *reinterpret_cast<typename K::raw *>(rows + i * N) = raw[u];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRotUnits; ++u) {
+    const int i = threadIdx.x + u * kRotThreads;
+    if (i >= units) break;
+    float x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = K::get(raw[u], e);
+    const float2 *const c = cs + tok[u] * width + c0[u];
+    const T *const other = rows + i * N - c0[u];
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c0[u] + e < width) {
+        const float2 z = c[e];
+        x[e] = fmaf(x[e], z.x, to_f32(other[partner[c0[u] + e]]) * z.y);
+      }
+    K::store(dst[u], x, P.D - c0[u]);
+  }
+}
+
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kRotThreads)
     k_rotary(RotProb P, const T *__restrict__ q, const T *__restrict__ k,
@@ -69,8 +148,9 @@ __global__ void __launch_bounds__(kRotThreads)
   typedef Chunk<T> K;
   constexpr int N = K::N;
   extern __shared__ __align__(16) char smem[];
-  float2 *const cs = reinterpret_cast<float2 *>(smem);            // [per_block][pairs]
-  double *const rate = reinterpret_cast<double *>(cs + P.per_block * P.pairs);  // [pairs]
+  constexpr int E = MODE == kRotStaged ? 2 : 1;  // table entries per pair
+  float2 *const cs = reinterpret_cast<float2 *>(smem);  // [per_block][E pairs]
+  double *const rate = reinterpret_cast<double *>(cs + P.per_block * E * P.pairs);  // [pairs]
   const int tid = threadIdx.x;
   const int t0 = blockIdx.x * P.per_block, nt = min(P.per_block, P.tokens - t0);
   const int h0 = blockIdx.y * P.heads_per, nh = min(P.heads_per, P.H + P.Hk - h0);
@@ -91,7 +171,18 @@ __global__ void __launch_bounds__(kRotThreads)
     const double turns = rot_position(P, pos, b, tok - b * P.fS.d, a) * rate[p];
     float sn, cn;
     sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
-    cs[i] = make_float2(cn, P.sign * sn);
+    sn *= P.sign;
+    if (MODE == kRotStaged) {
+      float2 *const c = cs + 2 * ((int)t * P.pairs + P.first[a]) + ((int)p - P.first[a]);
+      c[0] = make_float2(cn, -sn);
+      c[P.first[a + 1] - P.first[a]] = make_float2(cn, sn);
+    } else {
+      cs[i] = make_float2(cn, sn);
+    }
+  }
+  if (MODE == kRotStaged) {
+    rotate_staged<T>(P, smem, q, k, oq, ok, t0, nt, h0, nh);
+    return;
   }
   __syncthreads();
 
@@ -102,12 +193,9 @@ __global__ void __launch_bounds__(kRotThreads)
     const int j = i - (int)(row * P.fupr.d);
     const uint32_t t = fdiv(row, P.fheads);
     const int h = h0 + (int)(row - t * P.fheads.d);
-    const uint32_t tok = (uint32_t)t0 + t, b = fdiv(tok, P.fS), s = tok - b * P.fS.d;
-    const bool isq = h < P.H;
-    const int64_t *st = isq ? P.qs : P.ks;
-    const int hh = isq ? h : h - P.H;
-    const T *src = (isq ? q : k) + b * st[0] + s * st[1] + hh * st[2];
-    T *dst = isq ? oq + ((int64_t)tok * P.H + hh) * P.D : ok + ((int64_t)tok * P.Hk + hh) * P.D;
+    const RotRow<T> at(P, q, k, oq, ok, (uint32_t)t0 + t, h);
+    const T *const src = at.src;
+    T *const dst = at.dst;
     const float2 *c = cs + t * P.pairs;
     if (MODE == kRotHalves) {
       const int p0 = j * N;
@@ -148,17 +236,6 @@ __global__ void __launch_bounds__(kRotThreads)
         x[e + 1] = p < P.pairs ? fmaf(v, z.x, u * z.y) : v;
       }
       K::store(dst + c0, x, n);
-    } else if (j < P.pairs) {
-      int a = 0;
-#pragma unroll
-      for (int x = 1; x < kRotaryMaxAxes; ++x) a += x < P.axes && j >= P.first[x] ? 1 : 0;
-      const int c0 = j + P.first[a], c1 = c0 + P.first[a + 1] - P.first[a];
-      const float u = to_f32(src[c0]), v = to_f32(src[c1]);
-      const float2 z = c[j];
-      dst[c0] = from_f32<T>(u * z.x - v * z.y);
-      dst[c1] = from_f32<T>(fmaf(v, z.x, u * z.y));
-    } else {
-      dst[P.pairs + j] = src[P.pairs + j];
     }
   }
 }
@@ -188,34 +265,36 @@ void rotary(const na_rotary_params *p, const void *q, const void *k, const void 
     whole = whole && p->axis_dim[a] / 2 % n == 0;
   }
   for (int a = p->n_axes; a <= kRotaryMaxAxes; ++a) P.first[a] = P.pairs;
-  const int mode = p->interleaved ? kRotAdjacent : whole ? kRotHalves : kRotPairs;
+  const int mode = p->interleaved ? kRotAdjacent : whole ? kRotHalves : kRotStaged;
   const int rest = P.D - 2 * P.pairs;
-  P.upr = mode == kRotAdjacent ? (P.D + n - 1) / n
-          : mode == kRotHalves ? P.pairs / n + (rest + n - 1) / n
-                               : P.pairs + rest;
+  P.upr = mode == kRotHalves ? P.pairs / n + (rest + n - 1) / n : (P.D + n - 1) / n;
   for (int i = 0; i < 3; ++i) {
     P.qs[i] = p->q_stride[i];
     P.ks[i] = p->k_stride[i];
   }
-  // about four units per thread; fewer where the launch would not fill the chip
-  const int heads = P.H + P.Hk;
+  // kRotUnits units per thread; fewer where the launch would not fill the chip,
+  // and the heads of a token shared out where one token is too many or too few
+  const int heads = P.H + P.Hk, entries = P.pairs * (mode == kRotStaged ? 2 : 1);
   const int64_t row_units = (int64_t)heads * P.upr;
   int64_t per = std::max<int64_t>(1, kRotUnits * kRotThreads / row_units);
-  per = std::min<int64_t>(per, std::max(1, kRotTable / P.pairs));
+  per = std::min<int64_t>(per, std::max(1, kRotTable / entries));
   per = std::min<int64_t>(per, std::max<int64_t>(1, P.tokens / kRotBlocks));
   P.per_block = (int32_t)per;
-  P.heads_per = heads;
-  if (per == 1 && row_units > kRotThreads && P.tokens < kRotBlocks)
-    P.heads_per = std::max(1, kRotThreads / P.upr);
+  const bool few = per == 1 && P.tokens < kRotBlocks;
+  P.heads_per = (int32_t)std::min<int64_t>(
+      heads, std::max(1, (few ? 1 : kRotUnits) * kRotThreads / P.upr));
+  if (per > 1) P.heads_per = heads;
   P.fS = make_fastdiv((uint32_t)per_sample);
   P.fE1 = make_fastdiv((uint32_t)p->extent[1]);
   P.fE2 = make_fastdiv((uint32_t)p->extent[2]);
   P.fupr = make_fastdiv((uint32_t)P.upr);
-  P.fheads = make_fastdiv((uint32_t)std::min(P.heads_per, heads));
+  P.fheads = make_fastdiv((uint32_t)P.heads_per);
   P.fpairs = make_fastdiv((uint32_t)P.pairs);
   const dim3 grid((unsigned)((P.tokens + per - 1) / per),
                   (unsigned)((heads + P.heads_per - 1) / P.heads_per));
-  const size_t lds = sizeof(float2) * per * P.pairs + sizeof(double) * P.pairs;
+  size_t lds = sizeof(float2) * per * entries + sizeof(double) * rot_rates(P.pairs);
+  if (mode == kRotStaged)
+    lds += sizeof(uint16_t) * ((entries + 7) / 8 * 8) + 16 * (size_t)per * P.heads_per * P.upr;
   auto run = [&](auto tag) {
     using T = decltype(tag);
 #define R_(M)                                                                                   \
@@ -223,7 +302,7 @@ void rotary(const na_rotary_params *p, const void *q, const void *k, const void 
                      (const T *)k, pos, (T *)oq, (T *)ok)
     if (mode == kRotHalves) R_(kRotHalves);
     else if (mode == kRotAdjacent) R_(kRotAdjacent);
-    else R_(kRotPairs);
+    else R_(kRotStaged);
 #undef R_
   };
   if (p->dtype == NA_F32) run(float{});

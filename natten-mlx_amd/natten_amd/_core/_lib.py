@@ -164,6 +164,7 @@ class NaRotaryParams(ctypes.Structure):
     ]
 
 
+MAX_HEAD_DIM = 1024
 ROTARY_MAX_AXES = 4
 ROTARY_MAX_CHANNELS = 512
 # na_position_t by the positions' dtype

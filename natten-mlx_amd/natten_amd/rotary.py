@@ -52,6 +52,8 @@ def _check(query, key, positions, axis_dims, theta):
     if query.ndim not in (4, 5, 6):
         raise ValueError("rotary expects [B, *spatial, heads, dim] with one to three spatial "
                          f"axes, got shape {tuple(query.shape)}.")
+    if query.shape[-1] > _lib.MAX_HEAD_DIM:
+        raise ValueError(f"rotary takes up to {_lib.MAX_HEAD_DIM} channels, got {query.shape[-1]}.")
     lead = tuple(query.shape[:-2])
     if key is not None:
         if key.ndim != query.ndim or tuple(key.shape[:-2]) != lead:

@@ -84,6 +84,9 @@ CASES = {
     "one token": ((1, 1), 1, 1, 64, (64,)),
     "many heads of a token": ((3, 1), 70, 9, 64, (64,)),
     "widest": ((1, 3), 2, 1, 640, (512,)),
+    "widest, unlike halves": ((1, 3), 5, 2, 1024, (510,)),
+    "many wide heads, unlike halves": ((2, 2), 40, 7, 300, (118,)),
+    "many tokens, unlike halves": ((2, 40, 35), 2, 1, 26, (14, 10)),
     "many tokens": ((1, 5000), 1, 1, 16, (16,)),
 }
 
@@ -191,7 +194,7 @@ def test_gradient_against_differences():
 
     h = 0.5
     diff = (f(x + h * d) - f(x - h * d)) / (2 * h)
-    noise = 16 * E * float(x.norm() + d.norm()) * float(g.norm()) / h
+    noise = 16 * E * float(x.detach().norm() + d.norm()) * float(g.norm()) / h
     assert abs(diff - float((dx.double() * d.double()).sum())) <= noise
 
 
@@ -289,6 +292,7 @@ def test_refusals():
             ((q, k, None, (18,)), "rotate 18 channels"),
             ((torch.randn(1, 2, 1, 600), None, None, (514,)), "at most 512"),
             ((torch.randn(1, 2, 1, 15),), "must be even"),
+            ((torch.randn(1, 2, 1, 1026),), "up to 1024"),
             ((q, k, None, None, 0.0), "theta"),
             ((q, k, None, None, float("inf")), "theta")):
         with pytest.raises(ValueError, match=match):

@@ -487,6 +487,49 @@ typedef struct na_rotary_params {
 int na_rotary(const na_rotary_params *p, const void *q, const void *k,
               const void *positions, void *oq, void *ok, void *stream);
 
+/* ---- attention behind a shared prefix (serving) ------------------------------ */
+#define NA_PREFIX_MAX_HEAD_DIM 256
+
+/*
+ * The newest `tokens` tokens of every sample against keys in caches: `prefix`
+ * tokens that the whole batch shares, [prefix, kv_heads, D], and the sample's own,
+ * [B, capacity, kv_heads, D], of which the first seq_lens[b] are valid (the new
+ * tokens among them).  Query j of sample b is own token t = seq_lens[b] - tokens
+ * + j; it sees the prefix and the own tokens up to t (the last `window` of them
+ * where window > 0).  out [B, tokens, heads, D] is the softmax's mean of the values
+ * and lse [B, tokens, heads] (float32, natural log) the log of its sum; a query that
+ * sees no key gets zeros and -infinity.  This is causal neighborhood attention
+ * (causal windows of the reference's utils/window.py:8-34 at dilation 1) joined
+ * to global tokens, at the end of a sequence.
+ */
+typedef struct na_prefix_params {
+  int32_t batch;
+  int32_t tokens;      /* new tokens per sample */
+  int32_t heads;
+  int32_t kv_heads;    /* divides heads */
+  int32_t head_dim;    /* a multiple of 8, at most NA_PREFIX_MAX_HEAD_DIM */
+  int32_t dtype;
+  int32_t prefix;      /* shared tokens; 0: none */
+  int32_t capacity;    /* own tokens a sample can hold; 0: none */
+  int32_t window;      /* 0: all own tokens */
+  float scale;         /* positive and finite */
+  /* Optional device pointer to int32 [batch]; NULL: capacity.  Values outside
+   * [0, capacity] are taken as its ends. */
+  const int32_t *seq_lens;
+  int64_t q_stride[3];        /* elements: sample, token, head; channels adjacent */
+  int64_t prefix_k_stride[2]; /* token, head */
+  int64_t prefix_v_stride[2];
+  int64_t k_stride[3];        /* sample, token, head */
+  int64_t v_stride[3];
+} na_prefix_params;
+
+/* Bytes of device workspace na_prefix_fwd needs for these parameters. */
+size_t na_prefix_workspace_bytes(const na_prefix_params *p);
+/* lse may be NULL. */
+int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k,
+                  const void *prefix_v, const void *k, const void *v, void *out,
+                  float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

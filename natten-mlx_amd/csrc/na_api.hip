@@ -926,4 +926,56 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
   return launch_status("na_rotary");
 }
 
+namespace {
+
+int check_prefix(const na_prefix_params *p) {
+  if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
+  if (p->batch < 0 || p->tokens < 0 || p->heads < 1 || p->kv_heads < 1 || p->prefix < 0 ||
+      p->capacity < 0 || p->window < 0)
+    return fail(NA_ERR_INVALID, "a size is out of range (batch %d, tokens %d, heads %d, kv_heads %d, "
+                "prefix %d, capacity %d, window %d)", p->batch, p->tokens, p->heads, p->kv_heads,
+                p->prefix, p->capacity, p->window);
+  if (p->heads % p->kv_heads != 0)
+    return fail(NA_ERR_INVALID, "heads (%d) must be divisible by kv_heads (%d)", p->heads,
+                p->kv_heads);
+  if (p->dtype != NA_F32 && p->dtype != NA_F16 && p->dtype != NA_BF16)
+    return fail(NA_ERR_INVALID, "unknown dtype %d", p->dtype);
+  if (p->head_dim < 8 || p->head_dim % 8 != 0 || p->head_dim > NA_PREFIX_MAX_HEAD_DIM)
+    return fail(NA_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to %d, got %d",
+                NA_PREFIX_MAX_HEAD_DIM, p->head_dim);
+  if (!(p->scale > 0.f) || p->scale > 3e38f)
+    return fail(NA_ERR_INVALID, "scale must be positive and finite, got %g", (double)p->scale);
+  if (p->prefix > (1 << 30) || p->capacity > (1 << 30) || p->tokens > (1 << 30) ||
+      (int64_t)p->batch * p->tokens * p->heads >= ((int64_t)1 << 30))
+    return fail(NA_ERR_UNSUPPORTED, "more than 2^30 tokens, or batch * tokens * heads");
+  if (p->batch > 0 && p->tokens > 0 && !na::prefix_fits(p))
+    return fail(NA_ERR_UNSUPPORTED, "the call is too large for one launch");
+  return NA_OK;
+}
+
+}  // namespace
+
+size_t na_prefix_workspace_bytes(const na_prefix_params *p) {
+  if (check_prefix(p) != NA_OK || p->batch == 0 || p->tokens == 0) return 0;
+  return align256(na::prefix_workspace(p));
+}
+
+int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k,
+                  const void *prefix_v, const void *k, const void *v, void *out, float *lse,
+                  void *workspace, size_t workspace_bytes, void *stream) {
+  const int rc = check_prefix(p);
+  if (rc != NA_OK) return rc;
+  if (p->batch == 0 || p->tokens == 0) return NA_OK;
+  if (q == nullptr || out == nullptr ||
+      (p->prefix > 0 && (prefix_k == nullptr || prefix_v == nullptr)) ||
+      (p->capacity > 0 && (k == nullptr || v == nullptr)))
+    return fail(NA_ERR_INVALID, "q/prefix_k/prefix_v/k/v/out must be non-NULL");
+  const size_t need = align256(na::prefix_workspace(p));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(NA_ERR_WORKSPACE, "na_prefix_fwd needs a %zu-byte workspace (got %zu)", need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  na::prefix_attention(p, q, prefix_k, prefix_v, k, v, out, lse, workspace, as_stream(stream));
+  return launch_status("na_prefix_fwd");
+}
+
 }  // extern "C"

@@ -246,6 +246,14 @@ constexpr int kRotBlocks = 1024;  // workgroups that fill the chip
 void rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
             void *ok, hipStream_t st);
 
+// Attention against a shared prefix and own cached tokens (na_prefix.hip).
+constexpr int kPfxItems = 1024;  // workgroups that a call is split into
+bool prefix_fits(const na_prefix_params *p);
+size_t prefix_workspace(const na_prefix_params *p);
+void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, const void *pv,
+                      const void *k, const void *v, void *out, float *lse, void *workspace,
+                      hipStream_t st);
+
 // Generic pieces reused around the MFMA backward.
 void valu_delta(const Prob &P, int dtype, const void *out, const void *dout,
                 const float *dlse, float *delta, hipStream_t st);

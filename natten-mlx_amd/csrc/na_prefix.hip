@@ -1,0 +1,905 @@
+// na_prefix.hip — attention of new tokens against a cache whose prefix the whole
+// batch shares (serving).
+//
+// Query token j of sample b is token t = len_b - Lq + j of the sample's own
+// sequence.  It sees all N prefix tokens, of which there is one copy, and its own
+// tokens max(0, t - W + 1) .. t:
+//   out = softmax(scale q k^T) v over both, lse the log of the softmax's sum.
+//
+// The prefix's keys are one product for the batch: the rows of a key/value head
+// are all its query heads of all tokens of all samples, so every prefix tile is
+// read once per 128 rows instead of once per sample.  A sample's own keys meet
+// its own rows only.  Both are cut into chunks of keys; a workgroup takes a chunk
+// against a tile of rows and leaves (m, l, o) -- reference point, sum and
+// unnormalised output of an online softmax, float32 -- and k_pfx_join adds the
+// chunks of a row.  One launch holds the prefix's workgroups and the samples'.
+//
+// Two shapes of workgroup (four waves):
+//  * wide: 64 NQ rows, the waves share K / V tiles staged in LDS (as the dense
+//    forward does), one barrier per tile;
+//  * narrow: up to 16 rows, the waves take different tiles of 32 keys: K goes
+//    from memory straight into the matrix operand, V through the wave's own LDS
+//    (its transposing read), no barrier until the four results meet.
+// float32 runs narrow on the float32 matrix cores, without LDS tiles.
+#include "na_launch.h"
+#include "na_lean.h"
+
+#include <algorithm>
+
+namespace na {
+namespace {
+
+constexpr int kPfxThreads = 256;
+constexpr int kPfxNarrowKeys = 32;  // keys of a wave's tile
+
+struct PfxProb {
+  int32_t Lq, H, Hkv, rep, D;
+  int32_t M, Mo;            // rows per key/value head: of the batch, of a sample
+  int32_t N, S, W;          // prefix tokens, cached tokens a sample can hold, window
+  int32_t n_prefix, n_own;  // workgroups
+  int32_t prefix_launch;    // n_prefix up to a multiple of 8
+  int32_t own_launch;
+  int32_t rt_p, rt_o;       // row tiles
+  int32_t rows_p, rows_o;   // rows per tile: 16 narrow, more wide
+  int32_t chunk_p, chunk_o, SP, SO, NS;  // keys per chunk; chunks; slots per row
+  float sl2;                // scale * log2(e)
+  FastDiv frep, fLq, frt_p, fSP, frt_o, fSO, fHkv;
+  int64_t qs[3];            // element strides: sample, token, head
+  int64_t pks[2], pvs[2];   // prefix: token, head
+  int64_t ks[3], vs[3];     // own: sample, token, head
+  const int32_t *lens;      // own tokens per sample, or null: S
+};
+
+struct PfxArgs {
+  const void *q, *pk, *pv, *k, *v;
+  void *out;
+  float *lse;
+  float *po;    // [Hkv][M][NS][D] partial outputs, or null: one slot, written to out
+  float2 *pml;  // [Hkv][M][NS] reference points and sums
+};
+
+__device__ __forceinline__ int pfx_len(const PfxProb &P, int b) {
+  return P.lens == nullptr ? P.S : min(max(P.lens[b], 0), P.S);
+}
+
+// Own tokens [lo, hi) that token j of a sample of `len` tokens sees.
+struct PfxSpan {
+  int lo, hi;
+};
+__device__ __forceinline__ PfxSpan pfx_span(const PfxProb &P, int len, int j) {
+  const int t = len - P.Lq + j;
+  PfxSpan s;
+  s.hi = max(t + 1, 0);
+  s.lo = max(t - P.W + 1, 0);
+  return s;
+}
+
+// What a workgroup does: keys [k0, k1) of one head against rows [row0, row1).
+struct PfxItem {
+  const char *k, *v;    // of key 0
+  int64_t kst, vst;     // bytes from key to key
+  int g, b, len;        // b < 0: the prefix
+  int k0, k1, row0, row1, slot;
+  int lo_max, hi_min;   // keys that every row sees: [lo_max, hi_min)
+};
+
+// False where there is nothing to do.
+template <typename T>
+__device__ __forceinline__ bool pfx_item(const PfxProb &P, const PfxArgs &A, int bid, PfxItem &w) {
+  if (bid < P.prefix_launch) {
+    const int item = xcd_tile(bid, P.prefix_launch);  // a chunk's row tiles share an L2
+    if (item >= P.n_prefix) return false;
+    const int c = (int)fdiv((uint32_t)item, P.frt_p), rt = item - c * P.rt_p;
+    w.g = (int)fdiv((uint32_t)c, P.fSP);
+    w.slot = c - w.g * P.SP;
+    w.b = -1;
+    w.len = 0;
+    w.k0 = w.slot * P.chunk_p;
+    w.k1 = min(w.k0 + P.chunk_p, P.N);
+    w.row0 = rt * P.rows_p;
+    w.row1 = min(w.row0 + P.rows_p, P.M);
+    w.k = reinterpret_cast<const char *>(static_cast<const T *>(A.pk) + w.g * P.pks[1]);
+    w.v = reinterpret_cast<const char *>(static_cast<const T *>(A.pv) + w.g * P.pvs[1]);
+    w.kst = P.pks[0] * (int64_t)sizeof(T);
+    w.vst = P.pvs[0] * (int64_t)sizeof(T);
+    w.lo_max = 0;
+    w.hi_min = P.N;
+    return w.k0 < w.k1;
+  }
+  const int item = xcd_tile(bid - P.prefix_launch, P.own_launch);
+  if (item >= P.n_own) return false;
+  const int c = (int)fdiv((uint32_t)item, P.frt_o), rt = item - c * P.rt_o;
+  const int bg = (int)fdiv((uint32_t)c, P.fSO), cc = c - bg * P.SO;
+  w.b = (int)fdiv((uint32_t)bg, P.fHkv);
+  w.g = bg - w.b * P.Hkv;
+  w.slot = P.SP + cc;
+  w.len = pfx_len(P, w.b);
+  w.row0 = w.b * P.Mo + rt * P.rows_o;
+  w.row1 = min(w.row0 + P.rows_o, (w.b + 1) * P.Mo);
+  const int j0 = (int)fdiv((uint32_t)(w.row0 - w.b * P.Mo), P.frep);
+  const int j1 = (int)fdiv((uint32_t)(w.row1 - 1 - w.b * P.Mo), P.frep);
+  const PfxSpan first = pfx_span(P, w.len, j0), last = pfx_span(P, w.len, j1);
+  const int lo = pfx_span(P, w.len, 0).lo;  // the sample's chunks start here
+  w.k0 = max(lo + cc * P.chunk_o, first.lo);
+  w.k1 = min(lo + (cc + 1) * P.chunk_o, last.hi);
+  w.k = reinterpret_cast<const char *>(static_cast<const T *>(A.k) + w.b * P.ks[0] + w.g * P.ks[2]);
+  w.v = reinterpret_cast<const char *>(static_cast<const T *>(A.v) + w.b * P.vs[0] + w.g * P.vs[2]);
+  w.kst = P.ks[1] * (int64_t)sizeof(T);
+  w.vst = P.vs[1] * (int64_t)sizeof(T);
+  w.lo_max = last.lo;
+  w.hi_min = min(first.hi, w.k1);
+  return w.k0 < w.k1;
+}
+
+// A row of a workgroup's tile: its queries, and the keys of [k0, k1) it sees.
+template <typename T>
+struct PfxRow {
+  const T *q;
+  int lo, n;  // [lo, lo + n)
+  __device__ __forceinline__ PfxRow(const PfxProb &P, const PfxArgs &A, const PfxItem &w, int row) {
+    const int r = min(row, w.row1 - 1);
+    const int tt = (int)fdiv((uint32_t)r, P.frep), i = r - tt * P.rep;
+    const int b = (int)fdiv((uint32_t)tt, P.fLq), j = tt - b * P.Lq;
+    q = static_cast<const T *>(A.q) + b * P.qs[0] + j * P.qs[1] + (int64_t)(w.g * P.rep + i) * P.qs[2];
+    lo = w.k0;
+    int hi = w.k1;
+    if (w.b >= 0) {
+      const PfxSpan s = pfx_span(P, w.len, j);
+      lo = max(lo, s.lo);
+      hi = min(hi, s.hi);
+    }
+    n = max(hi - lo, 0);
+  }
+};
+
+// Row's element offset in out (its D channels) and index in lse.
+__device__ __forceinline__ int64_t pfx_out_row(const PfxProb &P, int g, int row) {
+  const int tt = (int)fdiv((uint32_t)row, P.frep);
+  return (int64_t)tt * P.H + g * P.rep + (row - tt * P.rep);
+}
+
+template <typename T>
+struct PfxStore;  // four results of a row, rounded
+template <>
+struct PfxStore<float> {
+  static __device__ __forceinline__ void put(float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; }
+};
+template <typename T>
+struct PfxStore16 {
+  static __device__ __forceinline__ void put(T *p, f32x4 x) {
+    typename L16<T>::v4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (typename L16<T>::e)x[r];
+    *reinterpret_cast<typename L16<T>::v4 *>(p) = o;
+  }
+};
+template <>
+struct PfxStore<bf16_t> : PfxStore16<bf16_t> {};
+template <>
+struct PfxStore<f16_t> : PfxStore16<f16_t> {};
+
+// A row's slot: four channels from c, or the row's (m, l).
+template <typename T>
+__device__ __forceinline__ void pfx_put(const PfxProb &P, const PfxArgs &A, const PfxItem &w, int row,
+                                        int c, f32x4 o, float l) {
+  if (c >= P.D) return;
+  if (A.po != nullptr) {
+    const int64_t r = ((int64_t)w.g * P.M + row) * P.NS + w.slot;
+    *reinterpret_cast<f32x4 *>(A.po + r * P.D + c) = o;
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    PfxStore<T>::put(static_cast<T *>(A.out) + pfx_out_row(P, w.g, row) * P.D + c, o * inv);
+  }
+}
+__device__ __forceinline__ void pfx_put_ml(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
+                                           int row, float m, float l) {
+  if (A.po != nullptr)
+    A.pml[((int64_t)w.g * P.M + row) * P.NS + w.slot] = make_float2(m, l);
+  else if (A.lse != nullptr)
+    A.lse[pfx_out_row(P, w.g, row)] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Any alignment of the elements.
+template <typename T>
+__device__ __forceinline__ typename L16<T>::v8 pfx_ld8(const char *p) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+  typedef uint32_t r4 __attribute__((ext_vector_type(4)));
+  const r4 x = *reinterpret_cast<const u4 *>(p);
+  return __builtin_bit_cast(typename L16<T>::v8, x);
+}
+template <typename T>
+__device__ __forceinline__ typename L16<T>::v8 pfx_zero8() {
+  typename L16<T>::v8 z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = (typename L16<T>::e)0.f;
+  return z;
+}
+
+// Online softmax step of a lane's CH * 4 scores of one row (the four lanes of a
+// row hold the others): scores to probabilities in place, m, l and o rescaled
+// where the reference point m moves.  It may trail the maximum by 8 (a factor
+// 2^8 in p): exact after the division by l.
+template <int CH, int NDB>
+__device__ __forceinline__ void pfx_softmax(float (&p)[CH][4], float sl2, float &m, float &l,
+                                            f32x4 (&o)[NDB]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, p[ch][r]);
+  mx = quad_max(mx) * sl2;
+  if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+    const float mn = fmaxf(m, mx);
+    const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= alpha;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+    m = mn;
+  }
+  const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[ch][r] = __builtin_amdgcn_exp2f(fmaf(p[ch][r], sl2, -mu));
+      l += p[ch][r];
+    }
+}
+
+// Whether 16-bit element x is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool pfx_odd16(uint32_t x) {
+  const uint32_t e = sizeof(T) == 2 && std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  return (x & e) == e;
+}
+
+// V rows [0, rows) of a tile in LDS hold an infinity or NaN (all lanes look).
+template <typename T, int D>
+__device__ __forceinline__ bool pfx_odd_tile(const typename L16<T>::e *vs, int stride, int rows,
+                                             int lane) {
+  bool odd = false;
+  for (int u = lane; u < rows * (D / 8); u += 64) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(vs + u / (D / 8) * stride + u % (D / 8) * 8);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= pfx_odd16<T>(w[i]) | pfx_odd16<T>(w[i] >> 16);
+  }
+  return __builtin_amdgcn_ballot_w64(odd) != 0;
+}
+
+// o += P V key by key, only over the keys that the lane's row sees: for tiles
+// where rows see different keys and V is not finite everywhere, where a product
+// with a probability of zero would not be zero.
+template <typename T, int CH, int NDB>
+__device__ __forceinline__ void pfx_odd_pv(const float (&p)[CH][4],
+                                                     const typename L16<T>::e *vs, int stride,
+                                                     int lane, int lo, int n, f32x4 (&o)[NDB]) {
+  const int row = lane & 15, gq = lane >> 4;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll 1
+      for (int g2 = 0; g2 < 4; ++g2) {
+        const int key = 16 * ch + 4 * g2 + r;
+        const float pk = __shfl(p[ch][r], row + 16 * g2, 64);
+        if ((unsigned)(key - lo) >= (unsigned)n) continue;
+        const typename L16<T>::e *v = vs + key * stride + 4 * gq;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[db][c] = fmaf(pk, (float)v[16 * db + c], o[db][c]);
+      }
+}
+
+template <int D>
+constexpr int pfx_tile() {
+  return D > 128 ? 32 : 64;  // keys of a wide tile
+}
+
+template <typename T, int D, int NQ>
+__device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
+                                         char *smem) {
+  typedef L16<T> M;
+  typedef typename M::v8 v8;
+  typedef typename M::v4 v4;
+  typedef typename M::e E;
+  constexpr int TK = pfx_tile<D>(), CH = TK / 16;
+  constexpr int NT = D / 32, NDB = D / 16, RSE = lds_row(D);
+  constexpr int UPR = D / 4, RPP = kPfxThreads / UPR, NU = TK / RPP;
+  E *const buf = reinterpret_cast<E *>(smem);
+  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63;
+  const int n = lane & 15, gq = lane >> 4;
+
+  // staging: the thread's column unit c and rows r0 + RPP i
+  const int c = tid % UPR, r0 = tid / UPR;
+  const bool isv = c >= D / 8;
+  const int col = 8 * (isv ? c - D / 8 : c);
+  const bool colok = col < P.D;
+  const int64_t st = isv ? w.vst : w.kst;
+  const char *const src = (isv ? w.v : w.k) + 2 * col + (int64_t)(w.k0 + r0) * st;
+  const int unit = r0 * RSE + 8 * c + (isv ? 8 : 0);
+  v8 pre[NU];
+  auto load_tile = [&](int t) {  // t: keys behind k0
+    const char *p = src + (int64_t)t * st;
+    const int left = w.k1 - w.k0 - t - r0;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      pre[i] = pfx_zero8<T>();
+      if (colok && RPP * i < left) pre[i] = pfx_ld8<T>(p);
+      p += RPP * st;
+    }
+  };
+  auto store_tile = [&](E *dst) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) *reinterpret_cast<v8 *>(dst + unit + RPP * i * RSE) = pre[i];
+  };
+  load_tile(0);
+
+  const int row0 = w.row0 + wv * (16 * NQ);
+  v8 qf[NQ][NT];
+  int lo[NQ], cnt[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const PfxRow<T> r(P, A, w, row0 + 16 * qi + n);
+    lo[qi] = r.lo - w.k0;
+    cnt[qi] = r.n;
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const int cq = 32 * s + 8 * gq;
+      qf[qi][s] = cq < P.D ? pfx_ld8<T>(reinterpret_cast<const char *>(r.q + cq)) : pfx_zero8<T>();
+    }
+  }
+  f32x4 o[NQ][NDB];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[qi][db] = zero4();
+    m[qi] = -INFINITY;
+    l[qi] = 0.f;
+  }
+  const float sl2 = P.sl2;
+  const int ka_off = n * RSE + 8 * gq;
+  const int tr_off = (4 * gq + (n >> 2)) * RSE + 4 * (n & 3);
+  const bool spans = w.b >= 0 && P.Lq > 1;  // rows may see different keys
+
+  store_tile(buf);
+  __syncthreads();
+  const int nkt = (w.k1 - w.k0 + TK - 1) / TK;
+  for (int j = 0; j < nkt; ++j) {
+    const int t0 = j * TK;
+    if (j + 1 < nkt) load_tile(t0 + TK);  // in flight during this tile
+    const E *ks = buf + (j & 1) * (TK * RSE);
+    const E *vs = ks + lds_y(D);
+    const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
+    const bool odd = !all && spans && pfx_odd_tile<T, D>(vs, RSE, TK, lane);
+    v8 bp[NQ][CH / 2];
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      float p[CH][4];
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        f32x4 s = zero4();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          s = M::mma(*reinterpret_cast<const v8 *>(ks + 16 * ch * RSE + ka_off + 32 * t), qf[qi][t], s);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[ch][r] = s[r];
+      }
+      if (!all) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((unsigned)(t0 + 16 * ch + 4 * gq + r - lo[qi]) >= (unsigned)cnt[qi])
+              p[ch][r] = -INFINITY;
+      }
+      pfx_softmax<CH, NDB>(p, sl2, m[qi], l[qi], o[qi]);
+      if (odd) pfx_odd_pv<T, CH, NDB>(p, vs, RSE, lane, lo[qi] - t0, cnt[qi], o[qi]);
+#pragma unroll
+      for (int jj = 0; jj < CH / 2; ++jj)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) bp[qi][jj][4 * hh + r] = (E)p[2 * jj + hh][r];
+    }
+    if (!odd) {
+#pragma unroll
+      for (int jj = 0; jj < CH / 2; ++jj) {
+        const E *ca = vs + 32 * jj * RSE + tr_off;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const v4 lo4 = M::tr(ca + 16 * db);
+          const v4 hi4 = M::tr(ca + 16 * RSE + 16 * db);
+          const v8 a = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+          for (int qi = 0; qi < NQ; ++qi) o[qi][db] = M::mma(a, bp[qi][jj], o[qi][db]);
+        }
+      }
+    }
+    if (j + 1 < nkt) store_tile(buf + ((j + 1) & 1) * (TK * RSE));
+    __syncthreads();
+  }
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const float lt = quad_sum(l[qi]);
+    const int row = row0 + 16 * qi + n;
+    if (row >= w.row1) continue;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) pfx_put<T>(P, A, w, row, 16 * db + 4 * gq, o[qi][db], lt);
+    if (gq == 0) pfx_put_ml(P, A, w, row, m[qi], lt);
+  }
+}
+
+// The four waves' results of up to 16 rows meet in LDS.  o: channel chan(db) ..
+// + 3 of row lane & 15.
+template <typename T, int D, int NDB, typename C>
+__device__ __forceinline__ void pfx_meet(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
+                                         char *smem, float m, float l, const f32x4 (&o)[NDB], C chan) {
+  constexpr int RS = D + 4;  // floats per row
+  float *const po = reinterpret_cast<float *>(smem);
+  float2 *const ml = reinterpret_cast<float2 *>(po + 4 * 16 * RS);  // [4][16]
+  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, n = lane & 15;
+  l = quad_sum(l);
+  __syncthreads();  // the tiles' LDS is free
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+    *reinterpret_cast<f32x4 *>(po + (wv * 16 + n) * RS + chan(db)) = o[db];
+  if (lane < 16) ml[wv * 16 + n] = make_float2(m, l);
+  __syncthreads();
+  const int r = tid >> 4, row = w.row0 + r;  // 16 threads per row
+  if (row >= w.row1) return;
+  float2 x[4];
+  float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = ml[i * 16 + r];
+    mt = fmaxf(mt, x[i].x);
+  }
+  float wt[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    wt[i] = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - mt);  // (NaN: a seen row)
+    lt = x[i].y == 0.f ? lt : fmaf(wt[i], x[i].y, lt);
+  }
+  for (int c = 4 * (tid & 15); c < D; c += 64) {
+    f32x4 s = zero4();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x[i].y != 0.f) s += wt[i] * *reinterpret_cast<const f32x4 *>(po + (i * 16 + r) * RS + c);
+    pfx_put<T>(P, A, w, row, c, s, lt);
+  }
+  if ((tid & 15) == 0) pfx_put_ml(P, A, w, row, mt, lt);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
+                                           char *smem) {
+  typedef L16<T> M;
+  typedef typename M::v8 v8;
+  typedef typename M::v4 v4;
+  typedef typename M::e E;
+  constexpr int TK = kPfxNarrowKeys, NT = D / 32, NDB = D / 16, RS = D + 8;
+  constexpr int UPR = D / 8, RPP = 64 / UPR, NU = TK / RPP;  // V: units per row, rows per pass
+  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63;
+  const int n = lane & 15, gq = lane >> 4;
+  E *const vs = reinterpret_cast<E *>(smem) + wv * (TK * RS);  // the wave's own
+  const PfxRow<T> row(P, A, w, w.row0 + n);
+  const int lo = row.lo - w.k0, cnt = row.n;
+  v8 qf[NT];
+#pragma unroll
+  for (int s = 0; s < NT; ++s) {
+    const int cq = 32 * s + 8 * gq;
+    qf[s] = cq < P.D ? pfx_ld8<T>(reinterpret_cast<const char *>(row.q + cq)) : pfx_zero8<T>();
+  }
+  const int vc = lane % UPR, vr = lane / UPR;
+  const int total = w.k1 - w.k0;
+  const char *const kp = w.k + (int64_t)(w.k0 + n) * w.kst + 16 * gq;
+  const char *const vp = w.v + (int64_t)(w.k0 + vr) * w.vst + 16 * vc;
+  v8 kr[2][NT], vr8[NU];
+  auto load = [&](int t0) {
+    const int left = total - t0;
+    const char *a = kp + (int64_t)t0 * w.kst, *b = vp + (int64_t)t0 * w.vst;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int s = 0; s < NT; ++s) {
+        kr[hh][s] = pfx_zero8<T>();
+        if (16 * hh + n < left && 32 * s + 8 * gq < P.D)
+          kr[hh][s] = pfx_ld8<T>(a + 16 * hh * w.kst + 64 * s);
+      }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      vr8[i] = pfx_zero8<T>();
+      if (RPP * i + vr < left && 8 * vc < P.D) vr8[i] = pfx_ld8<T>(b + RPP * i * w.vst);
+    }
+  };
+  f32x4 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = zero4();
+  float m = -INFINITY, l = 0.f;
+  const float sl2 = P.sl2;
+  const int tr_off = (4 * gq + (n >> 2)) * RS + 4 * (n & 3);
+  const bool spans = w.b >= 0 && P.Lq > 1;
+  int t0 = wv * TK;
+  if (t0 < total) load(t0);
+  for (; t0 < total; t0 += 4 * TK) {
+    f32x4 s[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      s[hh] = zero4();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[hh] = M::mma(kr[hh][t], qf[t], s[hh]);
+    }
+    __builtin_amdgcn_wave_barrier();  // the reads of the tile before are issued
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      *reinterpret_cast<v8 *>(vs + (RPP * i + vr) * RS + 8 * vc) = vr8[i];
+    if (t0 + 4 * TK < total) load(t0 + 4 * TK);  // in flight during the rest
+    const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
+    float p[2][4];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        p[hh][r] = all || (unsigned)(t0 + 16 * hh + 4 * gq + r - lo) < (unsigned)cnt ? s[hh][r]
+                                                                                     : -INFINITY;
+    pfx_softmax<2, NDB>(p, sl2, m, l, o);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (!all && spans && pfx_odd_tile<T, D>(vs, RS, TK, lane)) {
+      pfx_odd_pv<T, 2, NDB>(p, vs, RS, lane, lo - t0, cnt, o);
+    } else {
+      v8 bp;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bp[4 * hh + r] = (E)p[hh][r];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const v4 lo4 = M::tr(vs + tr_off + 16 * db);
+        const v4 hi4 = M::tr(vs + 16 * RS + tr_off + 16 * db);
+        o[db] = M::mma(__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7), bp, o[db]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  }
+  pfx_meet<T, D, NDB>(P, A, w, smem, m, l, o, [&](int db) { return 16 * db + 4 * gq; });
+}
+
+// Shape of a segment's workgroups: NQ of the wide ones, 0 the narrow ones.
+template <typename T, int D>
+__global__ void __launch_bounds__(kPfxThreads, D > 128 ? 1 : 2) k_pfx(PfxProb P, PfxArgs A) {
+  extern __shared__ __align__(16) char smem[];
+  PfxItem w;
+  if (!pfx_item<T>(P, A, blockIdx.x, w)) return;
+  const int shape = (w.b < 0 ? P.rows_p : P.rows_o) >> 6;
+  if (shape == 0) {
+    pfx_narrow<T, D>(P, A, w, smem);
+  } else if (D > 128 || shape == 1) {
+    pfx_wide<T, D, 1>(P, A, w, smem);
+  } else {
+    if constexpr (D <= 128) pfx_wide<T, D, 2>(P, A, w, smem);
+  }
+}
+
+// float32: 16 rows per workgroup, tiles of 16 keys per wave on 16x16x4 products.
+// Contraction slots are dealt so that every operand is a 16-byte load: a lane's
+// four channels 16 s + 4 gq .. of K feed four products, and its four channels
+// 64 u + 4 n .. of a V row four blocks of O^T, whose row i is then channel
+// 64 u + 4 i + e.
+template <int D>
+__global__ void __launch_bounds__(kPfxThreads) k_pfx32(PfxProb P, PfxArgs A) {
+  constexpr int TK = 16, NS = D / 16, NU = D / 64;
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+  extern __shared__ __align__(16) char smem[];
+  PfxItem w;
+  if (!pfx_item<float>(P, A, blockIdx.x, w)) return;
+  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63;
+  const int n = lane & 15, gq = lane >> 4;
+  const PfxRow<float> row(P, A, w, w.row0 + n);
+  const int lo = row.lo - w.k0, cnt = row.n;
+  auto ld = [&](const char *p, bool ok) {
+    f32x4 x = zero4();
+    if (ok) x = *reinterpret_cast<const f4u *>(p);
+    return x;
+  };
+  f32x4 qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    qf[s] = ld(reinterpret_cast<const char *>(row.q + 16 * s + 4 * gq), 16 * s + 4 * gq < P.D);
+  const int total = w.k1 - w.k0;
+  const char *const kp = w.k + (int64_t)(w.k0 + n) * w.kst + 16 * gq;
+  const char *const vp = w.v + (int64_t)(w.k0 + 4 * gq) * w.vst + 16 * n;
+  f32x4 o[4 * NU];
+#pragma unroll
+  for (int i = 0; i < 4 * NU; ++i) o[i] = zero4();
+  float m = -INFINITY, l = 0.f;
+  const bool spans = w.b >= 0 && P.Lq > 1;
+  for (int t0 = wv * TK; t0 < total; t0 += 4 * TK) {
+    const char *const a = kp + (int64_t)t0 * w.kst, *const b = vp + (int64_t)t0 * w.vst;
+    f32x4 kr[NS], vr[4][NU];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      kr[s] = ld(a + 64 * s, t0 + n < total && 16 * s + 4 * gq < P.D);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        vr[r][u] = ld(b + r * w.vst + 256 * u, t0 + 4 * gq + r < total && 64 * u + 4 * n < P.D);
+    f32x4 s4 = zero4();
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[s][e], qf[s][e], s4, 0, 0, 0);
+    const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
+    float p[1][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      p[0][r] = all || (unsigned)(t0 + 4 * gq + r - lo) < (unsigned)cnt ? s4[r] : -INFINITY;
+    pfx_softmax<1, 4 * NU>(p, P.sl2, m, l, o);
+    bool odd = false;
+    if (!all && spans) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            odd |= (__float_as_uint(vr[r][u][e]) & 0x7f800000u) == 0x7f800000u;
+    }
+    if (__builtin_amdgcn_ballot_w64(odd) == 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[4 * u + e] =
+                __builtin_amdgcn_mfma_f32_16x16x4f32(vr[r][u][e], p[0][r], o[4 * u + e], 0, 0, 0);
+    } else {  // as pfx_odd_pv: V's elements come from the lanes that hold them
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll 1
+        for (int g2 = 0; g2 < 4; ++g2) {
+          const float pk = __shfl(p[0][r], n + 16 * g2, 64);
+          const bool sees = (unsigned)(t0 + 4 * g2 + r - lo) < (unsigned)cnt;
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = __shfl(vr[r][u][e], 4 * gq + i + 16 * g2, 64);
+                if (sees) o[4 * u + e][i] = fmaf(pk, v, o[4 * u + e][i]);
+              }
+        }
+    }
+  }
+  // block e of group u, element i: channel 64 u + 4 (4 gq + i) + e; dealt to
+  // blocks of four adjacent channels
+  f32x4 q4[4 * NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q4[4 * u + i][e] = o[4 * u + e][i];
+  pfx_meet<float, D, 4 * NU>(P, A, w, smem, m, l, q4,
+                             [&](int x) { return 64 * (x >> 2) + 16 * gq + 4 * (x & 3); });
+}
+
+// The slots of a row added: lanes take four channels each, 2^lgG of them a row,
+// and 2^lgS such groups share the row's slots.
+template <typename T>
+__global__ void __launch_bounds__(256) k_pfx_join(PfxProb P, PfxArgs A, int lgG, int lgS) {
+  __shared__ f32x4 so[256];
+  __shared__ float2 sml[256];
+  const int tid = threadIdx.x, lane = tid & ((1 << lgG) - 1);
+  const int group = tid >> lgG, share = group & ((1 << lgS) - 1);
+  const int64_t rows = (int64_t)P.Hkv * P.M;
+  const int64_t mine = ((int64_t)blockIdx.x * 256 + tid) >> (lgG + lgS);
+  const int64_t r = min(mine, rows - 1);
+  const int g = (int)(r / P.M), row = (int)(r - (int64_t)g * P.M);
+  // the slots that were written: the prefix's, and the own chunks the row sees
+  const int tt = (int)fdiv((uint32_t)row, P.frep);
+  const int b = (int)fdiv((uint32_t)tt, P.fLq), j = tt - b * P.Lq;
+  int c0 = 0, c1 = 0;
+  if (P.SO > 0) {
+    const int len = pfx_len(P, b), base = pfx_span(P, len, 0).lo;
+    const PfxSpan s = pfx_span(P, len, j);
+    if (s.hi > s.lo) {
+      c0 = (s.lo - base) / P.chunk_o;
+      c1 = (s.hi - 1 - base) / P.chunk_o + 1;
+    }
+  }
+  const int count = P.SP + c1 - c0;
+  auto slot = [&](int i) { return i < P.SP ? i : i + c0; };
+  const float2 *const ml = A.pml + r * P.NS;
+  const float *const po = A.po + r * P.NS * P.D;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = zero4();
+  const int c = 4 * lane;
+  for (int i = share; i < count; i += 1 << lgS) m = fmaxf(m, ml[slot(i)].x);
+#pragma unroll 4
+  for (int i = share; i < count; i += 1 << lgS) {
+    const float2 x = ml[slot(i)];
+    f32x4 o = zero4();
+    if (c < P.D) o = *reinterpret_cast<const f32x4 *>(po + (int64_t)slot(i) * P.D + c);
+    if (x.y != 0.f) {  // (0: a row that sees nothing of the chunk)
+      const float wt = __builtin_amdgcn_exp2f(x.x - m);
+      l = fmaf(wt, x.y, l);
+      acc += wt * o;
+    }
+  }
+  if (lgS > 0) {
+    so[tid] = acc;
+    sml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (share != 0) return;
+    for (int i = 1; i < 1 << lgS; ++i) m = fmaxf(m, sml[tid + (i << lgG)].x);
+    l = 0.f;
+    acc = zero4();
+    for (int i = 0; i < 1 << lgS; ++i) {
+      const float2 x = sml[tid + (i << lgG)];
+      if (x.y != 0.f) {
+        const float wt = __builtin_amdgcn_exp2f(x.x - m);
+        l = fmaf(wt, x.y, l);
+        acc += wt * so[tid + (i << lgG)];
+      }
+    }
+  }
+  if (mine >= rows) return;
+  const int64_t out = pfx_out_row(P, g, row);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (c < P.D) PfxStore<T>::put(static_cast<T *>(A.out) + out * P.D + c, acc * inv);
+  if (lane == 0 && A.lse != nullptr) A.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+int pfx_width(int dtype, int D) {  // the kernels' head dim
+  if (dtype == NA_F32) return D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256;
+}
+
+// Rows of a tile: narrow up to 16, wide above, 128 where there are more than 64.
+int pfx_rows(int dtype, int D, int64_t rows) {
+  if (dtype == NA_F32 || rows <= 16) return 16;
+  return rows <= 64 || D > 128 ? 64 : 128;
+}
+
+// Keys per chunk: about kPfxItems workgroups in all, each with a chunk of at
+// least one tile per wave.
+PfxProb pfx_prob(const na_prefix_params *p) {
+  PfxProb P{};
+  P.Lq = p->tokens;
+  P.H = p->heads;
+  P.Hkv = p->kv_heads;
+  P.rep = p->heads / p->kv_heads;
+  P.D = p->head_dim;
+  P.Mo = P.Lq * P.rep;
+  P.M = (int32_t)(p->batch * P.Mo);
+  P.N = p->prefix;
+  P.S = p->capacity;
+  P.W = p->window > 0 ? p->window : 1 << 30;
+  P.rows_p = pfx_rows(p->dtype, P.D, P.M);
+  P.rows_o = pfx_rows(p->dtype, P.D, P.Mo);
+  P.rt_p = (P.M + P.rows_p - 1) / P.rows_p;
+  P.rt_o = (P.Mo + P.rows_o - 1) / P.rows_o;
+  const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
+  const int64_t tp = (int64_t)P.Hkv * P.rt_p, to = (int64_t)p->batch * P.Hkv * P.rt_o;
+  const int64_t visits = tp * P.N + to * span;
+  auto chunk = [&](int64_t keys, int rows) {
+    const int64_t least = rows > 16 ? 256 : 128;
+    const int64_t want = std::max((visits + kPfxItems - 1) / kPfxItems, least);
+    const int64_t parts = std::max<int64_t>(1, (keys + want - 1) / want);
+    return (int32_t)(((keys + parts - 1) / parts + 63) / 64 * 64);
+  };
+  if (P.N > 0) {
+    P.chunk_p = chunk(P.N, P.rows_p);
+    P.SP = (P.N + P.chunk_p - 1) / P.chunk_p;
+  }
+  if (span > 0) {
+    P.chunk_o = chunk(span, P.rows_o);
+    P.SO = (int32_t)((span + P.chunk_o - 1) / P.chunk_o);
+  }
+  P.NS = P.SP + P.SO;
+  P.n_prefix = (int32_t)(tp * P.SP);
+  P.n_own = (int32_t)(to * P.SO);
+  P.prefix_launch = (P.n_prefix + 7) & ~7;
+  P.own_launch = (P.n_own + 7) & ~7;
+  P.sl2 = p->scale * kLog2e;
+  P.frep = make_fastdiv((uint32_t)P.rep);
+  P.fLq = make_fastdiv((uint32_t)P.Lq);
+  P.frt_p = make_fastdiv((uint32_t)P.rt_p);
+  P.frt_o = make_fastdiv((uint32_t)P.rt_o);
+  P.fSP = make_fastdiv((uint32_t)std::max(P.SP, 1));
+  P.fSO = make_fastdiv((uint32_t)std::max(P.SO, 1));
+  P.fHkv = make_fastdiv((uint32_t)P.Hkv);
+  for (int i = 0; i < 3; ++i) {
+    P.qs[i] = p->q_stride[i];
+    P.ks[i] = p->k_stride[i];
+    P.vs[i] = p->v_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    P.pks[i] = p->prefix_k_stride[i];
+    P.pvs[i] = p->prefix_v_stride[i];
+  }
+  P.lens = p->seq_lens;
+  return P;
+}
+
+// One slot that every row fills needs no join.
+bool pfx_direct(const PfxProb &P) { return P.SP == 1 && P.SO == 0; }
+
+size_t pfx_part_bytes(const PfxProb &P) {
+  return ((size_t)P.Hkv * P.M * P.NS * P.D * sizeof(float) + 255) & ~(size_t)255;
+}
+
+template <typename T, int D>
+void pfx_launch(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
+  auto lds = [&](int rows) -> size_t {
+    if (rows > 16) return sizeof(T) * 2 * pfx_tile<D>() * lds_row(D);
+    const size_t meet = sizeof(float) * 4 * 16 * (D + 4) + sizeof(float2) * 64;
+    const size_t tiles = sizeof(T) == 2 ? sizeof(T) * 4 * kPfxNarrowKeys * (D + 8) : 0;
+    return std::max(meet, tiles);
+  };
+  const size_t bytes = std::max(P.SP > 0 ? lds(P.rows_p) : 0, P.SO > 0 ? lds(P.rows_o) : 0);
+  const dim3 grid((unsigned)(P.prefix_launch + P.own_launch));
+  if constexpr (sizeof(T) == 4)
+    hipLaunchKernelGGL((k_pfx32<D>), grid, dim3(kPfxThreads), bytes, st, P, A);
+  else
+    hipLaunchKernelGGL((k_pfx<T, D>), grid, dim3(kPfxThreads), bytes, st, P, A);
+}
+
+template <typename T>
+void pfx_run(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
+  if (P.NS > 0) {
+    const int width = pfx_width(sizeof(T) == 4 ? NA_F32 : NA_BF16, P.D);
+    if (width == 256) pfx_launch<T, 256>(P, A, st);
+    else if (width == 128) pfx_launch<T, 128>(P, A, st);
+    else if (sizeof(T) == 4 || width == 64) pfx_launch<T, 64>(P, A, st);
+    else if constexpr (sizeof(T) == 2) pfx_launch<T, 32>(P, A, st);
+  }
+  if (A.po == nullptr && P.NS > 0) return;
+  int lgG = 0, lgS = 0;
+  while ((4 << lgG) < P.D) ++lgG;
+  while (lgG + lgS < 8 && (8 << lgS) < P.NS) ++lgS;
+  const int64_t threads = ((int64_t)P.Hkv * P.M) << (lgG + lgS);
+  hipLaunchKernelGGL((k_pfx_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
+                     lgG, lgS);
+}
+
+}  // namespace
+
+bool prefix_fits(const na_prefix_params *p) {
+  const PfxProb P = pfx_prob(p);
+  const int64_t lim = ((int64_t)1 << 31) - 16;
+  return (int64_t)P.Hkv * P.rt_p * P.SP < lim && (int64_t)p->batch * P.Hkv * P.rt_o * P.SO < lim &&
+         (int64_t)P.prefix_launch + P.own_launch < lim &&
+         ((int64_t)P.Hkv * P.M) < (lim >> 1);
+}
+
+size_t prefix_workspace(const na_prefix_params *p) {
+  const PfxProb P = pfx_prob(p);
+  if (P.NS == 0 || pfx_direct(P)) return 0;
+  return pfx_part_bytes(P) + sizeof(float2) * (size_t)P.Hkv * P.M * P.NS;
+}
+
+void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, const void *pv,
+                      const void *k, const void *v, void *out, float *lse, void *workspace,
+                      hipStream_t st) {
+  const PfxProb P = pfx_prob(p);
+  PfxArgs A{q, pk, pv, k, v, out, lse, nullptr, nullptr};
+  if (P.NS > 0 && !pfx_direct(P)) {
+    A.po = static_cast<float *>(workspace);
+    A.pml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + pfx_part_bytes(P));
+  }
+  if (p->dtype == NA_F32) pfx_run<float>(P, A, st);
+  else if (p->dtype == NA_F16) pfx_run<f16_t>(P, A, st);
+  else pfx_run<bf16_t>(P, A, st);
+}
+
+}  // namespace na

@@ -961,6 +961,84 @@ std::tuple<at::Tensor, at::Tensor> na_rotary_op(const at::Tensor &q,
   return {r[0], r[1]};
 }
 
+// ---- attention behind a shared prefix (prefix.py) ---------------------------
+
+// t with its channels adjacent, and the strides of its other dimensions.
+at::Tensor rows_of(const at::Tensor &t, int64_t *stride) {
+  const int64_t nd = t.dim();
+  const bool ok = t.numel() == 0 || t.size(nd - 1) == 1 || t.stride(nd - 1) == 1;
+  const at::Tensor c = ok ? t : t.contiguous();
+  for (int64_t d = 0; d + 1 < nd; ++d) stride[d] = c.stride(d);
+  return c;
+}
+
+// The functional layer has validated the call; its shape rules are restated for
+// direct callers of the operator.
+std::tuple<at::Tensor, at::Tensor> na_prefix(
+    const at::Tensor &q, const at::Tensor &pk, const at::Tensor &pv,
+    const std::optional<at::Tensor> &k_opt, const std::optional<at::Tensor> &v_opt,
+    const std::optional<at::Tensor> &lens_opt, int64_t window, double scale, bool want_lse,
+    int64_t stream) {
+  const at::Tensor k = k_opt.value_or(at::Tensor()), v = v_opt.value_or(at::Tensor()),
+                   lens = lens_opt.value_or(at::Tensor());
+  TORCH_CHECK(!wants_grad({&q, &pk, &pv, &k, &v}),
+              "natten_amd prefix_attention serves: it has no backward (under torch.no_grad(), or "
+              "train with the prefix as additional_keys of na1d)");
+  TORCH_CHECK(q.dim() == 4 && pk.dim() == 3 && pk.sizes() == pv.sizes() && pk.size(2) == q.size(3) &&
+                  pk.size(1) > 0 && q.size(2) % pk.size(1) == 0,
+              "natten_amd na_prefix: q [B, L, H, D], prefix keys and values [N, H_kv, D], got ",
+              q.sizes(), " and ", pk.sizes());
+  TORCH_CHECK(k.defined() == v.defined() &&
+                  (!k.defined() || (k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                                    k.size(2) == pk.size(1) && k.size(3) == q.size(3))),
+              "natten_amd na_prefix: own keys and values [B, S, H_kv, D]");
+  for (const at::Tensor *t : {&pk, &pv, &k, &v})
+    TORCH_CHECK(!t->defined() || t->scalar_type() == q.scalar_type(),
+                "natten_amd na_prefix: all tensors share q's dtype");
+  if (lens.defined())
+    TORCH_CHECK(k.defined() && lens.dim() == 1 && lens.size(0) == q.size(0) &&
+                    (lens.scalar_type() == at::kInt || lens.scalar_type() == at::kLong),
+                "natten_amd na_prefix: seq_lens is an int32 or int64 [B] tensor beside own keys");
+  check_devices(q, {&pk, &pv, &k, &v, &lens});
+  for (const at::Tensor *t : {&q, &pk, &k})
+    for (int64_t d = 0; t->defined() && d < t->dim(); ++d)
+      TORCH_CHECK(t->size(d) <= INT32_MAX, "natten_amd na_prefix: a dimension is too long");
+  const c10::DeviceGuard guard(q.device());
+  na_prefix_params p{};
+  p.batch = (int32_t)q.size(0);
+  p.tokens = (int32_t)q.size(1);
+  p.heads = (int32_t)q.size(2);
+  p.kv_heads = (int32_t)pk.size(1);
+  p.head_dim = (int32_t)q.size(3);
+  p.dtype = dtype_code(q.scalar_type());
+  p.prefix = (int32_t)pk.size(0);
+  p.capacity = k.defined() ? (int32_t)k.size(1) : 0;
+  p.window = (int32_t)std::min<int64_t>(std::max<int64_t>(window, 0), 1 << 30);
+  p.scale = (float)scale;
+  const at::Tensor qc = rows_of(q, p.q_stride), pkc = rows_of(pk, p.prefix_k_stride),
+                   pvc = rows_of(pv, p.prefix_v_stride);
+  at::Tensor kc, vc, lc;
+  if (k.defined()) {
+    kc = rows_of(k, p.k_stride);
+    vc = rows_of(v, p.v_stride);
+  }
+  if (lens.defined()) {  // (64-bit lengths are clamped before they are narrowed)
+    lc = lens.scalar_type() == at::kLong ? lens.clamp(0, p.capacity).to(at::kInt) : lens.contiguous();
+    p.seq_lens = static_cast<const int32_t *>(lc.data_ptr());
+  }
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty(want_lse ? q.sizes().slice(0, 3) : at::IntArrayRef{0},
+                             q.options().dtype(at::kFloat));
+  const size_t bytes = na_prefix_workspace_bytes(&p);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_rc(na_prefix_fwd(&p, qc.data_ptr(), cptr(pkc), cptr(pvc), cptr(kc), cptr(vc), out.data_ptr(),
+                         want_lse ? static_cast<float *>(lse.data_ptr()) : nullptr, mptr(ws), bytes,
+                         as_stream(stream)),
+           "na_prefix_fwd");
+  return {out, lse};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(natten_amd, m) {
@@ -989,6 +1067,9 @@ TORCH_LIBRARY(natten_amd, m) {
   m.def(
       "na_rotary(Tensor q, Tensor? k, Tensor? positions, int[] axis_dims, float theta, "
       "bool interleaved, bool inverse, int stream) -> (Tensor, Tensor)");
+  m.def(
+      "na_prefix(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor? k, Tensor? v, "
+      "Tensor? seq_lens, int window, float scale, bool want_lse, int stream) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
@@ -1001,4 +1082,5 @@ TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
   m.impl("na_fused_qkv", na_fused_qkv);
   m.impl("na_layer_norm", na_layer_norm);
   m.impl("na_rotary", na_rotary_op);
+  m.impl("na_prefix", na_prefix);
 }

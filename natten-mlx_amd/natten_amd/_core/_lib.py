@@ -164,6 +164,30 @@ class NaRotaryParams(ctypes.Structure):
     ]
 
 
+class NaPrefixParams(ctypes.Structure):
+    """Mirror of ``na_prefix_params`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("prefix", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("seq_lens", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("prefix_k_stride", ctypes.c_int64 * 2),
+        ("prefix_v_stride", ctypes.c_int64 * 2),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+    ]
+
+
+PREFIX_MAX_HEAD_DIM = 256
 MAX_HEAD_DIM = 1024
 ROTARY_MAX_AXES = 4
 ROTARY_MAX_CHANNELS = 512
@@ -175,6 +199,7 @@ _R = ctypes.POINTER(NaRpbParams)
 _M = ctypes.POINTER(NaMergeParams)
 _N = ctypes.POINTER(NaNormParams)
 _RO = ctypes.POINTER(NaRotaryParams)
+_PF = ctypes.POINTER(NaPrefixParams)
 _PP = ctypes.POINTER(ctypes.c_void_p)  # host array of device pointers
 _V = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -217,6 +242,8 @@ SIGNATURES = {
     "na_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_N]),
     "na_norm_bwd": (ctypes.c_int, [_N] + [_V] * 8 + [ctypes.c_size_t, _V]),
     "na_rotary": (ctypes.c_int, [_RO] + [_V] * 6),
+    "na_prefix_workspace_bytes": (ctypes.c_size_t, [_PF]),
+    "na_prefix_fwd": (ctypes.c_int, [_PF] + [_V] * 8 + [ctypes.c_size_t, _V]),
 }
 
 _lib = None
@@ -263,7 +290,8 @@ def _load_fused_op() -> None:
     _node_ops = {"qk": ns.na_split_qk.default, "av": ns.na_split_av.default,
                  "rpb_qk": ns.na_rpb_qk.default, "rpb_av": ns.na_rpb_av.default,
                  "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default,
-                 "norm": ns.na_layer_norm.default, "rotary": ns.na_rotary.default}
+                 "norm": ns.na_layer_norm.default, "rotary": ns.na_rotary.default,
+                 "prefix": ns.na_prefix.default}
 
 
 def fused_op():
@@ -281,7 +309,8 @@ _OP_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 def node_op(name: str, a: torch.Tensor, b: torch.Tensor):
     """The C++ operator of a split ("qk", "av") or DiNAT ("rpb_qk", "rpb_av")
     op, of a layer's projection ("linear") and packed attention
-    ("fused_qkv"), of the layer norm ("norm") or of rotary positions ("rotary"), where it takes these tensors: built, and both of a supported dtype on
+    ("fused_qkv"), of the layer norm ("norm"), of rotary positions ("rotary") or of
+    attention behind a shared prefix ("prefix"), where it takes these tensors: built, and both of a supported dtype on
     one HIP device.  None otherwise (the Python autograd Function then runs
     the same kernels, or raises): under compilation, which can leave a Python
     Function to eager execution but not an operator without a fake kernel, while

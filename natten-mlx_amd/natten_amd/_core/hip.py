@@ -686,3 +686,35 @@ def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
                                          _lib.ptr(oq), _lib.ptr(ok), _lib.stream_of(x)),
                    "na_rotary")
     return oq, ok
+
+
+# ---------------------------------------------------------------------------
+# attention behind a shared prefix (C ABI na_prefix_fwd)
+
+def prefix_forward(q, pk, pv, k, v, lens, window, scale, want_lse):
+    """``(out, lse)``: lse float32 ``[B, L, H]``, or None where not wanted; ``window``
+    0 for none, ``lens`` int32 on the device or None."""
+    dev = _require_device(q, pk, pv, k, v, lens)
+    q, pk, pv, k, v, lens = map(_c, (q, pk, pv, k, v, lens))
+    p = _lib.NaPrefixParams()
+    p.batch, p.tokens, p.heads, p.head_dim = q.shape
+    p.kv_heads, p.prefix = pk.shape[1], pk.shape[0]
+    p.dtype, p.window, p.scale = _lib.dtype_code(q.dtype), min(int(window), 1 << 30), float(scale)
+    p.capacity = 0 if k is None else k.shape[1]
+    p.seq_lens = None if lens is None else lens.data_ptr()
+    row = p.kv_heads * p.head_dim
+    for st, t in ((p.q_stride, q), (p.k_stride, k), (p.v_stride, v)):
+        if t is not None:
+            st[0], st[1], st[2] = t.shape[1] * t.shape[2] * t.shape[3], t.shape[2] * t.shape[3], t.shape[3]
+    for st in (p.prefix_k_stride, p.prefix_v_stride):
+        st[0], st[1] = row, p.head_dim
+    lib = _lib.load()
+    out = torch.empty_like(q)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
+    nbytes = int(lib.na_prefix_workspace_bytes(p))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.na_prefix_fwd(p, _lib.ptr(q), _lib.ptr(pk), _lib.ptr(pv), _lib.ptr(k),
+                                     _lib.ptr(v), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), nbytes,
+                                     _lib.stream_of(q)), "na_prefix_fwd")
+    return out, lse

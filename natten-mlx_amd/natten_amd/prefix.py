@@ -1,0 +1,113 @@
+"""Serving: attention of a batch's newest tokens against key/value caches whose
+prefix the whole batch shares (no counterpart in the reference).
+
+It is causal 1D neighborhood attention at the end of a sequence, joined to tokens
+that every query sees -- ``na1d(..., is_causal=True, additional_keys=...)`` at its
+last rows -- with the caches as they lie and one copy of the shared tokens, whose
+keys are read once for all samples (``csrc/na_prefix.hip``).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from ._core import _lib
+from ._core import hip
+from .autograd import device_extents
+from .autograd import fused as _fused
+
+
+def _check(query, pk, pv, key, value, seq_lens, kernel_size, scale):
+    if query.ndim != 4:
+        raise ValueError(f"query must be [B, L, heads, dim], got {tuple(query.shape)}.")
+    b, _, h, d = query.shape
+    if pk.ndim != 3 or pk.shape != pv.shape or pk.shape[2] != d or pk.shape[1] < 1:
+        raise ValueError(f"prefix_key and prefix_value must be [N, heads_kv, {d}], got "
+                         f"{tuple(pk.shape)} and {tuple(pv.shape)}.")
+    hk = pk.shape[1]
+    if h < 1 or h % hk:
+        raise ValueError(f"heads_q ({h}) must be divisible by heads_kv ({hk}) for GQA.")
+    if d < 8 or d % 8 or d > _lib.PREFIX_MAX_HEAD_DIM:
+        raise ValueError(f"head dim must be a multiple of 8 up to {_lib.PREFIX_MAX_HEAD_DIM}, got {d}.")
+    if (key is None) != (value is None):
+        raise ValueError("key and value must both be provided or both None.")
+    if key is not None and (key.ndim != 4 or key.shape != value.shape or key.shape[0] != b
+                            or key.shape[2] != hk or key.shape[3] != d):
+        raise ValueError(f"key and value must be [{b}, S, {hk}, {d}], got {tuple(key.shape)} and "
+                         f"{tuple(value.shape)}.")
+    for t in (pk, pv, key, value):
+        if t is not None and t.dtype != query.dtype:
+            raise ValueError(f"keys and values must have query's dtype {query.dtype}, got {t.dtype}.")
+    if seq_lens is not None:
+        if key is None:
+            raise ValueError("seq_lens are the lengths of key and value, which are missing.")
+        if seq_lens.ndim != 1 or seq_lens.shape[0] != b:
+            raise ValueError(f"seq_lens must be a 1-D array of length B={b}, got shape "
+                             f"{tuple(seq_lens.shape)}.")
+        if seq_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"seq_lens must be int32 or int64, got {seq_lens.dtype}.")
+    if kernel_size is not None and (not isinstance(kernel_size, int) or kernel_size < 1):
+        raise ValueError(f"kernel_size must be a positive int or None, got {kernel_size!r}.")
+    if scale is not None and not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}.")
+
+
+def _host_lens(seq_lens, capacity, device):
+    host = seq_lens.tolist()
+    if host and (min(host) < 0 or max(host) > capacity):
+        raise ValueError(f"All seq_lens must be in [0, {capacity}], got {min(host)} to {max(host)}.")
+    return device_extents(seq_lens, len(host), 1, device).reshape(-1)
+
+
+def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value: torch.Tensor,
+                     key: Optional[torch.Tensor] = None, value: Optional[torch.Tensor] = None,
+                     seq_lens: Optional[torch.Tensor] = None, kernel_size: Optional[int] = None,
+                     scale: Optional[float] = None, return_lse: bool = False
+                     ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """The batch's newest tokens ``[B, L, H, D]`` (L = 1: one generated token each)
+    attend to shared tokens ``[N, H_kv, D]`` and to their samples' own caches
+    ``[B, S, H_kv, D]``.
+
+    ``seq_lens[b]`` (default S) counts the valid own tokens, the new ones among
+    them: query j of sample b is own token ``t = seq_lens[b] - L + j``.  It sees every
+    prefix token and the own tokens up to t; with ``kernel_size`` the last
+    ``kernel_size`` of them only, the causal window of ``na1d``.  What a cache holds
+    behind ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
+    clamped to ``[0, S]`` there (no synchronisation); lengths on the host are checked.
+
+    float32, float16 or bfloat16, all tensors alike; D a multiple of 8 up to 256;
+    query heads share key/value heads as in ``na1d``.  Caches and queries may be
+    views of any strides whose channels are adjacent, such as heads-first caches.
+    The output has query's type; the LSE (``return_lse``) is float32 ``[B, L, H]``,
+    ready for ``merge_attentions``.  A query that sees no key gets zeros and -inf.
+
+    There is no backward: inputs that require grad are refused outside
+    ``torch.no_grad()``.  To train with shared tokens, pass them to ``na1d`` as
+    ``additional_keys`` expanded over the batch.
+    """
+    _check(query, prefix_key, prefix_value, key, value, seq_lens, kernel_size, scale)
+    scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
+    if seq_lens is not None and not seq_lens.is_cuda and query.is_cuda:
+        seq_lens = _host_lens(seq_lens, key.shape[1], query.device)
+    window = 0 if kernel_size is None else kernel_size
+    op = None if _fused._py_autograd else _lib.node_op("prefix", query, prefix_key)
+    if op is not None:
+        out, lse = op(query, prefix_key, prefix_value, key, value, seq_lens, window, scale,
+                      return_lse, _lib.stream_of(query))
+    else:
+        if torch.is_grad_enabled() and any(
+                t is not None and t.requires_grad
+                for t in (query, prefix_key, prefix_value, key, value)):
+            raise RuntimeError("prefix_attention serves: it has no backward (under torch.no_grad(), "
+                               "or train with the prefix as additional_keys of na1d)")
+        if seq_lens is not None:
+            seq_lens = seq_lens.clamp(0, key.shape[1]).to(torch.int32)
+        out, lse = hip.prefix_forward(query, prefix_key, prefix_value, key, value, seq_lens, window,
+                                      scale, return_lse)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["prefix_attention"]

@@ -247,7 +247,7 @@ void rotary(const na_rotary_params *p, const void *q, const void *k, const void 
             void *ok, hipStream_t st);
 
 // Attention against a shared prefix and own cached tokens (na_prefix.hip).
-constexpr int kPfxItems = 1024;  // workgroups that a call is split into
+constexpr int kPfxItems = 512;  // workgroups that the chip holds at once
 bool prefix_fits(const na_prefix_params *p);
 size_t prefix_workspace(const na_prefix_params *p);
 void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, const void *pv,

@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kPfxThreads = 256;
 constexpr int kPfxNarrowKeys = 32;  // keys of a wave's tile
+constexpr int kPfxJoin = 8;         // slots that a thread of the join loads at once
 
 struct PfxProb {
   int32_t Lq, H, Hkv, rep, D;
@@ -320,21 +321,42 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
   const char *const src = (isv ? w.v : w.k) + 2 * col + (int64_t)(w.k0 + r0) * st;
   const int unit = r0 * RSE + 8 * c + (isv ? 8 : 0);
   v8 pre[NU];
-  auto load_tile = [&](int t) {  // t: keys behind k0
+  const int total = w.k1 - w.k0, nkt = (total + TK - 1) / TK;
+  // The tiles that every row sees in full are [ja, jb); they come first, then
+  // those behind them, then those before.
+  int ja = (max(w.lo_max - w.k0, 0) + TK - 1) / TK, jb = max(min(w.hi_min, w.k1) - w.k0, 0) / TK;
+  if (jb <= ja) ja = jb = 0;
+  auto first_key = [&](int i) {  // of the i-th tile, behind k0
+    const int j = ja + i;
+    return (j < nkt ? j : j - nkt) * TK;
+  };
+  // V of the i-th tile and K of the next: the scores run one tile ahead.
+  auto fetch = [&](int i) {
+    const int mine = isv ? i : i + 1;
+    const int t = first_key(max(min(mine, nkt - 1), 0));
     const char *p = src + (int64_t)t * st;
-    const int left = w.k1 - w.k0 - t - r0;
+    if (i >= 0 && i + 1 < nkt && max(first_key(i), first_key(i + 1)) + TK <= total && P.D == D) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      pre[i] = pfx_zero8<T>();
-      if (colok && RPP * i < left) pre[i] = pfx_ld8<T>(p);
-      p += RPP * st;
+      for (int u = 0; u < NU; ++u) {
+        pre[u] = pfx_ld8<T>(p);
+        p += RPP * st;
+      }
+    } else {  // zeros behind the last key and channel: 0 times them is 0
+      const int left = mine >= 0 && mine < nkt && colok ? total - t - r0 : 0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        pre[u] = pfx_zero8<T>();
+        if (RPP * u < left) pre[u] = pfx_ld8<T>(p);
+        p += RPP * st;
+      }
     }
   };
-  auto store_tile = [&](E *dst) {
+  auto put = [&](int i) {
+    E *const d = buf + ((isv ? i : i + 1) & 1) * (TK * RSE) + unit;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) *reinterpret_cast<v8 *>(dst + unit + RPP * i * RSE) = pre[i];
+    for (int u = 0; u < NU; ++u) *reinterpret_cast<v8 *>(d + RPP * u * RSE) = pre[u];
   };
-  load_tile(0);
+  fetch(-1);
 
   const int row0 = w.row0 + wv * (16 * NQ);
   v8 qf[NQ][NT];
@@ -364,62 +386,177 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
   const int tr_off = (4 * gq + (n >> 2)) * RSE + 4 * (n & 3);
   const bool spans = w.b >= 0 && P.Lq > 1;  // rows may see different keys
 
-  store_tile(buf);
-  __syncthreads();
-  const int nkt = (w.k1 - w.k0 + TK - 1) / TK;
-  for (int j = 0; j < nkt; ++j) {
-    const int t0 = j * TK;
-    if (j + 1 < nkt) load_tile(t0 + TK);  // in flight during this tile
-    const E *ks = buf + (j & 1) * (TK * RSE);
-    const E *vs = ks + lds_y(D);
-    const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
-    const bool odd = !all && spans && pfx_odd_tile<T, D>(vs, RSE, TK, lane);
-    v8 bp[NQ][CH / 2];
+  auto values = [&](const E *vs, int jj, int db) {  // V^T of 32 keys
+    const E *ca = vs + 32 * jj * RSE + tr_off + 16 * db;
+    const v4 lo4 = M::tr(ca), hi4 = M::tr(ca + 16 * RSE);
+    return (v8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  typedef f32x4 Scores[NQ][CH];
+  Scores sa, sb;  // of the tile at hand and of the next
+  float mx[NQ];   // the lane's largest score of the tile at hand
+  auto keys = [&](const E *ks, int ch, v8 (&ka)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      ka[t] = *reinterpret_cast<const v8 *>(ks + 16 * ch * RSE + 32 * t);
+  };
+  auto largest = [&](const Scores &s, int qi, int ch) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mx[qi] = fmaxf(mx[qi], s[qi][ch][r]);
+  };
+  // The i-th tile, its scores in `s`; the next tile's go to `next`.  EDGE: some
+  // row does not see some of its keys.  Matrix products are issued two at a time
+  // between the vector ALU's work, which fills the matrix unit's time: the next
+  // tile's scores beside the first half of the exponentials, O beside the second.
+  auto run_tile = [&](int i, Scores &s, Scores &next, auto edge_tile) {
+    constexpr bool EDGE = decltype(edge_tile)::value;
+    const E *vs = buf + (i & 1) * (TK * RSE) + lds_y(D);
+    const E *ks = buf + ((i + 1) & 1) * (TK * RSE) + ka_off;
+    fetch(i + 1);  // in flight during this tile
+    const int t0 = first_key(i);
+    bool moves = false;
 #pragma unroll
     for (int qi = 0; qi < NQ; ++qi) {
-      float p[CH][4];
+      if (EDGE) {
+        mx[qi] = -INFINITY;
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        f32x4 s = zero4();
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          s = M::mma(*reinterpret_cast<const v8 *>(ks + 16 * ch * RSE + ka_off + 32 * t), qf[qi][t], s);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[ch][r] = s[r];
-      }
-      if (!all) {
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
+        for (int ch = 0; ch < CH; ++ch) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if ((unsigned)(t0 + 16 * ch + 4 * gq + r - lo[qi]) >= (unsigned)cnt[qi])
-              p[ch][r] = -INFINITY;
-      }
-      pfx_softmax<CH, NDB>(p, sl2, m[qi], l[qi], o[qi]);
-      if (odd) pfx_odd_pv<T, CH, NDB>(p, vs, RSE, lane, lo[qi] - t0, cnt[qi], o[qi]);
-#pragma unroll
-      for (int jj = 0; jj < CH / 2; ++jj)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) bp[qi][jj][4 * hh + r] = (E)p[2 * jj + hh][r];
-    }
-    if (!odd) {
-#pragma unroll
-      for (int jj = 0; jj < CH / 2; ++jj) {
-        const E *ca = vs + 32 * jj * RSE + tr_off;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const v4 lo4 = M::tr(ca + 16 * db);
-          const v4 hi4 = M::tr(ca + 16 * RSE + 16 * db);
-          const v8 a = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int qi = 0; qi < NQ; ++qi) o[qi][db] = M::mma(a, bp[qi][jj], o[qi][db]);
+              s[qi][ch][r] = -INFINITY;
+          largest(s, qi, ch);
         }
       }
+      moves |= mx[qi] * sl2 > m[qi] + 8.f;
     }
-    if (j + 1 < nkt) store_tile(buf + ((j + 1) & 1) * (TK * RSE));
+    // the reference point may trail the maximum by 8 (a factor 2^8 in p): exact
+    // after the division by l
+    if (__builtin_amdgcn_ballot_w64(moves) != 0) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        const float mn = fmaxf(m[qi], quad_max(mx[qi]) * sl2);
+        const float alpha = __builtin_amdgcn_exp2f(m[qi] - (mn == -INFINITY ? 0.f : mn));
+        l[qi] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[qi][db] *= alpha;
+        m[qi] = mn;
+      }
+    }
+    float mu[NQ];
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) mu[qi] = m[qi] == -INFINITY ? 0.f : m[qi];
+    auto expo = [&](int qi, int x) {  // the x-th of the lane's CH * 4 probabilities
+      float &p = reinterpret_cast<float (&)[CH][4]>(s[qi])[x / 4][x % 4];
+      p = __builtin_amdgcn_exp2f(fmaf(p, sl2, -mu[qi]));
+      l[qi] += p;
+    };
+    auto rounded = [&](int qi, int jj) {
+      v8 bp;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) bp[x] = (E)s[qi][2 * jj + x / 4][x % 4];
+      return bp;
+    };
+    constexpr int ALL = CH * 4, FIRST = CH > 2 ? ALL / 2 : ALL;  // a lane's scores, beside QK
+    constexpr int QS = CH * NT, OS = CH / 2 * NDB;  // steps of the two products
+    constexpr int RING = 4;
+    v8 ka[RING];  // of the next steps
+    auto key = [&](int st) {
+      return *reinterpret_cast<const v8 *>(ks + 16 * (st / NT) * RSE + 32 * (st % NT));
+    };
+#pragma unroll
+    for (int st = 0; st < RING - 1; ++st) ka[st] = key(st);
+#pragma unroll
+    for (int st = 0; st < QS; ++st) {
+      const int ch = st / NT, t = st % NT;
+      if (st + RING - 1 < QS) ka[(st + RING - 1) % RING] = key(st + RING - 1);
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        next[qi][ch] = M::mma(ka[st % RING], qf[qi][t], t == 0 ? zero4() : next[qi][ch]);
+#pragma unroll
+        for (int x = st * FIRST / QS; x < (st + 1) * FIRST / QS; ++x) expo(qi, x);
+      }
+      __builtin_amdgcn_sched_barrier(0x124);
+    }
+    bool odd = false;
+    if (EDGE) odd = spans && pfx_odd_tile<T, D>(vs, RSE, TK, lane);
+    if (EDGE && odd) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        float p[CH][4];
+#pragma unroll
+        for (int x = FIRST; x < ALL; ++x) expo(qi, x);
+#pragma unroll
+        for (int x = 0; x < ALL; ++x) p[x / 4][x % 4] = s[qi][x / 4][x % 4];
+        pfx_odd_pv<T, CH, NDB>(p, vs, RSE, lane, lo[qi] - t0, cnt[qi], o[qi]);
+      }
+    } else {
+      v8 bp[NQ];
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) bp[qi] = rounded(qi, 0);
+      v8 va[2];
+      va[0] = values(vs, 0, 0);
+#pragma unroll
+      for (int st = 0; st < OS; ++st) {
+        const int jj = st / NDB, db = st % NDB;
+        if (jj > 0 && db == 0) {
+#pragma unroll
+          for (int qi = 0; qi < NQ; ++qi) bp[qi] = rounded(qi, jj);
+        }
+        if (st + 1 < OS) va[(st + 1) & 1] = values(vs, (st + 1) / NDB, (st + 1) % NDB);
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          o[qi][db] = M::mma(va[st & 1], bp[qi], o[qi][db]);
+          if (jj == 0) {
+#pragma unroll
+            for (int x = FIRST + db * (ALL - FIRST) / NDB; x < FIRST + (db + 1) * (ALL - FIRST) / NDB; ++x)
+              expo(qi, x);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0x124);
+      }
+    }
+    put(i + 1);
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      mx[qi] = -INFINITY;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) largest(next, qi, ch);
+    }
     __syncthreads();
+  };
+  put(-1);
+  __syncthreads();
+  fetch(0);
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) mx[qi] = -INFINITY;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    v8 ka[NT];
+    keys(buf + ka_off, ch, ka);
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      sa[qi][ch] = zero4();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sa[qi][ch] = M::mma(ka[t], qf[qi][t], sa[qi][ch]);
+      largest(sa, qi, ch);
+    }
+  }
+  put(0);
+  __syncthreads();
+  auto follow = [&]() {
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) sa[qi][ch] = sb[qi][ch];
+  };
+  int i = 0;
+  for (; i + 2 <= jb - ja; i += 2) {
+    run_tile(i, sa, sb, std::false_type{});
+    run_tile(i + 1, sb, sa, std::false_type{});
+  }
+  for (; i < nkt; ++i) {
+    run_tile(i, sa, sb, std::true_type{});
+    follow();
   }
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
@@ -499,20 +636,29 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
   const char *const vp = w.v + (int64_t)(w.k0 + vr) * w.vst + 16 * vc;
   v8 kr[2][NT], vr8[NU];
   auto load = [&](int t0) {
-    const int left = total - t0;
     const char *a = kp + (int64_t)t0 * w.kst, *b = vp + (int64_t)t0 * w.vst;
+    if (t0 + TK <= total && P.D == D) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+      for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int s = 0; s < NT; ++s) {
-        kr[hh][s] = pfx_zero8<T>();
-        if (16 * hh + n < left && 32 * s + 8 * gq < P.D)
-          kr[hh][s] = pfx_ld8<T>(a + 16 * hh * w.kst + 64 * s);
+        for (int s = 0; s < NT; ++s) kr[hh][s] = pfx_ld8<T>(a + 16 * hh * w.kst + 64 * s);
+#pragma unroll
+      for (int i = 0; i < NU; ++i) vr8[i] = pfx_ld8<T>(b + RPP * i * w.vst);
+    } else {  // zeros behind the last key and channel: 0 times them is 0
+      const int left = total - t0;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int s = 0; s < NT; ++s) {
+          kr[hh][s] = pfx_zero8<T>();
+          if (16 * hh + n < left && 32 * s + 8 * gq < P.D)
+            kr[hh][s] = pfx_ld8<T>(a + 16 * hh * w.kst + 64 * s);
+        }
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        vr8[i] = pfx_zero8<T>();
+        if (RPP * i + vr < left && 8 * vc < P.D) vr8[i] = pfx_ld8<T>(b + RPP * i * w.vst);
       }
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      vr8[i] = pfx_zero8<T>();
-      if (RPP * i + vr < left && 8 * vc < P.D) vr8[i] = pfx_ld8<T>(b + RPP * i * w.vst);
     }
   };
   f32x4 o[NDB];
@@ -522,34 +668,32 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
   const float sl2 = P.sl2;
   const int tr_off = (4 * gq + (n >> 2)) * RS + 4 * (n & 3);
   const bool spans = w.b >= 0 && P.Lq > 1;
-  int t0 = wv * TK;
-  if (t0 < total) load(t0);
-  for (; t0 < total; t0 += 4 * TK) {
-    f32x4 s[2];
+  const int all0 = w.lo_max - w.k0, all1 = min(w.hi_min, w.k1) - w.k0;  // seen by every row
+  auto run_tile = [&](int t0, auto edge_tile) {
+    constexpr bool EDGE = decltype(edge_tile)::value;
+    f32x4 s[2] = {zero4(), zero4()};
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      s[hh] = zero4();
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[hh] = M::mma(kr[hh][t], qf[t], s[hh]);
-    }
+      for (int hh = 0; hh < 2; ++hh) s[hh] = M::mma(kr[hh][t], qf[t], s[hh]);
     __builtin_amdgcn_wave_barrier();  // the reads of the tile before are issued
 #pragma unroll
     for (int i = 0; i < NU; ++i)
       *reinterpret_cast<v8 *>(vs + (RPP * i + vr) * RS + 8 * vc) = vr8[i];
     if (t0 + 4 * TK < total) load(t0 + 4 * TK);  // in flight during the rest
-    const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
     float p[2][4];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        p[hh][r] = all || (unsigned)(t0 + 16 * hh + 4 * gq + r - lo) < (unsigned)cnt ? s[hh][r]
-                                                                                     : -INFINITY;
+      for (int r = 0; r < 4; ++r) {
+        p[hh][r] = s[hh][r];
+        if (EDGE && (unsigned)(t0 + 16 * hh + 4 * gq + r - lo) >= (unsigned)cnt) p[hh][r] = -INFINITY;
+      }
     pfx_softmax<2, NDB>(p, sl2, m, l, o);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (!all && spans && pfx_odd_tile<T, D>(vs, RS, TK, lane)) {
+    if (EDGE && spans && pfx_odd_tile<T, D>(vs, RS, TK, lane)) {
       pfx_odd_pv<T, 2, NDB>(p, vs, RS, lane, lo - t0, cnt, o);
     } else {
       v8 bp;
@@ -565,6 +709,12 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  };
+  int t0 = wv * TK;
+  if (t0 < total) load(t0);
+  for (; t0 < total; t0 += 4 * TK) {
+    if (t0 >= all0 && t0 + TK <= all1) run_tile(t0, std::false_type{});
+    else run_tile(t0, std::true_type{});
   }
   pfx_meet<T, D, NDB>(P, A, w, smem, m, l, o, [&](int db) { return 16 * db + 4 * gq; });
 }
@@ -578,7 +728,7 @@ __global__ void __launch_bounds__(kPfxThreads, D > 128 ? 1 : 2) k_pfx(PfxProb P,
   const int shape = (w.b < 0 ? P.rows_p : P.rows_o) >> 6;
   if (shape == 0) {
     pfx_narrow<T, D>(P, A, w, smem);
-  } else if (D > 128 || shape == 1) {
+  } else if (shape == 1) {
     pfx_wide<T, D, 1>(P, A, w, smem);
   } else {
     if constexpr (D <= 128) pfx_wide<T, D, 2>(P, A, w, smem);
@@ -618,23 +768,31 @@ __global__ void __launch_bounds__(kPfxThreads) k_pfx32(PfxProb P, PfxArgs A) {
   for (int i = 0; i < 4 * NU; ++i) o[i] = zero4();
   float m = -INFINITY, l = 0.f;
   const bool spans = w.b >= 0 && P.Lq > 1;
-  for (int t0 = wv * TK; t0 < total; t0 += 4 * TK) {
-    const char *const a = kp + (int64_t)t0 * w.kst, *const b = vp + (int64_t)t0 * w.vst;
-    f32x4 kr[NS], vr[4][NU];
+  f32x4 kr[NS], vr[4][NU];
+  auto load_k = [&](int t0) {
+    const char *const a = kp + (int64_t)t0 * w.kst;
+    const bool ok = t0 + n < total;
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      kr[s] = ld(a + 64 * s, t0 + n < total && 16 * s + 4 * gq < P.D);
+    for (int s = 0; s < NS; ++s) kr[s] = ld(a + 64 * s, ok && 16 * s + 4 * gq < P.D);
+  };
+  auto load_v = [&](int t0) {
+    const char *const b = vp + (int64_t)t0 * w.vst;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int u = 0; u < NU; ++u)
         vr[r][u] = ld(b + r * w.vst + 256 * u, t0 + 4 * gq + r < total && 64 * u + 4 * n < P.D);
+  };
+  load_k(wv * TK);  // (past the last key: zeros)
+  load_v(wv * TK);
+  for (int t0 = wv * TK; t0 < total; t0 += 4 * TK) {
     f32x4 s4 = zero4();
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[s][e], qf[s][e], s4, 0, 0, 0);
+    load_k(t0 + 4 * TK);  // in flight during the softmax and the second product
     const bool all = w.k0 + t0 >= w.lo_max && w.k0 + t0 + TK <= min(w.hi_min, w.k1);
     float p[1][4];
 #pragma unroll
@@ -678,6 +836,7 @@ __global__ void __launch_bounds__(kPfxThreads) k_pfx32(PfxProb P, PfxArgs A) {
               }
         }
     }
+    load_v(t0 + 4 * TK);
   }
   // block e of group u, element i: channel 64 u + 4 (4 gq + i) + e; dealt to
   // blocks of four adjacent channels
@@ -723,17 +882,35 @@ __global__ void __launch_bounds__(256) k_pfx_join(PfxProb P, PfxArgs A, int lgG,
   float m = -INFINITY, l = 0.f;
   f32x4 acc = zero4();
   const int c = 4 * lane;
-  for (int i = share; i < count; i += 1 << lgS) m = fmaxf(m, ml[slot(i)].x);
-#pragma unroll 4
-  for (int i = share; i < count; i += 1 << lgS) {
-    const float2 x = ml[slot(i)];
-    f32x4 o = zero4();
-    if (c < P.D) o = *reinterpret_cast<const f32x4 *>(po + (int64_t)slot(i) * P.D + c);
-    if (x.y != 0.f) {  // (0: a row that sees nothing of the chunk)
-      const float wt = __builtin_amdgcn_exp2f(x.x - m);
-      l = fmaf(wt, x.y, l);
-      acc += wt * o;
+  for (int i0 = share; i0 < count; i0 += kPfxJoin << lgS) {  // a batch's loads together
+    float2 x[kPfxJoin];
+    f32x4 o[kPfxJoin];
+#pragma unroll
+    for (int u = 0; u < kPfxJoin; ++u) {
+      const int i = i0 + (u << lgS);
+      x[u] = make_float2(-INFINITY, 0.f);
+      o[u] = zero4();
+      if (i < count) {
+        x[u] = ml[slot(i)];
+        if (c < P.D) o[u] = *reinterpret_cast<const f32x4 *>(po + (int64_t)slot(i) * P.D + c);
+      }
     }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kPfxJoin; ++u) mn = fmaxf(mn, x[u].x);
+    if (l != 0.f) {
+      const float wt = __builtin_amdgcn_exp2f(m - mn);
+      l *= wt;
+      acc *= wt;
+    }
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < kPfxJoin; ++u)
+      if (x[u].y != 0.f) {  // (0: a row that sees nothing of the chunk)
+        const float wt = __builtin_amdgcn_exp2f(x[u].x - m);
+        l = fmaf(wt, x[u].y, l);
+        acc += wt * o[u];
+      }
   }
   if (lgS > 0) {
     so[tid] = acc;
@@ -764,14 +941,20 @@ int pfx_width(int dtype, int D) {  // the kernels' head dim
   return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256;
 }
 
-// Rows of a tile: narrow up to 16, wide above, 128 where there are more than 64.
+// Rows of a tile: narrow up to 16, wide above, as many as the registers hold
+// where there are more than 64.
 int pfx_rows(int dtype, int D, int64_t rows) {
   if (dtype == NA_F32 || rows <= 16) return 16;
   return rows <= 64 || D > 128 ? 64 : 128;
 }
 
-// Keys per chunk: about kPfxItems workgroups in all, each with a chunk of at
-// least one tile per wave.
+// Keys per chunk.  kPfxItems workgroups are on the chip at once (two on a CU): a
+// chunk is a workgroup's part of all keys and row tiles, the samples' lengths
+// taken as half their capacity.  Wide chunks are at least 512 keys (each leaves
+// rows * D floats for the join; 8 heads x 16384 keys x 128 rows of 128 channels:
+// 33.3 us in chunks of 256, 29.4 of 512, 32.7 of 768); a sample's are at most
+// 1024, which evens out ragged lengths (64 samples of up to 2048, 8 heads: 56.6
+// us, 69.2 in chunks of 2048).
 PfxProb pfx_prob(const na_prefix_params *p) {
   PfxProb P{};
   P.Lq = p->tokens;
@@ -790,19 +973,18 @@ PfxProb pfx_prob(const na_prefix_params *p) {
   P.rt_o = (P.Mo + P.rows_o - 1) / P.rows_o;
   const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
   const int64_t tp = (int64_t)P.Hkv * P.rt_p, to = (int64_t)p->batch * P.Hkv * P.rt_o;
-  const int64_t visits = tp * P.N + to * span;
-  auto chunk = [&](int64_t keys, int rows) {
-    const int64_t least = rows > 16 ? 256 : 128;
-    const int64_t want = std::max((visits + kPfxItems - 1) / kPfxItems, least);
-    const int64_t parts = std::max<int64_t>(1, (keys + want - 1) / want);
+  const int64_t want = (tp * P.N + to * span / 2) / kPfxItems;
+  auto chunk = [](int64_t keys, int64_t size) {  // even parts, whole tiles
+    const int64_t parts = (keys + size - 1) / size;
     return (int32_t)(((keys + parts - 1) / parts + 63) / 64 * 64);
   };
   if (P.N > 0) {
-    P.chunk_p = chunk(P.N, P.rows_p);
+    P.chunk_p = chunk(P.N, std::max<int64_t>(want, P.rows_p > 16 ? 512 : 128));
     P.SP = (P.N + P.chunk_p - 1) / P.chunk_p;
   }
   if (span > 0) {
-    P.chunk_o = chunk(span, P.rows_o);
+    const int64_t least = P.rows_o > 16 ? 256 : 128;
+    P.chunk_o = chunk(span, std::min<int64_t>(std::max(want, least), 1024));
     P.SO = (int32_t)((span + P.chunk_o - 1) / P.chunk_o);
   }
   P.NS = P.SP + P.SO;
@@ -866,7 +1048,7 @@ void pfx_run(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
   if (A.po == nullptr && P.NS > 0) return;
   int lgG = 0, lgS = 0;
   while ((4 << lgG) < P.D) ++lgG;
-  while (lgG + lgS < 8 && (8 << lgS) < P.NS) ++lgS;
+  while (lgG + lgS < 8 && (kPfxJoin << lgS) < P.NS) ++lgS;
   const int64_t threads = ((int64_t)P.Hkv * P.M) << (lgG + lgS);
   hipLaunchKernelGGL((k_pfx_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
                      lgG, lgS);

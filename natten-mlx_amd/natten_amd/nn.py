@@ -18,6 +18,10 @@ Routing follows the reference layer (``nn/na2d.py:80-154``):
 
 Key/value heads for GQA are not repeated: the kernels map query head ``h``
 to key/value head ``h // (num_heads // num_kv_heads)`` directly.
+
+Beyond the reference's arguments, ``qk_norm`` puts a layer norm over each head's
+channels on queries and keys (``q_norm``, ``k_norm``), and ``rotary`` turns them by
+their positions on the layer's axes; both come before the attention on every route.
 """
 
 from __future__ import annotations
@@ -31,6 +35,9 @@ from . import functional as F
 from ._core import _lib, ops
 from ._core import hip as _hip
 from .autograd import fused as _fused
+from .norm import layer_norm
+from .rotary import rotary as _rotary
+from .rotary import rotary_axis_dims
 from .utils.params import normalize_tuple_param
 
 IntOrTuple = Union[int, Tuple[int, ...]]
@@ -77,6 +84,25 @@ def _linear(m: _nn.Module, x: torch.Tensor) -> torch.Tensor:
     return m(x) if op is None else op(x, w, b, _lib.stream_of(x))
 
 
+class LayerNorm(_nn.Module):
+    """``layer_norm`` over the last dimension with a weight and, unless ``bias`` is
+    False, a bias."""
+
+    def __init__(self, channels: int, eps: float = 1e-5, bias: bool = True):
+        super().__init__()
+        if not 1 <= channels <= _lib.NORM_MAX_CHANNELS:
+            raise ValueError(f"channels must be 1 to {_lib.NORM_MAX_CHANNELS}, got {channels}")
+        self.channels, self.eps = int(channels), float(eps)
+        self.weight = _nn.Parameter(torch.ones(self.channels))
+        self.bias = _nn.Parameter(torch.zeros(self.channels)) if bias else None
+
+    def extra_repr(self) -> str:
+        return f"{self.channels}, eps={self.eps}, bias={self.bias is not None}"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class _NeighborhoodAttention(_nn.Module):
     """Rank-generic body of the three layers (``rank`` is set by each
     subclass).  Construction-time checks and messages follow
@@ -97,6 +123,9 @@ class _NeighborhoodAttention(_nn.Module):
         qk_scale: Optional[float] = None,
         attn_drop: float = 0.0,
         proj_drop: float = 0.0,
+        qk_norm: bool = False,
+        rotary: Union[bool, Tuple[int, ...]] = False,
+        rotary_theta: float = 10000.0,
     ):
         super().__init__()
         if embed_dim <= 0:
@@ -131,6 +160,17 @@ class _NeighborhoodAttention(_nn.Module):
         self.attn_drop_rate = float(attn_drop)
         self.attn_drop = _nn.Dropout(self.attn_drop_rate) if self.attn_drop_rate > 0.0 else None
         self.proj = _nn.Linear(self.embed_dim, self.embed_dim)
+        self.q_norm = LayerNorm(self.head_dim) if qk_norm else None
+        self.k_norm = LayerNorm(self.head_dim) if qk_norm else None
+        # rotated channels of each axis, or None
+        self.rotary_dims = (None if rotary is False else rotary_axis_dims(self.head_dim, r)
+                            if rotary is True else tuple(rotary))
+        if self.rotary_dims is not None and (
+                len(self.rotary_dims) != r or sum(self.rotary_dims) > self.head_dim
+                or any(not isinstance(d, int) or d < 2 or d % 2 for d in self.rotary_dims)):
+            raise ValueError(f"rotary must be {r} positive even ints that add up to at most "
+                             f"head_dim ({self.head_dim}), got {rotary}")
+        self.rotary_theta = float(rotary_theta)
         self.proj_drop_rate = float(proj_drop)
         self.proj_drop = _nn.Dropout(self.proj_drop_rate) if self.proj_drop_rate > 0.0 else None
 
@@ -143,7 +183,8 @@ class _NeighborhoodAttention(_nn.Module):
         """The fused op on the projection's packed output, where the operator
         takes it: q, k and v leave it in one pass instead of three copies, and
         their gradients return to it in one.  None otherwise."""
-        if (self._use_gqa or not x.is_cuda or type(x) is not torch.Tensor or _fused._py_autograd
+        if (self._use_gqa or self.q_norm is not None or self.rotary_dims is not None
+                or not x.is_cuda or type(x) is not torch.Tensor or _fused._py_autograd
                 or self.embed_dim * x.element_size() % 16
                 or 3 * x.numel() * x.element_size() >= 1 << 34
                 or torch.is_autocast_enabled("cuda") or ops.backend_module() is not _hip):
@@ -191,6 +232,10 @@ class _NeighborhoodAttention(_nn.Module):
             k, v = kv.unbind(dim=-3)
         else:
             q, k, v = self._split_qkv(_linear(self.qkv, x))
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
+        if self.rotary_dims is not None:
+            q, k = _rotary(q, k, axis_dims=self.rotary_dims, theta=self.rotary_theta)
         return q, k, v
 
     def _attend(self, x: torch.Tensor, sizes: Optional[torch.Tensor]) -> torch.Tensor:
@@ -241,4 +286,5 @@ class NeighborhoodAttention3D(_NeighborhoodAttention):
         return self._attend(x, spatial_sizes)
 
 
-__all__ = ["NeighborhoodAttention1D", "NeighborhoodAttention2D", "NeighborhoodAttention3D"]
+__all__ = ["LayerNorm", "NeighborhoodAttention1D", "NeighborhoodAttention2D",
+           "NeighborhoodAttention3D"]

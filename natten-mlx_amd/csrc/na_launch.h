@@ -223,8 +223,6 @@ void linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *g, con
 // kNormMaxChannels, rows below 2^30 (a group's next row stays in 32 bits).
 constexpr int kNormMaxChannels = 16384;
 constexpr int64_t kNormMaxRows = (int64_t)1 << 30;
-constexpr int kNormFewRows = 2048;
-constexpr int kNormFwdBlocks = 2048, kNormBwdBlocks = 512;
 struct NormArgs {
   int dtype, wdtype;  // wdtype: dtype or NA_F32
   int64_t rows;

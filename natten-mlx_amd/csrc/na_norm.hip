@@ -9,11 +9,11 @@
 // A row stays in registers between its sums (the squares are taken about the
 // mean, not as a difference of moments), so each pass reads its inputs once.
 // Lanes hold 16-byte chunks of a row: a group of 1..64 lanes for narrow rows
-// (several rows per wave), a wave with up to four chunks per lane, or 4 or 16
-// waves for wide ones.  A group walks over rows with a fixed step and keeps its
-// columns' weights -- and in the backward its columns' sums -- in registers; a
-// workgroup's sums leave as one row of partials, added in a fixed order by
-// k_norm_wsum, so results do not depend on the run.
+// (several rows per wave), a wave with two chunks per lane, or 4 or 16 waves for
+// wide ones.  A group walks over rows with a fixed step, the next row's loads in
+// flight, and keeps its columns' weights -- and in the backward its columns' sums
+// -- in registers; a workgroup's sums leave as one row of partials, added in a
+// fixed order by k_norm_wsum, so results do not depend on the run.
 #include "na_chunk.h"
 #include "na_launch.h"
 
@@ -191,15 +191,16 @@ __global__ void __launch_bounds__(norm_threads<WPR>())
   }
 }
 
-// part: [gridDim.x][2][C] sums of dy xh and dy, or null.
+// part: [gridDim.x][2][C] sums of dy xh and dy, or null; a single workgroup has
+// none and writes dw and db (nullable) itself.
 template <typename T, typename W, int NT, int WPR>
 __global__ void __launch_bounds__(norm_threads<WPR>())
     k_norm_bwd(NormProb P, const T *__restrict__ x, const W *__restrict__ w,
                const T *__restrict__ dy, const float2 *__restrict__ stats, T *__restrict__ dx,
-               float *__restrict__ part) {
+               float *__restrict__ part, W *__restrict__ dw, W *__restrict__ db) {
   typedef Chunk<T> K;
   constexpr int N = K::N;
-  extern __shared__ float smem[];  // one wave per row: [2][NT 64 N] column sums; else slots
+  extern __shared__ float smem[];  // one wave per row: [4][2][NT G N] column sums; else slots
   RowSum<WPR, 2> total(smem, P.lgG);
   const Place<WPR> at(P.lgG);
   typename K::raw nx[NT], ng[NT];
@@ -261,22 +262,31 @@ __global__ void __launch_bounds__(norm_threads<WPR>())
       if (d0 < P.C) K::store(dx + (int64_t)row * P.C + d0, o, P.C - d0);
     }
   }
-  if (part == nullptr) return;
+  if (part == nullptr && dw == nullptr && db == nullptr) return;
   float *const pw = part + (int64_t)blockIdx.x * 2 * P.C, *const pb = pw + P.C;
   if (WPR > 1) {  // a thread's columns are its own
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int d0 = (t * at.G + at.lane) * N;
-      if (d0 < P.C) {
-        Chunk<float>::store(pw + d0, aw[t], P.C - d0);
-        if (N == 8) Chunk<float>::store(pw + min(d0 + 4, P.C), aw[t] + 4 % N, P.C - d0 - 4);
-        Chunk<float>::store(pb + d0, ab[t], P.C - d0);
-        if (N == 8) Chunk<float>::store(pb + min(d0 + 4, P.C), ab[t] + 4 % N, P.C - d0 - 4);
+      if (d0 >= P.C) continue;
+      if (part != nullptr) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          Chunk<float>::store(pw + min(d0 + e, P.C), aw[t] + e, P.C - d0 - e);
+          Chunk<float>::store(pb + min(d0 + e, P.C), ab[t] + e, P.C - d0 - e);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (d0 + e >= P.C) continue;
+          if (dw != nullptr) dw[d0 + e] = from_f32<W>(aw[t][e]);
+          if (db != nullptr) db[d0 + e] = from_f32<W>(ab[t][e]);
+        }
       }
     }
     return;
   }
-  // the wave's groups, then the workgroup's four waves in turn
+  // the wave's groups, then the workgroup's four waves
   for (int off = at.G; off < 64; off <<= 1)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -286,23 +296,34 @@ __global__ void __launch_bounds__(norm_threads<WPR>())
         ab[t][e] += __shfl_xor(ab[t][e], off, 64);
       }
   const int width = NT * at.G * N;
-#pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    if ((int)(threadIdx.x >> 6) == k && (int)(threadIdx.x & 63) < at.G) {
+  if ((int)(threadIdx.x & 63) < at.G) {
+    float *const d = smem + (threadIdx.x >> 6) * 2 * width + at.lane * N;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int c = (t * at.G + at.lane) * N + e;
-          smem[c] = k == 0 ? aw[t][e] : smem[c] + aw[t][e];
-          smem[width + c] = k == 0 ? ab[t][e] : smem[width + c] + ab[t][e];
-        }
-    }
-    __syncthreads();
+      for (int e = 0; e < N; e += 4) {
+        const int c = t * at.G * N + e;
+        *reinterpret_cast<float4 *>(d + c) =
+            make_float4(aw[t][e], aw[t][e + 1], aw[t][e + 2], aw[t][e + 3]);
+        *reinterpret_cast<float4 *>(d + width + c) =
+            make_float4(ab[t][e], ab[t][e + 1], ab[t][e + 2], ab[t][e + 3]);
+      }
   }
+  __syncthreads();
   for (int c = threadIdx.x; c < P.C; c += 256) {
-    pw[c] = smem[c];
-    pb[c] = smem[width + c];
+    float sw = 0.f, sb = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sw += smem[k * 2 * width + c];
+      sb += smem[k * 2 * width + width + c];
+    }
+    if (part != nullptr) {
+      pw[c] = sw;
+      pb[c] = sb;
+    } else {
+      if (dw != nullptr) dw[c] = from_f32<W>(sw);
+      if (db != nullptr) db[c] = from_f32<W>(sb);
+    }
   }
 }
 
@@ -316,7 +337,7 @@ __global__ void __launch_bounds__(1024)
   const int col = blockIdx.x * 32 + c;
   float s = 0.f;
   if (col < 2 * C) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = j; k < n; k += 32) s += part[(int64_t)k * 2 * C + col];
   }
   sums[j][c] = s;
@@ -335,30 +356,37 @@ struct NormShape {
   int nt, wpr, lgG, per_block;  // chunks per lane, waves per row, lanes per row, rows per workgroup
 };
 
-// Lanes for a row of C channels.  Few rows spread over more lanes: the row's
-// own latency is what counts there.
-NormShape norm_shape(int dtype, int64_t rows, int C) {
+// Lanes for a row of C channels.  Two chunks per lane where a wave takes a row,
+// as the backward's column sums fill the registers beyond (2048 bf16 channels over
+// 4096 rows: four chunks per lane 38.9 us, four waves per row 16.7); the backward
+// of few rows spreads them over more lanes (768 channels over 2000 rows: 14.7 and
+// 11.0 us; the forward takes 4.0 and 5.0).
+NormShape norm_shape(int dtype, int64_t rows, int C, bool backward) {
   const int n = dtype == NA_F32 ? 4 : 8;
   const int chunks = (C + n - 1) / n;
   NormShape s{};
   if (chunks > 1024) {
     s.wpr = 16;
     s.nt = chunks > 2048 ? 4 : 2;
-  } else if (chunks > 256 || (chunks > 64 && rows <= kNormFewRows)) {
+  } else if (chunks > 128 || (chunks > 64 && backward && rows <= 2048)) {
     s.wpr = 4;
     s.nt = chunks > 512 ? 4 : chunks > 256 ? 2 : 1;
   } else {
     s.wpr = 1;
-    s.nt = chunks > 128 ? 4 : chunks > 64 ? 2 : 1;
+    s.nt = chunks > 64 ? 2 : 1;
     while ((s.nt << s.lgG) < chunks) ++s.lgG;
   }
   s.per_block = s.wpr > 1 ? 1 : 256 >> s.lgG;
   return s;
 }
 
+// The backward's workgroups each leave 2 C partial sums, so they take eight steps
+// over the rows at least, once they fill the chip (2048 rows of 16384 channels:
+// 256 workgroups 53 us, 512 72; 65536 of 2048: 240 and 159).
 int norm_blocks(const NormShape &s, int64_t rows, bool backward) {
-  const int64_t most = s.wpr == 16 ? 512 : backward ? kNormBwdBlocks : kNormFwdBlocks;
-  return (int)std::min<int64_t>((rows + s.per_block - 1) / s.per_block, most);
+  const int64_t steps = (rows + s.per_block - 1) / s.per_block;
+  if (!backward) return (int)std::min<int64_t>(steps, s.wpr == 16 ? 1024 : 8192);
+  return (int)std::min(steps, std::min<int64_t>(std::max<int64_t>(steps / 8, 256), 512));
 }
 
 NormProb norm_prob(const NormArgs &A, const NormShape &s, int blocks) {
@@ -390,8 +418,7 @@ void norm_by_shape(const NormShape &s, F &&f) {
     else S_(4, 4);
   } else {
     if (s.nt == 1) S_(1, 1);
-    else if (s.nt == 2) S_(2, 1);
-    else S_(4, 1);
+    else S_(2, 1);
   }
 #undef S_
 }
@@ -408,13 +435,13 @@ void norm_by_type(int dtype, int wdtype, F &&f) {
 }  // namespace
 
 size_t norm_workspace(int dtype, int64_t rows, int C) {
-  const NormShape s = norm_shape(dtype, rows, C);
-  return sizeof(float) * 2 * (size_t)C * (size_t)norm_blocks(s, rows, true);
+  const int blocks = norm_blocks(norm_shape(dtype, rows, C, true), rows, true);
+  return blocks > 1 ? sizeof(float) * 2 * (size_t)C * (size_t)blocks : 0;
 }
 
 void norm_fwd(const NormArgs &A, const void *x, const void *w, const void *b, void *y, float *stats,
               hipStream_t st) {
-  const NormShape s = norm_shape(A.dtype, A.rows, A.C);
+  const NormShape s = norm_shape(A.dtype, A.rows, A.C, false);
   const int blocks = norm_blocks(s, A.rows, false);
   const NormProb P = norm_prob(A, s, blocks);
   norm_by_type(A.dtype, A.wdtype, [&](auto t, auto wt) {
@@ -430,23 +457,23 @@ void norm_fwd(const NormArgs &A, const void *x, const void *w, const void *b, vo
 
 void norm_bwd(const NormArgs &A, const void *x, const void *w, const void *dy, const float *stats,
               void *dx, void *dw, void *db, void *workspace, hipStream_t st) {
-  const NormShape s = norm_shape(A.dtype, A.rows, A.C);
+  const NormShape s = norm_shape(A.dtype, A.rows, A.C, true);
   const int blocks = norm_blocks(s, A.rows, true);
   const NormProb P = norm_prob(A, s, blocks);
   const bool sums = dw != nullptr || db != nullptr;
-  float *const part = sums ? static_cast<float *>(workspace) : nullptr;
+  float *const part = sums && blocks > 1 ? static_cast<float *>(workspace) : nullptr;
   norm_by_type(A.dtype, A.wdtype, [&](auto t, auto wt) {
     using T = decltype(t);
     using W = decltype(wt);
     if (blocks > 0)
       norm_by_shape<sizeof(T) == 4>(s, [&](auto nt, auto wpr) {
         constexpr int NT = decltype(nt)::value, WPR = decltype(wpr)::value;
-        const size_t lds = sizeof(float) * (WPR > 1 ? 4 * WPR : 2 * NT * (16 / sizeof(T)) << s.lgG);
+        const size_t lds = sizeof(float) * (WPR > 1 ? 4 * WPR : 8 * NT * (16 / sizeof(T)) << s.lgG);
         hipLaunchKernelGGL((k_norm_bwd<T, W, NT, WPR>), dim3(blocks), dim3(norm_threads<WPR>()), lds,
                            st, P, (const T *)x, (const W *)w, (const T *)dy, (const float2 *)stats,
-                           (T *)dx, part);
+                           (T *)dx, part, (W *)dw, (W *)db);
       });
-    if (sums)  // no rows: no partials, zeros
+    if (sums && blocks != 1)  // no rows: no partials, zeros
       hipLaunchKernelGGL((k_norm_wsum<W>), dim3((2 * A.C + 31) / 32), dim3(1024), 0, st, part,
                          (W *)dw, (W *)db, A.C, blocks);
   });

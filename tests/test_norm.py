@@ -113,10 +113,11 @@ def test_missing_weights(has_w, has_b):
 
 
 @pytest.mark.gpu
-def test_only_some_gradients():
+@pytest.mark.parametrize("shape", [(33, 96), (5, 24), (1, 3000), (1, 20), (300, 9000)], ids=str)
+def test_only_some_gradients(shape):
     import natten_amd
 
-    x, w, b, g = (t.to(DEV) for t in _case((33, 96), BF16, BF16, 7))
+    x, w, b, g = (t.to(DEV) for t in _case(shape, BF16, BF16, 7))
     full = _step(x, w, b, g)
     for need in ((True, False, False), (False, True, False), (False, False, True)):
         ts = [t.detach().clone().requires_grad_(n) for t, n in zip((x, w, b), need)]

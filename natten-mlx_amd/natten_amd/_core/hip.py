@@ -625,6 +625,7 @@ def _norm_params(x, w, eps):
     return p
 
 
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
 def norm_forward(x, w, b, eps):
     """``(y, stats)``: stats float32 ``[*lead, 2]``, each row's mean and
     1 / sqrt(var + eps)."""
@@ -639,6 +640,7 @@ def norm_forward(x, w, b, eps):
     return y, stats
 
 
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
 def norm_backward(x, w, b, dy, stats, eps, need):
     """``(dx, dw, db)`` of ``norm_forward``; those not needed come back as None."""
     dev = _require_device(x, w, b, dy, stats)
@@ -660,6 +662,7 @@ def norm_backward(x, w, b, dy, stats, eps, need):
 # ---------------------------------------------------------------------------
 # rotary positions (C ABI na_rotary)
 
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
 def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
     """``(q, k)`` rotated by their tokens' positions; either may be None."""
     dev = _require_device(q, k, positions)
@@ -691,6 +694,7 @@ def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
 # ---------------------------------------------------------------------------
 # attention behind a shared prefix (C ABI na_prefix_fwd)
 
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
 def prefix_forward(q, pk, pv, k, v, lens, window, scale, want_lse):
     """``(out, lse)``: lse float32 ``[B, L, H]``, or None where not wanted; ``window``
     0 for none, ``lens`` int32 on the device or None."""

@@ -14,9 +14,9 @@
 // unnormalised output of an online softmax, float32 -- and k_pfx_join adds the
 // chunks of a row.  One launch holds the prefix's workgroups and the samples'.
 //
-// Two shapes of workgroup (four waves):
-//  * wide: 64 NQ rows, the waves share K / V tiles staged in LDS (as the dense
-//    forward does), one barrier per tile;
+// Two shapes of workgroup (NW waves, four or eight):
+//  * wide: 16 NQ rows per wave, the waves share K / V tiles staged in LDS, one
+//    barrier per tile;
 //  * narrow: up to 16 rows, the waves take different tiles of 32 keys: K goes
 //    from memory straight into the matrix operand, V through the wave's own LDS
 //    (its transposing read), no barrier until the four results meet.
@@ -29,7 +29,6 @@
 namespace na {
 namespace {
 
-constexpr int kPfxThreads = 256;
 constexpr int kPfxNarrowKeys = 32;  // keys of a wave's tile
 constexpr int kPfxJoin = 8;         // slots that a thread of the join loads at once
 
@@ -42,6 +41,7 @@ struct PfxProb {
   int32_t own_launch;
   int32_t rt_p, rt_o;       // row tiles
   int32_t rows_p, rows_o;   // rows per tile: 16 narrow, more wide
+  int32_t waves;            // of a workgroup: 4 or 8
   int32_t chunk_p, chunk_o, SP, SO, NS;  // keys per chunk; chunks; slots per row
   float sl2;                // scale * log2(e)
   FastDiv frep, fLq, frt_p, fSP, frt_o, fSO, fHkv;
@@ -298,7 +298,7 @@ constexpr int pfx_tile() {
   return D > 128 ? 32 : 64;  // keys of a wide tile
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int NW>
 __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
                                          char *smem) {
   typedef L16<T> M;
@@ -307,7 +307,7 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
   typedef typename M::e E;
   constexpr int TK = pfx_tile<D>(), CH = TK / 16;
   constexpr int NT = D / 32, NDB = D / 16, RSE = lds_row(D);
-  constexpr int UPR = D / 4, RPP = kPfxThreads / UPR, NU = TK / RPP;
+  constexpr int UPR = D / 4, RPP = 64 * NW / UPR, NU = TK / RPP;
   E *const buf = reinterpret_cast<E *>(smem);
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63;
   const int n = lane & 15, gq = lane >> 4;
@@ -335,11 +335,15 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
     const int mine = isv ? i : i + 1;
     const int t = first_key(max(min(mine, nkt - 1), 0));
     const char *p = src + (int64_t)t * st;
-    if (i >= 0 && i + 1 < nkt && max(first_key(i), first_key(i + 1)) + TK <= total && P.D == D) {
+    // (eight waves have registers left to hold the zeros of channels past D)
+    if (i >= 0 && i + 1 < nkt && max(first_key(i), first_key(i + 1)) + TK <= total &&
+        (NW > 4 || P.D == D)) {
+      if (NW == 4 || colok) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        pre[u] = pfx_ld8<T>(p);
-        p += RPP * st;
+        for (int u = 0; u < NU; ++u) {
+          pre[u] = pfx_ld8<T>(p);
+          p += RPP * st;
+        }
       }
     } else {  // zeros behind the last key and channel: 0 times them is 0
       const int left = mine >= 0 && mine < nkt && colok ? total - t - r0 : 0;
@@ -360,12 +364,9 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
 
   const int row0 = w.row0 + wv * (16 * NQ);
   v8 qf[NQ][NT];
-  int lo[NQ], cnt[NQ];
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
     const PfxRow<T> r(P, A, w, row0 + 16 * qi + n);
-    lo[qi] = r.lo - w.k0;
-    cnt[qi] = r.n;
 #pragma unroll
     for (int s = 0; s < NT; ++s) {
       const int cq = 32 * s + 8 * gq;
@@ -391,6 +392,7 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
     const v4 lo4 = M::tr(ca), hi4 = M::tr(ca + 16 * RSE);
     return (v8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
   };
+  int lo[NQ], cnt[NQ];  // keys of the tiles at the edges that a row sees
   typedef f32x4 Scores[NQ][CH];
   Scores sa, sb;  // of the tile at hand and of the next
   float mx[NQ];   // the lane's largest score of the tile at hand
@@ -554,6 +556,12 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
     run_tile(i, sa, sb, std::false_type{});
     run_tile(i + 1, sb, sa, std::false_type{});
   }
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {  // not before: the full tiles need the registers
+    const PfxRow<T> r(P, A, w, row0 + 16 * qi + n);
+    lo[qi] = r.lo - w.k0;
+    cnt[qi] = r.n;
+  }
   for (; i < nkt; ++i) {
     run_tile(i, sa, sb, std::true_type{});
     follow();
@@ -569,14 +577,14 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
   }
 }
 
-// The four waves' results of up to 16 rows meet in LDS.  o: channel chan(db) ..
+// The waves' results of up to 16 rows meet in LDS.  o: channel chan(db) ..
 // + 3 of row lane & 15.
-template <typename T, int D, int NDB, typename C>
+template <typename T, int D, int NW, int NDB, typename C>
 __device__ __forceinline__ void pfx_meet(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
                                          char *smem, float m, float l, const f32x4 (&o)[NDB], C chan) {
   constexpr int RS = D + 4;  // floats per row
   float *const po = reinterpret_cast<float *>(smem);
-  float2 *const ml = reinterpret_cast<float2 *>(po + 4 * 16 * RS);  // [4][16]
+  float2 *const ml = reinterpret_cast<float2 *>(po + NW * 16 * RS);  // [NW][16]
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, n = lane & 15;
   l = quad_sum(l);
   __syncthreads();  // the tiles' LDS is free
@@ -585,32 +593,33 @@ __device__ __forceinline__ void pfx_meet(const PfxProb &P, const PfxArgs &A, con
     *reinterpret_cast<f32x4 *>(po + (wv * 16 + n) * RS + chan(db)) = o[db];
   if (lane < 16) ml[wv * 16 + n] = make_float2(m, l);
   __syncthreads();
-  const int r = tid >> 4, row = w.row0 + r;  // 16 threads per row
+  constexpr int TPR = 4 * NW;  // threads per row
+  const int r = tid / TPR, row = w.row0 + r;
   if (row >= w.row1) return;
-  float2 x[4];
+  float2 x[NW];
   float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NW; ++i) {
     x[i] = ml[i * 16 + r];
     mt = fmaxf(mt, x[i].x);
   }
-  float wt[4];
+  float wt[NW];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NW; ++i) {
     wt[i] = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - mt);  // (NaN: a seen row)
     lt = x[i].y == 0.f ? lt : fmaf(wt[i], x[i].y, lt);
   }
-  for (int c = 4 * (tid & 15); c < D; c += 64) {
+  for (int c = 4 * (tid % TPR); c < D; c += 4 * TPR) {
     f32x4 s = zero4();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NW; ++i)
       if (x[i].y != 0.f) s += wt[i] * *reinterpret_cast<const f32x4 *>(po + (i * 16 + r) * RS + c);
     pfx_put<T>(P, A, w, row, c, s, lt);
   }
-  if ((tid & 15) == 0) pfx_put_ml(P, A, w, row, mt, lt);
+  if (tid % TPR == 0) pfx_put_ml(P, A, w, row, mt, lt);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NW>
 __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, const PfxItem &w,
                                            char *smem) {
   typedef L16<T> M;
@@ -680,7 +689,7 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
 #pragma unroll
     for (int i = 0; i < NU; ++i)
       *reinterpret_cast<v8 *>(vs + (RPP * i + vr) * RS + 8 * vc) = vr8[i];
-    if (t0 + 4 * TK < total) load(t0 + 4 * TK);  // in flight during the rest
+    if (t0 + NW * TK < total) load(t0 + NW * TK);  // in flight during the rest
     float p[2][4];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
@@ -712,26 +721,26 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
   };
   int t0 = wv * TK;
   if (t0 < total) load(t0);
-  for (; t0 < total; t0 += 4 * TK) {
+  for (; t0 < total; t0 += NW * TK) {
     if (t0 >= all0 && t0 + TK <= all1) run_tile(t0, std::false_type{});
     else run_tile(t0, std::true_type{});
   }
-  pfx_meet<T, D, NDB>(P, A, w, smem, m, l, o, [&](int db) { return 16 * db + 4 * gq; });
+  pfx_meet<T, D, NW, NDB>(P, A, w, smem, m, l, o, [&](int db) { return 16 * db + 4 * gq; });
 }
 
-// Shape of a segment's workgroups: NQ of the wide ones, 0 the narrow ones.
-template <typename T, int D>
-__global__ void __launch_bounds__(kPfxThreads, D > 128 ? 1 : 2) k_pfx(PfxProb P, PfxArgs A) {
+// NW waves; a segment's rows per tile say how its workgroups are shaped.
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_pfx(PfxProb P, PfxArgs A) {
   extern __shared__ __align__(16) char smem[];
   PfxItem w;
   if (!pfx_item<T>(P, A, blockIdx.x, w)) return;
-  const int shape = (w.b < 0 ? P.rows_p : P.rows_o) >> 6;
-  if (shape == 0) {
-    pfx_narrow<T, D>(P, A, w, smem);
-  } else if (shape == 1) {
-    pfx_wide<T, D, 1>(P, A, w, smem);
+  const int rows = w.b < 0 ? P.rows_p : P.rows_o;
+  if (rows == 16) {
+    pfx_narrow<T, D, NW>(P, A, w, smem);
+  } else if (rows == 16 * NW) {
+    pfx_wide<T, D, 1, NW>(P, A, w, smem);
   } else {
-    if constexpr (D <= 128) pfx_wide<T, D, 2>(P, A, w, smem);
+    if constexpr (D <= 128) pfx_wide<T, D, 2, NW>(P, A, w, smem);
   }
 }
 
@@ -741,7 +750,7 @@ __global__ void __launch_bounds__(kPfxThreads, D > 128 ? 1 : 2) k_pfx(PfxProb P,
 // 64 u + 4 n .. of a V row four blocks of O^T, whose row i is then channel
 // 64 u + 4 i + e.
 template <int D>
-__global__ void __launch_bounds__(kPfxThreads) k_pfx32(PfxProb P, PfxArgs A) {
+__global__ void __launch_bounds__(256) k_pfx32(PfxProb P, PfxArgs A) {
   constexpr int TK = 16, NS = D / 16, NU = D / 64;
   typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
   extern __shared__ __align__(16) char smem[];
@@ -847,7 +856,7 @@ __global__ void __launch_bounds__(kPfxThreads) k_pfx32(PfxProb P, PfxArgs A) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) q4[4 * u + i][e] = o[4 * u + e][i];
-  pfx_meet<float, D, 4 * NU>(P, A, w, smem, m, l, q4,
+  pfx_meet<float, D, 4, 4 * NU>(P, A, w, smem, m, l, q4,
                              [&](int x) { return 64 * (x >> 2) + 16 * gq + 4 * (x & 3); });
 }
 
@@ -941,11 +950,23 @@ int pfx_width(int dtype, int D) {  // the kernels' head dim
   return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256;
 }
 
-// Rows of a tile: narrow up to 16, wide above, as many as the registers hold
-// where there are more than 64.
-int pfx_rows(int dtype, int D, int64_t rows) {
+// Waves of the call's workgroups.  Eight where the batch's rows fill more than
+// half of 256 against a prefix that is most of the keys' work: every K / V tile is
+// then staged once for 256 rows, half the loads of four waves with 128 (256 rows
+// of 128 channels, 8 heads, 65536 prefix keys: 119 -> 100 us; of 80 channels: 94 ->
+// 77).  Where the samples' own keys are most of it, or a head fits 64 channels,
+// four are as good or better (80 channels, 16384 prefix keys and 64 samples of up
+// to 1024: 50.8 and 55.8 us; 64 channels, 65536 and up to 2048: 86 and 96).
+int pfx_waves(const na_prefix_params *p, int64_t span) {
+  const int64_t rows = (int64_t)p->batch * p->tokens * (p->heads / p->kv_heads);
+  return p->dtype != NA_F32 && p->head_dim > 64 && p->head_dim <= 128 && rows > 128 &&
+                 (rows + 255) / 256 * p->prefix >= p->batch * span / 2 ? 8 : 4;
+}
+
+// Rows of a tile: 16 narrow, above that 16 or, where there are more, 32 per wave.
+int pfx_rows(int dtype, int D, int64_t rows, int waves) {
   if (dtype == NA_F32 || rows <= 16) return 16;
-  return rows <= 64 || D > 128 ? 64 : 128;
+  return rows <= 16 * waves || D > 128 ? 16 * waves : 32 * waves;
 }
 
 // Keys per chunk.  kPfxItems workgroups are on the chip at once (two on a CU): a
@@ -967,13 +988,14 @@ PfxProb pfx_prob(const na_prefix_params *p) {
   P.N = p->prefix;
   P.S = p->capacity;
   P.W = p->window > 0 ? p->window : 1 << 30;
-  P.rows_p = pfx_rows(p->dtype, P.D, P.M);
-  P.rows_o = pfx_rows(p->dtype, P.D, P.Mo);
+  const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
+  P.waves = pfx_waves(p, span);
+  P.rows_p = pfx_rows(p->dtype, P.D, P.M, P.waves);
+  P.rows_o = pfx_rows(p->dtype, P.D, P.Mo, P.waves);
   P.rt_p = (P.M + P.rows_p - 1) / P.rows_p;
   P.rt_o = (P.Mo + P.rows_o - 1) / P.rows_o;
-  const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
   const int64_t tp = (int64_t)P.Hkv * P.rt_p, to = (int64_t)p->batch * P.Hkv * P.rt_o;
-  const int64_t want = (tp * P.N + to * span / 2) / kPfxItems;
+  const int64_t want = (tp * P.N + to * span / 2) / (4 * kPfxItems / P.waves);
   auto chunk = [](int64_t keys, int64_t size) {  // even parts, whole tiles
     const int64_t parts = (keys + size - 1) / size;
     return (int32_t)(((keys + parts - 1) / parts + 63) / 64 * 64);
@@ -1020,30 +1042,37 @@ size_t pfx_part_bytes(const PfxProb &P) {
   return ((size_t)P.Hkv * P.M * P.NS * P.D * sizeof(float) + 255) & ~(size_t)255;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NW>
 void pfx_launch(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
   auto lds = [&](int rows) -> size_t {
     if (rows > 16) return sizeof(T) * 2 * pfx_tile<D>() * lds_row(D);
-    const size_t meet = sizeof(float) * 4 * 16 * (D + 4) + sizeof(float2) * 64;
-    const size_t tiles = sizeof(T) == 2 ? sizeof(T) * 4 * kPfxNarrowKeys * (D + 8) : 0;
+    const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
+    const size_t tiles = sizeof(T) == 2 ? sizeof(T) * NW * kPfxNarrowKeys * (D + 8) : 0;
     return std::max(meet, tiles);
   };
   const size_t bytes = std::max(P.SP > 0 ? lds(P.rows_p) : 0, P.SO > 0 ? lds(P.rows_o) : 0);
   const dim3 grid((unsigned)(P.prefix_launch + P.own_launch));
   if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((k_pfx32<D>), grid, dim3(kPfxThreads), bytes, st, P, A);
+    hipLaunchKernelGGL((k_pfx32<D>), grid, dim3(256), bytes, st, P, A);
   else
-    hipLaunchKernelGGL((k_pfx<T, D>), grid, dim3(kPfxThreads), bytes, st, P, A);
+    hipLaunchKernelGGL((k_pfx<T, D, NW>), grid, dim3(64 * NW), bytes, st, P, A);
+}
+
+template <typename T, int D>
+void pfx_by_waves(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && D == 128)
+    if (P.waves == 8) return pfx_launch<T, D, 8>(P, A, st);
+  pfx_launch<T, D, 4>(P, A, st);
 }
 
 template <typename T>
 void pfx_run(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
   if (P.NS > 0) {
     const int width = pfx_width(sizeof(T) == 4 ? NA_F32 : NA_BF16, P.D);
-    if (width == 256) pfx_launch<T, 256>(P, A, st);
-    else if (width == 128) pfx_launch<T, 128>(P, A, st);
-    else if (sizeof(T) == 4 || width == 64) pfx_launch<T, 64>(P, A, st);
-    else if constexpr (sizeof(T) == 2) pfx_launch<T, 32>(P, A, st);
+    if (width == 256) pfx_by_waves<T, 256>(P, A, st);
+    else if (width == 128) pfx_by_waves<T, 128>(P, A, st);
+    else if (sizeof(T) == 4 || width == 64) pfx_by_waves<T, 64>(P, A, st);
+    else if constexpr (sizeof(T) == 2) pfx_by_waves<T, 32>(P, A, st);
   }
   if (A.po == nullptr && P.NS > 0) return;
   int lgG = 0, lgS = 0;

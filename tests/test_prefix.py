@@ -128,6 +128,11 @@ CASES = {
     "window, tokens narrow": (2, 5, 3, 1, 64, 0, 300, [300, 4], 7),
     "window, tokens wide": (2, 50, 4, 2, 64, 33, 300, [300, 60], 37),
     "window over all": (2, 3, 2, 1, 64, 10, 60, [60, 20], 5000),
+    "eight waves": (40, 1, 8, 2, 128, 600, 20, [20, 0, 7], None),
+    "eight waves, prefix only": (70, 2, 8, 2, 96, 333, None, None, None),
+    "eight waves, tokens": (6, 30, 4, 2, 80, 900, 60, [60, 31, 5, 0], None),
+    "eight waves, tokens of two tiles": (3, 100, 6, 2, 128, 700, 130, [130, 101, 40], None),
+    "eight waves, window": (5, 40, 4, 1, 120, 513, 150, [150, 90, 41], 33),
     "window, tokens of several tiles": (1, 130, 3, 1, 48, 64, 400, [390], 100),
 }
 
@@ -180,7 +185,8 @@ def _poison(x, at, value):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("case", ["small service", "tokens narrow", "tokens wide", "window",
-                                  "window, tokens wide", "256 wide, wide", "tokens of several tiles"])
+                                  "window, tokens wide", "256 wide, wide", "tokens of several tiles",
+                                  "eight waves", "eight waves, tokens", "eight waves, window"])
 def test_what_lies_behind_the_lengths_is_not_read(case, dtype):
     t = _make(CASES[case], dtype)
     want = _run(t)
@@ -198,7 +204,8 @@ def test_what_lies_behind_the_lengths_is_not_read(case, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("case", ["tokens narrow", "tokens wide", "window, tokens narrow",
-                                  "window, tokens wide", "256 wide, wide"])
+                                  "window, tokens wide", "256 wide, wide",
+                                  "eight waves, tokens of two tiles", "eight waves, window"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_tokens_that_a_row_does_not_see(case, dtype, value):
     """A token that holds infinities or NaN reaches the rows that see it alone: a

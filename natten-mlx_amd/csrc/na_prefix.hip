@@ -364,9 +364,12 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
 
   const int row0 = w.row0 + wv * (16 * NQ);
   v8 qf[NQ][NT];
+  int lo[NQ], cnt[NQ];  // keys that a row sees
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
     const PfxRow<T> r(P, A, w, row0 + 16 * qi + n);
+    lo[qi] = r.lo - w.k0;
+    cnt[qi] = r.n;
 #pragma unroll
     for (int s = 0; s < NT; ++s) {
       const int cq = 32 * s + 8 * gq;
@@ -392,7 +395,6 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
     const v4 lo4 = M::tr(ca), hi4 = M::tr(ca + 16 * RSE);
     return (v8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  int lo[NQ], cnt[NQ];  // keys of the tiles at the edges that a row sees
   typedef f32x4 Scores[NQ][CH];
   Scores sa, sb;  // of the tile at hand and of the next
   float mx[NQ];   // the lane's largest score of the tile at hand
@@ -555,12 +557,6 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
   for (; i + 2 <= jb - ja; i += 2) {
     run_tile(i, sa, sb, std::false_type{});
     run_tile(i + 1, sb, sa, std::false_type{});
-  }
-#pragma unroll
-  for (int qi = 0; qi < NQ; ++qi) {  // not before: the full tiles need the registers
-    const PfxRow<T> r(P, A, w, row0 + 16 * qi + n);
-    lo[qi] = r.lo - w.k0;
-    cnt[qi] = r.n;
   }
   for (; i < nkt; ++i) {
     run_tile(i, sa, sb, std::true_type{});

@@ -922,7 +922,9 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
       (p->kv_heads > 0 && (k == nullptr || ok == nullptr)) ||
       (p->pos_type != NA_POS_GRID && positions == nullptr))
     return fail(NA_ERR_INVALID, "q/k/positions and their outputs must be non-NULL");
-  na::rotary(p, q, k, positions, oq, ok, as_stream(stream));
+  if (!na::rotary(p, q, k, positions, oq, ok, as_stream(stream)))
+    return fail(NA_ERR_UNSUPPORTED, "%lld tokens of %lld heads are too many for one launch",
+                (long long)tokens, (long long)p->heads + p->kv_heads);
   return launch_status("na_rotary");
 }
 

@@ -238,10 +238,11 @@ void norm_fwd(const NormArgs &A, const void *x, const void *w, const void *b, vo
 void norm_bwd(const NormArgs &A, const void *x, const void *w, const void *dy, const float *stats,
               void *dx, void *dw, void *db, void *workspace, hipStream_t st);
 
-// Rotary positions of q and k in one launch (na_rotary.hip).
+// Rotary positions of q and k in one launch (na_rotary.hip); false, and nothing
+// launched, where they are more than a launch takes.
 constexpr int kRotaryMaxAxes = NA_ROTARY_MAX_AXES;
 constexpr int kRotBlocks = 1024;  // workgroups that fill the chip
-void rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
+bool rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
             void *ok, hipStream_t st);
 
 // Attention against a shared prefix and own cached tokens (na_prefix.hip).

@@ -971,7 +971,9 @@ int pfx_rows(int dtype, int D, int64_t rows, int waves) {
 // rows * D floats for the join; 8 heads x 16384 keys x 128 rows of 128 channels:
 // 33.3 us in chunks of 256, 29.4 of 512, 32.7 of 768); a sample's are at most
 // 1024, which evens out ragged lengths (64 samples of up to 2048, 8 heads: 56.6
-// us, 69.2 in chunks of 2048).
+// us, 69.2 in chunks of 2048) -- or an eighth of a workgroup's part, where there are
+// that many rounds of them anyway and slots would fill the memory (8192 tokens of 32
+// heads over 65536 own: 7.9 ms and 0.54 GB, 11.7 ms and 8.7 GB in chunks of 1024).
 PfxProb pfx_prob(const na_prefix_params *p) {
   PfxProb P{};
   P.Lq = p->tokens;
@@ -1002,7 +1004,7 @@ PfxProb pfx_prob(const na_prefix_params *p) {
   }
   if (span > 0) {
     const int64_t least = P.rows_o > 16 ? 256 : 128;
-    P.chunk_o = chunk(span, std::min<int64_t>(std::max(want, least), 1024));
+    P.chunk_o = chunk(span, std::min(std::max(want, least), std::max<int64_t>(want / 8, 1024)));
     P.SO = (int32_t)((span + P.chunk_o - 1) / P.chunk_o);
   }
   P.NS = P.SP + P.SO;
@@ -1033,6 +1035,18 @@ PfxProb pfx_prob(const na_prefix_params *p) {
 
 // One slot that every row fills needs no join.
 bool pfx_direct(const PfxProb &P) { return P.SP == 1 && P.SO == 0; }
+
+// Logs of the join's lanes per row and of the groups that share a row's slots.
+struct PfxJoinLanes {
+  int lgG = 0, lgS = 0;
+  int total() const { return lgG + lgS; }
+};
+PfxJoinLanes pfx_join_lanes(const PfxProb &P) {
+  PfxJoinLanes n;
+  while ((4 << n.lgG) < P.D) ++n.lgG;
+  while (n.total() < 8 && (kPfxJoin << n.lgS) < P.NS) ++n.lgS;
+  return n;
+}
 
 size_t pfx_part_bytes(const PfxProb &P) {
   return ((size_t)P.Hkv * P.M * P.NS * P.D * sizeof(float) + 255) & ~(size_t)255;
@@ -1071,22 +1085,21 @@ void pfx_run(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
     else if constexpr (sizeof(T) == 2) pfx_by_waves<T, 32>(P, A, st);
   }
   if (A.po == nullptr && P.NS > 0) return;
-  int lgG = 0, lgS = 0;
-  while ((4 << lgG) < P.D) ++lgG;
-  while (lgG + lgS < 8 && (kPfxJoin << lgS) < P.NS) ++lgS;
-  const int64_t threads = ((int64_t)P.Hkv * P.M) << (lgG + lgS);
+  const PfxJoinLanes n = pfx_join_lanes(P);
+  const int64_t threads = ((int64_t)P.Hkv * P.M) << n.total();
   hipLaunchKernelGGL((k_pfx_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
-                     lgG, lgS);
+                     n.lgG, n.lgS);
 }
 
 }  // namespace
 
+// A launch has fewer than 2^32 threads.
 bool prefix_fits(const na_prefix_params *p) {
   const PfxProb P = pfx_prob(p);
-  const int64_t lim = ((int64_t)1 << 31) - 16;
-  return (int64_t)P.Hkv * P.rt_p * P.SP < lim && (int64_t)p->batch * P.Hkv * P.rt_o * P.SO < lim &&
-         (int64_t)P.prefix_launch + P.own_launch < lim &&
-         ((int64_t)P.Hkv * P.M) < (lim >> 1);
+  const int64_t items =
+      (int64_t)P.Hkv * P.rt_p * P.SP + (int64_t)p->batch * P.Hkv * P.rt_o * P.SO + 16;
+  const int64_t rows = (int64_t)P.Hkv * P.M, lim = ((int64_t)1 << 32) - 256;
+  return items * (64 * P.waves) < lim && rows << pfx_join_lanes(P).total() < lim;
 }
 
 size_t prefix_workspace(const na_prefix_params *p) {

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kRotThreads)
 
 }  // namespace
 
-void rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
+bool rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
             void *ok, hipStream_t st) {
   RotProb P{};
   const int n = p->dtype == NA_F32 ? 4 : 8;
@@ -292,6 +292,7 @@ void rotary(const na_rotary_params *p, const void *q, const void *k, const void 
   P.fpairs = make_fastdiv((uint32_t)P.pairs);
   const dim3 grid((unsigned)((P.tokens + per - 1) / per),
                   (unsigned)((heads + P.heads_per - 1) / P.heads_per));
+  if (grid.x >= ((int64_t)1 << 32) / kRotThreads || grid.y > 65535) return false;  // a launch ends there
   size_t lds = sizeof(float2) * per * entries + sizeof(double) * rot_rates(P.pairs);
   if (mode == kRotStaged)
     lds += sizeof(uint16_t) * ((entries + 7) / 8 * 8) + 16 * (size_t)per * P.heads_per * P.upr;
@@ -308,6 +309,7 @@ void rotary(const na_rotary_params *p, const void *q, const void *k, const void 
   if (p->dtype == NA_F32) run(float{});
   else if (p->dtype == NA_F16) run(f16_t{});
   else run(bf16_t{});
+  return true;
 }
 
 }  // namespace na

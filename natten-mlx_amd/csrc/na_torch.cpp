@@ -849,8 +849,10 @@ variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at:
   na_rotary_params p{};
   p.batch = x.size(0);
   for (int a = 0; a < 3; ++a) p.extent[a] = 1;
+  for (const at::Tensor *t : {&q, &k})
+    for (int64_t d = 1; t->defined() && d < nd; ++d)
+      TORCH_CHECK(t->size(d) <= INT32_MAX, "natten_amd na_rotary: a dimension is too long");
   for (int64_t d = 1; d < nd - 2; ++d) {
-    TORCH_CHECK(x.size(d) <= INT32_MAX, "natten_amd na_rotary: axis too long");
     p.extent[3 - (nd - 3) + d - 1] = (int32_t)x.size(d);
   }
   p.heads = q.defined() ? (int32_t)q.size(-2) : 0;

@@ -74,8 +74,8 @@ def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value
     ``seq_lens[b]`` (default S) counts the valid own tokens, the new ones among
     them: query j of sample b is own token ``t = seq_lens[b] - L + j``.  It sees every
     prefix token and the own tokens up to t; with ``kernel_size`` the last
-    ``kernel_size`` of them only, the causal window of ``na1d``.  What a cache holds
-    behind ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
+    ``kernel_size`` of them only, the causal window of ``na1d``; a query before the
+    sequence's start (t < 0) sees the prefix alone.  What a cache holds behind ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
     clamped to ``[0, S]`` there (no synchronisation); lengths on the host are checked.
 
     float32, float16 or bfloat16, all tensors alike; D a multiple of 8 up to 256;

@@ -98,3 +98,46 @@ def test_compiled_calls_run_as_eager():
     assert torch.equal(torch.autograd.grad(got, x, g)[0], torch.autograd.grad(want, x, g)[0])
     q = want.detach()
     assert torch.equal(torch.compile(serve)(q, pk, pv), serve(q, pk, pv))
+
+
+def test_launches_end_at_their_limits():
+    """What does not fit one launch is refused before anything is launched."""
+    from natten_amd._core import _lib
+
+    lib = _lib.load()
+    somewhere = 256  # an address that a refused call does not touch
+
+    def rotary(**kw):
+        p = _lib.NaRotaryParams(**{**dict(batch=1, heads=1, kv_heads=0, head_dim=1024, dtype=0,
+                                          n_axes=1, theta=1e4), **kw})
+        p.extent[0], p.extent[1], p.extent[2], p.axis_dim[0] = 1, 1, 5, 16
+        return lib.na_rotary(p, *([somewhere] * 5), None)
+
+    if not torch.cuda.is_available():  # here nothing could be launched
+        assert rotary(heads=1 << 19) == 2 and b"one launch" in lib.na_last_error()
+        assert rotary(batch=1 << 27, heads=64) == 2 and b"one launch" in lib.na_last_error()
+
+    def prefix(**kw):
+        p = _lib.NaPrefixParams(**{**dict(batch=1, tokens=1, heads=16, kv_heads=16, head_dim=16,
+                                          dtype=2, prefix=5, capacity=7, scale=0.25), **kw})
+        return lib.na_prefix_fwd(p, *([None] * 8), 0, None)
+
+    assert prefix(batch=1 << 25) == 2 and b"one launch" in lib.na_last_error()
+    assert prefix(batch=1 << 25, kv_heads=1, head_dim=256) == 2
+
+
+def test_a_long_prompt_takes_a_workspace_of_few_slots():
+    """Rows that fill the chip many times over meet their own keys in few chunks: the
+    workspace is a small number of float32 rows per query, whatever the length."""
+    from natten_amd._core import _lib
+
+    lib = _lib.load()
+
+    def slots(tokens, capacity, batch=1):
+        p = _lib.NaPrefixParams(batch=batch, tokens=tokens, heads=32, kv_heads=8, head_dim=128,
+                                dtype=2, prefix=64, capacity=capacity, scale=0.1)
+        return lib.na_prefix_workspace_bytes(p) / (batch * tokens * 32 * (128 + 2) * 4)
+
+    assert slots(8192, 131072) < 10
+    assert slots(2048, 32768) < 20
+    assert slots(1, 32768) > 20  # few rows: the keys are shared out

@@ -14,6 +14,12 @@
 // flight, and keeps its columns' weights -- and in the backward its columns' sums
 // -- in registers; a workgroup's sums leave as one row of partials, added in a
 // fixed order by k_norm_wsum, so results do not depend on the run.
+//
+// Sums are float32; y, dx, dw and db are rounded once.  Bound: memory.  65536 rows
+// of 2048 bf16 channels: forward 89 us, reading 268 and writing 270 MB (6.0 TB/s,
+// the input partly from the last-level cache), backward 183 us for 545 and 277 MB
+// (4.5; a large copy moves 4.9), the partials' sum 5.  25088 rows of 256: 8.7, 12.6
+// and 3.9 us.  A call of few rows takes a launch's 2 us.
 #include "na_chunk.h"
 #include "na_launch.h"
 

@@ -8,10 +8,16 @@
 // The backward is the same kernel with the angle negated.
 //
 // The angle is formed in float64, in turns, and reduced to half a turn before it
-// is rounded: a float32 product of position and frequency is off by half a
-// radian at a million tokens.  A workgroup takes a run of tokens: its threads
+// is rounded: a float32 product of position and frequency is off by an eighth of
+// a radian at a million tokens.  A workgroup takes a run of tokens: its threads
 // first fill a table of (cos, sin) per token and pair in LDS, once for all heads,
 // then stream the rows of all heads of q and k past it in 16-byte chunks.
+//
+// The table and the products are float32, the result is rounded once.  Bound:
+// memory.  131072 tokens of 16 heads of 64 bf16 channels on three axes, whose
+// halves are no number of chunks: 124 us, reading and writing 268 MB each (4.3
+// TB/s; a large copy moves 4.9), 295 us where pairs are read and written singly
+// instead of through LDS.
 #include "na_chunk.h"
 #include "na_launch.h"
 

@@ -930,7 +930,9 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
 
 namespace {
 
-int check_prefix(const na_prefix_params *p) {
+// need: the workspace's bytes
+int check_prefix(const na_prefix_params *p, size_t *need) {
+  *need = 0;
   if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
   if (p->batch < 0 || p->tokens < 0 || p->heads < 1 || p->kv_heads < 1 || p->prefix < 0 ||
       p->capacity < 0 || p->window < 0)
@@ -950,29 +952,30 @@ int check_prefix(const na_prefix_params *p) {
   if (p->prefix > (1 << 30) || p->capacity > (1 << 30) || p->tokens > (1 << 30) ||
       (int64_t)p->batch * p->tokens * p->heads >= ((int64_t)1 << 30))
     return fail(NA_ERR_UNSUPPORTED, "more than 2^30 tokens, or batch * tokens * heads");
-  if (p->batch > 0 && p->tokens > 0 && !na::prefix_fits(p))
+  if (p->batch > 0 && p->tokens > 0 && !na::prefix_fits(p, need))
     return fail(NA_ERR_UNSUPPORTED, "the call is too large for one launch");
+  *need = align256(*need);
   return NA_OK;
 }
 
 }  // namespace
 
 size_t na_prefix_workspace_bytes(const na_prefix_params *p) {
-  if (check_prefix(p) != NA_OK || p->batch == 0 || p->tokens == 0) return 0;
-  return align256(na::prefix_workspace(p));
+  size_t need;
+  return check_prefix(p, &need) == NA_OK ? need : 0;
 }
 
 int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k,
                   const void *prefix_v, const void *k, const void *v, void *out, float *lse,
                   void *workspace, size_t workspace_bytes, void *stream) {
-  const int rc = check_prefix(p);
+  size_t need;
+  const int rc = check_prefix(p, &need);
   if (rc != NA_OK) return rc;
   if (p->batch == 0 || p->tokens == 0) return NA_OK;
   if (q == nullptr || out == nullptr ||
       (p->prefix > 0 && (prefix_k == nullptr || prefix_v == nullptr)) ||
       (p->capacity > 0 && (k == nullptr || v == nullptr)))
     return fail(NA_ERR_INVALID, "q/prefix_k/prefix_v/k/v/out must be non-NULL");
-  const size_t need = align256(na::prefix_workspace(p));
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(NA_ERR_WORKSPACE, "na_prefix_fwd needs a %zu-byte workspace (got %zu)", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);

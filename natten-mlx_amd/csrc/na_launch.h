@@ -247,8 +247,7 @@ bool rotary(const na_rotary_params *p, const void *q, const void *k, const void 
 
 // Attention against a shared prefix and own cached tokens (na_prefix.hip).
 constexpr int kPfxItems = 512;  // workgroups that the chip holds at once
-bool prefix_fits(const na_prefix_params *p);
-size_t prefix_workspace(const na_prefix_params *p);
+bool prefix_fits(const na_prefix_params *p, size_t *workspace_bytes);  // false: too large
 void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, const void *pv,
                       const void *k, const void *v, void *out, float *lse, void *workspace,
                       hipStream_t st);

@@ -1108,18 +1108,15 @@ void pfx_run(const PfxProb &P, const PfxArgs &A, hipStream_t st) {
 }  // namespace
 
 // A launch has fewer than 2^32 threads.
-bool prefix_fits(const na_prefix_params *p) {
+bool prefix_fits(const na_prefix_params *p, size_t *workspace_bytes) {
   const PfxProb P = pfx_prob(p);
+  *workspace_bytes = P.NS == 0 || pfx_direct(P)
+                         ? 0
+                         : pfx_part_bytes(P) + sizeof(float2) * (size_t)P.Hkv * P.M * P.NS;
   const int64_t items =
       (int64_t)P.Hkv * P.rt_p * P.SP + (int64_t)p->batch * P.Hkv * P.rt_o * P.SO + 16;
   const int64_t rows = (int64_t)P.Hkv * P.M, lim = ((int64_t)1 << 32) - 256;
   return items * (64 * P.waves) < lim && rows << pfx_join_lanes(P).total() < lim;
-}
-
-size_t prefix_workspace(const na_prefix_params *p) {
-  const PfxProb P = pfx_prob(p);
-  if (P.NS == 0 || pfx_direct(P)) return 0;
-  return pfx_part_bytes(P) + sizeof(float2) * (size_t)P.Hkv * P.M * P.NS;
 }
 
 void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, const void *pv,

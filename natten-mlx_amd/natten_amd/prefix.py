@@ -21,26 +21,31 @@ from .autograd import fused as _fused
 
 
 def _check(query, pk, pv, key, value, seq_lens, kernel_size, scale):
-    if query.ndim != 4:
-        raise ValueError(f"query must be [B, L, heads, dim], got {tuple(query.shape)}.")
-    b, _, h, d = query.shape
-    if pk.ndim != 3 or pk.shape != pv.shape or pk.shape[2] != d or pk.shape[1] < 1:
+    shape, dtype = query.shape, query.dtype
+    if len(shape) != 4:
+        raise ValueError(f"query must be [B, L, heads, dim], got {tuple(shape)}.")
+    b, _, h, d = shape
+    ps = pk.shape
+    if len(ps) != 3 or ps != pv.shape or ps[2] != d or ps[1] < 1:
         raise ValueError(f"prefix_key and prefix_value must be [N, heads_kv, {d}], got "
-                         f"{tuple(pk.shape)} and {tuple(pv.shape)}.")
-    hk = pk.shape[1]
+                         f"{tuple(ps)} and {tuple(pv.shape)}.")
+    hk = ps[1]
     if h < 1 or h % hk:
         raise ValueError(f"heads_q ({h}) must be divisible by heads_kv ({hk}) for GQA.")
     if d < 8 or d % 8 or d > _lib.PREFIX_MAX_HEAD_DIM:
         raise ValueError(f"head dim must be a multiple of 8 up to {_lib.PREFIX_MAX_HEAD_DIM}, got {d}.")
     if (key is None) != (value is None):
         raise ValueError("key and value must both be provided or both None.")
-    if key is not None and (key.ndim != 4 or key.shape != value.shape or key.shape[0] != b
-                            or key.shape[2] != hk or key.shape[3] != d):
-        raise ValueError(f"key and value must be [{b}, S, {hk}, {d}], got {tuple(key.shape)} and "
-                         f"{tuple(value.shape)}.")
-    for t in (pk, pv, key, value):
-        if t is not None and t.dtype != query.dtype:
-            raise ValueError(f"keys and values must have query's dtype {query.dtype}, got {t.dtype}.")
+    tensors = (pk, pv)
+    if key is not None:
+        tensors = (pk, pv, key, value)
+        ks = key.shape
+        if len(ks) != 4 or ks != value.shape or ks[0] != b or ks[2] != hk or ks[3] != d:
+            raise ValueError(f"key and value must be [{b}, S, {hk}, {d}], got {tuple(ks)} and "
+                             f"{tuple(value.shape)}.")
+    for t in tensors:
+        if t.dtype != dtype:
+            raise ValueError(f"keys and values must have query's dtype {dtype}, got {t.dtype}.")
     if seq_lens is not None:
         if key is None:
             raise ValueError("seq_lens are the lengths of key and value, which are missing.")

@@ -49,27 +49,31 @@ def rotary_axis_dims(head_dim: int, n_axes: int) -> Tuple[int, ...]:
 
 
 def _check(query, key, positions, axis_dims, theta):
-    if query.ndim not in (4, 5, 6):
+    shape = query.shape
+    if len(shape) not in (4, 5, 6):
         raise ValueError("rotary expects [B, *spatial, heads, dim] with one to three spatial "
-                         f"axes, got shape {tuple(query.shape)}.")
-    if query.shape[-1] > _lib.MAX_HEAD_DIM:
-        raise ValueError(f"rotary takes up to {_lib.MAX_HEAD_DIM} channels, got {query.shape[-1]}.")
-    lead = tuple(query.shape[:-2])
+                         f"axes, got shape {tuple(shape)}.")
+    d = shape[-1]
+    if d > _lib.MAX_HEAD_DIM:
+        raise ValueError(f"rotary takes up to {_lib.MAX_HEAD_DIM} channels, got {d}.")
+    lead = shape[:-2]
     if key is not None:
-        if key.ndim != query.ndim or tuple(key.shape[:-2]) != lead:
-            raise ValueError(f"key must have query's batch and spatial shape {lead}, got "
-                             f"{tuple(key.shape)}.")
-        if key.shape[-1] != query.shape[-1]:
-            raise ValueError(f"Head dim must match: Q has {query.shape[-1]}, K has {key.shape[-1]}.")
+        ks = key.shape
+        if len(ks) != len(shape) or ks[:-2] != lead:
+            raise ValueError(f"key must have query's batch and spatial shape {tuple(lead)}, got "
+                             f"{tuple(ks)}.")
+        if ks[-1] != d:
+            raise ValueError(f"Head dim must match: Q has {d}, K has {ks[-1]}.")
         if key.dtype != query.dtype:
             raise ValueError(f"query and key must have the same dtype, got {query.dtype} and "
                              f"{key.dtype}.")
     n = len(lead) - 1
     if positions is not None:
-        if tuple(positions.shape[:-1]) not in (lead, (1, *lead[1:]), lead[1:]):
+        *at, n = positions.shape or (0,)
+        at = tuple(at)
+        if at != lead and at != lead[1:] and at != (1, *lead[1:]):
             raise ValueError(f"positions must be [*spatial, axes] or [B, *spatial, axes] for "
-                             f"tokens {lead}, got {tuple(positions.shape)}.")
-        n = positions.shape[-1]
+                             f"tokens {tuple(lead)}, got {tuple(positions.shape)}.")
         if not 1 <= n <= _lib.ROTARY_MAX_AXES:
             raise ValueError(f"positions must have 1 to {_lib.ROTARY_MAX_AXES} axes, got {n}.")
         if positions.dtype not in _lib.POSITIONS:
@@ -77,13 +81,16 @@ def _check(query, key, positions, axis_dims, theta):
                              f"{positions.dtype}.")
         if positions.requires_grad:
             raise ValueError("positions are not differentiable; pass them detached.")
-    dims = rotary_axis_dims(query.shape[-1], n) if axis_dims is None else tuple(axis_dims)
+    dims = rotary_axis_dims(d, n) if axis_dims is None else tuple(axis_dims)
     if len(dims) != n:
         raise ValueError(f"axis_dims must have one entry per axis ({n}), got {dims}.")
-    if any(not isinstance(d, int) or d < 2 or d % 2 for d in dims):
-        raise ValueError(f"axis_dims must be positive even ints, got {dims}.")
-    if sum(dims) > min(query.shape[-1], _lib.ROTARY_MAX_CHANNELS):
-        raise ValueError(f"axis_dims {dims} rotate {sum(dims)} channels of {query.shape[-1]} "
+    total = 0
+    for a in dims:
+        if not isinstance(a, int) or a < 2 or a % 2:
+            raise ValueError(f"axis_dims must be positive even ints, got {dims}.")
+        total += a
+    if total > min(d, _lib.ROTARY_MAX_CHANNELS):
+        raise ValueError(f"axis_dims {dims} rotate {total} channels of {d} "
                          f"(at most {_lib.ROTARY_MAX_CHANNELS}).")
     if not (theta > 0.0 and math.isfinite(theta)):
         raise ValueError(f"theta must be positive and finite, got {theta}.")

@@ -81,7 +81,8 @@ def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value
     prefix token and the own tokens up to t; with ``kernel_size`` the last
     ``kernel_size`` of them only, the causal window of ``na1d``; a query before the
     sequence's start (t < 0) sees the prefix alone.  What a cache holds behind ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
-    clamped to ``[0, S]`` there (no synchronisation); lengths on the host are checked.
+    clamped to ``[0, S]`` there (no synchronisation); lengths on the host are checked
+    and copied, which a call under graph capture cannot do.
 
     float32, float16 or bfloat16, all tensors alike; D a multiple of 8 up to 256;
     query heads share key/value heads as in ``na1d``.  Caches and queries may be

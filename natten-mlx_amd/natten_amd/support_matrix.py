@@ -17,6 +17,8 @@ def get_support_matrix() -> dict[str, dict]:
                 "MI355X (gfx950) via libnatten_amd.so; tensors must be on a HIP device.",
                 "Any kernel size / dilation / stride / causal mask per axis, GQA, "
                 "return_lse and additional tokens in the fused kernels.",
+                "layer_norm and rotary forward and backward; prefix_attention (serving) "
+                "forward only.",
                 "float32 / float16 / bfloat16; fp32 accumulation.",
                 "No CPU fallback: an unavailable library raises.",
             ],

@@ -165,6 +165,22 @@ def test_chunks_of_many_tiles(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [None, 20000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_long_prompt(dtype, window):
+    """Rows that fill the chip many times over, their own keys in chunks of more than
+    1024; compared at some of the tokens."""
+    L, S, n = 8192, 32768, 30011
+    t = _make((1, L, 8, 2, 32, 70, S, [n], window), dtype, 11)
+    out, lse = _run(t)
+    for j in (0, 1, 4097, L - 1):
+        one = {**t, "q": t["q"][:, j:j + 1], "lens": torch.tensor([n - L + j + 1], dtype=torch.int32)}
+        ro, rl = _reference(one)
+        _near(out[:, j:j + 1], ro, f"token {j}")
+        _near(lse[:, j:j + 1], rl, f"token {j} lse")
+
+
+@pytest.mark.gpu
 def test_scores_far_apart_and_scales():
     for dtype in (F32, BF16, F16):
         t = _make((2, 3, 4, 2, 64, 150, 140, [140, 70], None), dtype, 3, std=12.0)

@@ -17,7 +17,7 @@
 // Two shapes of workgroup (NW waves, four or eight):
 //  * wide: 16 NQ rows per wave, the waves share K / V tiles staged in LDS, one
 //    barrier per tile;
-//  * narrow: up to 16 rows, the waves take different tiles of 32 keys: K goes
+//  * narrow: 16 rows, the waves take different tiles of 32 keys: K goes
 //    from memory straight into the matrix operand, V through the wave's own LDS
 //    (its transposing read), no barrier until the waves' results meet.
 // float32 runs narrow on the float32 matrix cores, without LDS tiles.
@@ -974,8 +974,13 @@ int pfx_waves(const na_prefix_params *p, int64_t span) {
 }
 
 // Rows of a tile: 16 narrow, above that 16 or, where there are more, 32 per wave.
-int pfx_rows(int dtype, int D, int64_t rows, int waves) {
-  if (dtype == NA_F32 || rows <= 16) return 16;
+// A sample's own rows are narrow up to two tiles, which read its keys one behind
+// the other through an L2 (64 samples of 32 heads over one key/value head of 128
+// channels: 49.6 us, 62.0 wide; 32 samples of 5 tokens, 8 groups of 64 channels and
+// up to 4096 tokens: 54.7 and 61.7), but not in heads of 256 (152 us, 117 wide); a
+// prefix is read once by wide tiles (32 rows, 65536 keys: 35.7 us, 40.7 narrow).
+int pfx_rows(int dtype, int D, int64_t rows, int waves, int narrow) {
+  if (dtype == NA_F32 || rows <= narrow) return 16;
   return rows <= 16 * waves || D > 128 ? 16 * waves : 32 * waves;
 }
 
@@ -1002,8 +1007,8 @@ PfxProb pfx_prob(const na_prefix_params *p) {
   P.W = p->window > 0 ? p->window : 1 << 30;
   const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
   P.waves = pfx_waves(p, span);
-  P.rows_p = pfx_rows(p->dtype, P.D, P.M, P.waves);
-  P.rows_o = pfx_rows(p->dtype, P.D, P.Mo, P.waves);
+  P.rows_p = pfx_rows(p->dtype, P.D, P.M, P.waves, 16);
+  P.rows_o = pfx_rows(p->dtype, P.D, P.Mo, P.waves, P.D > 128 ? 16 : 32);
   P.rt_p = (P.M + P.rows_p - 1) / P.rows_p;
   P.rt_o = (P.Mo + P.rows_o - 1) / P.rows_o;
   const int64_t tp = (int64_t)P.Hkv * P.rt_p, to = (int64_t)p->batch * P.Hkv * P.rt_o;

@@ -133,6 +133,9 @@ CASES = {
     "eight waves, tokens": (6, 30, 4, 2, 80, 900, 60, [60, 31, 5, 0], None),
     "eight waves, tokens of two tiles": (3, 100, 6, 2, 128, 700, 130, [130, 101, 40], None),
     "eight waves, window": (5, 40, 4, 1, 120, 513, 150, [150, 90, 41], 33),
+    "two narrow tiles": (3, 1, 32, 1, 128, 40, 300, [300, 0, 129], None),
+    "two narrow tiles, tokens": (3, 5, 8, 2, 64, 20, 400, [400, 3, 260], None),
+    "two narrow tiles, window": (2, 8, 4, 1, 40, 0, 300, [300, 150], 30),
     "window, tokens of several tiles": (1, 130, 3, 1, 48, 64, 400, [390], 100),
 }
 

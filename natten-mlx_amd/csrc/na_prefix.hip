@@ -23,9 +23,8 @@
 // float32 runs narrow on the float32 matrix cores, without LDS tiles.
 //
 // Scores, m, l and o are float32.  16-bit types round each probability to their
-// own type before the product with V, as the matrix cores take it (half a step of
-// a factor up to 2^8, next to which the output's own rounding stands); out is
-// rounded once.
+// own type before the product with V, as the matrix cores take it (off by at most
+// half a step each; l adds them unrounded); out is rounded once.
 //
 // Bound, each on its own: narrow workgroups by memory (32 samples of 8 heads and up
 // to 2048 own tokens of 128 bf16 channels against a prefix of 16384: k_pfx 44 us for

@@ -32,9 +32,11 @@ constexpr int kRotTable = 4096;  // (cos, sin) entries of a workgroup, 32 KB
 constexpr int kRotUnits = 4;     // units per thread of a full launch
 
 // How a row splits into the units that threads take: two chunks half an axis
-// apart; a chunk of adjacent pairs; or, where half an axis is no number of
-// chunks, any chunk, whose channels find their partners in a copy of the rows
-// in LDS (the table then holds an entry per channel).
+// apart, or two of the channels behind the axes (16384 tokens of 40 heads, 64 of
+// 128 channels rotated: 77 us, 85 where those took one each); a chunk of adjacent
+// pairs; or, where half an axis is no number of chunks, any chunk, whose channels
+// find their partners in a copy of the rows in LDS (the table then holds an entry
+// per channel).
 enum RotMode { kRotHalves, kRotAdjacent, kRotStaged };
 
 struct RotProb {
@@ -221,13 +223,19 @@ __global__ void __launch_bounds__(kRotThreads)
         }
         K::store(dst + c0, xu, N);
         K::store(dst + c1, xv, N);
-      } else {  // channels that pass through
-        const int c0 = P.pairs + p0, n = P.D - c0;
-        const typename K::raw r = K::load(src + c0, n);
-        float x[N];
+      } else {  // channels that pass through, as many to a unit
+        const int c0 = 2 * p0, c1 = c0 + N;
+        const typename K::raw ru = K::load(src + c0, P.D - c0);
+        typename K::raw rv{};
+        if (c1 < P.D) rv = K::load(src + c1, P.D - c1);
+        float xu[N], xv[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = K::get(r, e);
-        K::store(dst + c0, x, n);
+        for (int e = 0; e < N; ++e) {
+          xu[e] = K::get(ru, e);
+          xv[e] = K::get(rv, e);
+        }
+        K::store(dst + c0, xu, P.D - c0);
+        if (c1 < P.D) K::store(dst + c1, xv, P.D - c1);
       }
     } else if (MODE == kRotAdjacent) {
       const int c0 = j * N, n = P.D - c0;
@@ -273,7 +281,7 @@ bool rotary(const na_rotary_params *p, const void *q, const void *k, const void 
   for (int a = p->n_axes; a <= kRotaryMaxAxes; ++a) P.first[a] = P.pairs;
   const int mode = p->interleaved ? kRotAdjacent : whole ? kRotHalves : kRotStaged;
   const int rest = P.D - 2 * P.pairs;
-  P.upr = mode == kRotHalves ? P.pairs / n + (rest + n - 1) / n : (P.D + n - 1) / n;
+  P.upr = mode == kRotHalves ? P.pairs / n + (rest + 2 * n - 1) / (2 * n) : (P.D + n - 1) / n;
   for (int i = 0; i < 3; ++i) {
     P.qs[i] = p->q_stride[i];
     P.ks[i] = p->k_stride[i];

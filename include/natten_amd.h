@@ -511,7 +511,7 @@ typedef struct na_prefix_params {
   int32_t dtype;
   int32_t prefix;      /* shared tokens; 0: none */
   int32_t capacity;    /* own tokens a sample can hold; 0: none */
-  int32_t window;      /* 0: all own tokens */
+  int32_t window;      /* 0: all own tokens; any width, INT32_MAX among them */
   float scale;         /* positive and finite */
   /* Optional device pointer to int32 [batch]; NULL: capacity.  Values outside
    * [0, capacity] are taken as its ends. */

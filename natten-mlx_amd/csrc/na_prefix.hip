@@ -1003,7 +1003,9 @@ PfxProb pfx_prob(const na_prefix_params *p) {
   P.M = (int32_t)(p->batch * P.Mo);
   P.N = p->prefix;
   P.S = p->capacity;
-  P.W = p->window > 0 ? p->window : 1 << 30;
+  // No cache is longer than 2^30: a wider window is none, and a token's place less
+  // the window (at least -2^30 - 2^30) stays in 32 bits.
+  P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
   const int64_t span = std::min<int64_t>(P.S, (int64_t)P.W + P.Lq - 1);
   P.waves = pfx_waves(p, span);
   P.rows_p = pfx_rows(p->dtype, P.D, P.M, P.waves, 16);

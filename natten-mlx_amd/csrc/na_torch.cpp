@@ -688,10 +688,11 @@ at::Tensor viewed(const at::Tensor &t, RowView *v) {
   return c;
 }
 
+// Whether one of them carries a gradient or a forward-mode tangent.
 bool wants_grad(std::initializer_list<const at::Tensor *> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grads = at::GradMode::is_enabled();
   for (const at::Tensor *t : ts)
-    if (t->defined() && t->requires_grad()) return true;
+    if (t->defined() && ((grads && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 

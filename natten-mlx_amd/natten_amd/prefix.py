@@ -60,6 +60,15 @@ def _check(query, pk, pv, key, value, seq_lens, kernel_size, scale):
         raise ValueError(f"scale must be positive and finite, got {scale}.")
 
 
+class _Prefix(torch.autograd.Function):
+    """The call outside the operator: a Function without derivatives, so that
+    forward-mode levels and torch.func transforms are refused, not passed by."""
+
+    @staticmethod
+    def forward(ctx, q, pk, pv, k, v, lens, window, scale, want_lse):
+        return hip.prefix_forward(q, pk, pv, k, v, lens, window, scale, want_lse)
+
+
 def _host_lens(seq_lens, capacity, device):
     host = seq_lens.tolist()
     if host and (min(host) < 0 or max(host) > capacity):
@@ -90,8 +99,9 @@ def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value
     The output has query's type; the LSE (``return_lse``) is float32 ``[B, L, H]``,
     ready for ``merge_attentions``.  A query that sees no key gets zeros and -inf.
 
-    There is no backward: inputs that require grad are refused outside
-    ``torch.no_grad()``.  To train with shared tokens, pass them to ``na1d`` as
+    There is no derivative: inputs that require grad are refused outside
+    ``torch.no_grad()``, tangents of forward mode and torch.func transforms always.
+    To train with shared tokens, pass them to ``na1d`` as
     ``additional_keys`` expanded over the batch.
     """
     _check(query, prefix_key, prefix_value, key, value, seq_lens, kernel_size, scale)
@@ -111,8 +121,8 @@ def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value
                                "or train with the prefix as additional_keys of na1d)")
         if seq_lens is not None:
             seq_lens = seq_lens.clamp(0, key.shape[1]).to(torch.int32)
-        out, lse = hip.prefix_forward(query, prefix_key, prefix_value, key, value, seq_lens, window,
-                                      scale, return_lse)
+        out, lse = _Prefix.apply(query, prefix_key, prefix_value, key, value, seq_lens, window, scale,
+                                 return_lse)
     return (out, lse) if return_lse else out
 
 

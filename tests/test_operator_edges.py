@@ -1,10 +1,11 @@
 """Calls at the edges of what the layer norm, rotary positions and shared-prefix
-attention document: the widest windows of the C ABI."""
+attention document: the widest windows of the C ABI; forward-mode tangents and
+torch.func transforms, which none of them takes."""
 
 import pytest
 import torch
 
-from _helpers import DEV
+from _helpers import DEV, randn
 from test_prefix import _make, _near, _reference
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -46,3 +47,78 @@ def test_the_widest_windows_are_none(tokens, heads, dtype):
         out, lse = _prefix_c(t, window)
         _near(out, want_out, f"window {window} out")
         _near(lse, want_lse, f"window {window} lse")
+
+
+def _calls(device):
+    """Each operator as a function of its tensors, and the tensors."""
+    import natten_amd
+
+    def r(*shape):
+        return randn(shape, F32, len(shape)).to(device)
+
+    return {
+        "layer_norm": (natten_amd.layer_norm, [r(6, 16), r(16), r(16)]),
+        "rotary": (lambda q, k: torch.cat([t.flatten() for t in natten_amd.rotary(q, k)]),
+                   [r(2, 5, 4, 16), r(2, 5, 1, 16)]),
+        "prefix": (natten_amd.prefix_attention, [r(2, 1, 4, 16), r(5, 2, 16), r(5, 2, 16), r(2, 7, 2, 16),
+                                                 r(2, 7, 2, 16)]),
+    }
+
+
+def _dual(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("twin", [False, True])
+@pytest.mark.parametrize("name", ["layer_norm", "rotary", "prefix"])
+def test_tangents_and_transforms_are_refused(name, twin):
+    """No result without the tangent that the caller asks for, whichever input has
+    one; without a tangent a forward-mode level changes nothing."""
+    import natten_amd.autograd.fused as AF
+
+    fn, ts = _calls(DEV)[name]
+    with AF.python_autograd(twin):
+        want = fn(*ts)
+        for no_grad in (False, True):
+            for i in range(len(ts)):
+                with torch.set_grad_enabled(not no_grad), torch.autograd.forward_ad.dual_level():
+                    with pytest.raises(NotImplementedError):
+                        fn(*(_dual(t) if j == i else t for j, t in enumerate(ts)))
+                    assert torch.equal(fn(*ts), want)
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.func.jvp(fn, tuple(ts), tuple(torch.ones_like(t) for t in ts))
+        with pytest.raises(RuntimeError, match="functorch|no backward"):
+            torch.func.grad(lambda *a: fn(*a).sum())(*ts)
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.vmap(fn)(*(t[None].repeat(2, *[1] * t.dim()) for t in ts))
+
+
+def test_the_prefix_call_outside_the_operator_keeps_no_primal(monkeypatch):
+    """The Python path, its kernels replaced by a copy of the query."""
+    import natten_amd
+    from natten_amd._core import hip
+
+    monkeypatch.setattr(hip, "prefix_forward", lambda q, *rest: (q.clone(), None))
+    _, (q, pk, pv, k, v) = _calls("cpu")["prefix"]
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.equal(natten_amd.prefix_attention(q, pk, pv, k, v), q)
+        for args in ((_dual(q), pk, pv, k, v), (q, _dual(pk), pv, k, v), (q, pk, pv, k, _dual(v))):
+            with pytest.raises(NotImplementedError):
+                natten_amd.prefix_attention(*args)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.jvp(lambda q: natten_amd.prefix_attention(q, pk, pv, k, v), (q,), (q,))
+
+
+@pytest.mark.parametrize("at", range(5))
+def test_the_operators_refuse_tangents(at):
+    """Direct calls of the registered operators."""
+    from natten_amd._core import _lib
+
+    _lib.load()
+    ops = torch.ops.natten_amd
+    calls = _calls("cpu")
+    with torch.autograd.forward_ad.dual_level():
+        ts = [_dual(t) if i == at else t for i, t in enumerate(calls["prefix"][1])]
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.na_prefix(*ts, None, 0, 0.25, False, 0)

@@ -16,7 +16,6 @@ import torch
 
 from ._core import _lib
 from ._core import hip
-from .autograd import device_extents
 from .autograd import fused as _fused
 
 
@@ -70,10 +69,15 @@ class _Prefix(torch.autograd.Function):
 
 
 def _host_lens(seq_lens, capacity, device):
+    # lengths change with every generated token: nothing is kept of them
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("seq_lens on the host cannot be captured in a graph: pass them on "
+                               "query's device")
     host = seq_lens.tolist()
     if host and (min(host) < 0 or max(host) > capacity):
         raise ValueError(f"All seq_lens must be in [0, {capacity}], got {min(host)} to {max(host)}.")
-    return device_extents(seq_lens, len(host), 1, device).reshape(-1)
+    return seq_lens.to(torch.int32).to(device)
 
 
 def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value: torch.Tensor,
@@ -89,9 +93,11 @@ def prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value
     them: query j of sample b is own token ``t = seq_lens[b] - L + j``.  It sees every
     prefix token and the own tokens up to t; with ``kernel_size`` the last
     ``kernel_size`` of them only, the causal window of ``na1d``; a query before the
-    sequence's start (t < 0) sees the prefix alone.  What a cache holds behind ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
+    sequence's start (t < 0) sees the prefix alone.  What a cache holds behind
+    ``seq_lens[b]`` is not read.  Lengths on the device are taken as they are,
     clamped to ``[0, S]`` there (no synchronisation); lengths on the host are checked
-    and copied, which a call under graph capture cannot do.
+    and copied at every call, which waits for the stream; under graph capture they are
+    refused.
 
     float32, float16 or bfloat16, all tensors alike; D a multiple of 8 up to 256;
     query heads share key/value heads as in ``na1d``.  Caches and queries may be

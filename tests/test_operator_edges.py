@@ -1,6 +1,6 @@
 """Calls at the edges of what the layer norm, rotary positions and shared-prefix
-attention document: the widest windows of the C ABI; forward-mode tangents and
-torch.func transforms, which none of them takes."""
+attention document: the widest windows of the C ABI; lengths on the host; forward-mode
+tangents and torch.func transforms, which none of them takes."""
 
 import pytest
 import torch
@@ -122,3 +122,43 @@ def test_the_operators_refuse_tangents(at):
         ts = [_dual(t) if i == at else t for i, t in enumerate(calls["prefix"][1])]
         with pytest.raises(RuntimeError, match="no backward"):
             ops.na_prefix(*ts, None, 0, 0.25, False, 0)
+
+
+@pytest.mark.gpu
+def test_lengths_on_the_host_are_not_kept():
+    """Every step of a generation has other lengths: a copy of each, kept for calls to
+    come, would stay for the life of the process and crowd out the copies of lengths
+    that do come again."""
+    import natten_amd
+    from natten_amd.autograd import fused
+
+    t = {n: x.to(DEV) for n, x in _make((2, 1, 4, 2, 16, 5, 40, [0], None), F32).items()
+         if isinstance(x, torch.Tensor)}
+
+    def step(lens):
+        return natten_amd.prefix_attention(t["q"], t["pk"], t["pv"], t["k"], t["v"], seq_lens=lens)
+
+    before = dict(fused._extents_cache)
+    for n in range(1, 30):
+        lens = torch.tensor([n, 40 - n], dtype=(torch.int32, torch.int64)[n % 2])
+        assert torch.equal(step(lens), step(lens.to(DEV)))
+    assert fused._extents_cache == before
+
+    lens = torch.tensor([7, 9])
+    want = step(lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_device = lens.to(DEV)
+        step(on_device)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(RuntimeError, match="on the host"):
+                step(lens)
+            held = step(on_device)  # the capture goes on
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want) and torch.equal(step(lens), want)

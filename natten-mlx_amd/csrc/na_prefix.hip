@@ -24,7 +24,8 @@
 //
 // Scores, m, l and o are float32.  16-bit types round each probability to their
 // own type before the product with V, as the matrix cores take it (off by at most
-// half a step each; l adds them unrounded); out is rounded once.
+// half a step each, in fp16 at least 2^-32 of the row's largest; l adds them
+// unrounded); out is rounded once.
 //
 // Bound, each on its own: narrow workgroups by memory (32 samples of 8 heads and up
 // to 2048 own tokens of 128 bf16 channels against a prefix of 16384: k_pfx 44 us for
@@ -229,11 +230,21 @@ __device__ __forceinline__ typename L16<T>::v8 pfx_zero8() {
   return z;
 }
 
+// How far below a row's largest score its reference point m is put: a power of two
+// in every probability, which the division by l takes out.  In fp16, whose smallest
+// step is 2^-24, probabilities of an m at the maximum vanish below 2^-25 of the
+// largest, while l keeps them; from 2^7 up (with the factor 2^8 by which m may
+// trail, below 2^15) the products lose 2^-32 of the largest at most.
+template <typename T>
+__host__ __device__ constexpr float pfx_lead() {
+  return std::is_same<T, f16_t>::value ? 7.f : 0.f;
+}
+
 // Online softmax step of a lane's CH * 4 scores of one row (the four lanes of a
 // row hold the others): scores to probabilities in place, m, l and o rescaled
 // where the reference point m moves.  It may trail the maximum by 8 (a factor
-// 2^8 in p): exact after the division by l.
-template <int CH, int NDB>
+// 2^8 in p) beside its lead: exact after the division by l.
+template <typename T, int CH, int NDB>
 __device__ __forceinline__ void pfx_softmax(float (&p)[CH][4], float sl2, float &m, float &l,
                                             f32x4 (&o)[NDB]) {
   float mx = -INFINITY;
@@ -242,8 +253,8 @@ __device__ __forceinline__ void pfx_softmax(float (&p)[CH][4], float sl2, float 
 #pragma unroll
     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, p[ch][r]);
   mx = quad_max(mx) * sl2;
-  if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-    const float mn = fmaxf(m, mx);
+  if (__builtin_amdgcn_ballot_w64(mx > m + (8.f + pfx_lead<T>())) != 0) {
+    const float mn = fmaxf(m, mx - pfx_lead<T>());
     const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
     l *= alpha;
 #pragma unroll
@@ -444,14 +455,14 @@ __device__ __forceinline__ void pfx_wide(const PfxProb &P, const PfxArgs &A, con
           largest(s, qi, ch);
         }
       }
-      moves |= mx[qi] * sl2 > m[qi] + 8.f;
+      moves |= mx[qi] * sl2 > m[qi] + (8.f + pfx_lead<T>());
     }
-    // the reference point may trail the maximum by 8 (a factor 2^8 in p): exact
-    // after the division by l
+    // the reference point may trail the maximum by 8 (a factor 2^8 in p) beside its
+    // lead: exact after the division by l
     if (__builtin_amdgcn_ballot_w64(moves) != 0) {
 #pragma unroll
       for (int qi = 0; qi < NQ; ++qi) {
-        const float mn = fmaxf(m[qi], quad_max(mx[qi]) * sl2);
+        const float mn = fmaxf(m[qi], quad_max(mx[qi]) * sl2 - pfx_lead<T>());
         const float alpha = __builtin_amdgcn_exp2f(m[qi] - (mn == -INFINITY ? 0.f : mn));
         l[qi] *= alpha;
 #pragma unroll
@@ -707,7 +718,7 @@ __device__ __forceinline__ void pfx_narrow(const PfxProb &P, const PfxArgs &A, c
         p[hh][r] = s[hh][r];
         if (EDGE && (unsigned)(t0 + 16 * hh + 4 * gq + r - lo) >= (unsigned)cnt) p[hh][r] = -INFINITY;
       }
-    pfx_softmax<2, NDB>(p, sl2, m, l, o);
+    pfx_softmax<T, 2, NDB>(p, sl2, m, l, o);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -816,7 +827,7 @@ __global__ void __launch_bounds__(256) k_pfx32(PfxProb P, PfxArgs A) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       p[0][r] = all || (unsigned)(t0 + 4 * gq + r - lo) < (unsigned)cnt ? s4[r] : -INFINITY;
-    pfx_softmax<1, 4 * NU>(p, P.sl2, m, l, o);
+    pfx_softmax<float, 1, 4 * NU>(p, P.sl2, m, l, o);
     bool odd = false;
     if (!all && spans) {
 #pragma unroll

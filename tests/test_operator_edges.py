@@ -1,6 +1,9 @@
 """Calls at the edges of what the layer norm, rotary positions and shared-prefix
-attention document: the widest windows of the C ABI; lengths on the host; forward-mode
-tangents and torch.func transforms, which none of them takes."""
+attention document: the widest windows of the C ABI; lengths on the host;
+probabilities far below a row's largest; forward-mode tangents and torch.func
+transforms, which none of them takes."""
+
+import math
 
 import pytest
 import torch
@@ -9,6 +12,7 @@ from _helpers import DEV, randn
 from test_prefix import _make, _near, _reference
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+E = 2.0 ** -24
 
 
 def _prefix_c(t, window):
@@ -162,3 +166,54 @@ def test_lengths_on_the_host_are_not_kept():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want) and torch.equal(step(lens), want)
+
+
+SMALL = {  # B, tokens, heads, kv heads, dim, prefix, own capacity, lengths
+    "narrow": (2, 1, 4, 2, 64, 320, 200, [200, 33]),
+    "narrow, tokens": (2, 3, 4, 1, 32, 96, 300, [300, 70]),
+    "wide of 64": (8, 1, 8, 2, 128, 320, 130, [130, 0, 64]),
+    "wide of 128": (2, 70, 4, 1, 32, 160, 300, [300, 75]),
+    "wide of 128, 80 wide": (3, 40, 4, 1, 80, 352, 100, [100, 41]),
+    "256 wide": (5, 3, 8, 1, 256, 96, 64, [64, 7]),
+    "eight waves": (40, 1, 8, 2, 128, 640, 32, [32, 0]),
+    "eight waves, tokens": (3, 100, 6, 2, 128, 704, 130, [130, 101]),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", list(SMALL))
+def test_probabilities_far_below_the_largest(case, dtype):
+    """Every 32nd key scores 18 and holds zeros, the others score 0 and hold 1024: a
+    row of h and n of them is 1024 n e^-18 / (h + n e^-18), all of it probabilities of
+    2^-26 of the largest.
+
+    A score is off by d = 2^-24 (18 D + 2 * 18 + 16 + keys), with the sums over the keys
+    (as in test_prefix); 16-bit types round a probability by u = eps / 2 of it.  fp16
+    below 2^-14 rounds by 2^-25: with the largest at 2^7 at least, the n = 31 h (and up to
+    31 more where a sequence ends) move a row by 1024 (n / h) 2^-32."""
+    import natten_amd
+
+    B, L, H, Hk, D, N, S, lens = SMALL[case]
+    lens = torch.tensor([lens[b % len(lens)] for b in range(B)], dtype=torch.int32)
+    q, pk, k = torch.zeros(B, L, H, D), torch.zeros(N, Hk, D), torch.zeros(B, S, Hk, D)
+    q[..., 0], pk[::32, :, 0], k[:, ::32, :, 0] = 1.0, 18.0, 18.0
+    pv, v = torch.full_like(pk, 1024.0), torch.full_like(k, 1024.0)
+    pv[::32], v[:, ::32] = 0.0, 0.0
+    out, lse = natten_amd.prefix_attention(*(t.to(DEV, dtype) for t in (q, pk, pv, k, v)),
+                                           lens.to(DEV), scale=1.0, return_lse=True)
+    out, lse = out.cpu().double(), lse.cpu().double()
+    u, fi = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2, torch.finfo(dtype)
+    for b in range(B):
+        for j in range(L):
+            own = max(0, int(lens[b]) - L + j + 1)
+            h = N // 32 + -(-own // 32)
+            n = N + own - h
+            tail = n * math.exp(-18.0)
+            want, d = 1024 * tail / (h + tail), E * (18 * D + 52 + N + own)
+            tol = (u + 4 * d + fi.eps / 2) * want + fi.tiny
+            if dtype == F16:
+                tol += 1024 * n / h * 2.0 ** -32
+            assert ((out[b, j] - want).abs() <= tol).all(), (b, j, out[b, j].min(), out[b, j].max(), want)
+            ref = 18.0 + math.log(h + tail)
+            assert ((lse[b, j] - ref).abs() <= 4 * d + 4 * E * (1 + ref)).all(), (b, j)

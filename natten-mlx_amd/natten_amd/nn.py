@@ -26,6 +26,7 @@ their positions on the layer's axes; both come before the attention on every rou
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -92,6 +93,8 @@ class LayerNorm(_nn.Module):
         super().__init__()
         if not 1 <= channels <= _lib.NORM_MAX_CHANNELS:
             raise ValueError(f"channels must be 1 to {_lib.NORM_MAX_CHANNELS}, got {channels}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must be >= 0, got {eps}")
         self.channels, self.eps = int(channels), float(eps)
         self.weight = _nn.Parameter(torch.ones(self.channels))
         self.bias = _nn.Parameter(torch.zeros(self.channels)) if bias else None
@@ -165,12 +168,18 @@ class _NeighborhoodAttention(_nn.Module):
         # rotated channels of each axis, or None
         self.rotary_dims = (None if rotary is False else rotary_axis_dims(self.head_dim, r)
                             if rotary is True else tuple(rotary))
+        most = min(self.head_dim, _lib.ROTARY_MAX_CHANNELS)
         if self.rotary_dims is not None and (
-                len(self.rotary_dims) != r or sum(self.rotary_dims) > self.head_dim
-                or any(not isinstance(d, int) or d < 2 or d % 2 for d in self.rotary_dims)):
-            raise ValueError(f"rotary must be {r} positive even ints that add up to at most "
-                             f"head_dim ({self.head_dim}), got {rotary}")
+                len(self.rotary_dims) != r
+                or any(not isinstance(d, int) or d < 2 or d % 2 for d in self.rotary_dims)
+                or sum(self.rotary_dims) > most or self.head_dim > _lib.MAX_HEAD_DIM):
+            raise ValueError(f"rotary must be {r} positive even ints that add up to at most {most}, "
+                             f"in heads of up to {_lib.MAX_HEAD_DIM} channels (here "
+                             f"{self.head_dim}), got {self.rotary_dims}")
         self.rotary_theta = float(rotary_theta)
+        if self.rotary_dims is not None and not (
+                self.rotary_theta > 0.0 and math.isfinite(self.rotary_theta)):
+            raise ValueError(f"rotary_theta must be positive and finite, got {rotary_theta}")
         self.proj_drop_rate = float(proj_drop)
         self.proj_drop = _nn.Dropout(self.proj_drop_rate) if self.proj_drop_rate > 0.0 else None
 

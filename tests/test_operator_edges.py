@@ -1,7 +1,7 @@
 """Calls at the edges of what the layer norm, rotary positions and shared-prefix
 attention document: the widest windows of the C ABI; lengths on the host;
 probabilities far below a row's largest; forward-mode tangents and torch.func
-transforms, which none of them takes."""
+transforms, which none of them takes; layers of heads that rotary does not take."""
 
 import math
 
@@ -217,3 +217,23 @@ def test_probabilities_far_below_the_largest(case, dtype):
             assert ((out[b, j] - want).abs() <= tol).all(), (b, j, out[b, j].min(), out[b, j].max(), want)
             ref = 18.0 + math.log(h + tail)
             assert ((lse[b, j] - ref).abs() <= 4 * d + 4 * E * (1 + ref)).all(), (b, j)
+
+
+def test_layers_refuse_what_rotary_refuses():
+    """At construction, not at the first call: more rotated channels than a launch's
+    table holds, or heads too wide, also where the layer shares the channels out."""
+    from natten_amd import nn
+
+    for cls, dim, rotary in ((nn.NeighborhoodAttention1D, 1024, True), (nn.NeighborhoodAttention1D, 514, (514,)),
+                             (nn.NeighborhoodAttention2D, 520, (260, 254)),
+                             (nn.NeighborhoodAttention1D, 1026, (64,))):
+        with pytest.raises(ValueError, match="rotary must be"):
+            cls(dim, 1, 3, rotary=rotary)
+    assert nn.NeighborhoodAttention1D(1024, 1, 3, rotary=(512,)).rotary_dims == (512,)
+    assert nn.NeighborhoodAttention1D(1024, 2, 3, rotary=True).rotary_dims == (512,)
+    for theta in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="rotary_theta"):
+            nn.NeighborhoodAttention1D(32, 2, 3, rotary=True, rotary_theta=theta)
+    for eps in (-1e-5, math.nan):
+        with pytest.raises(ValueError, match="eps"):
+            nn.LayerNorm(8, eps)

@@ -183,6 +183,12 @@ class _NeighborhoodAttention(_nn.Module):
         self.proj_drop_rate = float(proj_drop)
         self.proj_drop = _nn.Dropout(self.proj_drop_rate) if self.proj_drop_rate > 0.0 else None
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "rotary_dims" not in state:  # pickled before the layers had these
+            self.q_norm = self.k_norm = self.rotary_dims = None
+            self.rotary_theta = 10000.0
+
     def extra_repr(self) -> str:
         return (f"embed_dim={self.embed_dim}, num_heads={self.num_heads}, "
                 f"num_kv_heads={self.num_kv_heads}, kernel_size={self.kernel_size}, "

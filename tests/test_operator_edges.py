@@ -1,8 +1,10 @@
 """Calls at the edges of what the layer norm, rotary positions and shared-prefix
 attention document: the widest windows of the C ABI; lengths on the host;
 probabilities far below a row's largest; forward-mode tangents and torch.func
-transforms, which none of them takes; layers of heads that rotary does not take."""
+transforms, which none of them takes; layers of heads that rotary does not take;
+layers pickled before they had norms and positions."""
 
+import io
 import math
 
 import pytest
@@ -237,3 +239,41 @@ def test_layers_refuse_what_rotary_refuses():
     for eps in (-1e-5, math.nan):
         with pytest.raises(ValueError, match="eps"):
             nn.LayerNorm(8, eps)
+
+
+def _pickled(m):
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+def _plain_and_older():
+    from natten_amd import nn
+
+    m = nn.NeighborhoodAttention2D(32, 2, 3)
+    older = nn.NeighborhoodAttention2D(32, 2, 3)
+    older.load_state_dict(m.state_dict())
+    for n in ("q_norm", "k_norm", "rotary_dims", "rotary_theta"):
+        del older.__dict__[n]
+    return m, _pickled(older)
+
+
+def test_layers_pickled_before_they_had_norms_and_positions():
+    m, older = _plain_and_older()
+    assert older.q_norm is None and older.k_norm is None and older.rotary_dims is None
+    with pytest.raises(RuntimeError, match="HIP"):
+        older(torch.randn(1, 4, 4, 32))
+    from natten_amd import nn
+
+    full = nn.NeighborhoodAttention2D(32, 2, 3, qk_norm=True, rotary=True, rotary_theta=7.0)
+    back = _pickled(full)
+    assert back.rotary_dims == (8, 8) and back.rotary_theta == 7.0
+    assert torch.equal(back.q_norm.weight, full.q_norm.weight)
+
+
+@pytest.mark.gpu
+def test_layers_pickled_before_run_as_plain_ones():
+    m, older = (t.to(DEV) for t in _plain_and_older())
+    x = randn((2, 9, 7, 32), F32, 1).to(DEV)
+    assert torch.equal(older(x), m(x))

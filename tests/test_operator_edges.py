@@ -2,7 +2,8 @@
 attention document: the widest windows of the C ABI; lengths on the host;
 probabilities far below a row's largest; forward-mode tangents and torch.func
 transforms, which none of them takes; layers of heads that rotary does not take;
-layers pickled before they had norms and positions."""
+layers pickled before they had norms and positions; second derivatives of rotary
+positions."""
 
 import io
 import math
@@ -277,3 +278,44 @@ def test_layers_pickled_before_run_as_plain_ones():
     m, older = (t.to(DEV) for t in _plain_and_older())
     x = randn((2, 9, 7, 32), F32, 1).to(DEV)
     assert torch.equal(older(x), m(x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("twin", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_second_derivatives_of_rotary(interleaved, twin):
+    """f = sum oq^2 ok with (oq, ok) the rotated (q, k), and the gradient of
+    <df/dq, u> + <df/dk, w>, which is R^T(2 ok Ru + 2 oq Rw) and R^T(2 oq Ru), against
+    float64 matrices.  Every rotation is two products and a sum of terms of at most b
+    and of a table off by 2 e; with the two factors that they meet, 64 e times the
+    largest term bounds the chain of four."""
+    import natten_amd
+    import natten_amd.autograd.fused as AF
+
+    q, k, u, w = (randn((2, 7, 3, 16), F32, s).to(DEV) for s in range(4))
+    q.requires_grad_(True), k.requires_grad_(True)
+    with AF.python_autograd(twin):
+        oq, ok = natten_amd.rotary(q, k, axis_dims=(12,), interleaved=interleaved)
+        assert ("CppNode" in oq.grad_fn.name()) != twin
+        gq, gk = torch.autograd.grad((oq.square() * ok).sum(), (q, k), create_graph=True)
+        hq, hk = torch.autograd.grad((gq * u).sum() + (gk * w).sum(), (q, k))
+
+    rot = torch.eye(16, dtype=torch.float64).repeat(7, 1, 1)  # [token, out, in]
+    for t in range(7):
+        for i in range(6):
+            a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + 6)
+            angle = t * 10000.0 ** (-2 * i / 12)
+            rot[t, a, a] = rot[t, b, b] = math.cos(angle)
+            rot[t, a, b], rot[t, b, a] = -math.sin(angle), math.sin(angle)
+
+    def turn(x):
+        return (rot[None, :, None] @ x.unsqueeze(-1)).squeeze(-1)
+
+    def back(x):
+        return (rot.transpose(1, 2)[None, :, None] @ x.unsqueeze(-1)).squeeze(-1)
+
+    q, k, u, w = (turn(t.detach().cpu().double()) for t in (q, k, u, w))
+    largest = 4 * max(float(t.abs().max()) for t in (q, k)) * max(float(t.abs().max()) for t in (u, w))
+    for got, want in ((gq, back(2 * q * k)), (gk, back(q * q)),
+                      (hq, back(2 * k * u + 2 * q * w)), (hk, back(2 * q * u))):
+        assert (got.detach().cpu().double() - want).abs().max() <= 64 * E * largest

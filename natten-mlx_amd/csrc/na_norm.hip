@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(norm_threads<WPR>())
       }
     if (r0 + P.per_iter < P.rows) fetch(row + P.per_iter);
     total(s);
-    const float mean = s[0] / (float)P.C;  // equal channels: their value, exactly
+    const float mean = s[0] / (float)P.C;  // equal channels: their value, where its sums are exact
     s[0] = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {

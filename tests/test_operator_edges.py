@@ -3,7 +3,7 @@ attention document: the widest windows of the C ABI; lengths on the host;
 probabilities far below a row's largest; forward-mode tangents and torch.func
 transforms, which none of them takes; layers of heads that rotary does not take;
 layers pickled before they had norms and positions; second derivatives of rotary
-positions."""
+positions; rows of equal channels."""
 
 import io
 import math
@@ -319,3 +319,22 @@ def test_second_derivatives_of_rotary(interleaved, twin):
     for got, want in ((gq, back(2 * q * k)), (gk, back(q * q)),
                       (hq, back(2 * k * u + 2 * q * w)), (hk, back(2 * q * u))):
         assert (got.detach().cpu().double() - want).abs().max() <= 64 * E * largest
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [24, 100, 200, 500, 777, 5000, 16384])
+def test_rows_of_equal_channels(width):
+    """The sum of equal channels rounds, so their mean is off by up to K e of it (K = 64,
+    as in test_norm) and the rows by that over sqrt(eps): no row leaves its bias by more,
+    and a value whose sums are exact not at all."""
+    import natten_amd
+
+    values = torch.tensor([0.1, 1.7, 3.14159, -1e-3, 12345.678, 0.75, 0.0])
+    x = values[:, None].expand(-1, width).contiguous().to(DEV)
+    w, b = (randn((width,), F32, s).to(DEV) for s in (1, 2))
+    for eps in (1e-5, 1e-2):
+        y = natten_amd.layer_norm(x, w, b, eps)
+        off = (y - b).abs().double() / w.abs().double()
+        bound = (64 * E * values.double().abs() / math.sqrt(eps))[:, None].to(DEV)
+        assert (off <= bound * (1 + 2 ** -10) + E * (y.abs() + b.abs()) / w.abs()).all()
+        assert torch.equal(y[-2:], b.expand(2, -1))

@@ -29,7 +29,7 @@
 namespace na {
 namespace {
 
-// A lane's columns of a weight vector, in the storage type; absent: `fill`.
+// A lane's columns of a weight vector, in the storage type.
 template <typename T, typename W, int NT>
 struct Cols {
   static constexpr int N = Chunk<T>::N, S = N * (int)sizeof(W) / 16;  // chunks of W per chunk of T
@@ -366,7 +366,12 @@ struct NormShape {
 // as the backward's column sums fill the registers beyond (2048 bf16 channels over
 // 4096 rows: four chunks per lane 38.9 us, four waves per row 16.7); the backward
 // of few rows spreads them over more lanes (768 channels over 2000 rows: 14.7 and
-// 11.0 us; the forward takes 4.0 and 5.0).
+// 11.0 us; the forward takes 4.0 and 5.0).  16-bit rows past 4096 channels take four
+// chunks per lane of four waves all the same, whose backward holds 255 registers, one
+// wave on a SIMD (8192 rows of 8192 bf16 channels: forward 58 us, backward 83, 4.7 and
+// 4.9 TB/s; of 5120, which leave 3 of 8 chunks empty: 47 and 73, 3.6 and 3.4; sixteen
+// waves of one chunk were not measured).  Past 8192 channels the backward spills 8 to
+// 14 registers in 16-bit types, 85 in float32.
 NormShape norm_shape(int dtype, int64_t rows, int C, bool backward) {
   const int n = dtype == NA_F32 ? 4 : 8;
   const int chunks = (C + n - 1) / n;

@@ -8,11 +8,13 @@
 //
 // The prefix's keys are one product for the batch: the rows of a key/value head
 // are all its query heads of all tokens of all samples, so every prefix tile is
-// read once per 128 or 256 rows instead of once per sample.  A sample's own keys
-// meet its own rows only.  Both are cut into chunks of keys; a workgroup takes a chunk
-// against a tile of rows and leaves (m, l, o) -- reference point, sum and
-// unnormalised output of an online softmax, float32 -- and k_pfx_join adds the
-// chunks of a row.  One launch holds the prefix's workgroups and the samples'.
+// read once per tile of rows instead of once per sample: 128 or 256 rows in 16-bit
+// types, 64 of them in heads past 128 channels or where there are no more, 16 in
+// float32 or where there are no more.  A sample's own keys meet its own rows only.
+// Both are cut into chunks of keys; a workgroup takes a chunk against a tile of rows
+// and leaves (m, l, o) -- reference point, sum and unnormalised output of an online
+// softmax, float32 -- and k_pfx_join adds the chunks of a row.  One launch holds the
+// prefix's workgroups and the samples'.
 //
 // Two shapes of workgroup (NW waves, four or eight):
 //  * wide: 16 NQ rows per wave, the waves share K / V tiles staged in LDS, one
@@ -28,13 +30,25 @@
 // unrounded); out is rounded once.
 //
 // Bound, each on its own: narrow workgroups by memory (32 samples of 8 heads and up
-// to 2048 own tokens of 128 bf16 channels against a prefix of 16384: k_pfx 44 us for
-// 202 MB, 4.6 TB/s; the join 6); wide ones by the exponentials beside the products:
+// to 2048 own tokens of 128 bf16 channels against a prefix of 16384: k_pfx 43 us for
+// 219 MB read, 5.0 TB/s; the join 6); wide ones by the exponentials beside the products:
 // a score costs a quarter-rate exp2 and four more vector instructions, as much as
 // its matrix work at 128 channels and twice it at 64 (1100 TFLOP/s with eight waves
-// at 128 channels, 720 at 64; a large product of the library reaches 1183).
-// Counters of 64 samples against 65536 prefix keys (168 us under the profiler, 147
-// without): 540 MB read, matrix unit busy 30%, waves waiting for memory 35%.
+// at 128 channels, 720 at 64; a large product of the library reaches 1183).  Both
+// wait for the last workgroups where those in use are no whole rounds of the chip's
+// 512 places: about 700 in the call above.
+// Counters of 64 samples against 65536 prefix keys (161 us under the profiler, 147
+// without): 551 MB read, matrix unit busy 30%, waves waiting for memory 35%.
+//
+// The wide instances of 128 channels use all 256 registers and spill 135 (four
+// waves) or 151 (eight), those of 64 spill 12: in the loop over tiles of which some
+// row sees a part, which causal diagonals and windows take (8 samples of 128 tokens,
+// 16 heads of 128 channels, window 255 over 640, prefix 8192: 126 us, 60 by
+// operations).  float32, whose workgroups hold 16 rows, takes 2.6 times its floor for
+// one token (32 samples of 8 heads, up to 2048 own tokens of 128 channels, prefix
+// 16384: 213 us, 83 by bytes) and 1.9 times for a prompt (8 samples of 128 tokens, 16
+// heads of 64 channels, prefix 8192: 433 us, 230 by operations at the 154 TFLOP/s of
+// a large product).
 #include "na_launch.h"
 #include "na_lean.h"
 

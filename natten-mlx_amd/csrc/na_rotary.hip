@@ -13,11 +13,12 @@
 // first fill a table of (cos, sin) per token and pair in LDS, once for all heads,
 // then stream the rows of all heads of q and k past it in 16-byte chunks.
 //
-// The table and the products are float32, the result is rounded once.  Bound:
-// memory.  131072 tokens of 16 heads of 64 bf16 channels on three axes, whose
-// halves are no number of chunks: 124 us, reading and writing 268 MB each (4.3
-// TB/s; a large copy moves 4.9), 295 us where pairs are read and written singly
-// instead of through LDS.
+// The reduced angle, the table and the products are float32 (float32 rows are off by
+// 4.2e-8 of their norm, 3.3e-8 with sines of the float64 angle), the result is
+// rounded once.  Bound: memory.  131072 tokens of 16 heads of 64 bf16 channels on
+// three axes, whose halves are no number of chunks: 125 us, reading and writing 268
+// MB each (4.3 TB/s; a large copy moves 4.9), 295 us where pairs are read and written
+// singly instead of through LDS.
 #include "na_chunk.h"
 #include "na_launch.h"
 

@@ -487,6 +487,38 @@ typedef struct na_rotary_params {
 int na_rotary(const na_rotary_params *p, const void *q, const void *k,
               const void *positions, void *oq, void *ok, void *stream);
 
+/* ---- norm of queries and keys with their rotation ------------------------------ */
+#define NA_NORM_ROTARY_MAX_HEAD_DIM 256
+
+/*
+ * Each head's channels of q and of k normed as na_norm_fwd norms a row (weights
+ * wq, bq [D] for the heads of q, wk, bk for those of k) and then rotated as
+ * na_rotary rotates them, in one pass.  No counterpart in the reference.
+ */
+typedef struct na_norm_rotary_params {
+  na_rotary_params rotary; /* sizes, axes, positions, strides of q and k; inverse 0;
+                              head_dim at most NA_NORM_ROTARY_MAX_HEAD_DIM */
+  int32_t weight_dtype;    /* of the weights and their gradients: dtype or NA_F32 */
+  float eps;
+  int64_t dq_stride[3];    /* of the outputs' gradients, as q_stride; backward only */
+  int64_t dk_stride[3];
+} na_norm_rotary_params;
+
+/* Writes oq and ok, contiguous.  Each of the weights may be NULL (ones, zeros). */
+int na_norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *k,
+                       const void *positions, const void *wq, const void *bq,
+                       const void *wk, const void *bk, void *oq, void *ok, void *stream);
+/* Bytes that na_norm_rotary_bwd needs when a weight's gradient is wanted. */
+size_t na_norm_rotary_bwd_workspace_bytes(const na_norm_rotary_params *p);
+/* Gradients from gq and gk, those of the outputs: dq and dk (contiguous), dwq, dbq,
+ * dwk, dbk, each NULL where it is not wanted; heads or kv_heads 0 leaves out q or k.
+ * Deterministic: no atomics. */
+int na_norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void *k,
+                       const void *positions, const void *wq, const void *wk,
+                       const void *gq, const void *gk, void *dq, void *dk, void *dwq,
+                       void *dbq, void *dwk, void *dbk, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
 /* ---- attention behind a shared prefix (serving) ------------------------------ */
 #define NA_PREFIX_MAX_HEAD_DIM 256
 

@@ -881,15 +881,18 @@ int na_norm_bwd(const na_norm_params *p, const void *x, const void *w, const voi
   return launch_status("na_norm_bwd");
 }
 
-int na_rotary(const na_rotary_params *p, const void *q, const void *k, const void *positions,
-              void *oq, void *ok, void *stream) {
+namespace {
+
+// count: the tokens
+int check_rotary(const na_rotary_params *p, int64_t *count) {
   if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
   if (p->dtype != NA_F32 && p->dtype != NA_F16 && p->dtype != NA_BF16)
     return fail(NA_ERR_INVALID, "unknown dtype %d", p->dtype);
   if (p->batch < 0 || p->heads < 0 || p->kv_heads < 0 || p->head_dim < 1)
     return fail(NA_ERR_INVALID, "batch/heads/kv_heads/head_dim out of range (got %lld/%d/%d/%d)",
                 (long long)p->batch, p->heads, p->kv_heads, p->head_dim);
-  int64_t tokens = p->batch;
+  int64_t &tokens = *count;
+  tokens = p->batch;
   for (int a = 0; a < 3; ++a) {
     if (p->extent[a] < 0) return fail(NA_ERR_INVALID, "extent[%d] is negative", a);
     if (p->extent[a] > 0 && tokens > (((int64_t)1 << 31) - 1) / p->extent[a])
@@ -917,6 +920,16 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
   if (p->head_dim > kMaxHeadDim || (int64_t)p->heads + p->kv_heads >= ((int64_t)1 << 20))
     return fail(NA_ERR_UNSUPPORTED, "rotary takes up to %d channels and 2^20 heads, got %d and %lld",
                 kMaxHeadDim, p->head_dim, (long long)p->heads + p->kv_heads);
+  return NA_OK;
+}
+
+}  // namespace
+
+int na_rotary(const na_rotary_params *p, const void *q, const void *k, const void *positions,
+              void *oq, void *ok, void *stream) {
+  int64_t tokens;
+  const int rc = check_rotary(p, &tokens);
+  if (rc != NA_OK) return rc;
   if (tokens == 0 || p->heads + p->kv_heads == 0) return NA_OK;
   if ((p->heads > 0 && (q == nullptr || oq == nullptr)) ||
       (p->kv_heads > 0 && (k == nullptr || ok == nullptr)) ||
@@ -926,6 +939,73 @@ int na_rotary(const na_rotary_params *p, const void *q, const void *k, const voi
     return fail(NA_ERR_UNSUPPORTED, "%lld tokens of %lld heads are too many for one launch",
                 (long long)tokens, (long long)p->heads + p->kv_heads);
   return launch_status("na_rotary");
+}
+
+namespace {
+
+int check_norm_rotary(const na_norm_rotary_params *p, int64_t *tokens) {
+  if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
+  const na_rotary_params &r = p->rotary;
+  const int rc = check_rotary(&r, tokens);
+  if (rc != NA_OK) return rc;
+  if (r.inverse != 0) return fail(NA_ERR_INVALID, "the rotation of norm_rotary is not inverse");
+  if (r.head_dim > NA_NORM_ROTARY_MAX_HEAD_DIM)
+    return fail(NA_ERR_UNSUPPORTED, "norm_rotary takes up to %d channels, got %d",
+                NA_NORM_ROTARY_MAX_HEAD_DIM, r.head_dim);
+  if (p->weight_dtype != r.dtype && p->weight_dtype != NA_F32)
+    return fail(NA_ERR_INVALID, "weight_dtype must be dtype or NA_F32, got %d", p->weight_dtype);
+  if (!(p->eps >= 0.f) || p->eps > 3e38f)
+    return fail(NA_ERR_INVALID, "eps must be >= 0 and finite, got %g", (double)p->eps);
+  return NA_OK;
+}
+
+}  // namespace
+
+int na_norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *k,
+                       const void *positions, const void *wq, const void *bq, const void *wk,
+                       const void *bk, void *oq, void *ok, void *stream) {
+  int64_t tokens;
+  const int rc = check_norm_rotary(p, &tokens);
+  if (rc != NA_OK) return rc;
+  const na_rotary_params &r = p->rotary;
+  if (tokens == 0 || r.heads + r.kv_heads == 0) return NA_OK;
+  if ((r.heads > 0 && (q == nullptr || oq == nullptr)) ||
+      (r.kv_heads > 0 && (k == nullptr || ok == nullptr)) ||
+      (r.pos_type != NA_POS_GRID && positions == nullptr))
+    return fail(NA_ERR_INVALID, "q/k/positions and their outputs must be non-NULL");
+  if (!na::norm_rotary_fwd(p, q, k, positions, wq, bq, wk, bk, oq, ok, as_stream(stream)))
+    return fail(NA_ERR_UNSUPPORTED, "%lld tokens of %lld heads are too many for one launch",
+                (long long)tokens, (long long)r.heads + r.kv_heads);
+  return launch_status("na_norm_rotary_fwd");
+}
+
+size_t na_norm_rotary_bwd_workspace_bytes(const na_norm_rotary_params *p) {
+  int64_t tokens;
+  if (check_norm_rotary(p, &tokens) != NA_OK || p->rotary.heads + p->rotary.kv_heads == 0) return 0;
+  return align256(na::norm_rotary_workspace(p));
+}
+
+int na_norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void *k,
+                       const void *positions, const void *wq, const void *wk, const void *gq,
+                       const void *gk, void *dq, void *dk, void *dwq, void *dbq, void *dwk,
+                       void *dbk, void *workspace, size_t workspace_bytes, void *stream) {
+  int64_t tokens;
+  const int rc = check_norm_rotary(p, &tokens);
+  if (rc != NA_OK) return rc;
+  const na_rotary_params &r = p->rotary;
+  const bool sums = dwq != nullptr || dbq != nullptr || dwk != nullptr || dbk != nullptr;
+  if (r.heads + r.kv_heads == 0 || (dq == nullptr && dk == nullptr && !sums)) return NA_OK;
+  if (tokens > 0 && ((r.heads > 0 && (q == nullptr || gq == nullptr)) ||
+                     (r.kv_heads > 0 && (k == nullptr || gk == nullptr)) ||
+                     (r.pos_type != NA_POS_GRID && positions == nullptr)))
+    return fail(NA_ERR_INVALID, "q/k/positions and the outputs' gradients must be non-NULL");
+  const size_t need = sums ? align256(na::norm_rotary_workspace(p)) : 0;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(NA_ERR_WORKSPACE, "na_norm_rotary_bwd needs a %zu-byte workspace (got %zu)", need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  na::norm_rotary_bwd(p, q, k, positions, wq, wk, gq, gk, dq, dk, dwq, dbq, dwk, dbk, workspace,
+                      as_stream(stream));
+  return launch_status("na_norm_rotary_bwd");
 }
 
 namespace {

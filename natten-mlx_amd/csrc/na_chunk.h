@@ -1,6 +1,6 @@
 // na_chunk.h — 16-byte chunks of a row at any alignment of its elements, with a
-// bounded last chunk: the kernels that stream rows of any width (na_norm.hip,
-// na_rotary.hip).
+// bounded last chunk, and sums over a group of lanes: the kernels that stream rows of
+// any width (na_norm.hip, na_rotary.hip, na_norm_rotary.hip).
 #pragma once
 
 #include "na_common.h"
@@ -80,6 +80,28 @@ __device__ __forceinline__ void Chunk<T>::store(T *p, const float *x, int n) {
     for (int e = 0; e < N; ++e)
       if (e < n) reinterpret_cast<H *>(p)[e] = (H)x[e];
   }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over an aligned group of 2^lg lanes (wave-uniform lg), in every lane.
+__device__ __forceinline__ float lanes_sum(float x, int lg) {
+  if (lg > 0) x = dpp_add<0xB1>(x);   // lane ^ 1
+  if (lg > 1) x = dpp_add<0x4E>(x);   // lane ^ 2
+  if (lg > 2) x = dpp_add<0x141>(x);  // mirror within 8 lanes
+  if (lg > 3) x = dpp_add<0x140>(x);  // mirror within 16 lanes
+  if (lg > 4) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  if (lg > 5) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  return x;
 }
 
 }  // namespace

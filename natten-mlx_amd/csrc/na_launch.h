@@ -245,6 +245,20 @@ constexpr int kRotBlocks = 1024;  // workgroups that fill the chip
 bool rotary(const na_rotary_params *p, const void *q, const void *k, const void *pos, void *oq,
             void *ok, hipStream_t st);
 
+// Layer norm of each head of q and k and their rotary positions in one pass
+// (na_norm_rotary.hip).  Forward: false, and nothing launched, where they are more
+// than a launch takes.  Backward: heads or kv_heads 0 leaves that part out; dq and dk
+// may be null (not wanted), the weights' gradients each too, or they are written
+// from the partial sums in `workspace`.
+bool norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *k, const void *pos,
+                     const void *wq, const void *bq, const void *wk, const void *bk, void *oq,
+                     void *ok, hipStream_t st);
+size_t norm_rotary_workspace(const na_norm_rotary_params *p);
+void norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void *k, const void *pos,
+                     const void *wq, const void *wk, const void *gq, const void *gk, void *dq,
+                     void *dk, void *dwq, void *dbq, void *dwk, void *dbk, void *workspace,
+                     hipStream_t st);
+
 // Attention against a shared prefix and own cached tokens (na_prefix.hip).
 constexpr int kPfxItems = 512;  // workgroups that the chip holds at once
 bool prefix_fits(const na_prefix_params *p, size_t *workspace_bytes);  // false: too large

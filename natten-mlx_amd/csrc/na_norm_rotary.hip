@@ -1,0 +1,516 @@
+// na_norm_rotary.hip — layer norm of each head of queries and keys and their rotary
+// positions in one pass, forward and backward, with the gradients of the norms'
+// weights and biases.
+//
+//   xh = (x - mean x) rstd, rstd = 1 / sqrt(mean (x - mean x)^2 + eps),
+//   y = R (xh w + b), R the rotation of the row's token (na_rotary.hip);
+//   g' = R^T g, gw = g' w, dx = rstd (gw - mean gw - xh mean(gw xh)),
+//   dw = sum over rows of g' xh, db = sum over rows of g',
+// one w and b for the heads of q, one for those of k.
+//
+// A group of 1 to 64 lanes takes a row, which stays in registers from its load to
+// its store: lanes hold the chunks that rotate together (two half an axis apart, or
+// one of adjacent pairs), so the rotation needs no other lane; where half an axis
+// is no number of chunks, each lane holds one chunk and takes the partners from a
+// copy of the wave's rows in LDS, laid out by element and lane, which no two banks
+// share.  A workgroup takes a run of tokens and fills the run's table of (cos, sin)
+// once for all heads, from float64 angles as na_rotary.hip does.
+//
+// The backward computes a row's mean and deviation again, which costs two sums over
+// registers where kept statistics would cost 8 bytes a row each way.  Its workgroups
+// take the rows of q or those of k (one pair of column sums in registers) over runs
+// of tokens; each leaves one row of partial sums, added in a fixed order by
+// k_nr_wsum, so results do not depend on the run.
+//
+// Sums are float32; y, dx, dw and db are rounded once.  Bound: memory.
+#include "na_rotary.h"
+
+namespace na {
+namespace {
+
+constexpr int kNrBlocks = 1024;  // most workgroups of a backward: four on a CU
+
+struct NrProb {
+  RotProb R;  // per_block: tokens of a run; backward: of q's, qs / ks the rows of x
+  int32_t lgG, wide;      // lanes per row; weights are float32
+  int32_t per_k, bq, bk;  // backward: tokens of a run of k, workgroups of q and of k
+  float eps, inv_d;
+  FastDiv fH, fHk;
+  int64_t gqs[3], gks[3];
+};
+
+// The lane's place in a row: first channels and channels left of its chunks.
+template <typename T, int MODE>
+struct NrLane {
+  static constexpr int N = Chunk<T>::N, NT = MODE == kRotHalves ? 2 : 1;
+  int c[NT], n[NT];
+  int p0;     // entry of the table of its first channel (halves, adjacent: pair)
+  bool turn;  // halves: its channels are rotated
+  __device__ __forceinline__ NrLane(const RotProb &P, int j) {
+    int c0 = j * N, c1 = P.D;
+    p0 = MODE == kRotAdjacent ? c0 / 2 : c0;
+    turn = false;
+    if (MODE == kRotHalves) {
+      turn = c0 < P.pairs;
+      const int a = rot_axis(P, c0);
+      c0 = turn ? p0 + P.first[a] : 2 * p0;
+      c1 = turn ? c0 + P.first[a + 1] - P.first[a] : c0 + N;
+    }
+    const bool live = j < P.upr;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int at = t == 0 ? c0 : c1;
+      n[t] = live ? max(P.D - at, 0) : 0;
+      c[t] = n[t] > 0 ? at : 0;
+    }
+  }
+};
+
+// The lane's partners in the wave's copy of its rows: channel c of the row whose
+// first lane is `base` lies at (c % N) * 64 + base + c / N.
+template <int N>
+struct NrPartner {
+  int16_t at[N];
+  __device__ __forceinline__ NrPartner(const RotProb &P, int c0, int base) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int ch = c0 + e, a = rot_axis(P, ch / 2);
+      const int half = P.first[a + 1] - P.first[a];
+      int o = ch - 2 * P.first[a] < half ? ch + half : ch - half;
+      o = ch < 2 * P.pairs ? o : ch;
+      at[e] = (int16_t)(o % N * 64 + base + o / N);
+    }
+  }
+};
+
+// x turned by the table's row `cs` of its token.
+template <typename T, int MODE, int NT, int N>
+__device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> &L,
+                                        const NrPartner<N> &other, float *rows, const float2 *cs,
+                                        float (&x)[NT][N]) {
+  if constexpr (MODE == kRotHalves) {
+    if (!L.turn) return;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float2 z = cs[L.p0 + e];
+      const float u = x[0][e], v = x[1][e];
+      x[0][e] = u * z.x - v * z.y;
+      x[1][e] = fmaf(v, z.x, u * z.y);
+    }
+  } else if constexpr (MODE == kRotAdjacent) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2)
+      if (L.p0 + e / 2 < P.pairs) {
+        const float2 z = cs[L.p0 + e / 2];
+        const float u = x[0][e], v = x[0][e + 1];
+        x[0][e] = u * z.x - v * z.y;
+        x[0][e + 1] = fmaf(v, z.x, u * z.y);
+      }
+  } else {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int e = 0; e < N; ++e) rows[e * 64 + lane] = x[0][e];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (L.p0 + e < 2 * P.pairs) {
+        const float2 z = cs[L.p0 + e];
+        x[0][e] = fmaf(x[0][e], z.x, rows[other.at[e]] * z.y);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // the next row's copy comes behind these reads
+  }
+}
+
+// A weight vector's values at the lane's channels.
+template <typename T, int MODE, int NT, int N>
+__device__ __forceinline__ void nr_weights(const NrLane<T, MODE> &L, const void *w, int wide,
+                                           float none, float (&x)[NT][N]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[t][e] = none;
+      if (w != nullptr && e < L.n[t])
+        x[t][e] = wide ? static_cast<const float *>(w)[L.c[t] + e]
+                       : to_f32(static_cast<const T *>(w)[L.c[t] + e]);
+    }
+}
+
+// The row less its mean in place; 1 / std.
+template <int NT, int N>
+__device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT], int D, int lgG,
+                                           float inv_d, float eps) {
+  float s = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += x[t][e];  // (zeros behind the last channel)
+  const float mean = lanes_sum(s, lgG) / (float)D;
+  s = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[t][e] -= mean;
+      s = fmaf(e < n[t] ? x[t][e] : 0.f, x[t][e], s);
+    }
+  return 1.f / sqrtf(fmaf(lanes_sum(s, lgG), inv_d, eps));
+}
+
+// LDS: the table, the rates, staged: the waves' copies of their rows.
+template <typename T, int MODE>
+struct NrSmem {
+  float2 *cs;
+  double *rate;
+  float *rows;
+  __device__ __forceinline__ NrSmem(char *smem, const RotProb &P, int per) {
+    cs = reinterpret_cast<float2 *>(smem);
+    rate = reinterpret_cast<double *>(cs + per * P.pairs * (MODE == kRotStaged ? 2 : 1));
+    rows = reinterpret_cast<float *>(rate + rot_rates(P.pairs)) +
+           (threadIdx.x >> 6) * (64 * Chunk<T>::N);
+  }
+};
+template <typename T>
+size_t nr_lds(const RotProb &P, int per, RotMode mode) {
+  return sizeof(float2) * per * P.pairs * (mode == kRotStaged ? 2 : 1) +
+         sizeof(double) * rot_rates(P.pairs) +
+         (mode == kRotStaged ? sizeof(float) * kRotThreads * Chunk<T>::N : 0);
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRotThreads)
+    k_nr_fwd(NrProb Q, const T *__restrict__ q, const T *__restrict__ k,
+             const void *__restrict__ pos, const void *__restrict__ wq, const void *__restrict__ bq,
+             const void *__restrict__ wk, const void *__restrict__ bk, T *__restrict__ oq,
+             T *__restrict__ ok) {
+  typedef Chunk<T> K;
+  typedef NrLane<T, MODE> Lane;
+  constexpr int N = K::N, NT = Lane::NT;
+  extern __shared__ __align__(16) char smem[];
+  const RotProb &P = Q.R;
+  const NrSmem<T, MODE> S(smem, P, P.per_block);
+  const int tid = threadIdx.x, G = 1 << Q.lgG;
+  const int t0 = blockIdx.x * P.per_block, nt = min(P.per_block, P.tokens - t0);
+  const int h0 = blockIdx.y * P.heads_per, nh = min(P.heads_per, P.H + P.Hk - h0);
+  const Lane L(P, tid & (G - 1));
+  const NrPartner<N> other(P, L.p0, tid & 63 & ~(G - 1));
+  rot_rate(P, S.rate);
+  __syncthreads();
+  rot_table<MODE == kRotStaged>(P, pos, S.rate, t0, nt, S.cs);
+  __syncthreads();
+  const int per_step = kRotThreads >> Q.lgG;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    // heads [ha, ha + hn) of q and k taken together; more than one token: all of them
+    const int ha = part == 0 ? h0 : max(h0, P.H);
+    const int hn = (part == 0 ? min(h0 + nh, P.H) : h0 + nh) - ha;
+    if (hn <= 0) continue;
+    float w[NT][N], b[NT][N];
+    nr_weights(L, part == 0 ? wq : wk, Q.wide, 1.f, w);
+    nr_weights(L, part == 0 ? bq : bk, Q.wide, 0.f, b);
+    const int rows = nt * hn;
+    auto place = [&](int r, int &t, int &h) {
+      r = min(r, rows - 1);
+      t = nt == 1 ? 0 : (int)fdiv((uint32_t)r, part == 0 ? Q.fH : Q.fHk);
+      h = ha + r - t * hn;
+    };
+    typename K::raw next[NT];
+    auto fetch = [&](int r) {
+      int t, h;
+      place(r, t, h);
+      const RotRow<T> at(P, q, k, oq, ok, (uint32_t)(t0 + t), h);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) next[i] = K::load(at.src + L.c[i], L.n[i]);
+    };
+    int r = tid >> Q.lgG;
+    fetch(r);
+    for (int r0 = 0; r0 < rows; r0 += per_step, r += per_step) {  // the same steps for every lane
+      float x[NT][N];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[i][e] = K::get(next[i], e);
+      if (r0 + per_step < rows) fetch(r + per_step);
+      const float rstd = nr_center(x, L.n, P.D, Q.lgG, Q.inv_d, Q.eps);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[i][e] = fmaf(x[i][e] * rstd, w[i][e], b[i][e]);
+      int t, h;
+      place(r, t, h);
+      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + t * P.pairs * (MODE == kRotStaged ? 2 : 1), x);
+      if (r >= rows) continue;
+      const RotRow<T> at(P, q, k, oq, ok, (uint32_t)(t0 + t), h);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (L.n[i] > 0) K::store(at.dst + L.c[i], x[i], L.n[i]);
+    }
+  }
+}
+
+struct NrGrads {
+  const void *q, *k, *wq, *wk, *gq, *gk;
+  void *dq, *dk;
+  float *part;  // [bq + bk][2][D], or null: no sums wanted
+};
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRotThreads)
+    k_nr_bwd(NrProb Q, NrGrads A, const void *__restrict__ pos) {
+  typedef Chunk<T> K;
+  typedef NrLane<T, MODE> Lane;
+  constexpr int N = K::N, NT = Lane::NT;
+  extern __shared__ __align__(16) char smem[];
+  const RotProb &P = Q.R;
+  const bool isq = (int)blockIdx.x < Q.bq;
+  const int per = isq ? P.per_block : Q.per_k, heads = isq ? P.H : P.Hk;
+  const int block = isq ? blockIdx.x : blockIdx.x - Q.bq, blocks = isq ? Q.bq : Q.bk;
+  const NrSmem<T, MODE> S(smem, P, per);
+  const int tid = threadIdx.x, G = 1 << Q.lgG;
+  const Lane L(P, tid & (G - 1));
+  const NrPartner<N> other(P, L.p0, tid & 63 & ~(G - 1));
+  const T *const x = static_cast<const T *>(isq ? A.q : A.k);
+  const T *const g = static_cast<const T *>(isq ? A.gq : A.gk);
+  T *const dx = static_cast<T *>(isq ? A.dq : A.dk);
+  const int64_t *const xs = isq ? P.qs : P.ks, *const gs = isq ? Q.gqs : Q.gks;
+  float w[NT][N];
+  nr_weights(L, isq ? A.wq : A.wk, Q.wide, 1.f, w);
+  float aw[NT][N], ab[NT][N];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) aw[i][e] = ab[i][e] = 0.f;
+  rot_rate(P, S.rate);
+  const int per_step = kRotThreads >> Q.lgG;
+  for (int64_t first = (int64_t)block * per; first < P.tokens; first += (int64_t)blocks * per) {
+    const int t0 = (int)first, nt = min(per, P.tokens - t0), rows = nt * heads;
+    auto place = [&](int r, int &t, int &h) {
+      r = min(r, rows - 1);
+      t = nt == 1 ? 0 : (int)fdiv((uint32_t)r, isq ? Q.fH : Q.fHk);
+      h = r - t * heads;
+    };
+    typename K::raw nx[NT], ng[NT];
+    auto fetch = [&](int r) {
+      int t, h;
+      place(r, t, h);
+      const uint32_t tok = (uint32_t)(t0 + t), b = fdiv(tok, P.fS), s = tok - b * P.fS.d;
+      const T *const px = x + b * xs[0] + s * xs[1] + h * xs[2];
+      const T *const pg = g + b * gs[0] + s * gs[1] + h * gs[2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        nx[i] = K::load(px + L.c[i], L.n[i]);
+        ng[i] = K::load(pg + L.c[i], r < rows ? L.n[i] : 0);  // rows past the last add nothing
+      }
+    };
+    int r = tid >> Q.lgG;
+    fetch(r);
+    __syncthreads();  // the rates are there; the run before is done with its table
+    rot_table<MODE == kRotStaged>(P, pos, S.rate, t0, nt, S.cs);
+    __syncthreads();
+    for (int r0 = 0; r0 < rows; r0 += per_step, r += per_step) {  // the same steps for every lane
+      float h[NT][N], d[NT][N];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          h[i][e] = K::get(nx[i], e);
+          d[i][e] = K::get(ng[i], e);
+        }
+      if (r0 + per_step < rows) fetch(r + per_step);
+      int t, hd;
+      place(r, t, hd);
+      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + t * P.pairs * (MODE == kRotStaged ? 2 : 1), d);
+      const float rstd = nr_center(h, L.n, P.D, Q.lgG, Q.inv_d, Q.eps);
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          h[i][e] *= rstd;
+          aw[i][e] = fmaf(d[i][e], h[i][e], aw[i][e]);
+          ab[i][e] += d[i][e];
+          d[i][e] *= w[i][e];
+          s0 += d[i][e];  // (zeros behind the last channel)
+          s1 = fmaf(d[i][e], h[i][e], s1);
+        }
+      if (dx == nullptr) continue;
+      s0 = lanes_sum(s0, Q.lgG) * Q.inv_d;
+      s1 = lanes_sum(s1, Q.lgG) * Q.inv_d;
+      if (r >= rows) continue;
+      T *const out = dx + ((int64_t)(t0 + t) * heads + hd) * P.D;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) d[i][e] = rstd * (d[i][e] - s0 - h[i][e] * s1);
+        if (L.n[i] > 0) K::store(out + L.c[i], d[i], L.n[i]);
+      }
+    }
+  }
+  if (A.part == nullptr) return;
+  // the wave's groups, then the workgroup's four waves
+  for (int off = G; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        aw[i][e] += __shfl_xor(aw[i][e], off, 64);
+        ab[i][e] += __shfl_xor(ab[i][e], off, 64);
+      }
+  __syncthreads();  // the table's LDS is free
+  float *const sums = reinterpret_cast<float *>(smem);  // [4][2][D]
+  if ((tid & 63) < G) {
+    float *const d = sums + (tid >> 6) * 2 * P.D;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < L.n[i]) {
+          d[L.c[i] + e] = aw[i][e];
+          d[P.D + L.c[i] + e] = ab[i][e];
+        }
+  }
+  __syncthreads();
+  for (int c = tid; c < 2 * P.D; c += kRotThreads)
+    A.part[(int64_t)blockIdx.x * 2 * P.D + c] =
+        (sums[c] + sums[2 * P.D + c]) + (sums[4 * P.D + c] + sums[6 * P.D + c]);
+}
+
+// Column sums of the partials of q's (blockIdx.y 0) or k's workgroups: 32 columns
+// per workgroup, 32 threads to a column, always added in the same order.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+    k_nr_wsum(const float *__restrict__ part, void *dwq, void *dbq, void *dwk, void *dbk, int D,
+              int bq, int bk, int wide) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x & 31, j = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + c, first = blockIdx.y == 0 ? 0 : bq;
+  const int n = blockIdx.y == 0 ? bq : bk;
+  float s = 0.f;
+  if (col < 2 * D) {
+#pragma unroll 8
+    for (int i = j; i < n; i += 32) s += part[(int64_t)(first + i) * 2 * D + col];
+  }
+  sums[j][c] = s;
+  __syncthreads();
+  s = sums[c][j];  // transposed: thread row j adds column j
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor(s, off, 32);
+  const int o = blockIdx.x * 32 + j;
+  if (c != 0 || o >= 2 * D) return;
+  void *const d = blockIdx.y == 0 ? (o < D ? dwq : dbq) : (o < D ? dwk : dbk);
+  if (d == nullptr) return;
+  const int at = o < D ? o : o - D;
+  if (wide) static_cast<float *>(d)[at] = s;
+  else static_cast<T *>(d)[at] = from_f32<T>(s);
+}
+
+NrProb nr_prob(const na_norm_rotary_params *p, RotMode *mode) {
+  NrProb Q{};
+  *mode = rot_prob(&p->rotary, Q.R);
+  Q.wide = p->weight_dtype == NA_F32;
+  Q.eps = p->eps;
+  Q.inv_d = 1.f / (float)Q.R.D;
+  while ((1 << Q.lgG) < Q.R.upr) ++Q.lgG;
+  Q.fH = make_fastdiv((uint32_t)std::max(Q.R.H, 1));
+  Q.fHk = make_fastdiv((uint32_t)std::max(Q.R.Hk, 1));
+  for (int i = 0; i < 3; ++i) {
+    Q.gqs[i] = p->dq_stride[i];
+    Q.gks[i] = p->dk_stride[i];
+  }
+  return Q;
+}
+
+// Tokens of a run: kRotUnits units per thread, as many as the table holds; fewer
+// where the runs would not be `blocks`.
+int nr_run(const RotProb &P, RotMode mode, int heads, int blocks) {
+  const int entries = P.pairs * (mode == kRotStaged ? 2 : 1);
+  const int64_t row_units = std::max<int64_t>((int64_t)heads * P.upr, 1);
+  int64_t per = std::max<int64_t>(1, kRotUnits * kRotThreads / row_units);
+  per = std::min<int64_t>(per, std::max(1, kRotTable / entries));
+  return (int)std::min<int64_t>(per, std::max<int64_t>(1, P.tokens / blocks));
+}
+
+// The backward's runs and workgroups, shared out by the heads of q and k.
+void nr_bwd_plan(NrProb &Q, RotMode mode) {
+  RotProb &P = Q.R;
+  auto part = [&](int heads, int32_t *per, int32_t *blocks) {
+    const int most = std::max(1, (int)((int64_t)kNrBlocks * heads / (P.H + P.Hk)));
+    *per = nr_run(P, mode, heads, most);
+    *blocks = heads == 0 ? 0 : (int)std::min<int64_t>(most, ((int64_t)P.tokens + *per - 1) / *per);
+  };
+  part(P.H, &P.per_block, &Q.bq);
+  part(P.Hk, &Q.per_k, &Q.bk);
+}
+
+template <typename F>
+void nr_by_type(int dtype, RotMode mode, F &&f) {
+  auto by_mode = [&](auto t) {
+    if (mode == kRotHalves) f(t, std::integral_constant<int, kRotHalves>{});
+    else if (mode == kRotAdjacent) f(t, std::integral_constant<int, kRotAdjacent>{});
+    else f(t, std::integral_constant<int, kRotStaged>{});
+  };
+  if (dtype == NA_F32) by_mode(float{});
+  else if (dtype == NA_F16) by_mode(f16_t{});
+  else by_mode(bf16_t{});
+}
+
+}  // namespace
+
+bool norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *k, const void *pos,
+                     const void *wq, const void *bq, const void *wk, const void *bk, void *oq,
+                     void *ok, hipStream_t st) {
+  RotMode mode;
+  NrProb Q = nr_prob(p, &mode);
+  RotProb &P = Q.R;
+  // the heads of a token are shared out where there are few tokens
+  const int heads = P.H + P.Hk;
+  P.per_block = nr_run(P, mode, heads, kRotBlocks);
+  P.heads_per = heads;
+  if (P.per_block == 1 && P.tokens < kRotBlocks)
+    P.heads_per = std::min(heads, kRotThreads >> Q.lgG);
+  const dim3 grid((unsigned)(((int64_t)P.tokens + P.per_block - 1) / P.per_block),
+                  (unsigned)((heads + P.heads_per - 1) / P.heads_per));
+  if (grid.x >= ((int64_t)1 << 32) / kRotThreads || grid.y > 65535) return false;  // a launch ends there
+  nr_by_type(p->rotary.dtype, mode, [&](auto t, auto m) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((k_nr_fwd<T, decltype(m)::value>), grid, dim3(kRotThreads),
+                       nr_lds<T>(P, P.per_block, mode), st, Q, (const T *)q, (const T *)k, pos, wq,
+                       bq, wk, bk, (T *)oq, (T *)ok);
+  });
+  return true;
+}
+
+size_t norm_rotary_workspace(const na_norm_rotary_params *p) {
+  RotMode mode;
+  NrProb Q = nr_prob(p, &mode);
+  nr_bwd_plan(Q, mode);
+  return sizeof(float) * 2 * (size_t)Q.R.D * (size_t)(Q.bq + Q.bk);
+}
+
+void norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void *k, const void *pos,
+                     const void *wq, const void *wk, const void *gq, const void *gk, void *dq,
+                     void *dk, void *dwq, void *dbq, void *dwk, void *dbk, void *workspace,
+                     hipStream_t st) {
+  RotMode mode;
+  NrProb Q = nr_prob(p, &mode);
+  Q.R.sign = -1.f;  // the gradients turn back
+  nr_bwd_plan(Q, mode);
+  const bool sums = dwq != nullptr || dbq != nullptr || dwk != nullptr || dbk != nullptr;
+  const NrGrads A{q, k, wq, wk, gq, gk, dq, dk, sums ? static_cast<float *>(workspace) : nullptr};
+  nr_by_type(p->rotary.dtype, mode, [&](auto t, auto m) {
+    using T = decltype(t);
+    const size_t lds = std::max(nr_lds<T>(Q.R, std::max(Q.R.per_block, Q.per_k), mode),
+                                sizeof(float) * 8 * Q.R.D);
+    if (Q.bq + Q.bk > 0)
+      hipLaunchKernelGGL((k_nr_bwd<T, decltype(m)::value>), dim3(Q.bq + Q.bk), dim3(kRotThreads), lds,
+                         st, Q, A, pos);
+    if (sums)  // (no rows: zeros)
+      hipLaunchKernelGGL((k_nr_wsum<T>), dim3((2 * Q.R.D + 31) / 32, 2), dim3(1024), 0, st, A.part,
+                         dwq, dbq, dwk, dbk, Q.R.D, Q.bq, Q.bk, Q.wide);
+  });
+}
+
+}  // namespace na

@@ -1,8 +1,8 @@
 // The differentiable ops as torch custom operators with their autograd nodes
 // in C++ over the C ABI of libnatten_amd.so: the fused op (natten_amd::na_fused),
 // the split ops (na_split_qk, na_split_av), the DiNAT ops (na_rpb_qk, na_rpb_av),
-// a layer's projections (na_linear), the layer norm (na_layer_norm) and rotary
-// positions (na_rotary).
+// a layer's projections (na_linear), the layer norm (na_layer_norm), rotary
+// positions (na_rotary) and both in one pass (na_norm_rotary).
 //
 // The reference's autograd layer (autograd/na1d.py:34-53, na2d.py:34-64,
 // na3d.py) wraps the fused forward / backward in an mx.custom_function; the
@@ -26,6 +26,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <array>
 #include <cstdint>
 #include <cstring>
 #include <vector>
@@ -833,11 +834,16 @@ at::Tensor token_view(const at::Tensor &t, int64_t *stride) {
   return t;
 }
 
+// A call's parameters, and its tensors as the kernels read them.
+struct RotaryCall {
+  na_rotary_params p{};
+  at::Tensor q, k, pos;
+};
+
 // q or k may be undefined; the shape rules restate the functional layer's for
 // direct callers of the operator.
-variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &pos,
-                             at::IntArrayRef dims, double theta, bool interleaved, bool inverse,
-                             int64_t stream) {
+RotaryCall rotary_call(const at::Tensor &q, const at::Tensor &k, const at::Tensor &pos,
+                       at::IntArrayRef dims, double theta, bool interleaved, bool inverse) {
   const at::Tensor &x = q.defined() ? q : k;
   const int64_t nd = x.dim();
   TORCH_CHECK(nd >= 4 && nd <= 6 &&
@@ -847,7 +853,8 @@ variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at:
               "natten_amd na_rotary: q and k [B, *spatial, heads, D] of one dtype, got ", x.sizes());
   TORCH_CHECK((int64_t)dims.size() >= 1 && dims.size() <= NA_ROTARY_MAX_AXES,
               "natten_amd na_rotary: 1 to 4 axes, got ", dims.size());
-  na_rotary_params p{};
+  RotaryCall r;
+  na_rotary_params &p = r.p;
   p.batch = x.size(0);
   for (int a = 0; a < 3; ++a) p.extent[a] = 1;
   for (const at::Tensor *t : {&q, &k})
@@ -866,7 +873,6 @@ variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at:
   p.interleaved = interleaved ? 1 : 0;
   p.inverse = inverse ? 1 : 0;
   p.theta = theta;
-  at::Tensor pc;
   if (pos.defined()) {
     const at::IntArrayRef lead = pos.sizes().slice(0, pos.dim() > 0 ? pos.dim() - 1 : 0);
     p.pos_batched = pos.dim() == nd - 1 ? 1 : 0;
@@ -882,23 +888,27 @@ variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at:
       default:
         TORCH_CHECK(false, "natten_amd na_rotary: positions are int32, int64, float32 or float64");
     }
-    pc = pos.contiguous();
   } else {
     TORCH_CHECK(p.n_axes == nd - 3, "natten_amd na_rotary: one axis_dims entry per spatial axis");
     p.pos_type = NA_POS_GRID;
   }
   check_devices(x, {&k, &pos});
   const c10::DeviceGuard guard(x.device());
-  at::Tensor qc, kc, oq, ok;
-  if (q.defined()) {
-    qc = token_view(q, p.q_stride);
-    oq = at::empty(q.sizes(), q.options());
-  }
-  if (k.defined()) {
-    kc = token_view(k, p.k_stride);
-    ok = at::empty(k.sizes(), k.options());
-  }
-  check_rc(na_rotary(&p, cptr(qc), cptr(kc), cptr(pc), mptr(oq), mptr(ok), as_stream(stream)),
+  if (q.defined()) r.q = token_view(q, p.q_stride);
+  if (k.defined()) r.k = token_view(k, p.k_stride);
+  if (pos.defined()) r.pos = pos.contiguous();
+  return r;
+}
+
+variable_list rotary_forward(const at::Tensor &q, const at::Tensor &k, const at::Tensor &pos,
+                             at::IntArrayRef dims, double theta, bool interleaved, bool inverse,
+                             int64_t stream) {
+  const RotaryCall r = rotary_call(q, k, pos, dims, theta, interleaved, inverse);
+  const c10::DeviceGuard guard((q.defined() ? q : k).device());
+  at::Tensor oq, ok;
+  if (q.defined()) oq = at::empty(q.sizes(), q.options());
+  if (k.defined()) ok = at::empty(k.sizes(), k.options());
+  check_rc(na_rotary(&r.p, cptr(r.q), cptr(r.k), cptr(r.pos), mptr(oq), mptr(ok), as_stream(stream)),
            "na_rotary");
   return {oq, ok};
 }
@@ -960,6 +970,130 @@ std::tuple<at::Tensor, at::Tensor> na_rotary_op(const at::Tensor &q,
   variable_list r =
       Rotary::apply_rotary(q, k.value_or(at::Tensor()), positions.value_or(at::Tensor()),
                            axis_dims.vec(), theta, interleaved, inverse, stream);
+  if (!r[1].defined()) r[1] = at::empty({0}, q.options());  // no key: an empty tensor
+  return {r[0], r[1]};
+}
+
+// ---- norm of queries and keys with their rotation (norm_rotary.py) -----------
+
+// The norms' weights and biases {wq, bq, wk, bk}, each of them possibly undefined.
+typedef std::array<at::Tensor, 4> NormWeights;
+
+na_norm_rotary_params norm_rotary_params(const RotaryCall &r, const NormWeights &w, double eps) {
+  na_norm_rotary_params p{};
+  p.rotary = r.p;
+  p.weight_dtype = r.p.dtype;
+  p.eps = (float)eps;
+  for (const at::Tensor &t : w)
+    if (t.defined()) p.weight_dtype = dtype_code(t.scalar_type());
+  return p;
+}
+
+variable_list norm_rotary_forward(const at::Tensor &q, const at::Tensor &k, const NormWeights &w,
+                                  const at::Tensor &pos, at::IntArrayRef dims, double theta,
+                                  bool interleaved, double eps, int64_t stream) {
+  at::ScalarType type = at::ScalarType::Undefined;
+  for (const at::Tensor &t : w) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == q.size(-1) &&
+                    (type == at::ScalarType::Undefined || t.scalar_type() == type),
+                "natten_amd na_norm_rotary: weights [D] of one dtype, got ", t.sizes());
+    type = t.scalar_type();
+  }
+  TORCH_CHECK(k.defined() || (!w[2].defined() && !w[3].defined()),
+              "natten_amd na_norm_rotary: weights of a missing key");
+  check_devices(q, {&k, &w[0], &w[1], &w[2], &w[3]});
+  const RotaryCall r = rotary_call(q, k, pos, dims, theta, interleaved, false);
+  const c10::DeviceGuard guard(q.device());
+  const na_norm_rotary_params p = norm_rotary_params(r, w, eps);
+  at::Tensor oq = at::empty(q.sizes(), q.options()), ok;
+  if (k.defined()) ok = at::empty(k.sizes(), k.options());
+  const at::Tensor wq = contig(w[0]), bq = contig(w[1]), wk = contig(w[2]), bk = contig(w[3]);
+  check_rc(na_norm_rotary_fwd(&p, cptr(r.q), cptr(r.k), cptr(r.pos), cptr(wq), cptr(bq), cptr(wk),
+                              cptr(bk), mptr(oq), mptr(ok), as_stream(stream)),
+           "na_norm_rotary_fwd");
+  return {oq, ok};
+}
+
+struct NormRotary : public torch::autograd::Function<NormRotary> {
+  static variable_list forward(AutogradContext *ctx, at::Tensor q, std::optional<at::Tensor> k,
+                               std::optional<at::Tensor> wq, std::optional<at::Tensor> bq,
+                               std::optional<at::Tensor> wk, std::optional<at::Tensor> bk,
+                               std::optional<at::Tensor> pos, std::vector<int64_t> dims,
+                               double theta, bool interleaved, double eps, int64_t stream) {
+    const at::Tensor none;
+    const NormWeights w{wq.value_or(none), bq.value_or(none), wk.value_or(none), bk.value_or(none)};
+    ctx->save_for_backward({q, k.value_or(none), w[0], w[1], w[2], w[3], pos.value_or(none)});
+    std::vector<int64_t> m{stream, interleaved ? 1 : 0};
+    m.insert(m.end(), dims.begin(), dims.end());
+    ctx->saved_data["p"] = m;
+    ctx->saved_data["theta"] = theta;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    variable_list out = norm_rotary_forward(q, k.value_or(none), w, pos.value_or(none), dims, theta,
+                                            interleaved, eps, stream);
+    if (!out[1].defined()) out.pop_back();
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "natten_amd norm_rotary: the backward is not differentiable");
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> m = ctx->saved_data["p"].toIntVector();
+    const std::vector<int64_t> dims(m.begin() + 2, m.end());
+    at::Tensor gq = grads[0], gk = s[1].defined() ? grads[1] : at::Tensor();
+    // the inputs whose gradients are wanted and follow from those that came
+    at::Tensor d[6];
+    bool any = false, sums = false;
+    for (int i = 0, present = 0; i < 6; ++i) {
+      if (!s[i].defined()) continue;
+      const bool ofq = i == 0 || i == 2 || i == 3;
+      if (ctx->needs_input_grad(present++) && (ofq ? gq : gk).defined()) {
+        d[i] = at::empty(s[i].sizes(), s[i].options());
+        any = true;
+        sums = sums || i >= 2;
+      }
+    }
+    variable_list out(12);
+    if (any) {
+      const c10::DeviceGuard guard(s[0].device());
+      const RotaryCall r =
+          rotary_call(gq.defined() ? s[0] : at::Tensor(), gk.defined() ? s[1] : at::Tensor(), s[6],
+                      dims, ctx->saved_data["theta"].toDouble(), m[1] != 0, false);
+      na_norm_rotary_params p =
+          norm_rotary_params(r, {s[2], s[3], s[4], s[5]}, ctx->saved_data["eps"].toDouble());
+      if (gq.defined()) gq = token_view(to_type(gq, s[0].scalar_type()), p.dq_stride);
+      if (gk.defined()) gk = token_view(to_type(gk, s[0].scalar_type()), p.dk_stride);
+      const size_t bytes = sums ? na_norm_rotary_bwd_workspace_bytes(&p) : 0;
+      at::Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes}, s[0].options().dtype(at::kByte));
+      const at::Tensor wq = contig(s[2]), wk = contig(s[4]);
+      check_rc(na_norm_rotary_bwd(&p, cptr(r.q), cptr(r.k), cptr(r.pos), cptr(wq), cptr(wk),
+                                  cptr(gq), cptr(gk), mptr(d[0]), mptr(d[1]), mptr(d[2]),
+                                  mptr(d[3]), mptr(d[4]), mptr(d[5]), mptr(ws), bytes,
+                                  as_stream(m[0])),
+               "na_norm_rotary_bwd");
+      for (int i = 0; i < 6; ++i) out[i] = d[i];
+    }
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> na_norm_rotary(
+    const at::Tensor &q, const std::optional<at::Tensor> &k, const std::optional<at::Tensor> &wq,
+    const std::optional<at::Tensor> &bq, const std::optional<at::Tensor> &wk,
+    const std::optional<at::Tensor> &bk, const std::optional<at::Tensor> &positions,
+    at::IntArrayRef axis_dims, double theta, bool interleaved, double eps, int64_t stream) {
+  const at::Tensor none;
+  const at::Tensor kt = k.value_or(none);
+  const NormWeights w{wq.value_or(none), bq.value_or(none), wk.value_or(none), bk.value_or(none)};
+  variable_list r =
+      wants_grad({&q, &kt, &w[0], &w[1], &w[2], &w[3]})
+          ? NormRotary::apply(q, k, wq, bq, wk, bk, positions, axis_dims.vec(), theta, interleaved,
+                              eps, stream)
+          : norm_rotary_forward(q, kt, w, positions.value_or(none), axis_dims, theta, interleaved,
+                                eps, stream);
+  if (r.size() < 2) r.emplace_back();
   if (!r[1].defined()) r[1] = at::empty({0}, q.options());  // no key: an empty tensor
   return {r[0], r[1]};
 }
@@ -1071,6 +1205,10 @@ TORCH_LIBRARY(natten_amd, m) {
       "na_rotary(Tensor q, Tensor? k, Tensor? positions, int[] axis_dims, float theta, "
       "bool interleaved, bool inverse, int stream) -> (Tensor, Tensor)");
   m.def(
+      "na_norm_rotary(Tensor q, Tensor? k, Tensor? q_weight, Tensor? q_bias, Tensor? k_weight, "
+      "Tensor? k_bias, Tensor? positions, int[] axis_dims, float theta, bool interleaved, "
+      "float eps, int stream) -> (Tensor, Tensor)");
+  m.def(
       "na_prefix(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor? k, Tensor? v, "
       "Tensor? seq_lens, int window, float scale, bool want_lse, int stream) -> (Tensor, Tensor)");
 }
@@ -1085,5 +1223,6 @@ TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
   m.impl("na_fused_qkv", na_fused_qkv);
   m.impl("na_layer_norm", na_layer_norm);
   m.impl("na_rotary", na_rotary_op);
+  m.impl("na_norm_rotary", na_norm_rotary);
   m.impl("na_prefix", na_prefix);
 }

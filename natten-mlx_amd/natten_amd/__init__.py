@@ -27,6 +27,7 @@ from .functional import (
 )
 from .merge import merge_attentions
 from .norm import layer_norm
+from .norm_rotary import norm_rotary
 from .prefix import prefix_attention
 from .rotary import rotary, rotary_axis_dims
 from .support_matrix import get_support_matrix
@@ -68,7 +69,7 @@ def __getattr__(name):
 __all__ = [
     "__version__", "na1d", "na1d_varlen", "na1d_varlen_gqa", "na2d", "na2d_varlen", "na1d_qk",
     "na1d_av", "na2d_qk", "na2d_av", "na3d", "na3d_varlen", "na3d_qk", "na3d_av",
-    "merge_attentions", "layer_norm", "rotary", "rotary_axis_dims", "prefix_attention",
+    "merge_attentions", "layer_norm", "rotary", "rotary_axis_dims", "norm_rotary", "prefix_attention",
     "NeighborhoodAttention1D", "NeighborhoodAttention2D",
     "NeighborhoodAttention3D", "has_hip", "has_metal", "has_nanobind", "get_backend", "set_backend", "get_support_matrix",
 ]

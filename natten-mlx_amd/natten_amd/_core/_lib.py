@@ -164,6 +164,18 @@ class NaRotaryParams(ctypes.Structure):
     ]
 
 
+class NaNormRotaryParams(ctypes.Structure):
+    """Mirror of ``na_norm_rotary_params`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("rotary", NaRotaryParams),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("dq_stride", ctypes.c_int64 * 3),
+        ("dk_stride", ctypes.c_int64 * 3),
+    ]
+
+
 class NaPrefixParams(ctypes.Structure):
     """Mirror of ``na_prefix_params`` (include/natten_amd.h)."""
 
@@ -188,6 +200,7 @@ class NaPrefixParams(ctypes.Structure):
 
 
 PREFIX_MAX_HEAD_DIM = 256
+NORM_ROTARY_MAX_HEAD_DIM = 256
 MAX_HEAD_DIM = 1024
 ROTARY_MAX_AXES = 4
 ROTARY_MAX_CHANNELS = 512
@@ -199,6 +212,7 @@ _R = ctypes.POINTER(NaRpbParams)
 _M = ctypes.POINTER(NaMergeParams)
 _N = ctypes.POINTER(NaNormParams)
 _RO = ctypes.POINTER(NaRotaryParams)
+_NR = ctypes.POINTER(NaNormRotaryParams)
 _PF = ctypes.POINTER(NaPrefixParams)
 _PP = ctypes.POINTER(ctypes.c_void_p)  # host array of device pointers
 _V = ctypes.c_void_p
@@ -242,6 +256,9 @@ SIGNATURES = {
     "na_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_N]),
     "na_norm_bwd": (ctypes.c_int, [_N] + [_V] * 8 + [ctypes.c_size_t, _V]),
     "na_rotary": (ctypes.c_int, [_RO] + [_V] * 6),
+    "na_norm_rotary_fwd": (ctypes.c_int, [_NR] + [_V] * 10),
+    "na_norm_rotary_bwd_workspace_bytes": (ctypes.c_size_t, [_NR]),
+    "na_norm_rotary_bwd": (ctypes.c_int, [_NR] + [_V] * 14 + [ctypes.c_size_t, _V]),
     "na_prefix_workspace_bytes": (ctypes.c_size_t, [_PF]),
     "na_prefix_fwd": (ctypes.c_int, [_PF] + [_V] * 8 + [ctypes.c_size_t, _V]),
 }
@@ -291,7 +308,7 @@ def _load_fused_op() -> None:
                  "rpb_qk": ns.na_rpb_qk.default, "rpb_av": ns.na_rpb_av.default,
                  "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default,
                  "norm": ns.na_layer_norm.default, "rotary": ns.na_rotary.default,
-                 "prefix": ns.na_prefix.default}
+                 "norm_rotary": ns.na_norm_rotary.default, "prefix": ns.na_prefix.default}
 
 
 def fused_op():
@@ -309,9 +326,9 @@ _OP_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 def node_op(name: str, a: torch.Tensor, b: torch.Tensor):
     """The C++ operator of a split ("qk", "av") or DiNAT ("rpb_qk", "rpb_av")
     op, of a layer's projection ("linear") and packed attention
-    ("fused_qkv"), of the layer norm ("norm"), of rotary positions ("rotary") or of
-    attention behind a shared prefix ("prefix"), where it takes these tensors: built, and both of a supported dtype on
-    one HIP device.  None otherwise (the Python autograd Function then runs
+    ("fused_qkv"), of the layer norm ("norm"), of rotary positions ("rotary"), of both
+    in one pass ("norm_rotary") or of attention behind a shared prefix ("prefix"), where
+    it takes these tensors: built, and both of a supported dtype on one HIP device.  None otherwise (the Python autograd Function then runs
     the same kernels, or raises): under compilation, which can leave a Python
     Function to eager execution but not an operator without a fake kernel, while
     tracing, and inside a torch.func transform or a forward-mode level, which a

@@ -662,13 +662,9 @@ def norm_backward(x, w, b, dy, stats, eps, need):
 # ---------------------------------------------------------------------------
 # rotary positions (C ABI na_rotary)
 
-@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
-def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
-    """``(q, k)`` rotated by their tokens' positions; either may be None."""
-    dev = _require_device(q, k, positions)
-    q, k, positions = map(_c, (q, k, positions))
+def _rotary_params(p, q, k, positions, axis_dims, theta, interleaved, inverse):
+    """``p`` for contiguous q and k, either of them None."""
     x = k if q is None else q
-    p = _lib.NaRotaryParams()
     spatial = tuple(x.shape[1:-2])
     p.batch, p.head_dim, p.dtype = x.shape[0], x.shape[-1], _lib.dtype_code(x.dtype)
     p.heads, p.kv_heads = (0 if t is None else t.shape[-2] for t in (q, k))
@@ -683,12 +679,76 @@ def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
     for st, t in ((p.q_stride, q), (p.k_stride, k)):
         if t is not None:
             st[0], st[1], st[2] = t.numel() // max(t.shape[0], 1), t.shape[-2] * t.shape[-1], t.shape[-1]
+    return p
+
+
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
+def rotary(q, k, positions, axis_dims, theta, interleaved, inverse=False):
+    """``(q, k)`` rotated by their tokens' positions; either may be None."""
+    dev = _require_device(q, k, positions)
+    q, k, positions = map(_c, (q, k, positions))
+    x = k if q is None else q
+    p = _rotary_params(_lib.NaRotaryParams(), q, k, positions, axis_dims, theta, interleaved, inverse)
     oq, ok = (None if t is None else torch.empty_like(t) for t in (q, k))
     with torch.cuda.device(dev):
         _lib.check(_lib.load().na_rotary(p, _lib.ptr(q), _lib.ptr(k), _lib.ptr(positions),
                                          _lib.ptr(oq), _lib.ptr(ok), _lib.stream_of(x)),
                    "na_rotary")
     return oq, ok
+
+
+# ---------------------------------------------------------------------------
+# norm of queries and keys with their rotation (C ABI na_norm_rotary_fwd / _bwd)
+
+def _norm_rotary_params(q, k, weights, positions, args, eps):
+    p = _lib.NaNormRotaryParams()
+    _rotary_params(p.rotary, q, k, positions, *args, False)
+    have = [w for w in weights if w is not None]
+    p.weight_dtype = _lib.dtype_code(have[0].dtype) if have else p.rotary.dtype
+    p.eps = float(eps)
+    p.dq_stride, p.dk_stride = p.rotary.q_stride, p.rotary.k_stride
+    return p
+
+
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
+def norm_rotary_forward(q, k, wq, bq, wk, bk, positions, args, eps):
+    """``(q, k)``, normed and rotated; k may be None."""
+    dev = _require_device(q, k, wq, bq, wk, bk, positions)
+    q, k, wq, bq, wk, bk, positions = map(_c, (q, k, wq, bq, wk, bk, positions))
+    p = _norm_rotary_params(q, k, (wq, bq, wk, bk), positions, args, eps)
+    oq, ok = (None if t is None else torch.empty_like(t) for t in (q, k))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().na_norm_rotary_fwd(
+            p, *map(_lib.ptr, (q, k, positions, wq, bq, wk, bk, oq, ok)), _lib.stream_of(q)),
+            "na_norm_rotary_fwd")
+    return oq, ok
+
+
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
+def norm_rotary_backward(q, k, wq, bq, wk, bk, positions, args, eps, gq, gk, need):
+    """Gradients of ``norm_rotary_forward``'s tensors ``(q, k, wq, bq, wk, bk)``; those
+    not needed, or of a part whose output has no gradient, come back as None."""
+    if gq is None:
+        q = wq = bq = None
+    if gk is None:
+        k = wk = bk = None
+    ts = [t if n else None for t, n in zip((q, k, wq, bq, wk, bk), need)]
+    if all(t is None for t in ts):
+        return [None] * 6
+    dev = _require_device(q, k, wq, wk, positions, gq, gk)
+    q, k, wq, wk, positions = map(_c, (q, k, wq, wk, positions))
+    gq, gk = (None if g is None else _c(g.to(t.dtype)) for g, t in ((gq, q), (gk, k)))
+    p = _norm_rotary_params(q, k, (wq, bq, wk, bk), positions, args, eps)
+    grads = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in ts]
+    lib = _lib.load()
+    sums = any(g is not None for g in grads[2:])
+    nbytes = int(lib.na_norm_rotary_bwd_workspace_bytes(p)) if sums else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.na_norm_rotary_bwd(
+            p, *map(_lib.ptr, (q, k, positions, wq, wk, gq, gk, *grads, ws)), nbytes,
+            _lib.stream_of(gk if gq is None else gq)), "na_norm_rotary_bwd")
+    return grads
 
 
 # ---------------------------------------------------------------------------

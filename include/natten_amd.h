@@ -562,6 +562,77 @@ int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k
                   const void *prefix_v, const void *k, const void *v, void *out,
                   float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- a paged cache of keys and values in 8 bits (serving) ---------------------- */
+#define NA_CACHE_MAX_HEAD_DIM 256
+#define NA_CACHE_MAX_PAGE 128
+
+/*
+ * Token i of sample b lies in slot i % page_size of page tables[b][i / page_size].
+ * An element of a page and head is its e4m3 code (4 exponent bits, 3 of mantissa,
+ * largest 448) times 2^(s - 127), s the scale byte of that page and head (e8m0), in
+ * [10, 246] as na_cache_append writes it.  A table's entry outside [0, pages) is no
+ * page: what would lie there is not written and not seen.  No counterpart in the
+ * reference.
+ */
+typedef struct na_cache {
+  void *key;                     /* codes of [pages, kv_heads, page_size, head_dim] */
+  void *value;
+  void *key_scale;               /* bytes of [pages, kv_heads] */
+  void *value_scale;
+  int64_t key_stride[3];         /* elements: page, head, token; channels adjacent, */
+  int64_t value_stride[3];       /* every row 16-byte aligned */
+  int64_t key_scale_stride[2];   /* page, head */
+  int64_t value_scale_stride[2];
+} na_cache;
+
+typedef struct na_cache_params {
+  int32_t batch;
+  int32_t tokens;       /* new tokens per sample */
+  int32_t heads;        /* attention: of the queries */
+  int32_t kv_heads;     /* divides heads */
+  int32_t head_dim;     /* a multiple of 16, at most NA_CACHE_MAX_HEAD_DIM */
+  int32_t dtype;        /* of new keys and values, of queries and outputs */
+  int32_t pages;        /* of the cache */
+  int32_t page_size;    /* 16, 32, 64 or 128 */
+  int32_t table_pages;  /* entries of a sample's table */
+  int32_t window;       /* attention: 0 for all tokens; any width */
+  float scale;          /* attention: positive and finite */
+  int64_t table_stride; /* elements from sample to sample */
+  int64_t q_stride[3];  /* attention: sample, token, head; channels adjacent */
+  int64_t k_stride[3];  /* append: of the new keys and values */
+  int64_t v_stride[3];
+} na_cache_params;
+
+/*
+ * Writes the new keys and values [batch, tokens, kv_heads, head_dim] into the cache:
+ * token j of sample b is token t = seq_lens[b] - tokens + j of its sequence; the last
+ * new_lens[b] of them (NULL: all) with t >= 0 are written.  seq_lens are the lengths
+ * with the new tokens; values outside [0, table_pages * page_size] are taken as its
+ * ends, new_lens as those of [0, tokens].  Per page and head the scale is the smallest
+ * power of two that puts the new tokens' largest finite magnitude at 448 at most, and
+ * at least the held one where tokens of the page lie in front of the new ones, whose
+ * codes are rescaled where it grows.  Codes are rounded to the nearest, ties to even;
+ * what is not finite becomes NaN.  Pages that one call writes belong to one sample
+ * each.  seq_lens, new_lens and tables: int32 on the device.
+ */
+int na_cache_append(const na_cache_params *p, const na_cache *cache, const void *key,
+                    const void *value, const int32_t *tables, const int32_t *seq_lens,
+                    const int32_t *new_lens, void *stream);
+
+/* Bytes of device workspace na_cache_attend needs for these parameters. */
+size_t na_cache_attend_workspace_bytes(const na_cache_params *p);
+/*
+ * Attention of the newest `tokens` tokens of every sample, q [batch, tokens, heads,
+ * head_dim], against the cache: query j is token t = seq_lens[b] - tokens + j and sees
+ * tokens up to t (the last `window` of them where window > 0).  out and lse
+ * (float32 [batch, tokens, heads], natural log, or NULL) as na_prefix_fwd writes them;
+ * a query that sees no key gets zeros and -infinity.  What lies behind a length, in
+ * front of every window or in no page is not read.
+ */
+int na_cache_attend(const na_cache_params *p, const na_cache *cache, const void *q,
+                    const int32_t *tables, const int32_t *seq_lens, void *out, float *lse,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -64,6 +64,7 @@ EXTRA_FLAGS = {
     "na_lean.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "na_dense.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "na_wave.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "na_cache_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "na_prefix.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "na_wsplit.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }

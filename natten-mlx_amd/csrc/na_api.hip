@@ -1063,4 +1063,94 @@ int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k
   return launch_status("na_prefix_fwd");
 }
 
+namespace {
+
+int check_cache(const na_cache_params *p) {
+  if (p == nullptr) return fail(NA_ERR_INVALID, "params is NULL");
+  if (p->batch < 0 || p->tokens < 0 || p->kv_heads < 1 || p->pages < 0 || p->table_pages < 0)
+    return fail(NA_ERR_INVALID, "a size is out of range (batch %d, tokens %d, kv_heads %d, pages %d, "
+                "table_pages %d)", p->batch, p->tokens, p->kv_heads, p->pages, p->table_pages);
+  if (p->dtype != NA_F32 && p->dtype != NA_F16 && p->dtype != NA_BF16)
+    return fail(NA_ERR_INVALID, "unknown dtype %d", p->dtype);
+  if (p->head_dim < 16 || p->head_dim % 16 != 0 || p->head_dim > NA_CACHE_MAX_HEAD_DIM)
+    return fail(NA_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 up to %d, got %d",
+                NA_CACHE_MAX_HEAD_DIM, p->head_dim);
+  if (p->page_size < 16 || p->page_size > NA_CACHE_MAX_PAGE || (p->page_size & (p->page_size - 1)))
+    return fail(NA_ERR_UNSUPPORTED, "page_size must be 16, 32, 64 or 128, got %d", p->page_size);
+  if ((int64_t)p->table_pages * p->page_size > (1 << 30) || p->tokens > (1 << 30))
+    return fail(NA_ERR_UNSUPPORTED, "more than 2^30 tokens of a sample");
+  return NA_OK;
+}
+
+int check_cache_attend(const na_cache_params *p, size_t *need) {
+  *need = 0;
+  const int rc = check_cache(p);
+  if (rc != NA_OK) return rc;
+  if (p->heads < 1 || p->heads % p->kv_heads != 0)
+    return fail(NA_ERR_INVALID, "heads (%d) must be divisible by kv_heads (%d)", p->heads,
+                p->kv_heads);
+  if (p->window < 0) return fail(NA_ERR_INVALID, "window is negative");
+  if (!(p->scale > 0.f) || p->scale > 3e38f)
+    return fail(NA_ERR_INVALID, "scale must be positive and finite, got %g", (double)p->scale);
+  if ((int64_t)p->batch * p->tokens >= ((int64_t)1 << 30) ||
+      (int64_t)p->batch * p->tokens * p->heads >= ((int64_t)1 << 30))
+    return fail(NA_ERR_UNSUPPORTED, "batch * tokens * heads is 2^30 or more");
+  if (p->batch > 0 && p->tokens > 0 && !na::cache_attend_fits(p, need))
+    return fail(NA_ERR_UNSUPPORTED, "the call is too large for one launch");
+  *need = align256(*need);
+  return NA_OK;
+}
+
+// Rows of codes start at multiples of 16 bytes.
+int check_pages(const na_cache *c) {
+  if (c == nullptr || c->key == nullptr || c->value == nullptr || c->key_scale == nullptr ||
+      c->value_scale == nullptr)
+    return fail(NA_ERR_INVALID, "the cache's key/value/key_scale/value_scale must be non-NULL");
+  uintptr_t bits = reinterpret_cast<uintptr_t>(c->key) | reinterpret_cast<uintptr_t>(c->value);
+  for (int i = 0; i < 3; ++i) bits |= (uintptr_t)c->key_stride[i] | (uintptr_t)c->value_stride[i];
+  if (bits & 15)
+    return fail(NA_ERR_INVALID, "the cache's rows must start at multiples of 16 bytes");
+  return NA_OK;
+}
+
+}  // namespace
+
+int na_cache_append(const na_cache_params *p, const na_cache *cache, const void *key,
+                    const void *value, const int32_t *tables, const int32_t *seq_lens,
+                    const int32_t *new_lens, void *stream) {
+  int rc = check_cache(p);
+  if (rc != NA_OK) return rc;
+  if (p->batch == 0 || p->tokens == 0 || p->pages == 0 || p->table_pages == 0) return NA_OK;
+  if ((rc = check_pages(cache)) != NA_OK) return rc;
+  if (key == nullptr || value == nullptr || tables == nullptr || seq_lens == nullptr)
+    return fail(NA_ERR_INVALID, "key/value/tables/seq_lens must be non-NULL");
+  if (!na::cache_append(p, cache, key, value, tables, seq_lens, new_lens, as_stream(stream)))
+    return fail(NA_ERR_UNSUPPORTED, "the call is too large for one launch");
+  return launch_status("na_cache_append");
+}
+
+size_t na_cache_attend_workspace_bytes(const na_cache_params *p) {
+  size_t need;
+  return check_cache_attend(p, &need) == NA_OK ? need : 0;
+}
+
+int na_cache_attend(const na_cache_params *p, const na_cache *cache, const void *q,
+                    const int32_t *tables, const int32_t *seq_lens, void *out, float *lse,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+  size_t need;
+  int rc = check_cache_attend(p, &need);
+  if (rc != NA_OK) return rc;
+  if (p->batch == 0 || p->tokens == 0) return NA_OK;
+  const bool keys = p->pages > 0 && p->table_pages > 0;
+  if (keys && (rc = check_pages(cache)) != NA_OK) return rc;
+  if (cache == nullptr || q == nullptr || out == nullptr || seq_lens == nullptr ||
+      (keys && tables == nullptr))
+    return fail(NA_ERR_INVALID, "cache/q/tables/seq_lens/out must be non-NULL");
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(NA_ERR_WORKSPACE, "na_cache_attend needs a %zu-byte workspace (got %zu)", need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  na::cache_attend(p, cache, q, tables, seq_lens, out, lse, workspace, as_stream(stream));
+  return launch_status("na_cache_attend");
+}
+
 }  // extern "C"

@@ -1,0 +1,736 @@
+// na_cache_attend.hip — attention of new tokens against a paged cache held in 8 bits
+// (serving).
+//
+// Query token j of sample b is token t = len_b - Lq + j of its sequence and sees
+// tokens max(0, t - W + 1) .. t:  out = softmax(scale q k^T) v,  lse the log of the
+// softmax's sum.  Token i lies in slot i mod T of page tables[b][i / T]; keys and values
+// are e4m3 codes times their page's and head's power of two, which every bf16 holds
+// exactly: they become bf16 as they are read, and products run on the bf16 matrix
+// cores.  Queries and probabilities meet them in parts of 8 bits each: bf16 in one,
+// fp16 in two (16 bits; its queries exactly), float32 in three (24 bits).  Scores, sums
+// and outputs are float32, probabilities lose half a step of their parts, out is
+// rounded once.
+//
+// The rows of a sample and key/value head (its query heads of all its new tokens)
+// are cut into tiles; a tile and the keys its rows see are an item, cut into units of
+// 64 keys.  The chip's workgroups share all units evenly, in order: lengths lie on the
+// device, so each finds its part by adding up the items' units, and ragged lengths
+// leave no workgroup waiting.  An item that lies in one workgroup is written by it;
+// the others leave (m, l, o) -- reference point, sum and unnormalised output of an
+// online softmax, float32 -- per workgroup, and k_cache_join adds those of a row.
+#include "na_cache.h"
+#include "na_chunk.h"
+#include "na_launch.h"
+#include "na_lean.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace na {
+namespace {
+
+constexpr int kUnit = 64;   // keys
+constexpr int kTile = 32;   // keys of a narrow wave's tile
+
+struct CacheProb {
+  int32_t B, Lq, H, Hkv, rep, D;
+  int32_t Mo, rows, rt;       // rows of a sample and key/value head, of a tile; tiles
+  int32_t items;              // B * rt
+  int32_t pages, lgT, M, W;   // W: window
+  int32_t wgs, least;         // workgroups, units that one takes at least
+  float sl2;                  // scale * log2(e)
+  FastDiv frep, frt;
+  int64_t qs[3];              // sample, token, head
+  int64_t ts;
+  const int32_t *tables, *lens;
+  CachePages k, v;
+};
+
+struct CacheArgs {
+  const void *q;
+  void *out;
+  float *lse;    // or null
+  float *po;     // [2 wgs][rows][D] parts: of an item begun before, of one begun here
+  float2 *pml;   // [2 wgs][rows] their reference points and sums
+  int2 *span;    // [Hkv][items] first and last workgroup
+};
+
+// The keys that an item's rows see, and units over them.
+struct CacheItem {
+  int b, row0, row1;     // rows of the sample
+  int len;
+  int k0, lo, hi;        // keys [lo, hi) of some row, units from k0
+  int lo_max, hi_min;    // keys that every row sees
+  int units;
+};
+
+__device__ __forceinline__ CacheItem cache_item(const CacheProb &P, int i) {
+  CacheItem w;
+  w.b = (int)fdiv((uint32_t)i, P.frt);
+  const int r = i - w.b * P.rt;
+  w.len = min(max(P.lens[w.b], 0), P.M << P.lgT);
+  w.row0 = r * P.rows;
+  w.row1 = min(w.row0 + P.rows, P.Mo);
+  const int first = w.len - P.Lq + (int)fdiv((uint32_t)w.row0, P.frep);
+  const int last = w.len - P.Lq + (int)fdiv((uint32_t)(w.row1 - 1), P.frep);
+  w.lo = max(first - P.W + 1, 0);
+  w.hi = max(last + 1, 0);
+  w.lo_max = max(last - P.W + 1, 0);
+  w.hi_min = max(first + 1, 0);
+  w.k0 = w.lo & ~(kUnit - 1);
+  w.units = w.hi > w.lo ? (w.hi - w.k0 + kUnit - 1) / kUnit : 0;
+  return w;
+}
+
+// Inclusive sum over the wave's lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off, 64);
+    x += lane >= off ? y : 0;
+  }
+  return x;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Units of all items of a head.
+__device__ __forceinline__ int64_t cache_total(const CacheProb &P) {
+  int64_t sum = 0;
+  for (int i0 = 0; i0 < P.items; i0 += 64) {
+    const int i = i0 + (threadIdx.x & 63);
+    const int u = i < P.items ? cache_item(P, i).units : 0;
+    sum += __builtin_amdgcn_readlane(wave_scan(u), 63);
+  }
+  return sum;
+}
+
+// The item that unit u of a head lies in; u becomes the unit within it.
+__device__ __forceinline__ int cache_find(const CacheProb &P, int64_t &u) {
+  for (int i0 = 0; i0 < P.items; i0 += 64) {
+    const int i = i0 + (threadIdx.x & 63);
+    const int mine = i < P.items ? cache_item(P, i).units : 0;
+    const int sum = wave_scan(mine);
+    const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (u < all) {
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > (int)u));
+      u -= __builtin_amdgcn_readlane(sum - mine, at);
+      return i0 + at;
+    }
+    u -= all;
+  }
+  return P.items;  // not reached: u is less than the total
+}
+
+// 64 entries of a sample's table, one a lane: the page or -1, its scales' bytes.
+struct PageWindow {
+  int base, page, sc;
+  __device__ __forceinline__ void load(const CacheProb &P, int sample, int g, int first) {
+    base = first;
+    const int i = first + (threadIdx.x & 63);
+    page = i < P.M ? P.tables[sample * P.ts + i] : -1;
+    if ((uint32_t)page >= (uint32_t)P.pages) page = -1;
+    sc = 0;
+    if (page >= 0) {  // (bytes past the largest scale, as unwritten pages hold them, stay finite)
+      const int a = P.k.scale[page * P.k.sc[0] + g * P.k.sc[1]];
+      const int b = P.v.scale[page * P.v.sc[0] + g * P.v.sc[1]];
+      sc = min(a, kScaleBias + kScaleHigh) | min(b, kScaleBias + kScaleHigh) << 8;
+    }
+  }
+  // Whether it holds table entry i (uniform).
+  __device__ __forceinline__ bool holds(int i) const { return (uint32_t)(i - base) < 64u; }
+  __device__ __forceinline__ int page_of(int i) const {
+    return __builtin_amdgcn_readlane(page, i - base);
+  }
+  __device__ __forceinline__ int scales_of(int i) const {
+    return __builtin_amdgcn_readlane(sc, i - base);
+  }
+};
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef L16<bf16_t> M16;
+
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+
+// Eight codes times a power of two.
+__device__ __forceinline__ bf8 decode8(uint32_t a, uint32_t b, float s) {
+  union {
+    bf2 p[4];
+    bf8 v;
+  } o;
+  o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false);
+  o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true);
+  o.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false);
+  o.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true);
+  return o.v;
+}
+
+template <typename T>
+constexpr int cache_parts() {
+  return std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3;
+}
+
+// Eight numbers as sums of parts.
+template <int NP>
+__device__ __forceinline__ void split8(const float (&x)[8], bf8 (&o)[NP]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[p][i] = (__bf16)r[i];
+      if (p + 1 < NP) r[i] -= (float)o[p][i];
+    }
+}
+
+// Eight channels of a query row.
+template <typename T, int NP>
+__device__ __forceinline__ void query8(const T *p, bool live, bf8 (&o)[NP]) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (live) {
+    typedef typename Mem16<sizeof(T)>::t m4;  // any alignment of the elements
+    if (sizeof(T) == 4) {
+      const u4 a = *reinterpret_cast<const m4 *>(p), b = *reinterpret_cast<const m4 *>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = __uint_as_float(a[i]);
+        x[4 + i] = __uint_as_float(b[i]);
+      }
+    } else {
+      const u4 a = *reinterpret_cast<const m4 *>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t h = (uint16_t)(a[i / 2] >> (16 * (i & 1)));
+        x[i] = std::is_same<T, f16_t>::value ? (float)__builtin_bit_cast(f16_t, h)
+                                             : __uint_as_float((uint32_t)h << 16);
+      }
+    }
+  }
+  split8<NP>(x, o);
+}
+
+// Four results of a row, rounded.
+template <typename T>
+__device__ __forceinline__ void cache_store4(T *p, f32x4 x) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4 *>(p) = x;
+  } else {
+    typename L16<T>::v4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (typename L16<T>::e)x[r];
+    *reinterpret_cast<typename L16<T>::v4 *>(p) = o;
+  }
+}
+
+// Index in lse of row r of sample b and key/value head g.
+__device__ __forceinline__ int64_t cache_out_row(const CacheProb &P, int b, int g, int r) {
+  const int j = (int)fdiv((uint32_t)r, P.frep);
+  return ((int64_t)b * P.Lq + j) * P.H + g * P.rep + (r - j * P.rep);
+}
+
+// Where a workgroup's rows of an item go: to out, or to its part.
+template <typename T>
+__device__ __forceinline__ void cache_put(const CacheProb &P, const CacheArgs &A, const CacheItem &w,
+                                          int g, int part, int r, int c, f32x4 o, float l) {
+  if (c >= P.D) return;
+  if (part >= 0) {
+    *reinterpret_cast<f32x4 *>(A.po + ((int64_t)part * P.rows + r) * P.D + c) = o;
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    cache_store4(static_cast<T *>(A.out) + cache_out_row(P, w.b, g, w.row0 + r) * P.D + c, o * inv);
+  }
+}
+__device__ __forceinline__ void cache_put_ml(const CacheProb &P, const CacheArgs &A,
+                                             const CacheItem &w, int g, int part, int r, float m,
+                                             float l) {
+  if (part >= 0)
+    A.pml[(int64_t)part * P.rows + r] = make_float2(m, l);
+  else if (A.lse != nullptr)
+    A.lse[cache_out_row(P, w.b, g, w.row0 + r)] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Online softmax step of a lane's N scores of one row (the four lanes of a row hold
+// the others): scores to probabilities in place, m, l and o rescaled where the
+// reference point m moves.  It may trail the maximum by 8 (a factor 2^8 in p): exact
+// after the division by l.
+template <int N, int NDB>
+__device__ __forceinline__ void cache_softmax(float (&p)[N], float sl2, float &m, float &l,
+                                              f32x4 (&o)[NDB]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mx = fmaxf(mx, p[i]);
+  mx = quad_max(mx) * sl2;
+  if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+    const float mn = fmaxf(m, mx);
+    const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= alpha;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+    m = mn;
+  }
+  const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], sl2, -mu));
+    l += p[i];
+  }
+}
+
+// Rows [0, rows) of a tile of values in LDS hold a NaN (all lanes look).
+template <int D>
+__device__ __forceinline__ bool cache_odd_tile(const __bf16 *vs, int stride, int rows, int lane) {
+  bool odd = false;
+  for (int u = lane; u < rows * (D / 8); u += 64) {
+    const u4 x = *reinterpret_cast<const u4 *>(vs + u / (D / 8) * stride + u % (D / 8) * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      odd |= (x[i] & 0x7f80u) == 0x7f80u || (x[i] & 0x7f800000u) == 0x7f800000u;
+  }
+  return __builtin_amdgcn_ballot_w64(odd) != 0;
+}
+
+// o += P V key by key, only over the keys that the lane's row sees: for tiles where
+// rows see different keys and V holds a NaN, which a probability of zero would not
+// take out.  p: the lane's scores of keys 16 (i / 4) + 4 gq + i % 4.
+template <int N, int NDB>
+__device__ __forceinline__ void cache_odd_pv(const float (&p)[N], const __bf16 *vs, int stride,
+                                             int lane, int lo, int n, f32x4 (&o)[NDB]) {
+  const int row = lane & 15, gq = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll 1
+    for (int g2 = 0; g2 < 4; ++g2) {
+      const int key = 16 * (i / 4) + 4 * g2 + i % 4;
+      const float pk = __shfl(p[i], row + 16 * g2, 64);
+      if ((unsigned)(key - lo) >= (unsigned)n) continue;
+      const __bf16 *v = vs + key * stride + 4 * gq;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[db][c] = fmaf(pk, (float)v[16 * db + c], o[db][c]);
+    }
+}
+
+// A row's queries, and the keys [lo, lo + n) that it sees.
+template <typename T>
+struct CacheRow {
+  const T *q;
+  int lo, n;
+  __device__ __forceinline__ CacheRow(const CacheProb &P, const CacheArgs &A, const CacheItem &w,
+                                      int g, int row) {
+    const int r = min(row, w.row1 - 1);
+    const int j = (int)fdiv((uint32_t)r, P.frep), i = r - j * P.rep;
+    q = static_cast<const T *>(A.q) + w.b * P.qs[0] + j * P.qs[1] + (int64_t)(g * P.rep + i) * P.qs[2];
+    const int t = w.len - P.Lq + j;
+    lo = max(t - P.W + 1, 0);
+    n = max(t + 1 - lo, 0);
+  }
+};
+
+// Narrow: 16 NQ rows, the waves take different tiles of 32 keys of [ka, kb): keys go
+// from memory into the matrix operand, values through the wave's own LDS (its
+// transposing read), no barrier until the waves' results meet.
+template <typename T, int D, int NQ, int NW>
+__device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs &A,
+                                             const CacheItem &w, int g, int ka, int kb, int part,
+                                             char *smem) {
+  constexpr int NP = cache_parts<T>(), NS = D / 64, NDB = D / 16, RS = D + 8;
+  constexpr int UPR = D / 16, RPP = 64 / UPR, NU = kTile / RPP;  // V: units per row, rows per pass
+  const int tid = threadIdx.x, wv = uniform(tid >> 6), lane = tid & 63;
+  const int n = lane & 15, gq = lane >> 4;
+  __bf16 *const vs = reinterpret_cast<__bf16 *>(smem) + wv * (kTile * RS);  // the wave's own
+  bf8 qf[NQ][2 * NS][NP];
+  int lo[NQ], cnt[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const CacheRow<T> row(P, A, w, g, w.row0 + 16 * qi + n);
+    lo[qi] = row.lo;
+    cnt[qi] = row.n;
+#pragma unroll
+    for (int s = 0; s < 2 * NS; ++s) {
+      const int c = 64 * (s / 2) + 16 * gq + 8 * (s & 1);
+      query8<T, NP>(row.q + c, c < P.D, qf[qi][s]);
+    }
+  }
+  const int vc = lane % UPR, vr = lane / UPR;
+  u4 kr[2][NS], vr8[NU];
+  float ksc[2], vsc[2];
+  bool bad = false;
+  PageWindow win;
+  win.base = -64;
+  const uint8_t *const kb0 = P.k.code + g * P.k.st[1] + (int64_t)n * P.k.st[2] + 16 * gq;
+  const uint8_t *const vb0 = P.v.code + g * P.v.st[1] + (int64_t)vr * P.v.st[2] + 16 * vc;
+  // Keys that no row sees are not read: zeros (0 times them is 0).
+  const int seen0 = max(ka, w.lo), seen1 = min(kb, w.hi);
+  auto load = [&](int t0) {
+    bad = false;
+    const bool whole = t0 >= seen0 && t0 + kTile <= seen1 && P.D == D;
+    int page[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int i = (t0 + 16 * hh) >> P.lgT;
+      if (!win.holds(i)) win.load(P, w.b, g, i);
+      page[hh] = win.page_of(i);
+      const int sc = win.scales_of(i);
+      ksc[hh] = scale_of(sc & 255);
+      vsc[hh] = scale_of(sc >> 8);
+      bad |= page[hh] < 0;
+    }
+    const int slot0 = t0 & ((1 << P.lgT) - 1), slot1 = (t0 + 16) & ((1 << P.lgT) - 1);
+    const uint8_t *const ap[2] = {kb0 + page[0] * P.k.st[0] + slot0 * P.k.st[2],
+                                  kb0 + page[1] * P.k.st[0] + slot1 * P.k.st[2]};
+    const uint8_t *const bp[2] = {vb0 + page[0] * P.v.st[0] + slot0 * P.v.st[2],
+                                  vb0 + page[1] * P.v.st[0] + slot1 * P.v.st[2]};
+    if (whole && !bad) {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+          kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s);
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+        vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2]);
+    } else {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int key = t0 + 16 * hh + n;
+        const bool live = page[hh] >= 0 && key >= seen0 && key < seen1;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          kr[hh][s] = u4{0, 0, 0, 0};
+          if (live && 64 * s + 16 * gq < P.D)
+            kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int key = t0 + RPP * i + vr;
+        vr8[i] = u4{0, 0, 0, 0};
+        if (page[RPP * i / 16] >= 0 && key >= seen0 && key < seen1 && 16 * vc < P.D)
+          vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2]);
+      }
+    }
+    // (a page that is none: its keys' scores are taken out below)
+    if (bad) {
+      if (page[0] < 0) ksc[0] = -1.f;
+      if (page[1] < 0) ksc[1] = -1.f;
+    }
+  };
+  f32x4 o[NQ][NDB];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[qi][db] = zero4();
+    m[qi] = -INFINITY;
+    l[qi] = 0.f;
+  }
+  const float sl2 = P.sl2;
+  const int tr_off = (4 * gq + (n >> 2)) * RS + 4 * (n & 3);
+  const bool spans = P.Lq > 1;
+  const int all0 = max(ka, w.lo_max), all1 = min(kb, w.hi_min);  // seen by every row
+  auto run_tile = [&](int t0, auto edge_tile) {
+    constexpr bool EDGE = decltype(edge_tile)::value;
+    f32x4 s[NQ][2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) s[qi][hh] = zero4();
+#pragma unroll
+      for (int t = 0; t < 2 * NS; ++t) {
+        const bf8 kf = decode8(kr[hh][t / 2][2 * (t & 1)], kr[hh][t / 2][2 * (t & 1) + 1], ksc[hh]);
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) s[qi][hh] = M16::mma(kf, qf[qi][t][p], s[qi][hh]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // the reads of the tile before are issued
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      __bf16 *const d = vs + (RPP * i + vr) * RS + 16 * vc;
+      const float sc = vsc[RPP * i / 16];
+      *reinterpret_cast<bf8 *>(d) = decode8(vr8[i][0], vr8[i][1], sc);
+      *reinterpret_cast<bf8 *>(d + 8) = decode8(vr8[i][2], vr8[i][3], sc);
+    }
+    const bool none[2] = {EDGE && ksc[0] < 0.f, EDGE && ksc[1] < 0.f};
+    if (t0 + NW * kTile < kb) load(t0 + NW * kTile);  // in flight during the rest
+    float p[NQ][8];
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[qi][i] = s[qi][i / 4][i % 4];
+        if (EDGE) {
+          const int key = t0 + 16 * (i / 4) + 4 * gq + i % 4;
+          if (none[i / 4] || key < ka || key >= kb || (unsigned)(key - lo[qi]) >= (unsigned)cnt[qi])
+            p[qi][i] = -INFINITY;
+        }
+      }
+      cache_softmax(p[qi], sl2, m[qi], l[qi], o[qi]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (EDGE && spans && cache_odd_tile<D>(vs, RS, kTile, lane)) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) cache_odd_pv(p[qi], vs, RS, lane, lo[qi] - t0, cnt[qi], o[qi]);
+    } else {
+      bf8 bp[NQ][NP];
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) split8<NP>(p[qi], bp[qi]);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const bf4 lo4 = M16::tr(vs + tr_off + 16 * db);
+        const bf4 hi4 = M16::tr(vs + 16 * RS + tr_off + 16 * db);
+        const bf8 va = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+          for (int x = NP - 1; x >= 0; --x) o[qi][db] = M16::mma(va, bp[qi][x], o[qi][db]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  };
+  int t0 = ka + wv * kTile;
+  if (t0 < kb) load(t0);
+  for (; t0 < kb; t0 += NW * kTile) {
+    if (t0 >= all0 && t0 + kTile <= all1 && !bad) run_tile(t0, std::false_type{});
+    else run_tile(t0, std::true_type{});
+  }
+  // The waves' results meet in LDS, 16 rows at a time.
+  constexpr int PS = D + 4;  // floats per row
+  float *const po = reinterpret_cast<float *>(smem);
+  float2 *const ml = reinterpret_cast<float2 *>(po + NW * 16 * PS);  // [NW][16]
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const float lt = quad_sum(l[qi]);
+    __syncthreads();  // the tiles' LDS is free
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      *reinterpret_cast<f32x4 *>(po + (wv * 16 + n) * PS + 16 * db + 4 * gq) = o[qi][db];
+    if (lane < 16) ml[wv * 16 + n] = make_float2(m[qi], lt);
+    __syncthreads();
+    constexpr int TPR = 4 * NW;  // threads per row
+    const int r = tid / TPR;
+    if (w.row0 + 16 * qi + r < w.row1) {
+      float2 x[NW];
+      float mt = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        x[i] = ml[i * 16 + r];
+        mt = fmaxf(mt, x[i].x);
+      }
+      float wt[NW];
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        wt[i] = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - mt);  // (NaN: a seen row)
+        sum = x[i].y == 0.f ? sum : fmaf(wt[i], x[i].y, sum);
+      }
+      for (int c = 4 * (tid % TPR); c < D; c += 4 * TPR) {
+        f32x4 a = zero4();
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+          if (x[i].y != 0.f) a += wt[i] * *reinterpret_cast<const f32x4 *>(po + (i * 16 + r) * PS + c);
+        cache_put<T>(P, A, w, g, part, 16 * qi + r, c, a, sum);
+      }
+      if (tid % TPR == 0) cache_put_ml(P, A, w, g, part, 16 * qi + r, mt, sum);
+    }
+  }
+  __syncthreads();  // before the next item's tiles
+}
+
+// This workgroup's part of all units, item by item.
+template <typename F>
+__device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheArgs &A, F &&run) {
+  const int64_t per_head = cache_total(P), all = per_head * P.Hkv;
+  if (all == 0) return;
+  const int64_t most = (all + P.least - 1) / P.least;
+  const int n = (int)(most < P.wgs ? most : P.wgs);
+  // tiles next to each other read the same keys: through one XCD's L2
+  const int me = P.rt > 1 && n == P.wgs ? xcd_tile(blockIdx.x, P.wgs) : blockIdx.x;
+  if (me >= n) return;
+  int64_t u = all * me / n;
+  const int64_t end = all * (me + 1) / n;
+  int g = (int)(u / per_head);
+  int64_t off = u - g * per_head;
+  int i = cache_find(P, off);
+  while (u < end) {
+    const CacheItem w = cache_item(P, i);
+    if (w.units > 0) {
+      const int take = (int)min((int64_t)w.units - off, end - u);
+      const bool begins = off == 0, whole = begins && take == w.units;
+      if (begins && threadIdx.x == 0) {
+        // the workgroup that unit x lies in is the largest whose part begins at x or before
+        const int64_t x = u + w.units;
+        A.span[(int64_t)g * P.items + i] = make_int2(me, (int)((x * n + all - 1) / all) - 1);
+      }
+      run(w, g, w.k0 + (int)off * kUnit, min(w.k0 + (int)(off + take) * kUnit, w.hi),
+          whole ? -1 : 2 * me + (begins ? 1 : 0));
+      u += take;
+    }
+    off = 0;
+    if (++i == P.items) {
+      i = 0;
+      ++g;
+    }
+  }
+}
+
+template <typename T, int D, int NQ, int NW>
+__global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_narrow(CacheProb P, CacheArgs A) {
+  extern __shared__ __align__(16) char smem[];
+  cache_parts_of(P, A, [&](const CacheItem &w, int g, int ka, int kb, int part) {
+    cache_narrow<T, D, NQ, NW>(P, A, w, g, ka, kb, part, smem);
+  });
+}
+
+// The parts of a row added: lanes take four channels each, 2^lgG of them a row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_cache_join(CacheProb P, CacheArgs A, int lgG) {
+  const int64_t mine = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lgG;
+  const int c = 4 * (threadIdx.x & ((1 << lgG) - 1));
+  if (mine >= (int64_t)P.B * P.Hkv * P.Mo) return;
+  const int64_t bg = mine / P.Mo;
+  const int row = (int)(mine - bg * P.Mo), b = (int)(bg / P.Hkv), g = (int)(bg - (int64_t)b * P.Hkv);
+  const int tile = row / P.rows, item = b * P.rt + tile, r = row - tile * P.rows;
+  const CacheItem w = cache_item(P, item);
+  int2 span = make_int2(0, -1);
+  if (w.units > 0) {
+    span = A.span[(int64_t)g * P.items + item];
+    if (span.x == span.y) return;  // written by its workgroup
+  }
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = zero4();
+  for (int i = span.x; i <= span.y; ++i) {
+    const int64_t at = (int64_t)(2 * i + (i == span.x ? 1 : 0)) * P.rows + r;
+    const float2 x = A.pml[at];
+    if (x.y == 0.f) continue;  // sees nothing of the part
+    f32x4 o = zero4();
+    if (c < P.D) o = *reinterpret_cast<const f32x4 *>(A.po + at * P.D + c);
+    const float mn = fmaxf(m, x.x);
+    const float a = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(x.x - mn);
+    l = l == 0.f ? e * x.y : fmaf(e, x.y, l * a);
+    acc = acc * a + e * o;
+    m = mn;
+  }
+  const int64_t out = cache_out_row(P, b, g, row);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (c < P.D) cache_store4(static_cast<T *>(A.out) + out * P.D + c, acc * inv);
+  if (c == 0 && A.lse != nullptr) A.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+int cache_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
+  CacheProb P{};
+  P.B = p->batch;
+  P.Lq = p->tokens;
+  P.H = p->heads;
+  P.Hkv = p->kv_heads;
+  P.rep = p->heads / p->kv_heads;
+  P.D = p->head_dim;
+  P.Mo = P.Lq * P.rep;
+  P.rows = P.Mo > 16 && p->dtype != NA_F32 && P.D <= 128 ? 32 : 16;
+  P.rt = (P.Mo + P.rows - 1) / P.rows;
+  P.items = P.B * P.rt;
+  P.pages = p->pages;
+  P.lgT = lg_page(p->page_size);
+  P.M = p->table_pages;
+  P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
+  P.wgs = 512;
+  P.least = 2;
+  P.sl2 = p->scale * kLog2e;
+  P.frep = make_fastdiv((uint32_t)P.rep);
+  P.frt = make_fastdiv((uint32_t)P.rt);
+  for (int i = 0; i < 3; ++i) P.qs[i] = p->q_stride[i];
+  P.ts = p->table_stride;
+  if (c != nullptr) {
+    P.k = {static_cast<uint8_t *>(c->key), static_cast<uint8_t *>(c->key_scale),
+           {c->key_stride[0], c->key_stride[1], c->key_stride[2]},
+           {c->key_scale_stride[0], c->key_scale_stride[1]}};
+    P.v = {static_cast<uint8_t *>(c->value), static_cast<uint8_t *>(c->value_scale),
+           {c->value_stride[0], c->value_stride[1], c->value_stride[2]},
+           {c->value_scale_stride[0], c->value_scale_stride[1]}};
+  }
+  return P;
+}
+
+struct CacheSizes {
+  size_t po, pml, span;
+  explicit CacheSizes(const CacheProb &P) {
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    po = up((size_t)2 * P.wgs * P.rows * P.D * sizeof(float));
+    pml = up((size_t)2 * P.wgs * P.rows * sizeof(float2));
+    span = up((size_t)P.Hkv * P.items * sizeof(int2));
+  }
+  size_t total() const { return po + pml + span; }
+};
+
+int cache_join_lanes(const CacheProb &P) {
+  int lgG = 0;
+  while ((4 << lgG) < P.D) ++lgG;
+  return lgG;
+}
+
+template <typename T, int D, int NQ>
+void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
+  constexpr int NW = 4;
+  const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
+  const size_t tiles = sizeof(__bf16) * NW * kTile * (D + 8);
+  hipLaunchKernelGGL((k_cache_narrow<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW),
+                     std::max(meet, tiles), st, P, A);
+}
+
+template <typename T>
+void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
+  auto by_rows = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if constexpr (sizeof(T) == 2 && D <= 128)
+      if (P.rows == 32) return cache_launch<T, D, 2>(P, A, st);
+    cache_launch<T, D, 1>(P, A, st);
+  };
+  const int width = cache_width(P.D);
+  if (width == 256) by_rows(std::integral_constant<int, 256>{});
+  else if (width == 128) by_rows(std::integral_constant<int, 128>{});
+  else by_rows(std::integral_constant<int, 64>{});
+  const int lgG = cache_join_lanes(P);
+  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << lgG;
+  hipLaunchKernelGGL((k_cache_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
+                     lgG);
+}
+
+}  // namespace
+
+// A launch has fewer than 2^32 threads.
+bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
+  const CacheProb P = cache_prob(p, nullptr);
+  *workspace_bytes = CacheSizes(P).total();
+  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << cache_join_lanes(P);
+  return threads < ((int64_t)1 << 32) - 256;
+}
+
+void cache_attend(const na_cache_params *p, const na_cache *c, const void *q, const int32_t *tables,
+                  const int32_t *lens, void *out, float *lse, void *workspace, hipStream_t st) {
+  CacheProb P = cache_prob(p, c);
+  P.tables = tables;
+  P.lens = lens;
+  const CacheSizes s(P);
+  char *const ws = static_cast<char *>(workspace);
+  const CacheArgs A{q, out, lse, reinterpret_cast<float *>(ws),
+                    reinterpret_cast<float2 *>(ws + s.po),
+                    reinterpret_cast<int2 *>(ws + s.po + s.pml)};
+  if (p->dtype == NA_F32) cache_run<float>(P, A, st);
+  else if (p->dtype == NA_F16) cache_run<f16_t>(P, A, st);
+  else cache_run<bf16_t>(P, A, st);
+}
+
+}  // namespace na

@@ -266,6 +266,16 @@ void prefix_attention(const na_prefix_params *p, const void *q, const void *pk, 
                       const void *k, const void *v, void *out, float *lse, void *workspace,
                       hipStream_t st);
 
+// A paged cache in 8 bits: new tokens into its pages (na_cache.hip; false, and nothing
+// launched, where they are more than a launch takes), attention over it
+// (na_cache_attend.hip).
+bool cache_append(const na_cache_params *p, const na_cache *c, const void *key, const void *value,
+                  const int32_t *tables, const int32_t *lens, const int32_t *fresh,
+                  hipStream_t st);
+bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes);  // false: too large
+void cache_attend(const na_cache_params *p, const na_cache *c, const void *q, const int32_t *tables,
+                  const int32_t *lens, void *out, float *lse, void *workspace, hipStream_t st);
+
 // Generic pieces reused around the MFMA backward.
 void valu_delta(const Prob &P, int dtype, const void *out, const void *dout,
                 const float *dlse, float *delta, hipStream_t st);

@@ -1176,6 +1176,131 @@ std::tuple<at::Tensor, at::Tensor> na_prefix(
   return {out, lse};
 }
 
+// ---- paged cache in 8 bits (cache.py) ------------------------------------------
+
+struct CacheCall {
+  na_cache_params p{};
+  na_cache c{};
+  at::Tensor tables, lens;
+};
+
+// Integers as the kernels read them; 64-bit ones are clamped before they are narrowed.
+at::Tensor narrow_ints(const at::Tensor &t, int64_t low, int64_t high) {
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong,
+              "natten_amd: tables and lengths are int32 or int64");
+  return t.scalar_type() == at::kLong ? t.clamp(low, high).to(at::kInt) : t;
+}
+
+// The functional layer has validated the call; its rules are restated for direct
+// callers of the operators.  x: the new keys or the queries.
+CacheCall cache_call(const at::Tensor &x, const at::Tensor &k, const at::Tensor &v,
+                     const at::Tensor &ks, const at::Tensor &vs, const at::Tensor &tables,
+                     const at::Tensor &lens) {
+  TORCH_CHECK(x.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && x.size(3) == k.size(3) &&
+                  k.size(1) > 0,
+              "natten_amd: new tokens [B, L, heads, D] and a cache [pages, H_kv, page_size, D], got ",
+              x.sizes(), " and ", k.sizes());
+  TORCH_CHECK(ks.dim() == 2 && ks.sizes() == k.sizes().slice(0, 2) && vs.sizes() == ks.sizes(),
+              "natten_amd: a cache's scales are [pages, H_kv]");
+  TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn &&
+                  ks.scalar_type() == at::kFloat8_e8m0fnu && vs.scalar_type() == at::kFloat8_e8m0fnu,
+              "natten_amd: a cache holds float8_e4m3fn and float8_e8m0fnu");
+  TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "natten_amd: a cache's channels are adjacent");
+  TORCH_CHECK(tables.dim() == 2 && tables.size(0) == x.size(0) && lens.dim() == 1 &&
+                  lens.size(0) == x.size(0),
+              "natten_amd: tables [B, pages of a sample] and seq_lens [B]");
+  for (const at::Tensor *t : {&x, &k, &tables})
+    for (int64_t d = 0; d < t->dim(); ++d)
+      TORCH_CHECK(t->size(d) <= INT32_MAX, "natten_amd: a dimension is too long");
+  check_devices(x, {&k, &v, &ks, &vs, &tables, &lens});
+  const c10::DeviceGuard guard(x.device());
+  CacheCall r;
+  r.p.batch = (int32_t)x.size(0);
+  r.p.tokens = (int32_t)x.size(1);
+  r.p.heads = (int32_t)x.size(2);
+  r.p.kv_heads = (int32_t)k.size(1);
+  r.p.head_dim = (int32_t)x.size(3);
+  r.p.dtype = dtype_code(x.scalar_type());
+  r.p.pages = (int32_t)k.size(0);
+  r.p.page_size = (int32_t)k.size(2);
+  r.p.table_pages = (int32_t)tables.size(1);
+  r.tables = narrow_ints(tables, -1, INT32_MAX);
+  if (r.tables.size(1) > 1 && r.tables.stride(1) != 1) r.tables = r.tables.contiguous();
+  r.p.table_stride = r.tables.stride(0);
+  r.lens = narrow_ints(lens, 0, (int64_t)1 << 30).contiguous();
+  r.c.key = k.data_ptr();
+  r.c.value = v.data_ptr();
+  r.c.key_scale = ks.data_ptr();
+  r.c.value_scale = vs.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    r.c.key_stride[i] = k.stride(i);
+    r.c.value_stride[i] = v.stride(i);
+  }
+  for (int i = 0; i < 2; ++i) {
+    r.c.key_scale_stride[i] = ks.stride(i);
+    r.c.value_scale_stride[i] = vs.stride(i);
+  }
+  return r;
+}
+
+void na_cache_append_op(const at::Tensor &k, const at::Tensor &v, const at::Tensor &ks,
+                        const at::Tensor &vs, const at::Tensor &key, const at::Tensor &value,
+                        const at::Tensor &tables, const at::Tensor &lens,
+                        const std::optional<at::Tensor> &new_opt, int64_t stream) {
+  TORCH_CHECK(!wants_grad({&key, &value, &k, &v, &ks, &vs}),
+              "natten_amd cache_append serves: it has no backward (under torch.no_grad(), or train "
+              "with na1d)");
+  TORCH_CHECK(key.sizes() == value.sizes() && key.dim() == 4 && key.size(2) == k.size(1) &&
+                  key.scalar_type() == value.scalar_type(),
+              "natten_amd na_cache_append: new keys and values [B, L, H_kv, D] of one dtype, got ",
+              key.sizes(), " and ", value.sizes());
+  CacheCall r = cache_call(key, k, v, ks, vs, tables, lens);
+  const at::Tensor count = new_opt.value_or(at::Tensor());
+  check_devices(key, {&value, &count});
+  const c10::DeviceGuard guard(key.device());
+  at::Tensor nc;
+  if (count.defined()) {
+    TORCH_CHECK(count.dim() == 1 && count.size(0) == key.size(0),
+                "natten_amd na_cache_append: new_lens [B]");
+    nc = narrow_ints(count, 0, key.size(1)).contiguous();
+  }
+  const at::Tensor kc = rows_of(key, r.p.k_stride), vc = rows_of(value, r.p.v_stride);
+  check_rc(na_cache_append(&r.p, &r.c, kc.data_ptr(), vc.data_ptr(),
+                           static_cast<const int32_t *>(r.tables.data_ptr()),
+                           static_cast<const int32_t *>(r.lens.data_ptr()),
+                           static_cast<const int32_t *>(cptr(nc)), as_stream(stream)),
+           "na_cache_append");
+  for (const at::Tensor *t : {&k, &v, &ks, &vs})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<at::Tensor, at::Tensor> na_cache_attend_op(
+    const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &ks,
+    const at::Tensor &vs, const at::Tensor &tables, const at::Tensor &lens, int64_t window,
+    double scale, bool want_lse, int64_t stream) {
+  TORCH_CHECK(!wants_grad({&q, &k, &v, &ks, &vs}),
+              "natten_amd cache_attention serves: it has no backward (under torch.no_grad(), or "
+              "train with na1d)");
+  CacheCall r = cache_call(q, k, v, ks, vs, tables, lens);
+  const c10::DeviceGuard guard(q.device());
+  r.p.window = (int32_t)std::min<int64_t>(std::max<int64_t>(window, 0), 1 << 30);
+  r.p.scale = (float)scale;
+  const at::Tensor qc = rows_of(q, r.p.q_stride);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty(want_lse ? q.sizes().slice(0, 3) : at::IntArrayRef{0},
+                             q.options().dtype(at::kFloat));
+  const size_t bytes = na_cache_attend_workspace_bytes(&r.p);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_rc(na_cache_attend(&r.p, &r.c, qc.data_ptr(),
+                           static_cast<const int32_t *>(r.tables.data_ptr()),
+                           static_cast<const int32_t *>(r.lens.data_ptr()), out.data_ptr(),
+                           want_lse ? static_cast<float *>(lse.data_ptr()) : nullptr, mptr(ws), bytes,
+                           as_stream(stream)),
+           "na_cache_attend");
+  return {out, lse};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(natten_amd, m) {
@@ -1211,6 +1336,14 @@ TORCH_LIBRARY(natten_amd, m) {
   m.def(
       "na_prefix(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor? k, Tensor? v, "
       "Tensor? seq_lens, int window, float scale, bool want_lse, int stream) -> (Tensor, Tensor)");
+  m.def(
+      "na_cache_append(Tensor(a!) k, Tensor(b!) v, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+      "Tensor key, Tensor value, Tensor tables, Tensor seq_lens, Tensor? new_lens, int stream) "
+      "-> ()");
+  m.def(
+      "na_cache_attend(Tensor q, Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, "
+      "Tensor tables, Tensor seq_lens, int window, float scale, bool want_lse, int stream) "
+      "-> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
@@ -1225,4 +1358,6 @@ TORCH_LIBRARY_IMPL(natten_amd, CompositeImplicitAutograd, m) {
   m.impl("na_rotary", na_rotary_op);
   m.impl("na_norm_rotary", na_norm_rotary);
   m.impl("na_prefix", na_prefix);
+  m.impl("na_cache_append", na_cache_append_op);
+  m.impl("na_cache_attend", na_cache_attend_op);
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 from ._core import hip as _hip
 from ._core import ops
+from .cache import PagedCache, cache_append, cache_attention, paged_cache
 from .functional import (
     na1d,
     na1d_av,
@@ -70,6 +71,7 @@ __all__ = [
     "__version__", "na1d", "na1d_varlen", "na1d_varlen_gqa", "na2d", "na2d_varlen", "na1d_qk",
     "na1d_av", "na2d_qk", "na2d_av", "na3d", "na3d_varlen", "na3d_qk", "na3d_av",
     "merge_attentions", "layer_norm", "rotary", "rotary_axis_dims", "norm_rotary", "prefix_attention",
+    "PagedCache", "paged_cache", "cache_append", "cache_attention",
     "NeighborhoodAttention1D", "NeighborhoodAttention2D",
     "NeighborhoodAttention3D", "has_hip", "has_metal", "has_nanobind", "get_backend", "set_backend", "get_support_matrix",
 ]

@@ -199,7 +199,46 @@ class NaPrefixParams(ctypes.Structure):
     ]
 
 
+class NaCache(ctypes.Structure):
+    """Mirror of ``na_cache`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_scale", ctypes.c_void_p),
+        ("value_scale", ctypes.c_void_p),
+        ("key_stride", ctypes.c_int64 * 3),
+        ("value_stride", ctypes.c_int64 * 3),
+        ("key_scale_stride", ctypes.c_int64 * 2),
+        ("value_scale_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class NaCacheParams(ctypes.Structure):
+    """Mirror of ``na_cache_params`` (include/natten_amd.h)."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("table_stride", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+    ]
+
+
 PREFIX_MAX_HEAD_DIM = 256
+CACHE_MAX_HEAD_DIM = 256
+CACHE_PAGE_SIZES = (16, 32, 64, 128)
 NORM_ROTARY_MAX_HEAD_DIM = 256
 MAX_HEAD_DIM = 1024
 ROTARY_MAX_AXES = 4
@@ -214,6 +253,8 @@ _N = ctypes.POINTER(NaNormParams)
 _RO = ctypes.POINTER(NaRotaryParams)
 _NR = ctypes.POINTER(NaNormRotaryParams)
 _PF = ctypes.POINTER(NaPrefixParams)
+_CA = ctypes.POINTER(NaCache)
+_CP = ctypes.POINTER(NaCacheParams)
 _PP = ctypes.POINTER(ctypes.c_void_p)  # host array of device pointers
 _V = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -261,6 +302,9 @@ SIGNATURES = {
     "na_norm_rotary_bwd": (ctypes.c_int, [_NR] + [_V] * 14 + [ctypes.c_size_t, _V]),
     "na_prefix_workspace_bytes": (ctypes.c_size_t, [_PF]),
     "na_prefix_fwd": (ctypes.c_int, [_PF] + [_V] * 8 + [ctypes.c_size_t, _V]),
+    "na_cache_append": (ctypes.c_int, [_CP, _CA] + [_V] * 6),
+    "na_cache_attend_workspace_bytes": (ctypes.c_size_t, [_CP]),
+    "na_cache_attend": (ctypes.c_int, [_CP, _CA] + [_V] * 6 + [ctypes.c_size_t, _V]),
 }
 
 _lib = None
@@ -308,7 +352,8 @@ def _load_fused_op() -> None:
                  "rpb_qk": ns.na_rpb_qk.default, "rpb_av": ns.na_rpb_av.default,
                  "linear": ns.na_linear.default, "fused_qkv": ns.na_fused_qkv.default,
                  "norm": ns.na_layer_norm.default, "rotary": ns.na_rotary.default,
-                 "norm_rotary": ns.na_norm_rotary.default, "prefix": ns.na_prefix.default}
+                 "norm_rotary": ns.na_norm_rotary.default, "prefix": ns.na_prefix.default,
+                 "cache_append": ns.na_cache_append.default, "cache_attend": ns.na_cache_attend.default}
 
 
 def fused_op():
@@ -327,8 +372,9 @@ def node_op(name: str, a: torch.Tensor, b: torch.Tensor):
     """The C++ operator of a split ("qk", "av") or DiNAT ("rpb_qk", "rpb_av")
     op, of a layer's projection ("linear") and packed attention
     ("fused_qkv"), of the layer norm ("norm"), of rotary positions ("rotary"), of both
-    in one pass ("norm_rotary") or of attention behind a shared prefix ("prefix"), where
-    it takes these tensors: built, and both of a supported dtype on one HIP device.  None otherwise (the Python autograd Function then runs
+    in one pass ("norm_rotary"), of attention behind a shared prefix ("prefix") or of a paged cache
+    ("cache_append", "cache_attend"), where it takes these tensors: built, and both of a
+    supported dtype on one HIP device.  None otherwise (the Python autograd Function then runs
     the same kernels, or raises): under compilation, which can leave a Python
     Function to eager execution but not an operator without a fake kernel, while
     tracing, and inside a torch.func transform or a forward-mode level, which a

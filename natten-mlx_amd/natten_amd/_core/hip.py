@@ -782,3 +782,59 @@ def prefix_forward(q, pk, pv, k, v, lens, window, scale, want_lse):
                                      _lib.ptr(v), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), nbytes,
                                      _lib.stream_of(q)), "na_prefix_fwd")
     return out, lse
+
+
+# ---------------------------------------------------------------------------
+# paged cache in 8 bits (C ABI na_cache_append, na_cache_attend)
+
+def _cache_params(cache, x, tables):
+    """``(parameters, cache block)`` for new tokens or queries x ``[B, L, heads, D]``."""
+    p, c = _lib.NaCacheParams(), _lib.NaCache()
+    p.batch, p.tokens, p.heads, p.head_dim = x.shape
+    p.pages, p.kv_heads, p.page_size = cache.key.shape[:3]
+    p.table_pages, p.table_stride = tables.shape[1], tables.stride(0)
+    p.dtype = _lib.dtype_code(x.dtype)
+    for n in ("key", "value"):
+        t, sc = getattr(cache, n), getattr(cache, n + "_scale")
+        setattr(c, n, t.data_ptr())
+        setattr(c, n + "_scale", sc.data_ptr())
+        getattr(c, n + "_stride")[:] = t.stride()[:3]
+        getattr(c, n + "_scale_stride")[:] = sc.stride()
+    return p, c
+
+
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
+def cache_append(cache, key, value, tables, seq_lens, new_lens):
+    """Writes into ``cache`` in place; ``tables``, ``seq_lens`` and ``new_lens`` (or None)
+    int32 on the device."""
+    dev = _require_device(*cache, key, value, tables, seq_lens, new_lens)
+    key, value, tables, seq_lens, new_lens = map(_c, (key, value, tables, seq_lens, new_lens))
+    p, c = _cache_params(cache, key, tables)
+    for st, t in ((p.k_stride, key), (p.v_stride, value)):
+        st[:] = t.stride()[:3]
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().na_cache_append(
+            p, c, *map(_lib.ptr, (key, value, tables, seq_lens, new_lens)), _lib.stream_of(key)),
+            "na_cache_append")
+    for t in cache:
+        torch.autograd.graph.increment_version(t)
+
+
+@torch.compiler.disable  # builds a parameter block, which a trace cannot follow
+def cache_attend(q, cache, tables, seq_lens, window, scale, want_lse):
+    """``(out, lse)``: lse float32 ``[B, L, H]``, or None where not wanted; ``window`` 0
+    for none."""
+    dev = _require_device(q, *cache, tables, seq_lens)
+    q, tables, seq_lens = map(_c, (q, tables, seq_lens))
+    p, c = _cache_params(cache, q, tables)
+    p.window, p.scale = min(int(window), 1 << 30), float(scale)
+    p.q_stride[:] = q.stride()[:3]
+    lib = _lib.load()
+    out = torch.empty_like(q)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if want_lse else None
+    nbytes = int(lib.na_cache_attend_workspace_bytes(p))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.na_cache_attend(p, c, *map(_lib.ptr, (q, tables, seq_lens, out, lse, ws)),
+                                       nbytes, _lib.stream_of(q)), "na_cache_attend")
+    return out, lse

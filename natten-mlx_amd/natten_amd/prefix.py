@@ -68,15 +68,15 @@ class _Prefix(torch.autograd.Function):
         return hip.prefix_forward(q, pk, pv, k, v, lens, window, scale, want_lse)
 
 
-def _host_lens(seq_lens, capacity, device):
+def _host_lens(seq_lens, capacity, device, name="seq_lens"):
     # lengths change with every generated token: nothing is kept of them
     with torch.cuda.device(device):
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("seq_lens on the host cannot be captured in a graph: pass them on "
+            raise RuntimeError(f"{name} on the host cannot be captured in a graph: pass them on "
                                "query's device")
     host = seq_lens.tolist()
     if host and (min(host) < 0 or max(host) > capacity):
-        raise ValueError(f"All seq_lens must be in [0, {capacity}], got {min(host)} to {max(host)}.")
+        raise ValueError(f"All {name} must be in [0, {capacity}], got {min(host)} to {max(host)}.")
     return seq_lens.to(torch.int32).to(device)
 
 

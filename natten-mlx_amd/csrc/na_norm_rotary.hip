@@ -29,10 +29,14 @@ namespace na {
 namespace {
 
 constexpr int kNrBlocks = 1024;  // most workgroups of a backward: four on a CU
+constexpr int kNrUnits = 16;     // units per thread of a run
+constexpr int kNrTable = 2048;   // entries of a run's table, 16 KB
 
 struct NrProb {
   RotProb R;  // per_block: tokens of a run; backward: of q's, qs / ks the rows of x
   int32_t lgG, wide;      // lanes per row; weights are float32
+  int32_t fast;           // no chunk is cut off by a row's end, and a run's rows lie within
+                          // 2^31 bytes of its first token's, samples behind each other
   int32_t per_k, bq, bk;  // backward: tokens of a run of k, workgroups of q and of k
   float eps, inv_d;
   FastDiv fH, fHk;
@@ -44,27 +48,39 @@ template <typename T, int MODE>
 struct NrLane {
   static constexpr int N = Chunk<T>::N, NT = MODE == kRotHalves ? 2 : 1;
   int c[NT], n[NT];
-  int p0;     // entry of the table of its first channel (halves, adjacent: pair)
+  int j, c0;  // unit, its first channel (halves: pair)
   bool turn;  // halves: its channels are rotated
-  __device__ __forceinline__ NrLane(const RotProb &P, int j) {
-    int c0 = j * N, c1 = P.D;
-    p0 = MODE == kRotAdjacent ? c0 / 2 : c0;
+  __device__ __forceinline__ NrLane(const RotProb &P, int unit) : j(unit), c0(unit * N) {
+    int first = c0, second = P.D;
     turn = false;
     if (MODE == kRotHalves) {
       turn = c0 < P.pairs;
       const int a = rot_axis(P, c0);
-      c0 = turn ? p0 + P.first[a] : 2 * p0;
-      c1 = turn ? c0 + P.first[a + 1] - P.first[a] : c0 + N;
+      first = turn ? c0 + P.first[a] : 2 * c0;
+      second = turn ? first + P.first[a + 1] - P.first[a] : first + N;
     }
     const bool live = j < P.upr;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int at = t == 0 ? c0 : c1;
+      const int at = t == 0 ? first : second;
       n[t] = live ? max(P.D - at, 0) : 0;
       c[t] = n[t] > 0 ? at : 0;
     }
   }
 };
+
+// A chunk of which n elements belong to the row.
+template <bool FAST, typename T>
+__device__ __forceinline__ typename Chunk<T>::raw nr_load(const T *p, int n) {
+  if (!FAST) return Chunk<T>::load(p, n);
+  typename Chunk<T>::raw r = {0, 0, 0, 0};
+  if (n > 0) r = *reinterpret_cast<const typename Chunk<T>::mem *>(p);
+  return r;
+}
+template <bool FAST, typename T>
+__device__ __forceinline__ void nr_store(T *p, const float *x, int n) {
+  if (n > 0) Chunk<T>::store(p, x, FAST ? Chunk<T>::N : n);
+}
 
 // The lane's partners in the wave's copy of its rows: channel c of the row whose
 // first lane is `base` lies at (c % N) * 64 + base + c / N.
@@ -83,16 +99,51 @@ struct NrPartner {
   }
 };
 
-// x turned by the table's row `cs` of its token.
+// The table of a token: entry (e, j) is what element e of unit j turns by -- its
+// pair's (cos, sin), staged with the sign that its place in the pair takes -- so that
+// the lanes of a row read next to each other.
+template <typename T, int MODE>
+struct NrTable {
+  static constexpr int N = Chunk<T>::N, E = MODE == kRotAdjacent ? N / 2 : N;
+  static __host__ __device__ __forceinline__ int units(const RotProb &P) {
+    return MODE == kRotHalves ? P.pairs / N : P.upr;
+  }
+  static __host__ __device__ __forceinline__ int size(const RotProb &P) { return E * units(P); }
+  static __device__ __forceinline__ int at(const RotProb &P, int i) {  // i: pair, or channel
+    return i % E * units(P) + i / E;
+  }
+  // Of tokens t0 .. t0 + nt.  A barrier before they are read.
+  static __device__ __forceinline__ void fill(const RotProb &P, const void *pos, const double *rate,
+                                              int t0, int nt, float2 *cs) {
+    const int n = size(P);
+    for (int i = threadIdx.x; i < nt * P.pairs; i += kRotThreads) {
+      const uint32_t t = fdiv((uint32_t)i, P.fpairs), p = (uint32_t)i - t * P.fpairs.d;
+      const int a = rot_axis(P, (int)p);
+      const float2 z = rot_cos_sin(P, pos, rate, (uint32_t)t0 + t, (int)p, a);
+      float2 *const c = cs + (int)t * n;
+      if (MODE == kRotStaged) {
+        const int ch = (int)p + P.first[a];
+        c[at(P, ch)] = make_float2(z.x, -z.y);
+        c[at(P, ch + P.first[a + 1] - P.first[a])] = z;
+      } else {
+        c[at(P, (int)p)] = z;
+      }
+    }
+  }
+};
+
+// x turned by the table `cs` of its token.
 template <typename T, int MODE, int NT, int N>
 __device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> &L,
                                         const NrPartner<N> &other, float *rows, const float2 *cs,
                                         float (&x)[NT][N]) {
+  typedef NrTable<T, MODE> Table;
+  const int units = Table::units(P);
   if constexpr (MODE == kRotHalves) {
     if (!L.turn) return;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float2 z = cs[L.p0 + e];
+      const float2 z = cs[e * units + L.j];
       const float u = x[0][e], v = x[1][e];
       x[0][e] = u * z.x - v * z.y;
       x[1][e] = fmaf(v, z.x, u * z.y);
@@ -100,8 +151,8 @@ __device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> 
   } else if constexpr (MODE == kRotAdjacent) {
 #pragma unroll
     for (int e = 0; e < N; e += 2)
-      if (L.p0 + e / 2 < P.pairs) {
-        const float2 z = cs[L.p0 + e / 2];
+      if (L.c0 + e < 2 * P.pairs) {
+        const float2 z = cs[e / 2 * units + L.j];
         const float u = x[0][e], v = x[0][e + 1];
         x[0][e] = u * z.x - v * z.y;
         x[0][e + 1] = fmaf(v, z.x, u * z.y);
@@ -115,8 +166,8 @@ __device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> 
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (L.p0 + e < 2 * P.pairs) {
-        const float2 z = cs[L.p0 + e];
+      if (L.c0 + e < 2 * P.pairs) {
+        const float2 z = cs[e * units + L.j];
         x[0][e] = fmaf(x[0][e], z.x, rows[other.at[e]] * z.y);
       }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -129,36 +180,66 @@ template <typename T, int MODE, int NT, int N>
 __device__ __forceinline__ void nr_weights(const NrLane<T, MODE> &L, const void *w, int wide,
                                            float none, float (&x)[NT][N]) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      x[t][e] = none;
-      if (w != nullptr && e < L.n[t])
-        x[t][e] = wide ? static_cast<const float *>(w)[L.c[t] + e]
-                       : to_f32(static_cast<const T *>(w)[L.c[t] + e]);
+    for (int e = 0; e < N; ++e) x[t][e] = none;
+    if (w == nullptr) continue;
+    if (wide) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const auto r = Chunk<float>::load(static_cast<const float *>(w) + L.c[t] + min(e, L.n[t]),
+                                          L.n[t] - e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[t][e + i] = Chunk<float>::get(r, i);
+      }
+    } else {
+      const auto r = Chunk<T>::load(static_cast<const T *>(w) + L.c[t], L.n[t]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[t][e] = Chunk<T>::get(r, e);
     }
+  }
 }
 
 // The row less its mean in place; 1 / std.
-template <int NT, int N>
-__device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT], int D, int lgG,
-                                           float inv_d, float eps) {
+template <bool FAST, int NT, int N>
+__device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT], const NrProb &Q) {
   float s = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < N; ++e) s += x[t][e];  // (zeros behind the last channel)
-  const float mean = lanes_sum(s, lgG) / (float)D;
+  const float mean = lanes_sum(s, Q.lgG) / (float)Q.R.D;
   s = 0.f;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    float part = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       x[t][e] -= mean;
-      s = fmaf(e < n[t] ? x[t][e] : 0.f, x[t][e], s);
+      part = fmaf(FAST || e < n[t] ? x[t][e] : 0.f, x[t][e], part);
     }
-  return 1.f / sqrtf(fmaf(lanes_sum(s, lgG), inv_d, eps));
+    s += n[t] > 0 ? part : 0.f;
+  }
+  return 1.f / sqrtf(fmaf(lanes_sum(s, Q.lgG), Q.inv_d, Q.eps));
 }
+
+// Rows of a tensor [.., heads, D] by token and head, from a run's first token.
+template <bool FAST, typename T>
+struct NrRows {
+  const T *p, *run;
+  const int64_t *st;
+  int t0;
+  __device__ __forceinline__ NrRows(const T *tensor, const int64_t *stride, int first)
+      : p(tensor), run(tensor + (int64_t)first * stride[1]), st(stride), t0(first) {}
+  // Row of head h of the run's token t.
+  __device__ __forceinline__ const T *at(const NrProb &Q, int t, int h) const {
+    if (FAST)
+      return reinterpret_cast<const T *>(reinterpret_cast<const char *>(run) +
+                                         (uint32_t)((t * (int)st[1] + h * (int)st[2]) * (int)sizeof(T)));
+    const uint32_t tok = (uint32_t)(t0 + t), b = fdiv(tok, Q.R.fS), s = tok - b * Q.R.fS.d;
+    return p + b * st[0] + s * st[1] + h * st[2];
+  }
+};
 
 // LDS: the table, the rates, staged: the waves' copies of their rows.
 template <typename T, int MODE>
@@ -166,21 +247,20 @@ struct NrSmem {
   float2 *cs;
   double *rate;
   float *rows;
-  __device__ __forceinline__ NrSmem(char *smem, const RotProb &P, int per) {
-    cs = reinterpret_cast<float2 *>(smem);
-    rate = reinterpret_cast<double *>(cs + per * P.pairs * (MODE == kRotStaged ? 2 : 1));
-    rows = reinterpret_cast<float *>(rate + rot_rates(P.pairs)) +
-           (threadIdx.x >> 6) * (64 * Chunk<T>::N);
+  __device__ __forceinline__ NrSmem(char *smem, const RotProb &P) {
+    rate = reinterpret_cast<double *>(smem);
+    rows = reinterpret_cast<float *>(rate + rot_rates(P.pairs));
+    cs = reinterpret_cast<float2 *>(rows + (MODE == kRotStaged ? kRotThreads * Chunk<T>::N : 0));
+    rows += (threadIdx.x >> 6) * (64 * Chunk<T>::N);
+  }
+  static size_t bytes(const RotProb &P, int per) {
+    return sizeof(double) * rot_rates(P.pairs) +
+           (MODE == kRotStaged ? sizeof(float) * kRotThreads * Chunk<T>::N : 0) +
+           sizeof(float2) * per * NrTable<T, MODE>::size(P);
   }
 };
-template <typename T>
-size_t nr_lds(const RotProb &P, int per, RotMode mode) {
-  return sizeof(float2) * per * P.pairs * (mode == kRotStaged ? 2 : 1) +
-         sizeof(double) * rot_rates(P.pairs) +
-         (mode == kRotStaged ? sizeof(float) * kRotThreads * Chunk<T>::N : 0);
-}
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool FAST>
 __global__ void __launch_bounds__(kRotThreads)
     k_nr_fwd(NrProb Q, const T *__restrict__ q, const T *__restrict__ k,
              const void *__restrict__ pos, const void *__restrict__ wq, const void *__restrict__ bq,
@@ -191,42 +271,49 @@ __global__ void __launch_bounds__(kRotThreads)
   constexpr int N = K::N, NT = Lane::NT;
   extern __shared__ __align__(16) char smem[];
   const RotProb &P = Q.R;
-  const NrSmem<T, MODE> S(smem, P, P.per_block);
+  const NrSmem<T, MODE> S(smem, P);
   const int tid = threadIdx.x, G = 1 << Q.lgG;
   const int t0 = blockIdx.x * P.per_block, nt = min(P.per_block, P.tokens - t0);
   const int h0 = blockIdx.y * P.heads_per, nh = min(P.heads_per, P.H + P.Hk - h0);
   const Lane L(P, tid & (G - 1));
-  const NrPartner<N> other(P, L.p0, tid & 63 & ~(G - 1));
+  const NrPartner<N> other(P, L.c0, tid & 63 & ~(G - 1));
+  const int per_step = kRotThreads >> Q.lgG, table = NrTable<T, MODE>::size(P);
   rot_rate(P, S.rate);
-  __syncthreads();
-  rot_table<MODE == kRotStaged>(P, pos, S.rate, t0, nt, S.cs);
-  __syncthreads();
-  const int per_step = kRotThreads >> Q.lgG;
+  bool ready = false;  // the table is there
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
     // heads [ha, ha + hn) of q and k taken together; more than one token: all of them
     const int ha = part == 0 ? h0 : max(h0, P.H);
     const int hn = (part == 0 ? min(h0 + nh, P.H) : h0 + nh) - ha;
     if (hn <= 0) continue;
-    float w[NT][N], b[NT][N];
-    nr_weights(L, part == 0 ? wq : wk, Q.wide, 1.f, w);
-    nr_weights(L, part == 0 ? bq : bk, Q.wide, 0.f, b);
     const int rows = nt * hn;
-    auto place = [&](int r, int &t, int &h) {
-      r = min(r, rows - 1);
-      t = nt == 1 ? 0 : (int)fdiv((uint32_t)r, part == 0 ? Q.fH : Q.fHk);
-      h = ha + r - t * hn;
+    const int first = part == 0 ? ha : ha - P.H;  // head of the first row
+    const NrRows<FAST, T> in(part == 0 ? q : k, part == 0 ? P.qs : P.ks, t0);
+    // (the heads of a token lie behind each other, so do the rows of a run)
+    T *const out = (part == 0 ? oq : ok) +
+                   ((int64_t)t0 * (part == 0 ? P.H : P.Hk) + first) * P.D;
+    auto token = [&](int r) {
+      return nt == 1 ? 0 : (int)fdiv((uint32_t)r, part == 0 ? Q.fH : Q.fHk);
     };
     typename K::raw next[NT];
     auto fetch = [&](int r) {
-      int t, h;
-      place(r, t, h);
-      const RotRow<T> at(P, q, k, oq, ok, (uint32_t)(t0 + t), h);
+      r = min(r, rows - 1);
+      const int t = token(r);
+      const T *const x = in.at(Q, t, first + r - t * hn);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) next[i] = K::load(at.src + L.c[i], L.n[i]);
+      for (int i = 0; i < NT; ++i) next[i] = nr_load<FAST>(x + L.c[i], L.n[i]);
     };
     int r = tid >> Q.lgG;
     fetch(r);
+    float w[NT][N], b[NT][N];
+    nr_weights(L, part == 0 ? wq : wk, Q.wide, 1.f, w);
+    nr_weights(L, part == 0 ? bq : bk, Q.wide, 0.f, b);
+    if (!ready) {
+      __syncthreads();  // the rates are there
+      NrTable<T, MODE>::fill(P, pos, S.rate, t0, nt, S.cs);
+      __syncthreads();
+      ready = true;
+    }
     for (int r0 = 0; r0 < rows; r0 += per_step, r += per_step) {  // the same steps for every lane
       float x[NT][N];
 #pragma unroll
@@ -234,19 +321,16 @@ __global__ void __launch_bounds__(kRotThreads)
 #pragma unroll
         for (int e = 0; e < N; ++e) x[i][e] = K::get(next[i], e);
       if (r0 + per_step < rows) fetch(r + per_step);
-      const float rstd = nr_center(x, L.n, P.D, Q.lgG, Q.inv_d, Q.eps);
+      const float rstd = nr_center<FAST>(x, L.n, Q);
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < N; ++e) x[i][e] = fmaf(x[i][e] * rstd, w[i][e], b[i][e]);
-      int t, h;
-      place(r, t, h);
-      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + t * P.pairs * (MODE == kRotStaged ? 2 : 1), x);
+      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + token(min(r, rows - 1)) * table, x);
       if (r >= rows) continue;
-      const RotRow<T> at(P, q, k, oq, ok, (uint32_t)(t0 + t), h);
+      T *const y = out + r * P.D;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (L.n[i] > 0) K::store(at.dst + L.c[i], x[i], L.n[i]);
+      for (int i = 0; i < NT; ++i) nr_store<FAST>(y + L.c[i], x[i], L.n[i]);
     }
   }
 }
@@ -257,7 +341,7 @@ struct NrGrads {
   float *part;  // [bq + bk][2][D], or null: no sums wanted
 };
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool FAST>
 __global__ void __launch_bounds__(kRotThreads)
     k_nr_bwd(NrProb Q, NrGrads A, const void *__restrict__ pos) {
   typedef Chunk<T> K;
@@ -268,10 +352,11 @@ __global__ void __launch_bounds__(kRotThreads)
   const bool isq = (int)blockIdx.x < Q.bq;
   const int per = isq ? P.per_block : Q.per_k, heads = isq ? P.H : P.Hk;
   const int block = isq ? blockIdx.x : blockIdx.x - Q.bq, blocks = isq ? Q.bq : Q.bk;
-  const NrSmem<T, MODE> S(smem, P, per);
+  const NrSmem<T, MODE> S(smem, P);
+  const int table = NrTable<T, MODE>::size(P);
   const int tid = threadIdx.x, G = 1 << Q.lgG;
   const Lane L(P, tid & (G - 1));
-  const NrPartner<N> other(P, L.p0, tid & 63 & ~(G - 1));
+  const NrPartner<N> other(P, L.c0, tid & 63 & ~(G - 1));
   const T *const x = static_cast<const T *>(isq ? A.q : A.k);
   const T *const g = static_cast<const T *>(isq ? A.gq : A.gk);
   T *const dx = static_cast<T *>(isq ? A.dq : A.dk);
@@ -287,28 +372,24 @@ __global__ void __launch_bounds__(kRotThreads)
   const int per_step = kRotThreads >> Q.lgG;
   for (int64_t first = (int64_t)block * per; first < P.tokens; first += (int64_t)blocks * per) {
     const int t0 = (int)first, nt = min(per, P.tokens - t0), rows = nt * heads;
-    auto place = [&](int r, int &t, int &h) {
-      r = min(r, rows - 1);
-      t = nt == 1 ? 0 : (int)fdiv((uint32_t)r, isq ? Q.fH : Q.fHk);
-      h = r - t * heads;
-    };
+    const NrRows<FAST, T> xin(x, xs, t0), gin(g, gs, t0);
+    T *const out = dx == nullptr ? nullptr : dx + (int64_t)t0 * heads * P.D;
+    auto token = [&](int r) { return nt == 1 ? 0 : (int)fdiv((uint32_t)r, isq ? Q.fH : Q.fHk); };
     typename K::raw nx[NT], ng[NT];
     auto fetch = [&](int r) {
-      int t, h;
-      place(r, t, h);
-      const uint32_t tok = (uint32_t)(t0 + t), b = fdiv(tok, P.fS), s = tok - b * P.fS.d;
-      const T *const px = x + b * xs[0] + s * xs[1] + h * xs[2];
-      const T *const pg = g + b * gs[0] + s * gs[1] + h * gs[2];
+      const int in = min(r, rows - 1), t = token(in), h = in - t * heads;
+      const T *const px = xin.at(Q, t, h), *const pg = gin.at(Q, t, h);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        nx[i] = K::load(px + L.c[i], L.n[i]);
-        ng[i] = K::load(pg + L.c[i], r < rows ? L.n[i] : 0);  // rows past the last add nothing
+        nx[i] = nr_load<FAST>(px + L.c[i], L.n[i]);
+        // rows past the last add nothing
+        ng[i] = nr_load<FAST>(pg + L.c[i], r < rows ? L.n[i] : 0);
       }
     };
     int r = tid >> Q.lgG;
     fetch(r);
     __syncthreads();  // the rates are there; the run before is done with its table
-    rot_table<MODE == kRotStaged>(P, pos, S.rate, t0, nt, S.cs);
+    NrTable<T, MODE>::fill(P, pos, S.rate, t0, nt, S.cs);
     __syncthreads();
     for (int r0 = 0; r0 < rows; r0 += per_step, r += per_step) {  // the same steps for every lane
       float h[NT][N], d[NT][N];
@@ -320,10 +401,8 @@ __global__ void __launch_bounds__(kRotThreads)
           d[i][e] = K::get(ng[i], e);
         }
       if (r0 + per_step < rows) fetch(r + per_step);
-      int t, hd;
-      place(r, t, hd);
-      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + t * P.pairs * (MODE == kRotStaged ? 2 : 1), d);
-      const float rstd = nr_center(h, L.n, P.D, Q.lgG, Q.inv_d, Q.eps);
+      nr_turn<T, MODE>(P, L, other, S.rows, S.cs + token(min(r, rows - 1)) * table, d);
+      const float rstd = nr_center<FAST>(h, L.n, Q);
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
@@ -336,16 +415,15 @@ __global__ void __launch_bounds__(kRotThreads)
           s0 += d[i][e];  // (zeros behind the last channel)
           s1 = fmaf(d[i][e], h[i][e], s1);
         }
-      if (dx == nullptr) continue;
+      if (out == nullptr) continue;
       s0 = lanes_sum(s0, Q.lgG) * Q.inv_d;
       s1 = lanes_sum(s1, Q.lgG) * Q.inv_d;
       if (r >= rows) continue;
-      T *const out = dx + ((int64_t)(t0 + t) * heads + hd) * P.D;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
 #pragma unroll
         for (int e = 0; e < N; ++e) d[i][e] = rstd * (d[i][e] - s0 - h[i][e] * s1);
-        if (L.n[i] > 0) K::store(out + L.c[i], d[i], L.n[i]);
+        nr_store<FAST>(out + r * P.D + L.c[i], d[i], L.n[i]);
       }
     }
   }
@@ -420,29 +498,9 @@ NrProb nr_prob(const na_norm_rotary_params *p, RotMode *mode) {
     Q.gqs[i] = p->dq_stride[i];
     Q.gks[i] = p->dk_stride[i];
   }
+  if (Q.R.fS.d == 1)  // one token a sample: the next one is the next sample's
+    for (int64_t *st : {Q.R.qs, Q.R.ks, Q.gqs, Q.gks}) st[1] = st[0];
   return Q;
-}
-
-// Tokens of a run: kRotUnits units per thread, as many as the table holds; fewer
-// where the runs would not be `blocks`.
-int nr_run(const RotProb &P, RotMode mode, int heads, int blocks) {
-  const int entries = P.pairs * (mode == kRotStaged ? 2 : 1);
-  const int64_t row_units = std::max<int64_t>((int64_t)heads * P.upr, 1);
-  int64_t per = std::max<int64_t>(1, kRotUnits * kRotThreads / row_units);
-  per = std::min<int64_t>(per, std::max(1, kRotTable / entries));
-  return (int)std::min<int64_t>(per, std::max<int64_t>(1, P.tokens / blocks));
-}
-
-// The backward's runs and workgroups, shared out by the heads of q and k.
-void nr_bwd_plan(NrProb &Q, RotMode mode) {
-  RotProb &P = Q.R;
-  auto part = [&](int heads, int32_t *per, int32_t *blocks) {
-    const int most = std::max(1, (int)((int64_t)kNrBlocks * heads / (P.H + P.Hk)));
-    *per = nr_run(P, mode, heads, most);
-    *blocks = heads == 0 ? 0 : (int)std::min<int64_t>(most, ((int64_t)P.tokens + *per - 1) / *per);
-  };
-  part(P.H, &P.per_block, &Q.bq);
-  part(P.Hk, &Q.per_k, &Q.bk);
 }
 
 template <typename F>
@@ -457,6 +515,47 @@ void nr_by_type(int dtype, RotMode mode, F &&f) {
   else by_mode(bf16_t{});
 }
 
+// Entries of a token's table.
+int nr_entries(const RotProb &P, int dtype, RotMode mode) {
+  int n = 0;
+  nr_by_type(dtype, mode, [&](auto t, auto m) {
+    n = NrTable<decltype(t), decltype(m)::value>::size(P);
+  });
+  return n;
+}
+
+// Whether rows of runs of up to `per` tokens are and lie as NrProb::fast says.
+bool nr_fast(const RotProb &P, int dtype, const int64_t *st, int heads, int per) {
+  if (P.D % (dtype == NA_F32 ? 4 : 8) != 0) return false;
+  if (P.fS.d > 1 && (uint32_t)P.tokens > P.fS.d && st[0] != st[1] * (int64_t)P.fS.d) return false;
+  if (st[1] < 0 || st[2] < 0 || st[1] >= (1 << 30) || st[2] >= (1 << 30)) return false;
+  return (per * st[1] + heads * st[2]) * (dtype == NA_F32 ? 4 : 2) < ((int64_t)1 << 31);
+}
+
+// Tokens of a run: kNrUnits units per thread, as many as the table holds; fewer
+// where the runs would not be `blocks`.
+int nr_run(const RotProb &P, int entries, int heads, int blocks) {
+  const int64_t row_units = std::max<int64_t>((int64_t)heads * P.upr, 1);
+  int64_t per = std::max<int64_t>(1, kNrUnits * kRotThreads / row_units);
+  per = std::min<int64_t>(per, std::max(1, kNrTable / entries));
+  return (int)std::min<int64_t>(per, std::max<int64_t>(1, P.tokens / blocks));
+}
+
+// The backward's runs and workgroups, shared out by the heads of q and k.
+void nr_bwd_plan(NrProb &Q, int dtype, RotMode mode) {
+  RotProb &P = Q.R;
+  const int entries = nr_entries(P, dtype, mode);
+  auto part = [&](int heads, int32_t *per, int32_t *blocks) {
+    const int most = std::max(1, (int)((int64_t)kNrBlocks * heads / (P.H + P.Hk)));
+    *per = nr_run(P, entries, heads, most);
+    *blocks = heads == 0 ? 0 : (int)std::min<int64_t>(most, ((int64_t)P.tokens + *per - 1) / *per);
+  };
+  part(P.H, &P.per_block, &Q.bq);
+  part(P.Hk, &Q.per_k, &Q.bk);
+  Q.fast = nr_fast(P, dtype, P.qs, P.H, P.per_block) && nr_fast(P, dtype, Q.gqs, P.H, P.per_block) &&
+           nr_fast(P, dtype, P.ks, P.Hk, Q.per_k) && nr_fast(P, dtype, Q.gks, P.Hk, Q.per_k);
+}
+
 }  // namespace
 
 bool norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *k, const void *pos,
@@ -467,17 +566,21 @@ bool norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *
   RotProb &P = Q.R;
   // the heads of a token are shared out where there are few tokens
   const int heads = P.H + P.Hk;
-  P.per_block = nr_run(P, mode, heads, kRotBlocks);
+  P.per_block = nr_run(P, nr_entries(P, p->rotary.dtype, mode), heads, kRotBlocks);
   P.heads_per = heads;
   if (P.per_block == 1 && P.tokens < kRotBlocks)
     P.heads_per = std::min(heads, kRotThreads >> Q.lgG);
+  Q.fast = nr_fast(P, p->rotary.dtype, P.qs, P.H, P.per_block) &&
+           nr_fast(P, p->rotary.dtype, P.ks, P.Hk, P.per_block);
   const dim3 grid((unsigned)(((int64_t)P.tokens + P.per_block - 1) / P.per_block),
                   (unsigned)((heads + P.heads_per - 1) / P.heads_per));
   if (grid.x >= ((int64_t)1 << 32) / kRotThreads || grid.y > 65535) return false;  // a launch ends there
   nr_by_type(p->rotary.dtype, mode, [&](auto t, auto m) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_nr_fwd<T, decltype(m)::value>), grid, dim3(kRotThreads),
-                       nr_lds<T>(P, P.per_block, mode), st, Q, (const T *)q, (const T *)k, pos, wq,
+    const size_t lds = NrSmem<T, decltype(m)::value>::bytes(P, P.per_block);
+    const auto kernel = Q.fast ? k_nr_fwd<T, decltype(m)::value, true>
+                               : k_nr_fwd<T, decltype(m)::value, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kRotThreads), lds, st, Q, (const T *)q, (const T *)k, pos, wq,
                        bq, wk, bk, (T *)oq, (T *)ok);
   });
   return true;
@@ -486,7 +589,7 @@ bool norm_rotary_fwd(const na_norm_rotary_params *p, const void *q, const void *
 size_t norm_rotary_workspace(const na_norm_rotary_params *p) {
   RotMode mode;
   NrProb Q = nr_prob(p, &mode);
-  nr_bwd_plan(Q, mode);
+  nr_bwd_plan(Q, p->rotary.dtype, mode);
   return sizeof(float) * 2 * (size_t)Q.R.D * (size_t)(Q.bq + Q.bk);
 }
 
@@ -497,15 +600,17 @@ void norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void *
   RotMode mode;
   NrProb Q = nr_prob(p, &mode);
   Q.R.sign = -1.f;  // the gradients turn back
-  nr_bwd_plan(Q, mode);
+  nr_bwd_plan(Q, p->rotary.dtype, mode);
   const bool sums = dwq != nullptr || dbq != nullptr || dwk != nullptr || dbk != nullptr;
   const NrGrads A{q, k, wq, wk, gq, gk, dq, dk, sums ? static_cast<float *>(workspace) : nullptr};
   nr_by_type(p->rotary.dtype, mode, [&](auto t, auto m) {
     using T = decltype(t);
-    const size_t lds = std::max(nr_lds<T>(Q.R, std::max(Q.R.per_block, Q.per_k), mode),
-                                sizeof(float) * 8 * Q.R.D);
+    const size_t lds = std::max(
+        NrSmem<T, decltype(m)::value>::bytes(Q.R, std::max(Q.R.per_block, Q.per_k)),
+        sizeof(float) * 8 * Q.R.D);
     if (Q.bq + Q.bk > 0)
-      hipLaunchKernelGGL((k_nr_bwd<T, decltype(m)::value>), dim3(Q.bq + Q.bk), dim3(kRotThreads), lds,
+      hipLaunchKernelGGL((Q.fast ? k_nr_bwd<T, decltype(m)::value, true>
+                                 : k_nr_bwd<T, decltype(m)::value, false>), dim3(Q.bq + Q.bk), dim3(kRotThreads), lds,
                          st, Q, A, pos);
     if (sums)  // (no rows: zeros)
       hipLaunchKernelGGL((k_nr_wsum<T>), dim3((2 * Q.R.D + 31) / 32, 2), dim3(1024), 0, st, A.part,

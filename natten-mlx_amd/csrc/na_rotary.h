@@ -91,25 +91,31 @@ __device__ __forceinline__ void rot_rate(const RotProb &P, double *rate) {
               0.15915494309189533577;
 }
 
-// (cos, sin) of tokens t0 .. t0 + nt: [nt][pairs], or [nt][2 pairs] by channel with
-// the sine's sign in it.  A barrier before they are read.
+// (cos, sin) of the angle by which token `tok` turns pair p of axis a.
+__device__ __forceinline__ float2 rot_cos_sin(const RotProb &P, const void *pos, const double *rate,
+                                              uint32_t tok, int p, int a) {
+  const uint32_t b = fdiv(tok, P.fS);
+  const double turns = rot_position(P, pos, b, tok - b * P.fS.d, a) * rate[p];
+  float sn, cn;
+  sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
+  return make_float2(cn, sn * P.sign);
+}
+
+// Those of tokens t0 .. t0 + nt: [nt][pairs], or [nt][2 pairs] by channel with the
+// sine's sign in it.  A barrier before they are read.
 template <bool BY_CHANNEL>
 __device__ __forceinline__ void rot_table(const RotProb &P, const void *pos, const double *rate,
                                           int t0, int nt, float2 *cs) {
   for (int i = threadIdx.x; i < nt * P.pairs; i += kRotThreads) {
     const uint32_t t = fdiv((uint32_t)i, P.fpairs), p = (uint32_t)i - t * P.fpairs.d;
     const int a = rot_axis(P, (int)p);
-    const uint32_t tok = (uint32_t)t0 + t, b = fdiv(tok, P.fS);
-    const double turns = rot_position(P, pos, b, tok - b * P.fS.d, a) * rate[p];
-    float sn, cn;
-    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
-    sn *= P.sign;
+    const float2 z = rot_cos_sin(P, pos, rate, (uint32_t)t0 + t, (int)p, a);
     if (BY_CHANNEL) {
       float2 *const c = cs + 2 * ((int)t * P.pairs + P.first[a]) + ((int)p - P.first[a]);
-      c[0] = make_float2(cn, -sn);
-      c[P.first[a + 1] - P.first[a]] = make_float2(cn, sn);
+      c[0] = make_float2(z.x, -z.y);
+      c[P.first[a + 1] - P.first[a]] = z;
     } else {
-      cs[i] = make_float2(cn, sn);
+      cs[i] = z;
     }
   }
 }

@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
+constexpr int kJoin = 8;    // parts that a thread of the join loads at once
 
 struct CacheProb {
   int32_t B, Lq, H, Hkv, rep, D;
@@ -95,33 +96,40 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Units of all items of a head.
-__device__ __forceinline__ int64_t cache_total(const CacheProb &P) {
-  int64_t sum = 0;
-  for (int i0 = 0; i0 < P.items; i0 += 64) {
+// The items of a head in order, 64 at a time, their units added up.
+struct CacheScan {
+  int i0 = -64, sum = 0, mine = 0, all = 0;  // first item, the lane's sums, of all 64
+  __device__ __forceinline__ void load(const CacheProb &P, int first) {
+    if (first == i0) return;
+    i0 = first;
     const int i = i0 + (threadIdx.x & 63);
-    const int u = i < P.items ? cache_item(P, i).units : 0;
-    sum += __builtin_amdgcn_readlane(wave_scan(u), 63);
+    mine = i < P.items ? cache_item(P, i).units : 0;
+    sum = wave_scan(mine);
+    all = __builtin_amdgcn_readlane(sum, 63);
   }
-  return sum;
-}
-
-// The item that unit u of a head lies in; u becomes the unit within it.
-__device__ __forceinline__ int cache_find(const CacheProb &P, int64_t &u) {
-  for (int i0 = 0; i0 < P.items; i0 += 64) {
-    const int i = i0 + (threadIdx.x & 63);
-    const int mine = i < P.items ? cache_item(P, i).units : 0;
-    const int sum = wave_scan(mine);
-    const int all = __builtin_amdgcn_readlane(sum, 63);
-    if (u < all) {
-      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > (int)u));
-      u -= __builtin_amdgcn_readlane(sum - mine, at);
-      return i0 + at;
+  // Units of all items.
+  __device__ __forceinline__ int64_t total(const CacheProb &P) {
+    int64_t t = 0;
+    for (int i = 0; i < P.items; i += 64) {
+      load(P, i);
+      t += all;
     }
-    u -= all;
+    return t;
   }
-  return P.items;  // not reached: u is less than the total
-}
+  // The item that unit u lies in; u becomes the unit within it.
+  __device__ __forceinline__ int find(const CacheProb &P, int64_t &u) {
+    for (int i = 0; i < P.items; i += 64) {
+      load(P, i);
+      if (u < all) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > (int)u));
+        u -= __builtin_amdgcn_readlane(sum - mine, at);
+        return i0 + at;
+      }
+      u -= all;
+    }
+    return P.items;  // not reached: u is less than the total
+  }
+};
 
 // 64 entries of a sample's table, one a lane: the page or -1, its scales' bytes.
 struct PageWindow {
@@ -313,9 +321,11 @@ __device__ __forceinline__ void cache_odd_pv(const float (&p)[N], const __bf16 *
       if ((unsigned)(key - lo) >= (unsigned)n) continue;
       const __bf16 *v = vs + key * stride + 4 * gq;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+      for (int db = 0; db < NDB; ++db) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[db][c] = fmaf(pk, (float)v[16 * db + c], o[db][c]);
+        __builtin_amdgcn_sched_barrier(0);  // few registers rather than loads ahead
+      }
     }
 }
 
@@ -362,42 +372,38 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   }
   const int vc = lane % UPR, vr = lane / UPR;
   u4 kr[2][NS], vr8[NU];
-  float ksc[2], vsc[2];
+  int entry[2];  // of the table, of the loaded tile's halves
   bool bad = false;
   PageWindow win;
   win.base = -64;
-  const uint8_t *const kb0 = P.k.code + g * P.k.st[1] + (int64_t)n * P.k.st[2] + 16 * gq;
-  const uint8_t *const vb0 = P.v.code + g * P.v.st[1] + (int64_t)vr * P.v.st[2] + 16 * vc;
+  const uint8_t *const kg = P.k.code + g * P.k.st[1], *const vg = P.v.code + g * P.v.st[1];
+  const uint32_t ko = (uint32_t)(n * (int)P.k.st[2] + 16 * gq);
+  const uint32_t vo = (uint32_t)(vr * (int)P.v.st[2] + 16 * vc);
   // Keys that no row sees are not read: zeros (0 times them is 0).
   const int seen0 = max(ka, w.lo), seen1 = min(kb, w.hi);
   auto load = [&](int t0) {
-    bad = false;
     const bool whole = t0 >= seen0 && t0 + kTile <= seen1 && P.D == D;
     int page[2];
+    entry[0] = t0 >> P.lgT;
+    entry[1] = (t0 + 16) >> P.lgT;
+    if (!win.holds(entry[0]) || !win.holds(entry[1])) win.load(P, w.b, g, entry[0]);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int i = (t0 + 16 * hh) >> P.lgT;
-      if (!win.holds(i)) win.load(P, w.b, g, i);
-      page[hh] = win.page_of(i);
-      const int sc = win.scales_of(i);
-      ksc[hh] = scale_of(sc & 255);
-      vsc[hh] = scale_of(sc >> 8);
-      bad |= page[hh] < 0;
-    }
-    const int slot0 = t0 & ((1 << P.lgT) - 1), slot1 = (t0 + 16) & ((1 << P.lgT) - 1);
-    const uint8_t *const ap[2] = {kb0 + page[0] * P.k.st[0] + slot0 * P.k.st[2],
-                                  kb0 + page[1] * P.k.st[0] + slot1 * P.k.st[2]};
-    const uint8_t *const bp[2] = {vb0 + page[0] * P.v.st[0] + slot0 * P.v.st[2],
-                                  vb0 + page[1] * P.v.st[0] + slot1 * P.v.st[2]};
+    for (int hh = 0; hh < 2; ++hh) page[hh] = win.page_of(entry[hh]);
+    bad = page[0] < 0 || page[1] < 0;
+    const int mask = (1 << P.lgT) - 1;
+    const uint8_t *const ap[2] = {kg + page[0] * P.k.st[0] + (t0 & mask) * P.k.st[2],
+                                  kg + page[1] * P.k.st[0] + ((t0 + 16) & mask) * P.k.st[2]};
+    const uint8_t *const bp[2] = {vg + page[0] * P.v.st[0] + (t0 & mask) * P.v.st[2],
+                                  vg + page[1] * P.v.st[0] + ((t0 + 16) & mask) * P.v.st[2]};
     if (whole && !bad) {
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s);
+          kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s + ko);
 #pragma unroll
       for (int i = 0; i < NU; ++i)
-        vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2]);
+        vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2] + vo);
     } else {
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
@@ -407,7 +413,7 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
         for (int s = 0; s < NS; ++s) {
           kr[hh][s] = u4{0, 0, 0, 0};
           if (live && 64 * s + 16 * gq < P.D)
-            kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s);
+            kr[hh][s] = *reinterpret_cast<const u4 *>(ap[hh] + 64 * s + ko);
         }
       }
 #pragma unroll
@@ -415,13 +421,8 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
         const int key = t0 + RPP * i + vr;
         vr8[i] = u4{0, 0, 0, 0};
         if (page[RPP * i / 16] >= 0 && key >= seen0 && key < seen1 && 16 * vc < P.D)
-          vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2]);
+          vr8[i] = *reinterpret_cast<const u4 *>(bp[RPP * i / 16] + (RPP * i % 16) * P.v.st[2] + vo);
       }
-    }
-    // (a page that is none: its keys' scores are taken out below)
-    if (bad) {
-      if (page[0] < 0) ksc[0] = -1.f;
-      if (page[1] < 0) ksc[1] = -1.f;
     }
   };
   f32x4 o[NQ][NDB];
@@ -440,6 +441,15 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   auto run_tile = [&](int t0, auto edge_tile) {
     constexpr bool EDGE = decltype(edge_tile)::value;
     f32x4 s[NQ][2];
+    float ksc[2], vsc[2];
+    bool none[2] = {false, false};  // no page: keys that nothing sees
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int sc = win.scales_of(entry[hh]);
+      ksc[hh] = scale_of(sc & 255);
+      vsc[hh] = scale_of(sc >> 8);
+      if (EDGE) none[hh] = win.page_of(entry[hh]) < 0;
+    }
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
@@ -461,7 +471,6 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
       *reinterpret_cast<bf8 *>(d) = decode8(vr8[i][0], vr8[i][1], sc);
       *reinterpret_cast<bf8 *>(d + 8) = decode8(vr8[i][2], vr8[i][3], sc);
     }
-    const bool none[2] = {EDGE && ksc[0] < 0.f, EDGE && ksc[1] < 0.f};
     if (t0 + NW * kTile < kb) load(t0 + NW * kTile);  // in flight during the rest
     float p[NQ][8];
 #pragma unroll
@@ -548,10 +557,313 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   __syncthreads();  // before the next item's tiles
 }
 
+template <int D>
+constexpr int cache_tile() {
+  return D > 128 ? 32 : 64;  // keys of a wide tile
+}
+
+// Wide: 16 NQ rows per wave; half of the waves stage the keys of a tile in LDS as
+// bf16, half the values, for all of them, one barrier per tile.
+template <typename T, int D, int NQ, int NW>
+__device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &A,
+                                           const CacheItem &w, int g, int ka, int kb, int part,
+                                           char *smem) {
+  constexpr int NP = cache_parts<T>();
+  constexpr int TK = cache_tile<D>(), CH = TK / 16;
+  constexpr int NT = D / 32, NDB = D / 16, RSE = lds_row(D);
+  constexpr int UPR = D / 16, RPW = 64 / UPR, RPP = RPW * NW / 2, NU = TK / RPP;
+  __bf16 *const buf = reinterpret_cast<__bf16 *>(smem);
+  const int tid = threadIdx.x, wv = uniform(tid >> 6), lane = tid & 63;
+  const int n = lane & 15, gq = lane >> 4;
+
+  // staging: the lane's unit and row of the wave's RPW; the wave's first row of a pass
+  const bool isv = wv >= NW / 2;
+  const CachePages &G = isv ? P.v : P.k;
+  const int col = 16 * (lane % UPR), rl = lane / UPR, rw = (isv ? wv - NW / 2 : wv) * RPW;
+  const uint8_t *const code = G.code + g * G.st[1];
+  const uint32_t off = (uint32_t)(rl * (int)G.st[2] + col);
+  const int unit = (rw + rl) * RSE + (isv ? lds_y(D) : 0) + col;
+  const int seen0 = max(ka, w.lo), seen1 = min(kb, w.hi);
+  PageWindow win;
+  win.base = -64;
+  auto entry_of = [&](int key) {  // of the table, in the window
+    const int e = key >> P.lgT;
+    if (!win.holds(e)) win.load(P, w.b, g, e);
+    return e;
+  };
+  bool bad = false;  // the part's table names a page that is none
+  for (int e = (kb - 1) >> P.lgT; e >= ka >> P.lgT; e -= 64) {
+    const int first = max(e - 63, ka >> P.lgT);
+    win.load(P, w.b, g, first);
+    const int mine = first + lane;
+    bad |= __builtin_amdgcn_ballot_w64(mine <= e && win.page < 0) != 0;
+  }
+  u4 pre[NU];
+  float sc[NU];
+  const int nkt = (kb - ka + TK - 1) / TK;
+  // The tiles that every row sees in full are [ja, jb); they come first, then
+  // those behind them, then those before.
+  int ja = (max(w.lo_max - ka, 0) + TK - 1) / TK, jb = max(min(w.hi_min, kb) - ka, 0) / TK;
+  if (jb <= ja || bad) ja = jb = 0;
+  auto first_key = [&](int i) {  // of the i-th tile
+    const int j = ja + i;
+    return ka + (j < nkt ? j : j - nkt) * TK;
+  };
+  // V of the i-th tile and K of the next: the scores run one tile ahead.
+  auto fetch = [&](int i) {
+    const int mine = isv ? i : i + 1;
+    const int t0 = first_key(max(min(mine, nkt - 1), 0));
+    const bool some = mine >= 0 && mine < nkt;
+    const bool whole = some && !bad && t0 >= seen0 && t0 + TK <= seen1 && P.D == D;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int key = t0 + rw + RPP * u;  // the wave's rows: one page's
+      const int e = entry_of(key), page = win.page_of(e), both = win.scales_of(e);
+      sc[u] = scale_of(isv ? both >> 8 : both & 255);
+      const uint8_t *const p = code + page * G.st[0] + (key & ((1 << P.lgT) - 1)) * G.st[2];
+      if (whole) {
+        pre[u] = *reinterpret_cast<const u4 *>(p + off);
+      } else {  // zeros for keys that no row sees and channels past the last: 0 times them is 0
+        pre[u] = u4{0, 0, 0, 0};
+        if (some && page >= 0 && key + rl >= seen0 && key + rl < seen1 && col < P.D)
+          pre[u] = *reinterpret_cast<const u4 *>(p + off);
+      }
+    }
+  };
+  auto put = [&](int i) {
+    __bf16 *const d = buf + ((isv ? i : i + 1) & 1) * (TK * RSE) + unit;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      *reinterpret_cast<bf8 *>(d + RPP * u * RSE) = decode8(pre[u][0], pre[u][1], sc[u]);
+      *reinterpret_cast<bf8 *>(d + RPP * u * RSE + 8) = decode8(pre[u][2], pre[u][3], sc[u]);
+    }
+  };
+  fetch(-1);
+
+  const int row0 = w.row0 + wv * (16 * NQ);
+  bf8 qf[NQ][NT][NP];
+  int lo[NQ], cnt[NQ];  // keys that a row sees
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const CacheRow<T> r(P, A, w, g, row0 + 16 * qi + n);
+    lo[qi] = r.lo;
+    cnt[qi] = r.n;
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const int c = 32 * s + 8 * gq;
+      query8<T, NP>(r.q + c, c < P.D, qf[qi][s]);
+    }
+  }
+  f32x4 o[NQ][NDB];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[qi][db] = zero4();
+    m[qi] = -INFINITY;
+    l[qi] = 0.f;
+  }
+  const float sl2 = P.sl2;
+  const int ka_off = n * RSE + 8 * gq;
+  const int tr_off = (4 * gq + (n >> 2)) * RSE + 4 * (n & 3);
+  const bool spans = P.Lq > 1;  // rows may see different keys
+
+  auto values = [&](const __bf16 *vs, int jj, int db) {  // V^T of 32 keys
+    const __bf16 *ca = vs + 32 * jj * RSE + tr_off + 16 * db;
+    const bf4 lo4 = M16::tr(ca), hi4 = M16::tr(ca + 16 * RSE);
+    return (bf8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto product = [&](bf8 a, const bf8 (&b)[NP], f32x4 c) {
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p) c = M16::mma(a, b[p], c);
+    return c;
+  };
+  typedef f32x4 Scores[NQ][CH];
+  Scores sa, sb;  // of the tile at hand and of the next
+  float mx[NQ];   // the lane's largest score of the tile at hand
+  auto largest = [&](const Scores &s, int qi, int ch) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mx[qi] = fmaxf(mx[qi], s[qi][ch][r]);
+  };
+  // The i-th tile, its scores in `s`; the next tile's go to `next`.  EDGE: some
+  // row does not see some of its keys.  Matrix products are issued between the vector
+  // ALU's work, which fills the matrix unit's time: the next tile's scores beside the
+  // first half of the exponentials, O beside the second.
+  auto run_tile = [&](int i, Scores &s, Scores &next, auto edge_tile) {
+    constexpr bool EDGE = decltype(edge_tile)::value;
+    const __bf16 *vs = buf + (i & 1) * (TK * RSE) + lds_y(D);
+    const __bf16 *ks = buf + ((i + 1) & 1) * (TK * RSE) + ka_off;
+    const int t0 = first_key(i);
+    int none = 0;  // groups of 16 keys of no page, one a bit
+    if (EDGE && bad) {
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+        none |= win.page_of(entry_of(t0 + 16 * ch)) < 0 ? 1 << ch : 0;
+    }
+    fetch(i + 1);  // in flight during this tile
+    bool moves = false;
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      if (EDGE) {
+        mx[qi] = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = t0 + 16 * ch + 4 * gq + r;
+            if ((none >> ch & 1) || key < ka || key >= kb || (unsigned)(key - lo[qi]) >= (unsigned)cnt[qi])
+              s[qi][ch][r] = -INFINITY;
+          }
+          largest(s, qi, ch);
+        }
+      }
+      moves |= mx[qi] * sl2 > m[qi] + 8.f;
+    }
+    // the reference point may trail the maximum by 8 (a factor 2^8 in p): exact after
+    // the division by l
+    if (__builtin_amdgcn_ballot_w64(moves) != 0) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        const float mn = fmaxf(m[qi], quad_max(mx[qi]) * sl2);
+        const float alpha = __builtin_amdgcn_exp2f(m[qi] - (mn == -INFINITY ? 0.f : mn));
+        l[qi] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[qi][db] *= alpha;
+        m[qi] = mn;
+      }
+    }
+    float mu[NQ];
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) mu[qi] = m[qi] == -INFINITY ? 0.f : m[qi];
+    auto expo = [&](int qi, int x) {  // the x-th of the lane's CH * 4 probabilities
+      float &p = reinterpret_cast<float (&)[CH][4]>(s[qi])[x / 4][x % 4];
+      p = __builtin_amdgcn_exp2f(fmaf(p, sl2, -mu[qi]));
+      l[qi] += p;
+    };
+    auto rounded = [&](int qi, int jj, bf8 (&b)[NP]) {
+      float p[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) p[x] = s[qi][2 * jj + x / 4][x % 4];
+      split8<NP>(p, b);
+    };
+    constexpr int ALL = CH * 4, FIRST = CH > 2 ? ALL / 2 : ALL;  // a lane's scores, beside QK
+    constexpr int QS = CH * NT, OS = CH / 2 * NDB;  // steps of the two products
+    constexpr int RING = 4;
+    bf8 kf[RING];  // of the next steps
+    auto key = [&](int st) {
+      return *reinterpret_cast<const bf8 *>(ks + 16 * (st / NT) * RSE + 32 * (st % NT));
+    };
+#pragma unroll
+    for (int st = 0; st < RING - 1; ++st) kf[st] = key(st);
+#pragma unroll
+    for (int st = 0; st < QS; ++st) {
+      const int ch = st / NT, t = st % NT;
+      if (st + RING - 1 < QS) kf[(st + RING - 1) % RING] = key(st + RING - 1);
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        next[qi][ch] = product(kf[st % RING], qf[qi][t], t == 0 ? zero4() : next[qi][ch]);
+#pragma unroll
+        for (int x = st * FIRST / QS; x < (st + 1) * FIRST / QS; ++x) expo(qi, x);
+      }
+      __builtin_amdgcn_sched_barrier(0x124);
+    }
+    bool odd = false;
+    if (EDGE) odd = spans && cache_odd_tile<D>(vs, RSE, TK, lane);
+    if (EDGE && odd) {
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        float p[ALL];
+#pragma unroll
+        for (int x = FIRST; x < ALL; ++x) expo(qi, x);
+#pragma unroll
+        for (int x = 0; x < ALL; ++x) p[x] = s[qi][x / 4][x % 4];
+        cache_odd_pv(p, vs, RSE, lane, lo[qi] - t0, cnt[qi], o[qi]);
+      }
+    } else {
+      bf8 bp[NQ][NP];
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) rounded(qi, 0, bp[qi]);
+      bf8 va[2];
+      va[0] = values(vs, 0, 0);
+#pragma unroll
+      for (int st = 0; st < OS; ++st) {
+        const int jj = st / NDB, db = st % NDB;
+        if (jj > 0 && db == 0) {
+#pragma unroll
+          for (int qi = 0; qi < NQ; ++qi) rounded(qi, jj, bp[qi]);
+        }
+        if (st + 1 < OS) va[(st + 1) & 1] = values(vs, (st + 1) / NDB, (st + 1) % NDB);
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          o[qi][db] = product(va[st & 1], bp[qi], o[qi][db]);
+          if (jj == 0) {
+#pragma unroll
+            for (int x = FIRST + db * (ALL - FIRST) / NDB; x < FIRST + (db + 1) * (ALL - FIRST) / NDB; ++x)
+              expo(qi, x);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0x124);
+      }
+    }
+    put(i + 1);
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      mx[qi] = -INFINITY;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) largest(next, qi, ch);
+    }
+    __syncthreads();
+  };
+  put(-1);
+  __syncthreads();
+  fetch(0);
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) mx[qi] = -INFINITY;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    bf8 kf[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      kf[t] = *reinterpret_cast<const bf8 *>(buf + ka_off + 16 * ch * RSE + 32 * t);
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) {
+      sa[qi][ch] = zero4();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sa[qi][ch] = product(kf[t], qf[qi][t], sa[qi][ch]);
+      largest(sa, qi, ch);
+    }
+  }
+  put(0);
+  __syncthreads();
+  int i = 0;
+  for (; i + 2 <= jb - ja; i += 2) {
+    run_tile(i, sa, sb, std::false_type{});
+    run_tile(i + 1, sb, sa, std::false_type{});
+  }
+  for (; i < nkt; ++i) {
+    run_tile(i, sa, sb, std::true_type{});
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) sa[qi][ch] = sb[qi][ch];
+  }
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const float lt = quad_sum(l[qi]);
+    const int r = wv * (16 * NQ) + 16 * qi + n;
+    if (w.row0 + r >= w.row1) continue;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      cache_put<T>(P, A, w, g, part, r, 16 * db + 4 * gq, o[qi][db], lt);
+    if (gq == 0) cache_put_ml(P, A, w, g, part, r, m[qi], lt);
+  }
+}
+
 // This workgroup's part of all units, item by item.
 template <typename F>
 __device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheArgs &A, F &&run) {
-  const int64_t per_head = cache_total(P), all = per_head * P.Hkv;
+  CacheScan scan;
+  const int64_t per_head = scan.total(P), all = per_head * P.Hkv;
   if (all == 0) return;
   const int64_t most = (all + P.least - 1) / P.least;
   const int n = (int)(most < P.wgs ? most : P.wgs);
@@ -562,7 +874,7 @@ __device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheAr
   const int64_t end = all * (me + 1) / n;
   int g = (int)(u / per_head);
   int64_t off = u - g * per_head;
-  int i = cache_find(P, off);
+  int i = scan.find(P, off);
   while (u < end) {
     const CacheItem w = cache_item(P, i);
     if (w.units > 0) {
@@ -593,35 +905,82 @@ __global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_narrow(Cache
   });
 }
 
-// The parts of a row added: lanes take four channels each, 2^lgG of them a row.
+template <typename T, int D, int NQ, int NW>
+__global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_wide(CacheProb P, CacheArgs A) {
+  extern __shared__ __align__(16) char smem[];
+  cache_parts_of(P, A, [&](const CacheItem &w, int g, int ka, int kb, int part) {
+    cache_wide<T, D, NQ, NW>(P, A, w, g, ka, kb, part, smem);
+  });
+}
+
+// The parts of a row added: lanes take four channels each, 2^lgG of them a row, and
+// 2^lgS such groups share the row's parts, each kJoin at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) k_cache_join(CacheProb P, CacheArgs A, int lgG) {
-  const int64_t mine = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lgG;
-  const int c = 4 * (threadIdx.x & ((1 << lgG) - 1));
-  if (mine >= (int64_t)P.B * P.Hkv * P.Mo) return;
-  const int64_t bg = mine / P.Mo;
-  const int row = (int)(mine - bg * P.Mo), b = (int)(bg / P.Hkv), g = (int)(bg - (int64_t)b * P.Hkv);
+__global__ void __launch_bounds__(256) k_cache_join(CacheProb P, CacheArgs A, int lgG, int lgS) {
+  __shared__ f32x4 so[256];
+  __shared__ float2 sml[256];
+  const int tid = threadIdx.x, c = 4 * (tid & ((1 << lgG) - 1));
+  const int share = (tid >> lgG) & ((1 << lgS) - 1);
+  const int64_t rows = (int64_t)P.B * P.Hkv * P.Mo;
+  const int64_t mine = ((int64_t)blockIdx.x * 256 + tid) >> (lgG + lgS);
+  const int64_t at = min(mine, rows - 1), bg = at / P.Mo;
+  const int row = (int)(at - bg * P.Mo), b = (int)(bg / P.Hkv), g = (int)(bg - (int64_t)b * P.Hkv);
   const int tile = row / P.rows, item = b * P.rt + tile, r = row - tile * P.rows;
-  const CacheItem w = cache_item(P, item);
   int2 span = make_int2(0, -1);
-  if (w.units > 0) {
-    span = A.span[(int64_t)g * P.items + item];
-    if (span.x == span.y) return;  // written by its workgroup
-  }
+  if (cache_item(P, item).units > 0) span = A.span[(int64_t)g * P.items + item];
   float m = -INFINITY, l = 0.f;
   f32x4 acc = zero4();
-  for (int i = span.x; i <= span.y; ++i) {
-    const int64_t at = (int64_t)(2 * i + (i == span.x ? 1 : 0)) * P.rows + r;
-    const float2 x = A.pml[at];
-    if (x.y == 0.f) continue;  // sees nothing of the part
-    f32x4 o = zero4();
-    if (c < P.D) o = *reinterpret_cast<const f32x4 *>(A.po + at * P.D + c);
-    const float mn = fmaxf(m, x.x);
-    const float a = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(x.x - mn);
-    l = l == 0.f ? e * x.y : fmaf(e, x.y, l * a);
-    acc = acc * a + e * o;
-    m = mn;
+  if (span.x != span.y) {  // (else its workgroup has written it)
+    for (int i0 = span.x + share; i0 <= span.y; i0 += kJoin << lgS) {  // a batch's loads together
+      float2 x[kJoin];
+      f32x4 o[kJoin];
+#pragma unroll
+      for (int u = 0; u < kJoin; ++u) {
+        const int i = i0 + (u << lgS);
+        x[u] = make_float2(-INFINITY, 0.f);
+        o[u] = zero4();
+        if (i <= span.y) {
+          const int64_t part = (int64_t)(2 * i + (i == span.x ? 1 : 0)) * P.rows + r;
+          x[u] = A.pml[part];
+          if (c < P.D) o[u] = *reinterpret_cast<const f32x4 *>(A.po + part * P.D + c);
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < kJoin; ++u) mn = fmaxf(mn, x[u].x);
+      if (l != 0.f) {
+        const float wt = __builtin_amdgcn_exp2f(m - mn);
+        l *= wt;
+        acc *= wt;
+      }
+      m = mn;
+#pragma unroll
+      for (int u = 0; u < kJoin; ++u)
+        if (x[u].y != 0.f) {  // (0: a row that sees nothing of the part)
+          const float wt = __builtin_amdgcn_exp2f(x[u].x - m);
+          l = fmaf(wt, x[u].y, l);
+          acc += wt * o[u];
+        }
+    }
   }
+  if (lgS > 0) {
+    so[tid] = acc;
+    sml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (share != 0) return;
+    for (int i = 1; i < 1 << lgS; ++i) m = fmaxf(m, sml[tid + (i << lgG)].x);
+    l = 0.f;
+    acc = zero4();
+    for (int i = 0; i < 1 << lgS; ++i) {
+      const float2 x = sml[tid + (i << lgG)];
+      if (x.y != 0.f) {
+        const float wt = __builtin_amdgcn_exp2f(x.x - m);
+        l = fmaf(wt, x.y, l);
+        acc += wt * so[tid + (i << lgG)];
+      }
+    }
+  }
+  if (mine >= rows || span.x == span.y) return;
   const int64_t out = cache_out_row(P, b, g, row);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (c < P.D) cache_store4(static_cast<T *>(A.out) + out * P.D + c, acc * inv);
@@ -629,6 +988,19 @@ __global__ void __launch_bounds__(256) k_cache_join(CacheProb P, CacheArgs A, in
 }
 
 int cache_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+// Rows of a tile, the workgroup's waves, workgroups that the chip holds at once, and
+// units that one takes at least (of 64 keys; a part costs its rows * D floats).
+struct CacheShape {
+  int rows, waves, wgs, least;
+};
+CacheShape cache_shape(int dtype, int D, int64_t rows) {
+  if (dtype == NA_F32 || rows <= 16) return {16, 4, 512, 2};
+  if (D > 128) return {64, 4, 256, 4};
+  if (rows <= 32) return {32, 4, 512, 2};
+  if (rows <= 64) return {64, 4, 512, 4};
+  return {128, dtype == NA_F16 ? 8 : 4, dtype == NA_F16 ? 256 : 512, 4};
+}
 
 CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   CacheProb P{};
@@ -639,15 +1011,16 @@ CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   P.rep = p->heads / p->kv_heads;
   P.D = p->head_dim;
   P.Mo = P.Lq * P.rep;
-  P.rows = P.Mo > 16 && p->dtype != NA_F32 && P.D <= 128 ? 32 : 16;
+  const CacheShape shape = cache_shape(p->dtype, P.D, P.Mo);
+  P.rows = shape.rows;
   P.rt = (P.Mo + P.rows - 1) / P.rows;
   P.items = P.B * P.rt;
   P.pages = p->pages;
   P.lgT = lg_page(p->page_size);
   P.M = p->table_pages;
   P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
-  P.wgs = 512;
-  P.least = 2;
+  P.wgs = shape.wgs;
+  P.least = shape.least;
   P.sl2 = p->scale * kLog2e;
   P.frep = make_fastdiv((uint32_t)P.rep);
   P.frt = make_fastdiv((uint32_t)P.rt);
@@ -675,37 +1048,56 @@ struct CacheSizes {
   size_t total() const { return po + pml + span; }
 };
 
-int cache_join_lanes(const CacheProb &P) {
-  int lgG = 0;
-  while ((4 << lgG) < P.D) ++lgG;
-  return lgG;
-}
+// Logs of the join's lanes per row and of the groups that share a row's parts: kJoin
+// of them each where the workgroups are shared evenly by the items.
+struct CacheJoinLanes {
+  int lgG = 0, lgS = 0;
+  explicit CacheJoinLanes(const CacheProb &P) {
+    while ((4 << lgG) < P.D) ++lgG;
+    const int64_t parts = P.wgs / std::max<int64_t>((int64_t)P.items * P.Hkv, 1) + 2;
+    while (lgG + lgS < 8 && ((int64_t)kJoin << lgS) < parts) ++lgS;
+  }
+  int total() const { return lgG + lgS; }
+};
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int NW, bool WIDE>
 void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
-  constexpr int NW = 4;
-  const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
-  const size_t tiles = sizeof(__bf16) * NW * kTile * (D + 8);
-  hipLaunchKernelGGL((k_cache_narrow<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW),
-                     std::max(meet, tiles), st, P, A);
+  if constexpr (WIDE) {
+    const size_t lds = sizeof(__bf16) * 2 * cache_tile<D>() * lds_row(D);
+    hipLaunchKernelGGL((k_cache_wide<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW), lds, st, P, A);
+  } else {
+    const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
+    const size_t tiles = sizeof(__bf16) * NW * kTile * (D + 8);
+    hipLaunchKernelGGL((k_cache_narrow<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW),
+                       std::max(meet, tiles), st, P, A);
+  }
 }
 
 template <typename T>
 void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   auto by_rows = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if constexpr (sizeof(T) == 2 && D <= 128)
-      if (P.rows == 32) return cache_launch<T, D, 2>(P, A, st);
-    cache_launch<T, D, 1>(P, A, st);
+    if constexpr (sizeof(T) == 2) {
+      if (P.rows == 64) return cache_launch<T, D, 1, 4, true>(P, A, st);
+      if constexpr (D <= 128) {
+        if (P.rows == 32) return cache_launch<T, D, 2, 4, false>(P, A, st);
+        if constexpr (std::is_same<T, f16_t>::value) {
+          if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
+        } else {
+          if (P.rows == 128) return cache_launch<T, D, 2, 4, true>(P, A, st);
+        }
+      }
+    }
+    cache_launch<T, D, 1, 4, false>(P, A, st);
   };
   const int width = cache_width(P.D);
   if (width == 256) by_rows(std::integral_constant<int, 256>{});
   else if (width == 128) by_rows(std::integral_constant<int, 128>{});
   else by_rows(std::integral_constant<int, 64>{});
-  const int lgG = cache_join_lanes(P);
-  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << lgG;
+  const CacheJoinLanes n(P);
+  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << n.total();
   hipLaunchKernelGGL((k_cache_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
-                     lgG);
+                     n.lgG, n.lgS);
 }
 
 }  // namespace
@@ -714,7 +1106,7 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
 bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
   const CacheProb P = cache_prob(p, nullptr);
   *workspace_bytes = CacheSizes(P).total();
-  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << cache_join_lanes(P);
+  const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << CacheJoinLanes(P).total();
   return threads < ((int64_t)1 << 32) - 256;
 }
 

@@ -78,8 +78,8 @@ def _check_cache(cache):
                          f"{[str(t.dtype) for t in cache]}.")
     _check_sizes(shape[3], shape[2])
     for t in (k, v):  # (a copy would not be the cache)
-        if shape[0] and (t.stride(3) != 1 or t.data_ptr() % 16
-                         or any(s % 16 for s in t.stride()[:3])):
+        if shape[0] and (t.data_ptr() % 16 or not t.is_contiguous() and (
+                t.stride(3) != 1 or any(s % 16 for s in t.stride()[:3]))):
             raise ValueError("cache.key and cache.value must have adjacent channels and rows that "
                              f"start at multiples of 16, got strides {t.stride()}.")
     return shape

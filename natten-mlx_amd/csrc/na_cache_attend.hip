@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
+constexpr int kEntries = 512;  // of a sample's table, in the LDS of a wide workgroup
 constexpr int kJoin = 8;    // parts that a thread of the join loads at once
 
 struct CacheProb {
@@ -131,20 +132,25 @@ struct CacheScan {
   }
 };
 
-// 64 entries of a sample's table, one a lane: the page or -1, its scales' bytes.
+// Entry i of a sample's table: the page or -1, and the bytes of its scales, of keys and
+// above of values.
+__device__ __forceinline__ int2 cache_entry(const CacheProb &P, int sample, int g, int i) {
+  int page = i < P.M ? P.tables[sample * P.ts + i] : -1;
+  if ((uint32_t)page >= (uint32_t)P.pages) return make_int2(-1, 0);
+  const int a = P.k.scale[page * P.k.sc[0] + g * P.k.sc[1]];
+  const int b = P.v.scale[page * P.v.sc[0] + g * P.v.sc[1]];
+  // (bytes past the largest scale, as unwritten pages hold them, stay finite)
+  return make_int2(page, min(a, kScaleBias + kScaleHigh) | min(b, kScaleBias + kScaleHigh) << 8);
+}
+
+// 64 entries of a sample's table, one a lane.
 struct PageWindow {
   int base, page, sc;
   __device__ __forceinline__ void load(const CacheProb &P, int sample, int g, int first) {
     base = first;
-    const int i = first + (threadIdx.x & 63);
-    page = i < P.M ? P.tables[sample * P.ts + i] : -1;
-    if ((uint32_t)page >= (uint32_t)P.pages) page = -1;
-    sc = 0;
-    if (page >= 0) {  // (bytes past the largest scale, as unwritten pages hold them, stay finite)
-      const int a = P.k.scale[page * P.k.sc[0] + g * P.k.sc[1]];
-      const int b = P.v.scale[page * P.v.sc[0] + g * P.v.sc[1]];
-      sc = min(a, kScaleBias + kScaleHigh) | min(b, kScaleBias + kScaleHigh) << 8;
-    }
+    const int2 x = cache_entry(P, sample, g, first + (threadIdx.x & 63));
+    page = x.x;
+    sc = x.y;
   }
   // Whether it holds table entry i (uniform).
   __device__ __forceinline__ bool holds(int i) const { return (uint32_t)(i - base) < 64u; }
@@ -292,40 +298,35 @@ __device__ __forceinline__ void cache_softmax(float (&p)[N], float sl2, float &m
   }
 }
 
-// Rows [0, rows) of a tile of values in LDS hold a NaN (all lanes look).
-template <int D>
-__device__ __forceinline__ bool cache_odd_tile(const __bf16 *vs, int stride, int rows, int lane) {
-  bool odd = false;
-  for (int u = lane; u < rows * (D / 8); u += 64) {
-    const u4 x = *reinterpret_cast<const u4 *>(vs + u / (D / 8) * stride + u % (D / 8) * 8);
+// Takes the NaNs out of 16 codes; a bit for each.  A value that some rows of a tile
+// see and others do not may be one, which a probability of zero would not take out.
+__device__ __forceinline__ uint32_t take_nans(u4 &x) {
+  uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      odd |= (x[i] & 0x7f80u) == 0x7f80u || (x[i] & 0x7f800000u) == 0x7f800000u;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = ((x[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // codes 7f and ff
+    x[i] &= ~(t | (t - (t >> 7)));
+    mask |= ((t >> 7) * 0x01020408u >> 24) << (4 * i);
   }
-  return __builtin_amdgcn_ballot_w64(odd) != 0;
+  return mask;
 }
 
-// o += P V key by key, only over the keys that the lane's row sees: for tiles where
-// rows see different keys and V holds a NaN, which a probability of zero would not
-// take out.  p: the lane's scores of keys 16 (i / 4) + 4 gq + i % 4.
-template <int N, int NDB>
-__device__ __forceinline__ void cache_odd_pv(const float (&p)[N], const __bf16 *vs, int stride,
-                                             int lane, int lo, int n, f32x4 (&o)[NDB]) {
-  const int row = lane & 15, gq = lane >> 4;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
+// What take_nans took out of a tile's values, back into the outputs of the rows that
+// see it: nan[key * D / 16 + unit], the lane's row sees keys [lo, lo + n) of `keys`.
+template <int D, int NDB>
+__device__ __forceinline__ void put_nans(const uint16_t *nan, int keys, int lo, int n, int gq,
+                                         f32x4 (&o)[NDB]) {
+  static_assert(NDB == D / 16, "a unit is a block of 16 channels");
 #pragma unroll 1
-    for (int g2 = 0; g2 < 4; ++g2) {
-      const int key = 16 * (i / 4) + 4 * g2 + i % 4;
-      const float pk = __shfl(p[i], row + 16 * g2, 64);
-      if ((unsigned)(key - lo) >= (unsigned)n) continue;
-      const __bf16 *v = vs + key * stride + 4 * gq;
+  for (int key = 0; key < keys; ++key)
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
+    for (int db = 0; db < NDB; ++db) {
+      const uint32_t bits = (uint32_t)nan[key * NDB + db] >> (4 * gq);
+      const bool sees = (unsigned)(key - lo) < (unsigned)n;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[db][c] = fmaf(pk, (float)v[16 * db + c], o[db][c]);
-        __builtin_amdgcn_sched_barrier(0);  // few registers rather than loads ahead
-      }
+      for (int c = 0; c < 4; ++c)
+        if (sees && (bits >> c & 1)) o[db][c] = __uint_as_float(0x7fc00000u);
+      __builtin_amdgcn_sched_barrier(0);  // few registers rather than loads ahead
     }
 }
 
@@ -357,6 +358,8 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   const int tid = threadIdx.x, wv = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 15, gq = lane >> 4;
   __bf16 *const vs = reinterpret_cast<__bf16 *>(smem) + wv * (kTile * RS);  // the wave's own
+  uint16_t *const nan = reinterpret_cast<uint16_t *>(smem + sizeof(__bf16) * NW * kTile * RS) +
+                        wv * (kTile * UPR);
   bf8 qf[NQ][2 * NS][NP];
   int lo[NQ], cnt[NQ];
 #pragma unroll
@@ -464,6 +467,21 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
       }
     }
     __builtin_amdgcn_wave_barrier();  // the reads of the tile before are issued
+    bool odd = false;
+    if (EDGE && spans) {
+      uint32_t mask[NU];
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        mask[i] = take_nans(vr8[i]);
+        some |= mask[i] != 0;
+      }
+      odd = __builtin_amdgcn_ballot_w64(some) != 0;
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) nan[(RPP * i + vr) * UPR + vc] = (uint16_t)mask[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       __bf16 *const d = vs + (RPP * i + vr) * RS + 16 * vc;
@@ -489,23 +507,23 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (EDGE && spans && cache_odd_tile<D>(vs, RS, kTile, lane)) {
+    bf8 bp[NQ][NP];
 #pragma unroll
-      for (int qi = 0; qi < NQ; ++qi) cache_odd_pv(p[qi], vs, RS, lane, lo[qi] - t0, cnt[qi], o[qi]);
-    } else {
-      bf8 bp[NQ][NP];
+    for (int qi = 0; qi < NQ; ++qi) split8<NP>(p[qi], bp[qi]);
 #pragma unroll
-      for (int qi = 0; qi < NQ; ++qi) split8<NP>(p[qi], bp[qi]);
+    for (int db = 0; db < NDB; ++db) {
+      const bf4 lo4 = M16::tr(vs + tr_off + 16 * db);
+      const bf4 hi4 = M16::tr(vs + 16 * RS + tr_off + 16 * db);
+      const bf8 va = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const bf4 lo4 = M16::tr(vs + tr_off + 16 * db);
-        const bf4 hi4 = M16::tr(vs + 16 * RS + tr_off + 16 * db);
-        const bf8 va = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int qi = 0; qi < NQ; ++qi)
 #pragma unroll
-        for (int qi = 0; qi < NQ; ++qi)
+        for (int x = NP - 1; x >= 0; --x) o[qi][db] = M16::mma(va, bp[qi][x], o[qi][db]);
+    }
+    if (EDGE && odd) {
 #pragma unroll
-          for (int x = NP - 1; x >= 0; --x) o[qi][db] = M16::mma(va, bp[qi][x], o[qi][db]);
-      }
+      for (int qi = 0; qi < NQ; ++qi)
+        put_nans<D>(nan, kTile, lo[qi] - t0, cnt[qi], gq, o[qi]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   };
@@ -580,65 +598,16 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   const bool isv = wv >= NW / 2;
   const CachePages &G = isv ? P.v : P.k;
   const int col = 16 * (lane % UPR), rl = lane / UPR, rw = (isv ? wv - NW / 2 : wv) * RPW;
-  const uint8_t *const code = G.code + g * G.st[1];
-  const uint32_t off = (uint32_t)(rl * (int)G.st[2] + col);
+  const int page_st = (int)G.st[0], slot_st = (int)G.st[2];
+  const uint8_t *const code = G.code + g * G.st[1] + rl * slot_st + col;
   const int unit = (rw + rl) * RSE + (isv ? lds_y(D) : 0) + col;
-  const int seen0 = max(ka, w.lo), seen1 = min(kb, w.hi);
-  PageWindow win;
-  win.base = -64;
-  auto entry_of = [&](int key) {  // of the table, in the window
-    const int e = key >> P.lgT;
-    if (!win.holds(e)) win.load(P, w.b, g, e);
-    return e;
-  };
-  bool bad = false;  // the part's table names a page that is none
-  for (int e = (kb - 1) >> P.lgT; e >= ka >> P.lgT; e -= 64) {
-    const int first = max(e - 63, ka >> P.lgT);
-    win.load(P, w.b, g, first);
-    const int mine = first + lane;
-    bad |= __builtin_amdgcn_ballot_w64(mine <= e && win.page < 0) != 0;
-  }
-  u4 pre[NU];
-  float sc[NU];
-  const int nkt = (kb - ka + TK - 1) / TK;
-  // The tiles that every row sees in full are [ja, jb); they come first, then
-  // those behind them, then those before.
-  int ja = (max(w.lo_max - ka, 0) + TK - 1) / TK, jb = max(min(w.hi_min, kb) - ka, 0) / TK;
-  if (jb <= ja || bad) ja = jb = 0;
-  auto first_key = [&](int i) {  // of the i-th tile
-    const int j = ja + i;
-    return ka + (j < nkt ? j : j - nkt) * TK;
-  };
-  // V of the i-th tile and K of the next: the scores run one tile ahead.
-  auto fetch = [&](int i) {
-    const int mine = isv ? i : i + 1;
-    const int t0 = first_key(max(min(mine, nkt - 1), 0));
-    const bool some = mine >= 0 && mine < nkt;
-    const bool whole = some && !bad && t0 >= seen0 && t0 + TK <= seen1 && P.D == D;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int key = t0 + rw + RPP * u;  // the wave's rows: one page's
-      const int e = entry_of(key), page = win.page_of(e), both = win.scales_of(e);
-      sc[u] = scale_of(isv ? both >> 8 : both & 255);
-      const uint8_t *const p = code + page * G.st[0] + (key & ((1 << P.lgT) - 1)) * G.st[2];
-      if (whole) {
-        pre[u] = *reinterpret_cast<const u4 *>(p + off);
-      } else {  // zeros for keys that no row sees and channels past the last: 0 times them is 0
-        pre[u] = u4{0, 0, 0, 0};
-        if (some && page >= 0 && key + rl >= seen0 && key + rl < seen1 && col < P.D)
-          pre[u] = *reinterpret_cast<const u4 *>(p + off);
-      }
-    }
-  };
-  auto put = [&](int i) {
-    __bf16 *const d = buf + ((isv ? i : i + 1) & 1) * (TK * RSE) + unit;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      *reinterpret_cast<bf8 *>(d + RPP * u * RSE) = decode8(pre[u][0], pre[u][1], sc[u]);
-      *reinterpret_cast<bf8 *>(d + RPP * u * RSE + 8) = decode8(pre[u][2], pre[u][3], sc[u]);
-    }
-  };
-  fetch(-1);
+  // the part's pages, kEntries at a time: page or -1, scale bytes
+  int2 *const table = reinterpret_cast<int2 *>(buf + 2 * TK * RSE);
+  int *const flags = reinterpret_cast<int *>(table + kEntries);  // [NW]
+  // NaNs among the values of a tile that rows see differently: whether a wave found
+  // some, and which
+  int *const odds = flags + NW;                                     // [2][NW / 2]
+  uint16_t *const nan = reinterpret_cast<uint16_t *>(odds + NW);    // [2][TK][UPR]
 
   const int row0 = w.row0 + wv * (16 * NQ);
   bf8 qf[NQ][NT][NP];
@@ -685,6 +654,86 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
 #pragma unroll
     for (int r = 0; r < 4; ++r) mx[qi] = fmaxf(mx[qi], s[qi][ch][r]);
   };
+  const int per_chunk = kEntries << P.lgT;
+  for (int ca = ka; ca < kb;) {
+  const int e0 = ca >> P.lgT, cb = min(kb, (e0 << P.lgT) + per_chunk), e1 = (cb - 1) >> P.lgT;
+  const int seen0 = max(ca, w.lo), seen1 = min(cb, w.hi);
+  {
+    __syncthreads();  // the chunk before is done with the table
+    bool none = false;
+    for (int e = e0 + tid; e <= e1; e += 64 * NW) {
+      const int2 x = cache_entry(P, w.b, g, e);
+      table[e - e0] = x;
+      none |= x.x < 0;
+    }
+    if (lane == 0) flags[wv] = 0;
+    if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) flags[wv] = 1;
+    __syncthreads();
+  }
+  bool bad = false;  // the table names a page that is none
+#pragma unroll
+  for (int i = 0; i < NW; ++i) bad |= flags[i] != 0;
+  bad = uniform(bad);
+  u4 pre[NU];
+  float sc[NU];
+  const int nkt = (cb - ca + TK - 1) / TK;
+  // The tiles that every row sees in full are [ja, jb); they come first, then
+  // those behind them, then those before.
+  int ja = (max(w.lo_max - ca, 0) + TK - 1) / TK, jb = max(min(w.hi_min, cb) - ca, 0) / TK;
+  if (jb <= ja || bad) ja = jb = 0;
+  auto first_key = [&](int i) {  // of the i-th tile
+    const int j = ja + i;
+    return ca + (j < nkt ? j : j - nkt) * TK;
+  };
+  // V of the i-th tile and K of the next: the scores run one tile ahead.
+  auto fetch = [&](int i) {
+    const int mine = isv ? i : i + 1;
+    const int t0 = first_key(max(min(mine, nkt - 1), 0));
+    const bool some = mine >= 0 && mine < nkt;
+    const bool whole = some && !bad && t0 >= seen0 && t0 + TK <= seen1 && P.D == D;
+    const uint8_t *p[NU];
+    int page[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int key = t0 + rw + RPP * u;  // the wave's rows: one page's
+      const int2 x = table[min(key >> P.lgT, e1) - e0];
+      page[u] = x.x;
+      sc[u] = scale_of(isv ? x.y >> 8 : x.y & 255);
+      p[u] = code + (int64_t)x.x * page_st + (key & ((1 << P.lgT) - 1)) * slot_st;
+    }
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) pre[u] = *reinterpret_cast<const u4 *>(p[u]);
+    } else {  // zeros for keys that no row sees and channels past the last: 0 times them is 0
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int key = t0 + rw + RPP * u + rl;
+        pre[u] = u4{0, 0, 0, 0};
+        if (some && page[u] >= 0 && key >= seen0 && key < seen1 && col < P.D)
+          pre[u] = *reinterpret_cast<const u4 *>(p[u]);
+      }
+    }
+  };
+  const int full = (jb - ja) & ~1;  // tiles that run as seen by every row
+  auto put = [&](int i) {
+    __bf16 *const d = buf + ((isv ? i : i + 1) & 1) * (TK * RSE) + unit;
+    if (isv && spans && i >= full) {
+      bool some = false;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const uint32_t mask = take_nans(pre[u]);
+        nan[(i & 1) * (TK * UPR) + (rw + RPP * u + rl) * UPR + lane % UPR] = (uint16_t)mask;
+        some |= mask != 0;
+      }
+      some = __builtin_amdgcn_ballot_w64(some) != 0;
+      if (lane == 0) odds[(i & 1) * (NW / 2) + wv - NW / 2] = some;
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      *reinterpret_cast<bf8 *>(d + RPP * u * RSE) = decode8(pre[u][0], pre[u][1], sc[u]);
+      *reinterpret_cast<bf8 *>(d + RPP * u * RSE + 8) = decode8(pre[u][2], pre[u][3], sc[u]);
+    }
+  };
   // The i-th tile, its scores in `s`; the next tile's go to `next`.  EDGE: some
   // row does not see some of its keys.  Matrix products are issued between the vector
   // ALU's work, which fills the matrix unit's time: the next tile's scores beside the
@@ -698,7 +747,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     if (EDGE && bad) {
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
-        none |= win.page_of(entry_of(t0 + 16 * ch)) < 0 ? 1 << ch : 0;
+        none |= table[min((t0 + 16 * ch) >> P.lgT, e1) - e0].x < 0 ? 1 << ch : 0;
     }
     fetch(i + 1);  // in flight during this tile
     bool moves = false;
@@ -711,7 +760,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int key = t0 + 16 * ch + 4 * gq + r;
-            if ((none >> ch & 1) || key < ka || key >= kb || (unsigned)(key - lo[qi]) >= (unsigned)cnt[qi])
+            if ((none >> ch & 1) || key < ca || key >= cb || (unsigned)(key - lo[qi]) >= (unsigned)cnt[qi])
               s[qi][ch][r] = -INFINITY;
           }
           largest(s, qi, ch);
@@ -767,42 +816,38 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
       }
       __builtin_amdgcn_sched_barrier(0x124);
     }
-    bool odd = false;
-    if (EDGE) odd = spans && cache_odd_tile<D>(vs, RSE, TK, lane);
-    if (EDGE && odd) {
+    bf8 bp[NQ][NP];
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) rounded(qi, 0, bp[qi]);
+    bf8 va[2];
+    va[0] = values(vs, 0, 0);
+#pragma unroll
+    for (int st = 0; st < OS; ++st) {
+      const int jj = st / NDB, db = st % NDB;
+      if (jj > 0 && db == 0) {
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) rounded(qi, jj, bp[qi]);
+      }
+      if (st + 1 < OS) va[(st + 1) & 1] = values(vs, (st + 1) / NDB, (st + 1) % NDB);
 #pragma unroll
       for (int qi = 0; qi < NQ; ++qi) {
-        float p[ALL];
+        o[qi][db] = product(va[st & 1], bp[qi], o[qi][db]);
+        if (jj == 0) {
 #pragma unroll
-        for (int x = FIRST; x < ALL; ++x) expo(qi, x);
-#pragma unroll
-        for (int x = 0; x < ALL; ++x) p[x] = s[qi][x / 4][x % 4];
-        cache_odd_pv(p, vs, RSE, lane, lo[qi] - t0, cnt[qi], o[qi]);
+          for (int x = FIRST + db * (ALL - FIRST) / NDB; x < FIRST + (db + 1) * (ALL - FIRST) / NDB; ++x)
+            expo(qi, x);
+        }
       }
-    } else {
-      bf8 bp[NQ][NP];
+      __builtin_amdgcn_sched_barrier(0x124);
+    }
+    if (EDGE && spans) {
+      int odd = 0;
 #pragma unroll
-      for (int qi = 0; qi < NQ; ++qi) rounded(qi, 0, bp[qi]);
-      bf8 va[2];
-      va[0] = values(vs, 0, 0);
+      for (int x = 0; x < NW / 2; ++x) odd |= odds[(i & 1) * (NW / 2) + x];
+      if (uniform(odd) != 0) {
 #pragma unroll
-      for (int st = 0; st < OS; ++st) {
-        const int jj = st / NDB, db = st % NDB;
-        if (jj > 0 && db == 0) {
-#pragma unroll
-          for (int qi = 0; qi < NQ; ++qi) rounded(qi, jj, bp[qi]);
-        }
-        if (st + 1 < OS) va[(st + 1) & 1] = values(vs, (st + 1) / NDB, (st + 1) % NDB);
-#pragma unroll
-        for (int qi = 0; qi < NQ; ++qi) {
-          o[qi][db] = product(va[st & 1], bp[qi], o[qi][db]);
-          if (jj == 0) {
-#pragma unroll
-            for (int x = FIRST + db * (ALL - FIRST) / NDB; x < FIRST + (db + 1) * (ALL - FIRST) / NDB; ++x)
-              expo(qi, x);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0x124);
+        for (int qi = 0; qi < NQ; ++qi)
+          put_nans<D>(nan + (i & 1) * (TK * UPR), TK, lo[qi] - t0, cnt[qi], gq, o[qi]);
       }
     }
     put(i + 1);
@@ -814,6 +859,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     }
     __syncthreads();
   };
+  fetch(-1);
   put(-1);
   __syncthreads();
   fetch(0);
@@ -836,7 +882,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   put(0);
   __syncthreads();
   int i = 0;
-  for (; i + 2 <= jb - ja; i += 2) {
+  for (; i < full; i += 2) {
     run_tile(i, sa, sb, std::false_type{});
     run_tile(i + 1, sb, sa, std::false_type{});
   }
@@ -846,6 +892,8 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     for (int qi = 0; qi < NQ; ++qi)
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) sa[qi][ch] = sb[qi][ch];
+  }
+  ca = cb;
   }
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
@@ -999,7 +1047,9 @@ CacheShape cache_shape(int dtype, int D, int64_t rows) {
   if (D > 128) return {64, 4, 256, 4};
   if (rows <= 32) return {32, 4, 512, 2};
   if (rows <= 64) return {64, 4, 512, 4};
-  return {128, dtype == NA_F16 ? 8 : 4, dtype == NA_F16 ? 256 : 512, 4};
+  if (dtype == NA_F16) return {128, 8, 256, 4};
+  if (rows <= 128) return {128, 4, 512, 4};
+  return D > 64 ? CacheShape{256, 8, 256, 4} : CacheShape{128, 4, 512, 4};
 }
 
 CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
@@ -1063,11 +1113,13 @@ struct CacheJoinLanes {
 template <typename T, int D, int NQ, int NW, bool WIDE>
 void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   if constexpr (WIDE) {
-    const size_t lds = sizeof(__bf16) * 2 * cache_tile<D>() * lds_row(D);
+    const size_t lds = sizeof(__bf16) * 2 * cache_tile<D>() * lds_row(D) +
+                       sizeof(int2) * kEntries + sizeof(int) * 2 * NW +
+                       sizeof(uint16_t) * 2 * cache_tile<D>() * (D / 16);
     hipLaunchKernelGGL((k_cache_wide<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW), lds, st, P, A);
   } else {
     const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
-    const size_t tiles = sizeof(__bf16) * NW * kTile * (D + 8);
+    const size_t tiles = NW * kTile * (sizeof(__bf16) * (D + 8) + sizeof(uint16_t) * (D / 16));
     hipLaunchKernelGGL((k_cache_narrow<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW),
                        std::max(meet, tiles), st, P, A);
   }
@@ -1085,6 +1137,7 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
           if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
         } else {
           if (P.rows == 128) return cache_launch<T, D, 2, 4, true>(P, A, st);
+          if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
         }
       }
     }

@@ -203,33 +203,32 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf8 (&o)[NP]) {
     }
 }
 
-// Eight channels of a query row.
-template <typename T, int NP>
-__device__ __forceinline__ void query8(const T *p, bool live, bf8 (&o)[NP]) {
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (live) {
+// Eight channels of a query row, as they lie and as sums of parts.
+template <typename T>
+struct Query8 {
+  u4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p, bool live) {
     typedef typename Mem16<sizeof(T)>::t m4;  // any alignment of the elements
-    if (sizeof(T) == 4) {
-      const u4 a = *reinterpret_cast<const m4 *>(p), b = *reinterpret_cast<const m4 *>(p + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = __uint_as_float(a[i]);
-        x[4 + i] = __uint_as_float(b[i]);
-      }
-    } else {
-      const u4 a = *reinterpret_cast<const m4 *>(p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint16_t h = (uint16_t)(a[i / 2] >> (16 * (i & 1)));
-        x[i] = std::is_same<T, f16_t>::value ? (float)__builtin_bit_cast(f16_t, h)
-                                             : __uint_as_float((uint32_t)h << 16);
-      }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      r[i] = u4{0, 0, 0, 0};
+      if (live) r[i] = *reinterpret_cast<const m4 *>(p + 4 * i);
     }
   }
-  split8<NP>(x, o);
-}
+  template <int NP>
+  __device__ __forceinline__ void parts(bf8 (&o)[NP]) const {
+    if constexpr (std::is_same<T, bf16_t>::value) {
+      o[0] = __builtin_bit_cast(bf8, r[0]);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = sizeof(T) == 4 ? __uint_as_float(r[i / 4 % (sizeof(T) / 2)][i % 4])
+                              : (float)__builtin_bit_cast(f16_t, (uint16_t)(r[0][i / 2] >> (16 * (i & 1))));
+      split8<NP>(x, o);
+    }
+  }
+};
 
 // Four results of a row, rounded.
 template <typename T>
@@ -370,7 +369,9 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
 #pragma unroll
     for (int s = 0; s < 2 * NS; ++s) {
       const int c = 64 * (s / 2) + 16 * gq + 8 * (s & 1);
-      query8<T, NP>(row.q + c, c < P.D, qf[qi][s]);
+      Query8<T> x;
+      x.load(row.q + c, c < P.D);
+      x.template parts<NP>(qf[qi][s]);
     }
   }
   const int vc = lane % UPR, vr = lane / UPR;
@@ -590,6 +591,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   constexpr int TK = cache_tile<D>(), CH = TK / 16;
   constexpr int NT = D / 32, NDB = D / 16, RSE = lds_row(D);
   constexpr int UPR = D / 16, RPW = 64 / UPR, RPP = RPW * NW / 2, NU = TK / RPP;
+  static_assert(CH / 2 * NDB % NU == 0, "a unit is staged every so many products");
   __bf16 *const buf = reinterpret_cast<__bf16 *>(smem);
   const int tid = threadIdx.x, wv = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 15, gq = lane >> 4;
@@ -603,14 +605,13 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   const int unit = (rw + rl) * RSE + (isv ? lds_y(D) : 0) + col;
   // the part's pages, kEntries at a time: page or -1, scale bytes
   int2 *const table = reinterpret_cast<int2 *>(buf + 2 * TK * RSE);
-  int *const flags = reinterpret_cast<int *>(table + kEntries);  // [NW]
   // NaNs among the values of a tile that rows see differently: whether a wave found
   // some, and which
-  int *const odds = flags + NW;                                     // [2][NW / 2]
+  int *const odds = reinterpret_cast<int *>(table + kEntries);      // [2][NW / 2]
   uint16_t *const nan = reinterpret_cast<uint16_t *>(odds + NW);    // [2][TK][UPR]
 
   const int row0 = w.row0 + wv * (16 * NQ);
-  bf8 qf[NQ][NT][NP];
+  Query8<T> qr[NQ][NT];
   int lo[NQ], cnt[NQ];  // keys that a row sees
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
@@ -618,11 +619,9 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     lo[qi] = r.lo;
     cnt[qi] = r.n;
 #pragma unroll
-    for (int s = 0; s < NT; ++s) {
-      const int c = 32 * s + 8 * gq;
-      query8<T, NP>(r.q + c, c < P.D, qf[qi][s]);
-    }
+    for (int s = 0; s < NT; ++s) qr[qi][s].load(r.q + 32 * s + 8 * gq, 32 * s + 8 * gq < P.D);
   }
+  bf8 qf[NQ][NT][NP];
   f32x4 o[NQ][NDB];
   float m[NQ], l[NQ];
 #pragma unroll
@@ -658,80 +657,73 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   for (int ca = ka; ca < kb;) {
   const int e0 = ca >> P.lgT, cb = min(kb, (e0 << P.lgT) + per_chunk), e1 = (cb - 1) >> P.lgT;
   const int seen0 = max(ca, w.lo), seen1 = min(cb, w.hi);
-  {
-    __syncthreads();  // the chunk before is done with the table
-    bool none = false;
-    for (int e = e0 + tid; e <= e1; e += 64 * NW) {
-      const int2 x = cache_entry(P, w.b, g, e);
-      table[e - e0] = x;
-      none |= x.x < 0;
-    }
-    if (lane == 0) flags[wv] = 0;
-    if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) flags[wv] = 1;
-    __syncthreads();
-  }
-  bool bad = false;  // the table names a page that is none
-#pragma unroll
-  for (int i = 0; i < NW; ++i) bad |= flags[i] != 0;
-  bad = uniform(bad);
   u4 pre[NU];
   float sc[NU];
   const int nkt = (cb - ca + TK - 1) / TK;
   // The tiles that every row sees in full are [ja, jb); they come first, then
   // those behind them, then those before.
   int ja = (max(w.lo_max - ca, 0) + TK - 1) / TK, jb = max(min(w.hi_min, cb) - ca, 0) / TK;
-  if (jb <= ja || bad) ja = jb = 0;
+  if (jb <= ja) ja = jb = 0;
   auto first_key = [&](int i) {  // of the i-th tile
     const int j = ja + i;
     return ca + (j < nkt ? j : j - nkt) * TK;
   };
-  // V of the i-th tile and K of the next: the scores run one tile ahead.
-  auto fetch = [&](int i) {
-    const int mine = isv ? i : i + 1;
+  bool bad = false;  // the table names a page that is none
+  // The lane's units of a tile; entry(i): entry i of the table.
+  auto load = [&](int mine, u4 (&x)[NU], float (&scale)[NU], auto entry) {
     const int t0 = first_key(max(min(mine, nkt - 1), 0));
     const bool some = mine >= 0 && mine < nkt;
     const bool whole = some && !bad && t0 >= seen0 && t0 + TK <= seen1 && P.D == D;
-    const uint8_t *p[NU];
-    int page[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int key = t0 + rw + RPP * u;  // the wave's rows: one page's
-      const int2 x = table[min(key >> P.lgT, e1) - e0];
-      page[u] = x.x;
-      sc[u] = scale_of(isv ? x.y >> 8 : x.y & 255);
-      p[u] = code + (int64_t)x.x * page_st + (key & ((1 << P.lgT) - 1)) * slot_st;
-    }
-    if (whole) {
-#pragma unroll
-      for (int u = 0; u < NU; ++u) pre[u] = *reinterpret_cast<const u4 *>(p[u]);
-    } else {  // zeros for keys that no row sees and channels past the last: 0 times them is 0
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const int key = t0 + rw + RPP * u + rl;
-        pre[u] = u4{0, 0, 0, 0};
-        if (some && page[u] >= 0 && key >= seen0 && key < seen1 && col < P.D)
-          pre[u] = *reinterpret_cast<const u4 *>(p[u]);
+      const int key = t0 + rw + RPP * u;  // the wave's rows of a pass: one page's
+      const int2 at = entry(min(key >> P.lgT, e1));
+      scale[u] = scale_of(isv ? at.y >> 8 : at.y & 255);
+      const uint8_t *const p = code + (int64_t)at.x * page_st + (key & ((1 << P.lgT) - 1)) * slot_st;
+      if (whole) {
+        x[u] = *reinterpret_cast<const u4 *>(p);
+      } else {  // zeros for keys that no row sees and channels past the last: 0 times them is 0
+        x[u] = u4{0, 0, 0, 0};
+        if (some && at.x >= 0 && key + rl >= seen0 && key + rl < seen1 && col < P.D)
+          x[u] = *reinterpret_cast<const u4 *>(p);
       }
     }
   };
-  const int full = (jb - ja) & ~1;  // tiles that run as seen by every row
-  auto put = [&](int i) {
-    __bf16 *const d = buf + ((isv ? i : i + 1) & 1) * (TK * RSE) + unit;
-    if (isv && spans && i >= full) {
+  // V of the i-th tile and K of the next: the scores run one tile ahead.
+  auto fetch = [&](int i) {
+    load(isv ? i : i + 1, pre, sc, [&](int e) { return table[e - e0]; });
+  };
+  // The first tiles' loads go out beside the table's: K of two, V of one.
+  u4 head[NU];
+  float head_sc[NU];
+  __syncthreads();  // the chunk before is done with the table
+  {
+    auto direct = [&](int e) { return cache_entry(P, w.b, g, e); };
+    bool none = false;
+    for (int e = e0 + lane; e <= e1; e += 64)
+      none |= (uint32_t)(e < P.M ? P.tables[w.b * P.ts + e] : -1) >= (uint32_t)P.pages;
+    bad = __builtin_amdgcn_ballot_w64(none) != 0;
+    load(0, head, head_sc, direct);
+    if (!isv) load(1, pre, sc, direct);
+    for (int e = e0 + tid; e <= e1; e += 64 * NW) table[e - e0] = direct(e);
+  }
+  const int full = bad ? 0 : (jb - ja) & ~1;  // tiles that run as seen by every row
+  auto put_unit = [&](int tile, int u, const u4 &x, float scale) {
+    __bf16 *const d = buf + (tile & 1) * (TK * RSE) + unit + RPP * u * RSE;
+    *reinterpret_cast<bf8 *>(d) = decode8(x[0], x[1], scale);
+    *reinterpret_cast<bf8 *>(d + 8) = decode8(x[2], x[3], scale);
+  };
+  auto note_nans = [&](int tile, u4 (&x)[NU]) {
+    if (isv && spans && tile >= full) {
       bool some = false;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const uint32_t mask = take_nans(pre[u]);
-        nan[(i & 1) * (TK * UPR) + (rw + RPP * u + rl) * UPR + lane % UPR] = (uint16_t)mask;
+        const uint32_t mask = take_nans(x[u]);
+        nan[(tile & 1) * (TK * UPR) + (rw + RPP * u + rl) * UPR + lane % UPR] = (uint16_t)mask;
         some |= mask != 0;
       }
       some = __builtin_amdgcn_ballot_w64(some) != 0;
-      if (lane == 0) odds[(i & 1) * (NW / 2) + wv - NW / 2] = some;
-    }
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      *reinterpret_cast<bf8 *>(d + RPP * u * RSE) = decode8(pre[u][0], pre[u][1], sc[u]);
-      *reinterpret_cast<bf8 *>(d + RPP * u * RSE + 8) = decode8(pre[u][2], pre[u][3], sc[u]);
+      if (lane == 0) odds[(tile & 1) * (NW / 2) + wv - NW / 2] = some;
     }
   };
   // The i-th tile, its scores in `s`; the next tile's go to `next`.  EDGE: some
@@ -797,7 +789,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     };
     constexpr int ALL = CH * 4, FIRST = CH > 2 ? ALL / 2 : ALL;  // a lane's scores, beside QK
     constexpr int QS = CH * NT, OS = CH / 2 * NDB;  // steps of the two products
-    constexpr int RING = 4;
+    constexpr int RING = 3;
     bf8 kf[RING];  // of the next steps
     auto key = [&](int st) {
       return *reinterpret_cast<const bf8 *>(ks + 16 * (st / NT) * RSE + 32 * (st % NT));
@@ -838,6 +830,12 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
             expo(qi, x);
         }
       }
+      // the next tiles' units between the products, which go on meanwhile
+      if (st == 0) note_nans(i + 1, pre);
+      if ((st + 1) % (OS / NU) == 0) {
+        constexpr int EVERY = OS / NU;
+        put_unit(isv ? i + 1 : i + 2, st / EVERY, pre[st / EVERY], sc[st / EVERY]);
+      }
       __builtin_amdgcn_sched_barrier(0x124);
     }
     if (EDGE && spans) {
@@ -850,7 +848,6 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
           put_nans<D>(nan + (i & 1) * (TK * UPR), TK, lo[qi] - t0, cnt[qi], gq, o[qi]);
       }
     }
-    put(i + 1);
 #pragma unroll
     for (int qi = 0; qi < NQ; ++qi) {
       mx[qi] = -INFINITY;
@@ -859,10 +856,19 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     }
     __syncthreads();
   };
-  fetch(-1);
-  put(-1);
+  if (ca == ka) {
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+      for (int x = 0; x < NT; ++x) qr[qi][x].template parts<NP>(qf[qi][x]);
+  }
+  note_nans(0, head);
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    put_unit(0, u, head[u], head_sc[u]);
+    if (!isv) put_unit(1, u, pre[u], sc[u]);
+  }
   __syncthreads();
-  fetch(0);
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) mx[qi] = -INFINITY;
 #pragma unroll
@@ -879,8 +885,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
       largest(sa, qi, ch);
     }
   }
-  put(0);
-  __syncthreads();
+  __syncthreads();  // these keys' place is the tile's after next
   int i = 0;
   for (; i < full; i += 2) {
     run_tile(i, sa, sb, std::false_type{});
@@ -1044,12 +1049,12 @@ struct CacheShape {
 };
 CacheShape cache_shape(int dtype, int D, int64_t rows) {
   if (dtype == NA_F32 || rows <= 16) return {16, 4, 512, 2};
-  if (D > 128) return {64, 4, 256, 4};
+  if (D > 128) return {64, 4, 256, 1};
   if (rows <= 32) return {32, 4, 512, 2};
-  if (rows <= 64) return {64, 4, 512, 4};
-  if (dtype == NA_F16) return {128, 8, 256, 4};
-  if (rows <= 128) return {128, 4, 512, 4};
-  return D > 64 ? CacheShape{256, 8, 256, 4} : CacheShape{128, 4, 512, 4};
+  if (rows <= 64) return {64, 4, 512, 1};
+  if (dtype == NA_F16) return {128, 8, 256, 1};
+  if (rows <= 128) return {128, 4, 512, 1};
+  return D > 64 ? CacheShape{256, 8, 256, 1} : CacheShape{128, 4, 512, 1};
 }
 
 CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
@@ -1114,7 +1119,7 @@ template <typename T, int D, int NQ, int NW, bool WIDE>
 void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   if constexpr (WIDE) {
     const size_t lds = sizeof(__bf16) * 2 * cache_tile<D>() * lds_row(D) +
-                       sizeof(int2) * kEntries + sizeof(int) * 2 * NW +
+                       sizeof(int2) * kEntries + sizeof(int) * NW +
                        sizeof(uint16_t) * 2 * cache_tile<D>() * (D / 16);
     hipLaunchKernelGGL((k_cache_wide<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW), lds, st, P, A);
   } else {

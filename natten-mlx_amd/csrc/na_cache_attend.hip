@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
+constexpr int kAligned = 24;  // units
 constexpr int kEntries = 512;  // of a sample's table, in the LDS of a wide workgroup
 constexpr int kJoin = 8;    // parts that a thread of the join loads at once
 
@@ -95,34 +96,41 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
+// A value that all lanes hold, as one scalar (quotients come in vector registers).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The items of a head in order, 64 at a time, their units added up.
+// The items of a head in order, 64 at a time, their chunks of `size` units added up.
 struct CacheScan {
-  int i0 = -64, sum = 0, mine = 0, all = 0;  // first item, the lane's sums, of all 64
-  __device__ __forceinline__ void load(const CacheProb &P, int first) {
-    if (first == i0) return;
-    i0 = first;
-    const int i = i0 + (threadIdx.x & 63);
-    mine = i < P.items ? cache_item(P, i).units : 0;
+  int i0 = -1, size = 0, units = 0;  // first item, the lane's units
+  int mine = 0, sum = 0, all = 0;    // the lane's chunks, up to it, of all 64
+  __device__ __forceinline__ void load(const CacheProb &P, int first, int chunk) {
+    if (first != i0) {
+      i0 = first;
+      size = 0;
+      const int i = i0 + (threadIdx.x & 63);
+      units = i < P.items ? cache_item(P, i).units : 0;
+    }
+    if (chunk == size) return;
+    size = chunk;
+    mine = (int)((unsigned)(units + size - 1) / (unsigned)size);
     sum = wave_scan(mine);
     all = __builtin_amdgcn_readlane(sum, 63);
   }
-  // Units of all items.
-  __device__ __forceinline__ int64_t total(const CacheProb &P) {
-    int64_t t = 0;
+  // Chunks of all items.
+  __device__ __forceinline__ int total(const CacheProb &P, int chunk) {
+    int t = 0;
     for (int i = 0; i < P.items; i += 64) {
-      load(P, i);
+      load(P, i, chunk);
       t += all;
     }
     return t;
   }
-  // The item that unit u lies in; u becomes the unit within it.
-  __device__ __forceinline__ int find(const CacheProb &P, int64_t &u) {
+  // The item that chunk u lies in; u becomes the chunk within it.
+  __device__ __forceinline__ int find(const CacheProb &P, int &u, int chunk) {
     for (int i = 0; i < P.items; i += 64) {
-      load(P, i);
+      load(P, i, chunk);
       if (u < all) {
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > (int)u));
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > u));
         u -= __builtin_amdgcn_readlane(sum - mine, at);
         return i0 + at;
       }
@@ -611,7 +619,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   uint16_t *const nan = reinterpret_cast<uint16_t *>(odds + NW);    // [2][TK][UPR]
 
   const int row0 = w.row0 + wv * (16 * NQ);
-  Query8<T> qr[NQ][NT];
+  bf8 qf[NQ][NT][NP];
   int lo[NQ], cnt[NQ];  // keys that a row sees
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
@@ -619,9 +627,12 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     lo[qi] = r.lo;
     cnt[qi] = r.n;
 #pragma unroll
-    for (int s = 0; s < NT; ++s) qr[qi][s].load(r.q + 32 * s + 8 * gq, 32 * s + 8 * gq < P.D);
+    for (int s = 0; s < NT; ++s) {
+      Query8<T> x;
+      x.load(r.q + 32 * s + 8 * gq, 32 * s + 8 * gq < P.D);
+      x.template parts<NP>(qf[qi][s]);
+    }
   }
-  bf8 qf[NQ][NT][NP];
   f32x4 o[NQ][NDB];
   float m[NQ], l[NQ];
 #pragma unroll
@@ -856,12 +867,6 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     }
     __syncthreads();
   };
-  if (ca == ka) {
-#pragma unroll
-    for (int qi = 0; qi < NQ; ++qi)
-#pragma unroll
-      for (int x = 0; x < NT; ++x) qr[qi][x].template parts<NP>(qf[qi][x]);
-  }
   note_nans(0, head);
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
@@ -912,34 +917,53 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   }
 }
 
-// This workgroup's part of all units, item by item.
+// This workgroup's part of the keys.  All units are shared out evenly, in order, so
+// that a workgroup may end one item and begin others; or, where its even share is at
+// most kAligned units and the items are fewer than the workgroups, each takes one chunk
+// of one item, as beginning an item costs the time of several units.
 template <typename F>
 __device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheArgs &A, F &&run) {
   CacheScan scan;
-  const int64_t per_head = scan.total(P), all = per_head * P.Hkv;
+  int per_head = scan.total(P, 1), all = per_head * P.Hkv;  // (below 2^31: the host's check)
   if (all == 0) return;
-  const int64_t most = (all + P.least - 1) / P.least;
-  const int n = (int)(most < P.wgs ? most : P.wgs);
+  const int share = uniform(max((all - 1) / P.wgs + 1, P.least));
+  int chunk = 1, n;
+  if (share <= kAligned && P.items * P.Hkv <= P.wgs) {
+    for (chunk = share; (per_head = scan.total(P, chunk)) * P.Hkv > P.wgs;) chunk += (chunk + 7) / 8;
+    n = all = per_head * P.Hkv;
+  } else {
+    n = uniform(min((all - 1) / P.least + 1, P.wgs));
+  }
+  chunk = uniform(chunk);
+  per_head = uniform(per_head);
+  all = uniform(all);
+  n = uniform(n);
   // tiles next to each other read the same keys: through one XCD's L2
   const int me = P.rt > 1 && n == P.wgs ? xcd_tile(blockIdx.x, P.wgs) : blockIdx.x;
   if (me >= n) return;
-  int64_t u = all * me / n;
-  const int64_t end = all * (me + 1) / n;
-  int g = (int)(u / per_head);
-  int64_t off = u - g * per_head;
-  int i = scan.find(P, off);
+  int u = uniform((int)((int64_t)all * me / n));
+  const int end = uniform((int)((int64_t)all * (me + 1) / n));
+  int g = uniform(u / per_head);
+  int off = u - g * per_head;
+  int i = uniform(scan.find(P, off, chunk));
+  off = uniform(off);
   while (u < end) {
-    const CacheItem w = cache_item(P, i);
+    CacheItem w = cache_item(P, i);
+    for (int *x : {&w.b, &w.row0, &w.row1, &w.len, &w.k0, &w.lo, &w.hi, &w.lo_max, &w.hi_min, &w.units})
+      *x = uniform(*x);
     if (w.units > 0) {
-      const int take = (int)min((int64_t)w.units - off, end - u);
-      const bool begins = off == 0, whole = begins && take == w.units;
+      const int chunks = uniform((w.units + chunk - 1) / chunk);
+      const int take = min(chunks - off, end - u);
+      const bool begins = off == 0, whole = begins && take == chunks;
       if (begins && threadIdx.x == 0) {
-        // the workgroup that unit x lies in is the largest whose part begins at x or before
-        const int64_t x = u + w.units;
+        // the workgroup that chunk x lies in is the largest whose part begins at x or before
+        const int64_t x = u + chunks;
         A.span[(int64_t)g * P.items + i] = make_int2(me, (int)((x * n + all - 1) / all) - 1);
       }
-      run(w, g, w.k0 + (int)off * kUnit, min(w.k0 + (int)(off + take) * kUnit, w.hi),
-          whole ? -1 : 2 * me + (begins ? 1 : 0));
+      // (a chunk of several units: no more than kAligned a workgroup, the products are small)
+      const int ua = chunk == 1 ? off : uniform(w.units * off / chunks);
+      const int ub = chunk == 1 ? off + take : uniform(w.units * (off + take) / chunks);
+      run(w, g, w.k0 + ua * kUnit, min(w.k0 + ub * kUnit, w.hi), whole ? -1 : 2 * me + (begins ? 1 : 0));
       u += take;
     }
     off = 0;
@@ -1165,7 +1189,9 @@ bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
   const CacheProb P = cache_prob(p, nullptr);
   *workspace_bytes = CacheSizes(P).total();
   const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << CacheJoinLanes(P).total();
-  return threads < ((int64_t)1 << 32) - 256;
+  // all units, as the kernels count them, of full tables
+  const int64_t units = (int64_t)P.items * P.Hkv * (((int64_t)P.M << P.lgT) / kUnit + 2);
+  return threads < ((int64_t)1 << 32) - 256 && units < ((int64_t)1 << 31);
 }
 
 void cache_attend(const na_cache_params *p, const na_cache *c, const void *q, const int32_t *tables,

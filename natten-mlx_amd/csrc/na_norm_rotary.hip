@@ -25,6 +25,10 @@
 // Sums are float32; y, dx, dw and db are rounded once.  Bound: memory.
 #include "na_rotary.h"
 
+// Sums and products are fused where it says so and nowhere else: the kernels of rows
+// that lie as one and of others give the same bits.
+#pragma clang fp contract(off)
+
 namespace na {
 namespace {
 
@@ -145,7 +149,7 @@ __device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> 
     for (int e = 0; e < N; ++e) {
       const float2 z = cs[e * units + L.j];
       const float u = x[0][e], v = x[1][e];
-      x[0][e] = u * z.x - v * z.y;
+      x[0][e] = fmaf(u, z.x, -(v * z.y));
       x[1][e] = fmaf(v, z.x, u * z.y);
     }
   } else if constexpr (MODE == kRotAdjacent) {
@@ -154,7 +158,7 @@ __device__ __forceinline__ void nr_turn(const RotProb &P, const NrLane<T, MODE> 
       if (L.c0 + e < 2 * P.pairs) {
         const float2 z = cs[e / 2 * units + L.j];
         const float u = x[0][e], v = x[0][e + 1];
-        x[0][e] = u * z.x - v * z.y;
+        x[0][e] = fmaf(u, z.x, -(v * z.y));
         x[0][e + 1] = fmaf(v, z.x, u * z.y);
       }
   } else {
@@ -200,6 +204,15 @@ __device__ __forceinline__ void nr_weights(const NrLane<T, MODE> &L, const void 
   }
 }
 
+// 1 / sqrt(x): the hardware's estimate and one step of Newton's, off by less than two
+// steps; outside the range where the step's products are normal, the exact quotient.
+__device__ __forceinline__ float nr_rsqrt(float x) {
+  float y = __builtin_amdgcn_rsqf(x);
+  y = fmaf(0.5f * y, fmaf(-x * y, y, 1.f), y);
+  if (!(x > 0x1p-60f && x < 0x1p+60f)) y = 1.f / sqrtf(x);
+  return y;
+}
+
 // The row less its mean in place; 1 / std.
 template <bool FAST, int NT, int N>
 __device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT], const NrProb &Q) {
@@ -208,7 +221,11 @@ __device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT]
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < N; ++e) s += x[t][e];  // (zeros behind the last channel)
-  const float mean = lanes_sum(s, Q.lgG) / (float)Q.R.D;
+  // the quotient by D, to its last place: equal channels, where their sums are exact,
+  // have their value for a mean
+  s = lanes_sum(s, Q.lgG);
+  float mean = s * Q.inv_d;
+  mean = fmaf(fmaf(-mean, (float)Q.R.D, s), Q.inv_d, mean);
   s = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -220,7 +237,7 @@ __device__ __forceinline__ float nr_center(float (&x)[NT][N], const int (&n)[NT]
     }
     s += n[t] > 0 ? part : 0.f;
   }
-  return 1.f / sqrtf(fmaf(lanes_sum(s, Q.lgG), Q.inv_d, Q.eps));
+  return nr_rsqrt(fmaf(lanes_sum(s, Q.lgG), Q.inv_d, Q.eps));
 }
 
 // Rows of a tensor [.., heads, D] by token and head, from a run's first token.
@@ -422,7 +439,7 @@ __global__ void __launch_bounds__(kRotThreads)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) d[i][e] = rstd * (d[i][e] - s0 - h[i][e] * s1);
+        for (int e = 0; e < N; ++e) d[i][e] = rstd * fmaf(-h[i][e], s1, d[i][e] - s0);
         nr_store<FAST>(out + r * P.D + L.c[i], d[i], L.n[i]);
       }
     }

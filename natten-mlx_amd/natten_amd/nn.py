@@ -22,6 +22,8 @@ to key/value head ``h // (num_heads // num_kv_heads)`` directly.
 Beyond the reference's arguments, ``qk_norm`` puts a layer norm over each head's
 channels on queries and keys (``q_norm``, ``k_norm``), and ``rotary`` turns them by
 their positions on the layer's axes; both come before the attention on every route.
+With ``qk_fused`` a layer that has both runs them in one pass, ``norm_rotary``, which
+rounds queries and keys once where the two operators round twice.
 """
 
 from __future__ import annotations
@@ -37,6 +39,7 @@ from ._core import _lib, ops
 from ._core import hip as _hip
 from .autograd import fused as _fused
 from .norm import layer_norm
+from .norm_rotary import norm_rotary
 from .rotary import rotary as _rotary
 from .rotary import rotary_axis_dims
 from .utils.params import normalize_tuple_param
@@ -129,6 +132,7 @@ class _NeighborhoodAttention(_nn.Module):
         qk_norm: bool = False,
         rotary: Union[bool, Tuple[int, ...]] = False,
         rotary_theta: float = 10000.0,
+        qk_fused: bool = False,
     ):
         super().__init__()
         if embed_dim <= 0:
@@ -180,6 +184,11 @@ class _NeighborhoodAttention(_nn.Module):
         if self.rotary_dims is not None and not (
                 self.rotary_theta > 0.0 and math.isfinite(self.rotary_theta)):
             raise ValueError(f"rotary_theta must be positive and finite, got {rotary_theta}")
+        self.qk_fused = bool(qk_fused)
+        if self.qk_fused and (self.q_norm is None or self.rotary_dims is None
+                              or self.head_dim > _lib.NORM_ROTARY_MAX_HEAD_DIM):
+            raise ValueError("qk_fused needs qk_norm, rotary and heads of up to "
+                             f"{_lib.NORM_ROTARY_MAX_HEAD_DIM} channels (here {self.head_dim})")
         self.proj_drop_rate = float(proj_drop)
         self.proj_drop = _nn.Dropout(self.proj_drop_rate) if self.proj_drop_rate > 0.0 else None
 
@@ -188,6 +197,8 @@ class _NeighborhoodAttention(_nn.Module):
         if "rotary_dims" not in state:  # pickled before the layers had these
             self.q_norm = self.k_norm = self.rotary_dims = None
             self.rotary_theta = 10000.0
+        if "qk_fused" not in state:
+            self.qk_fused = False
 
     def extra_repr(self) -> str:
         return (f"embed_dim={self.embed_dim}, num_heads={self.num_heads}, "
@@ -247,11 +258,25 @@ class _NeighborhoodAttention(_nn.Module):
             k, v = kv.unbind(dim=-3)
         else:
             q, k, v = self._split_qkv(_linear(self.qkv, x))
+        if self.qk_fused and self._fuses_norms():
+            q, k = norm_rotary(q, k, self.q_norm.weight, self.q_norm.bias, self.k_norm.weight,
+                               self.k_norm.bias, axis_dims=self.rotary_dims,
+                               theta=self.rotary_theta, eps=self.q_norm.eps)
+            return q, k, v
         if self.q_norm is not None:
             q, k = self.q_norm(q), self.k_norm(k)
         if self.rotary_dims is not None:
             q, k = _rotary(q, k, axis_dims=self.rotary_dims, theta=self.rotary_theta)
         return q, k, v
+
+    def _fuses_norms(self) -> bool:
+        """Whether the norms are the layer's plain ones: a replaced or hooked module is
+        called itself."""
+        return (self.q_norm.eps == self.k_norm.eps
+                and not torch.nn.modules.module._has_any_global_hook()
+                and all(type(m) is LayerNorm and "forward" not in m.__dict__
+                        and not any(getattr(m, h) for h in _HOOKS)
+                        for m in (self.q_norm, self.k_norm)))
 
     def _attend(self, x: torch.Tensor, sizes: Optional[torch.Tensor]) -> torch.Tensor:
         r = self.rank

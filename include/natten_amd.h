@@ -579,8 +579,8 @@ typedef struct na_cache {
   void *value;
   void *key_scale;               /* bytes of [pages, kv_heads] */
   void *value_scale;
-  int64_t key_stride[3];         /* elements: page, head, token; channels adjacent, */
-  int64_t value_stride[3];       /* every row 16-byte aligned */
+  int64_t key_stride[3];         /* elements: page (below 2^31), head, token (below */
+  int64_t value_stride[3];       /* 2^24); channels adjacent, rows 16-byte aligned */
   int64_t key_scale_stride[2];   /* page, head */
   int64_t value_scale_stride[2];
 } na_cache;

@@ -1101,7 +1101,8 @@ int check_cache_attend(const na_cache_params *p, size_t *need) {
   return NA_OK;
 }
 
-// Rows of codes start at multiples of 16 bytes.
+// Rows of codes start at multiples of 16 bytes; the kernels hold the strides of pages and
+// tokens, times up to 127 of the latter, in 32 bits.
 int check_pages(const na_cache *c) {
   if (c == nullptr || c->key == nullptr || c->value == nullptr || c->key_scale == nullptr ||
       c->value_scale == nullptr)
@@ -1110,6 +1111,12 @@ int check_pages(const na_cache *c) {
   for (int i = 0; i < 3; ++i) bits |= (uintptr_t)c->key_stride[i] | (uintptr_t)c->value_stride[i];
   if (bits & 15)
     return fail(NA_ERR_INVALID, "the cache's rows must start at multiples of 16 bytes");
+  for (const int64_t *st : {c->key_stride, c->value_stride})
+    if (st[0] < 0 || st[1] < 0 || st[2] < 0 || st[0] >= ((int64_t)1 << 31) ||
+        st[2] >= (1 << 24))
+      return fail(NA_ERR_UNSUPPORTED, "the cache's strides must be below 2^31 bytes from page to "
+                  "page and 2^24 from token to token, got %lld and %lld", (long long)st[0],
+                  (long long)st[2]);
   return NA_OK;
 }
 

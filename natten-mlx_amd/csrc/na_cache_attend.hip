@@ -679,7 +679,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     const int j = ja + i;
     return ca + (j < nkt ? j : j - nkt) * TK;
   };
-  bool bad = false;  // the table names a page that is none
+  bool bad = false;  // the table names a page that is none, among those that rows see
   // The lane's units of a tile; entry(i): entry i of the table.
   auto load = [&](int mine, u4 (&x)[NU], float (&scale)[NU], auto entry) {
     const int t0 = first_key(max(min(mine, nkt - 1), 0));
@@ -711,7 +711,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
   {
     auto direct = [&](int e) { return cache_entry(P, w.b, g, e); };
     bool none = false;
-    for (int e = e0 + lane; e <= e1; e += 64)
+    for (int e = (seen0 >> P.lgT) + lane; e <= (seen1 - 1) >> P.lgT; e += 64)
       none |= (uint32_t)(e < P.M ? P.tables[w.b * P.ts + e] : -1) >= (uint32_t)P.pages;
     bad = __builtin_amdgcn_ballot_w64(none) != 0;
     load(0, head, head_sc, direct);
@@ -1166,7 +1166,9 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
           if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
         } else {
           if (P.rows == 128) return cache_launch<T, D, 2, 4, true>(P, A, st);
-          if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
+          if constexpr (D > 64) {
+            if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
+          }
         }
       }
     }
@@ -1190,7 +1192,8 @@ bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
   *workspace_bytes = CacheSizes(P).total();
   const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << CacheJoinLanes(P).total();
   // all units, as the kernels count them, of full tables
-  const int64_t units = (int64_t)P.items * P.Hkv * (((int64_t)P.M << P.lgT) / kUnit + 2);
+  const int64_t keys = std::min((int64_t)P.M << P.lgT, (int64_t)P.W + P.rows);  // of an item
+  const int64_t units = (int64_t)P.items * P.Hkv * (keys / kUnit + 2);
   return threads < ((int64_t)1 << 32) - 256 && units < ((int64_t)1 << 31);
 }
 

@@ -1233,8 +1233,8 @@ CacheCall cache_call(const at::Tensor &x, const at::Tensor &k, const at::Tensor 
   r.c.key_scale = ks.data_ptr();
   r.c.value_scale = vs.data_ptr();
   for (int i = 0; i < 3; ++i) {
-    r.c.key_stride[i] = k.stride(i);
-    r.c.value_stride[i] = v.stride(i);
+    r.c.key_stride[i] = k.size(i) > 1 ? k.stride(i) : 0;
+    r.c.value_stride[i] = v.size(i) > 1 ? v.stride(i) : 0;
   }
   for (int i = 0; i < 2; ++i) {
     r.c.key_scale_stride[i] = ks.stride(i);

@@ -798,7 +798,7 @@ def _cache_params(cache, x, tables):
         t, sc = getattr(cache, n), getattr(cache, n + "_scale")
         setattr(c, n, t.data_ptr())
         setattr(c, n + "_scale", sc.data_ptr())
-        getattr(c, n + "_stride")[:] = t.stride()[:3]
+        getattr(c, n + "_stride")[:] = [st if size > 1 else 0 for size, st in zip(t.shape[:3], t.stride())]
         getattr(c, n + "_scale_stride")[:] = sc.stride()
     return p, c
 

@@ -78,10 +78,15 @@ def _check_cache(cache):
                          f"{[str(t.dtype) for t in cache]}.")
     _check_sizes(shape[3], shape[2])
     for t in (k, v):  # (a copy would not be the cache)
-        if shape[0] and (t.data_ptr() % 16 or not t.is_contiguous() and (
-                t.stride(3) != 1 or any(s % 16 for s in t.stride()[:3]))):
+        if not shape[0] or t.is_contiguous() and not t.data_ptr() % 16 and t.stride(0) < 1 << 31:
+            continue
+        st = [s if n > 1 else 0 for n, s in zip(shape, t.stride())]
+        if t.data_ptr() % 16 or st[3] != 1 or any(s % 16 for s in st[:3]):
             raise ValueError("cache.key and cache.value must have adjacent channels and rows that "
                              f"start at multiples of 16, got strides {t.stride()}.")
+        if st[0] >= 1 << 31 or st[2] >= 1 << 24:
+            raise ValueError("cache.key and cache.value must have strides below 2^31 from page to "
+                             f"page and 2^24 from token to token, got {t.stride()}.")
     return shape
 
 

@@ -846,3 +846,145 @@ def test_refusals():
         assert append(params(**bad)) == 2 and attend(params(**bad)) == 2, bad
     assert attend(params(batch=1 << 20, tokens=1 << 9)) == 2
     assert append(params(batch=1 << 20, tokens=1 << 12, table_pages=1 << 12), pages, 1) == 2
+
+
+# ---- layouts and sizes at the kernels' limits --------------------------------
+
+def _codes(t):
+    return t.view(torch.uint8)
+
+
+def test_strides_and_sizes_that_are_refused():
+    import natten_amd
+    from natten_amd._core import _lib
+
+    lib = _lib.load()
+    p = dict(batch=2, tokens=1, heads=4, kv_heads=2, head_dim=32, dtype=2, pages=5, page_size=16,
+             table_pages=4, scale=0.25)
+
+    def both(n, strides, **kw):
+        c = _lib.NaCache(key=256, value=256, key_scale=1, value_scale=1)
+        for m in ("key_stride", "value_stride"):
+            getattr(c, m)[:] = (1024, 512, 32)
+        getattr(c, n)[:] = strides
+        q = _lib.NaCacheParams(**{**p, **kw})
+        return {lib.na_cache_append(q, c, 1, 1, 1, 1, None, None),
+                lib.na_cache_attend(q, c, 1, 1, 1, 1, None, None, 0, None)}
+
+    for n in ("key_stride", "value_stride"):
+        for strides in ((1 << 31, 512, 32), (1024, 512, 1 << 24), (-1024, 512, 32), (1024, -512, 32),
+                        (1024, 512, -32)):
+            assert both(n, strides) == {2}, strides
+            assert b"strides" in lib.na_last_error()
+    # a call's units of 64 keys are counted in 31 bits; a window keeps them few
+    big = dict(p, batch=1 << 13, kv_heads=64, heads=64, table_pages=1 << 16)
+    assert lib.na_cache_attend_workspace_bytes(_lib.NaCacheParams(**big)) == 0
+    assert b"too large" in lib.na_last_error()
+    assert lib.na_cache_attend_workspace_bytes(_lib.NaCacheParams(**big, window=4096)) > 0
+    cache = natten_amd.paged_cache(2, 2, 32, 16, device="cpu")
+    tables, lens = torch.zeros(2, 4, dtype=torch.int32), torch.tensor([5, 7])
+    k = torch.randn(2, 3, 2, 32)
+    for st in ((1 << 31, 512, 32, 1), (1024, 512, 1 << 24, 1)):
+        far = torch.empty_strided((2, 2, 16, 32), st, dtype=torch.uint8, device="meta").view(E4M3)
+        with pytest.raises(ValueError, match="2\\^31"):
+            natten_amd.cache_append(cache._replace(value=far), k, k, tables, lens)
+        with pytest.raises(ValueError, match="2\\^31"):
+            natten_amd.cache_attention(k, cache._replace(key=far), tables, lens)
+
+
+def _twins(cache, twin, q, k, v, tables, lens, **kw):
+    """Appends to both caches and attends over both: the same bits."""
+    import natten_amd
+
+    out = []
+    for c in (cache, twin):
+        natten_amd.cache_append(c, k, v, tables, lens)
+        out.append(natten_amd.cache_attention(q, c, tables, lens, return_lse=True, **kw))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    assert out[0][0].isfinite().all() and out[0][0].abs().max() > 0
+    used = tables.unique().long()
+    for a, b in zip(cache, twin):
+        assert torch.equal(_codes(a)[used], _codes(b)[used])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_strides_at_their_limits(n):
+    """Pages 2^31 - 16 bytes apart, tokens 2^24 - 16: offsets past 32 bits."""
+    import natten_amd
+
+    big = torch.zeros(3 << 31, dtype=torch.uint8, device=DEV)
+    st = ((1 << 31) - 16, 64, (1 << 24) - 16, 1)
+    cache = natten_amd.paged_cache(3, 2, 64, 128)
+    k8, v8 = (big.as_strided((3, 2, 128, 64), st, at).view(E4M3) for at in (0, 4096))
+    cache = cache._replace(key=k8, value=v8)
+    twin = natten_amd.paged_cache(3, 2, 64, 128)
+    tables = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=DEV)
+    for length in (n, 384 if n > 84 else 300 + n) if n < 300 else (300,):
+        k, v = (randn((1, length, 2, 64), BF16, s).to(DEV) for s in (1, 2))
+        lens = torch.tensor([length], device=DEV)
+        q = randn((1, n, 4, 64), BF16, 3).to(DEV)
+        _twins(cache, twin, q, k, v, tables, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 24])
+def test_a_pool_past_four_gigabytes(n):
+    import natten_amd
+
+    pages = (1 << 32) // (2 * 128 * 256) + 300
+    cache = natten_amd.paged_cache(pages, 2, 256, 128)
+    twin = natten_amd.paged_cache(6, 2, 256, 128)
+    near = torch.arange(6, dtype=torch.int32, device=DEV).view(2, 3)
+    far = torch.tensor([[pages - 1, 0, pages - 2], [32768, 65536, 65535]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([350, 129], device=DEV)
+    k, v = (randn((2, 350, 2, 256), BF16, s).to(DEV) for s in (1, 2))
+    q = randn((2, n, 8, 256), BF16, 3).to(DEV)
+    outs = []
+    for c, t in ((cache, far), (twin, near)):
+        natten_amd.cache_append(c, k, v, t, lens)
+        outs.append(natten_amd.cache_attention(q, c, t, lens))
+    assert torch.equal(*outs) and outs[0].isfinite().all() and outs[0].abs().max() > 0
+    for a, b in zip(cache, twin):
+        assert torch.equal(_codes(a)[far.long().flatten()], _codes(b)[near.long().flatten()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("python", [False, True])
+def test_strides_of_dimensions_of_one(python, monkeypatch):
+    """One head, whose stride is no multiple of 16 and means nothing."""
+    import natten_amd
+    from natten_amd.autograd import fused
+
+    monkeypatch.setattr(fused, "_py_autograd", python)
+    twin = natten_amd.paged_cache(4, 1, 32, 16)
+    cache = natten_amd.paged_cache(4, 1, 32, 16)
+    cache = natten_amd.PagedCache(*(_codes(t).as_strided((4, 1, 16, 32), (512, 7, 32, 1)).view(E4M3)
+                                    for t in cache[:2]), *cache[2:])
+    k, v = (randn((2, 20, 1, 32), BF16, s).to(DEV) for s in (1, 2))
+    q = randn((2, 3, 2, 32), BF16, 3).to(DEV)
+    tables = torch.tensor([[0, 2], [3, 1]], device=DEV)
+    _twins(cache, twin, q, k, v, tables, torch.tensor([20, 17], device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 70, 200])
+def test_pages_in_front_of_every_window_are_given_back(n):
+    """Their entries are -1, or name pages of NaNs: the same bits either way."""
+    import natten_amd
+
+    cache = natten_amd.paged_cache(130, 2, 64, 16)
+    tables = torch.randperm(128, generator=torch.Generator().manual_seed(1)).view(1, 128).int().to(DEV)
+    k, v = (randn((1, 2000, 2, 64), BF16, s).to(DEV) for s in (1, 2))
+    lens = torch.tensor([2000], device=DEV)
+    natten_amd.cache_append(cache, k, v, tables, lens)
+    _codes(cache[0])[129], _codes(cache[1])[129] = 127, 127
+    q = randn((1, n, 8, 64), BF16, 3).to(DEV)
+    want = natten_amd.cache_attention(q, cache, tables, lens, kernel_size=700, return_lse=True)
+    for entry in (-1, 129):
+        t = tables.clone()
+        t[:, :(2000 - n - 699) // 16] = entry
+        t[:, 125:] = entry
+        got = natten_amd.cache_attention(q, cache, t, lens, kernel_size=700, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), entry

@@ -31,8 +31,11 @@ namespace {
 
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
-constexpr int kAligned = 24;  // units
-constexpr int kEntries = 512;  // of a sample's table, in the LDS of a wide workgroup
+// Units of an even share up to which each workgroup takes one chunk of one item: 8 x 128
+// tokens of 4 heads of 64 against 4096 keys 37 us (46 with 0), 4 tokens against 1000 7.8
+// (10.2); at 80, 32 tokens of 8 heads of 128 against 16384 102 us (98).
+constexpr int kAligned = 24;
+constexpr int kEntries = 512;  // of a sample's table at a time, 4 KB of a wide workgroup's LDS
 constexpr int kJoin = 8;    // parts that a thread of the join loads at once
 
 struct CacheProb {
@@ -679,7 +682,10 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     const int j = ja + i;
     return ca + (j < nkt ? j : j - nkt) * TK;
   };
-  bool bad = false;  // the table names a page that is none, among those that rows see
+  // The table names a page that is none, among those that rows see.  (Pages in front of
+  // every window may have been given back: 2048 tokens of 32 heads of 64, a window of
+  // 4000, pages of 16: 209 us; 289 where those count.)
+  bool bad = false;
   // The lane's units of a tile; entry(i): entry i of the table.
   auto load = [&](int mine, u4 (&x)[NU], float (&scale)[NU], auto entry) {
     const int t0 = first_key(max(min(mine, nkt - 1), 0));
@@ -1071,14 +1077,25 @@ int cache_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 struct CacheShape {
   int rows, waves, wgs, least;
 };
+// Times in us, 8192 keys, bf16 but where said; heads: samples x key/value heads.
 CacheShape cache_shape(int dtype, int D, int64_t rows) {
-  if (dtype == NA_F32 || rows <= 16) return {16, 4, 512, 2};
-  if (D > 128) return {64, 4, 256, 1};
-  if (rows <= 32) return {32, 4, 512, 2};
+  // Float32's three parts leave registers for 16 rows; so do 32 of more than 64 channels
+  // (16 x 8 heads, 32 rows of 128: 76, narrow tiles of 32 rows 106, a wide one of 64 83;
+  // 8 x 4 heads, 24 of 256: 50 and the wide one 52).  More than 128 channels: one
+  // workgroup a CU (16 x 1 heads, 16 rows: 27, two of them 36).
+  if (dtype == NA_F32 || rows <= (D > 64 ? 32 : 16)) return {16, 4, D > 128 ? 256 : 512, 2};
+  if (rows <= 32) return {32, 4, 512, 2};  // (37; 16 rows 47, a wide tile 48)
+  // fp16's two parts leave registers for one workgroup a CU (2 x 8 heads, 2048 rows: 735,
+  // grids of two 750; bf16 439, of one 629)
+  if (D > 128) return {64, 4, dtype == NA_F16 ? 256 : 512, 1};
+  // (16 x 8 heads, 48 rows of 128: 87, three narrow tiles 128; 64 rows: 85, in a tile of
+  // 128 159; of 64 channels 49 and 64)
   if (rows <= 64) return {64, 4, 512, 1};
+  // (8 x 8 heads, 256 rows of 128: fp16 135, in tiles of 64 156; bf16 89, in tiles of 64 or
+  // 128 130; 2 x 8 heads, 4096 rows: 267, 449 and 386)
   if (dtype == NA_F16) return {128, 8, 256, 1};
-  if (rows <= 128) return {128, 4, 512, 1};
-  return D > 64 ? CacheShape{256, 8, 256, 1} : CacheShape{128, 4, 512, 1};
+  if (D > 64) return {256, 8, 256, 1};
+  return {128, 4, 512, 1};  // (8 x 8 heads, 512 rows: 118, in tiles of 64 145)
 }
 
 CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
@@ -1160,15 +1177,16 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
     constexpr int D = decltype(d)::value;
     if constexpr (sizeof(T) == 2) {
       if (P.rows == 64) return cache_launch<T, D, 1, 4, true>(P, A, st);
-      if constexpr (D <= 128) {
+      if constexpr (D <= 64) {
         if (P.rows == 32) return cache_launch<T, D, 2, 4, false>(P, A, st);
+      }
+      if constexpr (D <= 128) {
         if constexpr (std::is_same<T, f16_t>::value) {
           if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
+        } else if constexpr (D > 64) {
+          if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
         } else {
           if (P.rows == 128) return cache_launch<T, D, 2, 4, true>(P, A, st);
-          if constexpr (D > 64) {
-            if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
-          }
         }
       }
     }

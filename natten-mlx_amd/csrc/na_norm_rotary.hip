@@ -22,7 +22,9 @@
 // of tokens; each leaves one row of partial sums, added in a fixed order by
 // k_nr_wsum, so results do not depend on the run.
 //
-// Sums are float32; y, dx, dw and db are rounded once.  Bound: memory.
+// Sums are float32; y, dx, dw and db are rounded once.  Bound: memory: 131072 tokens of
+// 8 + 8 bf16 heads of 64, forward 537 MB in 124 us, backward 805 MB in 189, both 4.3 TB/s
+// where a large copy reaches 4.7; 64 tokens of 32 + 8 heads of 128 take 5.8 us.
 #include "na_rotary.h"
 
 // Sums and products are fused where it says so and nowhere else: the kernels of rows
@@ -32,9 +34,12 @@
 namespace na {
 namespace {
 
-constexpr int kNrBlocks = 1024;  // most workgroups of a backward: four on a CU
-constexpr int kNrUnits = 16;     // units per thread of a run
-constexpr int kNrTable = 2048;   // entries of a run's table, 16 KB
+// Most workgroups of a backward, four on a CU, and units per thread of a run: 25088
+// tokens of 8 + 8 heads of 32 bf16 channels, backward: 30 us, 37 with 2048 workgroups;
+// 131072 of 8 + 8 heads of 64, forward: 139, 146 with 8 units and 171 with 4.
+constexpr int kNrBlocks = 1024;
+constexpr int kNrUnits = 16;
+constexpr int kNrTable = 2048;  // entries of a run's table, 16 KB
 
 struct NrProb {
   RotProb R;  // per_block: tokens of a run; backward: of q's, qs / ks the rows of x

@@ -988,3 +988,45 @@ def test_pages_in_front_of_every_window_are_given_back(n):
         t[:, 125:] = entry
         got = natten_amd.cache_attention(q, cache, t, lens, kernel_size=700, return_lse=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), entry
+
+
+# ---- short and long tables ---------------------------------------------------
+# Single tokens against short tables run without a division of the keys; entries behind
+# every length that are no page make the tables long.
+
+def _lengthen(t):
+    size = t["cache"].key.shape[2]
+    t["tables"] = torch.cat([t["tables"], torch.full((t["tables"].shape[0], 4096 // size), -1, dtype=torch.int32)], 1)
+    return t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", list(CASES))
+def test_long_tables_of_short_sequences(case, dtype):
+    t = _lengthen(_make(CASES[case], dtype, 3))
+    _check(t, f"{case} {dtype}")
+    want = _run(t)
+    hidden = _unseen(t)
+    for i in (0, 1):
+        t["cache"][i].view(torch.uint8).masked_fill_(hidden[:, None, :, None], 0x7f)
+        t["cache"][2 + i].view(torch.uint8)[hidden.all(1)] = 255
+    for a, b in zip(_run(t), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("pages", [15, 16, 17, 24, 25, 80, 81])
+def test_on_both_sides_of_the_division(pages, dim, dtype):
+    """Tables of up to 256, 384 and 1280 keys and one page more, all of them full."""
+    _check(_make((2, 1, 4, 2, dim, 16, [16 * pages, 16 * pages - 9], None), dtype, pages))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_a_long_sequence_with_a_short_window(dtype):
+    """Keys from 60000 on, windows on either side of the division."""
+    for window in (1, 300, 1264, 1265, 3000):
+        _check(_make((1, 1, 4, 2, 64, 64, [61001], window), dtype, window), f"{window}")

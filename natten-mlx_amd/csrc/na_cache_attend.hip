@@ -1176,7 +1176,7 @@ struct CacheSizes {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     po = up((size_t)2 * P.wgs * P.rows * P.D * sizeof(float));
     pml = up((size_t)2 * P.wgs * P.rows * sizeof(float2));
-    span = P.wgs == 0 ? 0 : up((size_t)P.Hkv * P.items * sizeof(int2));
+    span = up((size_t)P.Hkv * P.items * sizeof(int2));  // (never nothing: a caller may count on it)
   }
   size_t total() const { return po + pml + span; }
 };

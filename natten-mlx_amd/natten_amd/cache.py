@@ -61,24 +61,29 @@ def _check_sizes(dim, page_size):
         raise ValueError(f"page_size must be one of {_lib.CACHE_PAGE_SIZES}, got {page_size}.")
 
 
+_DTYPES = (torch.float8_e4m3fn,) * 2 + (torch.float8_e8m0fnu,) * 2
+
+
 def _check_cache(cache):
+    """The shape ``(pages, heads, page_size, dim)``."""
     if not isinstance(cache, tuple) or len(cache) != 4:
         raise ValueError(f"cache must be a PagedCache, got {type(cache).__name__}.")
     k, v, ks, vs = cache
-    shape = k.shape
+    shape = tuple(k.shape)
     if len(shape) != 4 or v.shape != shape or shape[1] < 1:
         raise ValueError(f"cache.key and cache.value must be [pages, heads, page_size, dim], got "
-                         f"{tuple(shape)} and {tuple(v.shape)}.")
-    if ks.shape != shape[:2] or vs.shape != shape[:2]:
-        raise ValueError(f"cache.key_scale and cache.value_scale must be {tuple(shape[:2])}, got "
+                         f"{shape} and {tuple(v.shape)}.")
+    pages = shape[:2]
+    if ks.shape != pages or vs.shape != pages:
+        raise ValueError(f"cache.key_scale and cache.value_scale must be {pages}, got "
                          f"{tuple(ks.shape)} and {tuple(vs.shape)}.")
-    if (k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn
-            or ks.dtype != torch.float8_e8m0fnu or vs.dtype != torch.float8_e8m0fnu):
+    if (k.dtype, v.dtype, ks.dtype, vs.dtype) != _DTYPES:
         raise ValueError("cache must hold float8_e4m3fn and float8_e8m0fnu, got "
                          f"{[str(t.dtype) for t in cache]}.")
     _check_sizes(shape[3], shape[2])
+    flat = shape[1] * shape[2] * shape[3] < 1 << 31
     for t in (k, v):  # (a copy would not be the cache)
-        if not shape[0] or t.is_contiguous() and not t.data_ptr() % 16 and t.stride(0) < 1 << 31:
+        if flat and t.is_contiguous() and not t.data_ptr() % 16 or not shape[0]:
             continue
         st = [s if n > 1 else 0 for n, s in zip(shape, t.stride())]
         if t.data_ptr() % 16 or st[3] != 1 or any(s % 16 for s in st[:3]):
@@ -90,7 +95,7 @@ def _check_cache(cache):
     return shape
 
 
-def _check_lens(name, t, b, tables=None):
+def _check_lens(name, t, b):
     if t.ndim != 1 or t.shape[0] != b:
         raise ValueError(f"{name} must be a 1-D array of length B={b}, got shape {tuple(t.shape)}.")
     if t.dtype not in (torch.int32, torch.int64):
@@ -149,12 +154,13 @@ def cache_append(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, tabl
     ``torch.no_grad()``.
     """
     shape = _check_cache(cache)
-    if key.ndim != 4 or key.shape != value.shape or key.shape[2:] != (shape[1], shape[3]):
+    new = tuple(key.shape)
+    if len(new) != 4 or value.shape != new or new[2:] != (shape[1], shape[3]):
         raise ValueError(f"key and value must be [B, L, {shape[1]}, {shape[3]}], got "
                          f"{tuple(key.shape)} and {tuple(value.shape)}.")
     if key.dtype != value.dtype:
         raise ValueError(f"key and value must have the same dtype, got {key.dtype} and {value.dtype}.")
-    b, n = key.shape[:2]
+    b, n = new[:2]
     _check_tables(tables, b, shape[2])
     _check_lens("seq_lens", seq_lens, b)
     capacity = tables.shape[1] * shape[2]

@@ -1153,7 +1153,9 @@ CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   P.M = p->table_pages;
   P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
   P.least = shape.least;
-  P.wgs = P.rows == 16 && cache_keys(P) <= cache_whole(P.D).keys ? 0 : shape.wgs;
+  const CacheWhole whole = cache_whole(cache_width(P.D));
+  const bool one_launch = (int64_t)P.items * P.Hkv * 64 * whole.waves < ((int64_t)1 << 32);
+  P.wgs = P.rows == 16 && cache_keys(P) <= whole.keys && one_launch ? 0 : shape.wgs;
   P.sl2 = p->scale * kLog2e;
   P.frep = make_fastdiv((uint32_t)P.rep);
   P.frt = make_fastdiv((uint32_t)P.rt);
@@ -1260,8 +1262,6 @@ bool cache_attend_fits(const na_cache_params *p, size_t *workspace_bytes) {
   const int64_t threads = ((int64_t)P.B * P.Hkv * P.Mo) << CacheJoinLanes(P).total();
   // all units, as the kernels count them, of full tables
   const int64_t units = (int64_t)P.items * P.Hkv * (cache_keys(P) / kUnit + 2);
-  if (P.wgs == 0 && (int64_t)P.items * P.Hkv * 64 * cache_whole(P.D).waves >= ((int64_t)1 << 32))
-    return false;
   return threads < ((int64_t)1 << 32) - 256 && units < ((int64_t)1 << 31);
 }
 

@@ -226,3 +226,92 @@ def test_fused_layer_arguments():
     torch.save(two, f)
     f.seek(0)
     assert torch.load(f, weights_only=False).qk_fused is False
+
+
+@pytest.mark.gpu
+def test_compiled():
+    """A compiled step leaves the operators to eager execution: the same bits."""
+    import natten_amd
+
+    B, hk, size = 3, 2, 16
+    q, k, v = (randn((B, 4, h, 32), BF16, s).to(DEV) for s, h in ((1, 4), (2, hk), (3, hk)))
+    w = randn((32,), BF16, 4).to(DEV)
+    tables = torch.arange(B * 4, device=DEV).view(B, 4)
+    lens = torch.tensor([40, 4, 17], device=DEV)
+
+    def step(cache, q, k, v, lens):
+        a, b = natten_amd.norm_rotary(q * 2, k, w, None, w, None, axis_dims=(32,))
+        natten_amd.cache_append(cache, b, v, tables, lens)
+        return natten_amd.cache_attention(a, cache, tables, lens, kernel_size=20) + 1
+
+    with torch.no_grad():
+        caches = [natten_amd.paged_cache(B * 4, hk, 32, size) for _ in range(2)]
+        want = step(caches[0], q, k, v, lens)
+        assert torch.equal(torch.compile(step, backend="eager")(caches[1], q, k, v, lens), want)
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_two_steps_at_once():
+    """Two streams, each its own samples and pages of one cache; the same calls one after
+    the other."""
+    import natten_amd
+
+    B, hk, D, size = 6, 2, 64, 32
+    start = randn((2 * B, 300, hk, D), BF16, 1).to(DEV)
+    q, k, v = (randn((2 * B, 1, h, D), BF16, s).to(DEV) for s, h in ((2, 8), (3, hk), (4, hk)))
+    for width in (11, 64):  # tables of one launch and of two
+        tables = torch.randperm(2 * B * 11, generator=torch.Generator().manual_seed(1)).view(2 * B, 11)
+        tables = torch.cat([tables, torch.full((2 * B, width - 11), -1)], 1).to(DEV)
+        lens = torch.arange(290, 290 + 2 * B, device=DEV)
+        outs = []
+        for together in (True, False):
+            cache = natten_amd.paged_cache(2 * B * 11, hk, D, size)
+            natten_amd.cache_append(cache, start, start, tables, lens - 1)
+            streams = [torch.cuda.Stream() for _ in "ab"]
+            torch.cuda.synchronize()
+            got = [None, None]
+            for rep in range(5):
+                for i, s in enumerate(streams):
+                    part = slice(i * B, (i + 1) * B)
+                    with torch.cuda.stream(s):
+                        natten_amd.cache_append(cache, k[part], v[part], tables[part], lens[part])
+                        got[i] = natten_amd.cache_attention(q[part], cache, tables[part], lens[part])
+                    if not together:
+                        torch.cuda.synchronize()
+            torch.cuda.synchronize()
+            outs.append((torch.cat(got), *(t.view(torch.uint8) for t in cache)))
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_queries():
+    """norm_rotary and its gradients at the end of a tensor of more than 2^31 elements, and
+    a prompt's attention into an output of more: the last rows alone, the same bits."""
+    import natten_amd
+
+    n, D = (1 << 21) + 77, 128
+    w, b = (randn((D,), BF16, s).to(DEV) for s in (1, 2))
+    q = torch.empty((1, n, 8, D), dtype=BF16, device=DEV).normal_().requires_grad_(True)
+    g = torch.empty_like(q, requires_grad=False).normal_()
+    out = natten_amd.norm_rotary(q, None, w, b, axis_dims=(D,))
+    dq, = torch.autograd.grad(out, q, g)
+    for at in (0, n - 5):
+        part = q.detach()[:, at:at + 5].clone().requires_grad_(True)
+        pos = torch.arange(at, at + 5, device=DEV).unsqueeze(-1)
+        few = natten_amd.norm_rotary(part, None, w, b, positions=pos, axis_dims=(D,))
+        assert torch.equal(out[:, at:at + 5], few)
+        assert torch.equal(dq[:, at:at + 5], torch.autograd.grad(few, part, g[:, at:at + 5])[0])
+    del out, dq, g
+    cache = natten_amd.paged_cache(4, 8, D, 16)
+    kv = randn((1, 64, 8, D), BF16, 5).to(DEV)
+    tables = torch.tensor([[2, 0, 3, 1]], device=DEV)
+    with torch.no_grad():
+        natten_amd.cache_append(cache, kv, kv, tables, torch.tensor([64], device=DEV))
+        # (all but the last 64 of the rows lie before the sequence's start)
+        out = natten_amd.cache_attention(q, cache, tables, torch.tensor([64], device=DEV))
+        few = natten_amd.cache_attention(q[:, -64:], cache, tables, torch.tensor([64], device=DEV))
+    assert torch.allclose(out[:, -64:].float(), few.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+    assert few.abs().max() > 0 and not out[:, :-64].any()

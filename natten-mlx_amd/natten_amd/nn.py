@@ -270,9 +270,10 @@ class _NeighborhoodAttention(_nn.Module):
         return q, k, v
 
     def _fuses_norms(self) -> bool:
-        """Whether the norms are the layer's plain ones: a replaced or hooked module is
-        called itself."""
+        """Whether the norms are the layer's plain ones, alike: a replaced or hooked module
+        is called itself."""
         return (self.q_norm.eps == self.k_norm.eps
+                and self.q_norm.weight.dtype == self.k_norm.weight.dtype
                 and not torch.nn.modules.module._has_any_global_hook()
                 and all(type(m) is LayerNorm and "forward" not in m.__dict__
                         and not any(getattr(m, h) for h in _HOOKS)

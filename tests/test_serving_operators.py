@@ -315,3 +315,42 @@ def test_more_than_32_bits_of_queries():
         few = natten_amd.cache_attention(q[:, -64:], cache, tables, torch.tensor([64], device=DEV))
     assert torch.allclose(out[:, -64:].float(), few.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
     assert few.abs().max() > 0 and not out[:, :-64].any()
+
+
+@pytest.mark.gpu
+def test_inference_mode():
+    """A cache made under inference mode, by both routes, and one made outside it."""
+    import natten_amd
+    from natten_amd.autograd import fused
+
+    k, q = randn((2, 5, 2, 32), BF16, 1).to(DEV), randn((2, 5, 4, 32), BF16, 2).to(DEV)
+    tables, lens = torch.tensor([[0], [1]], device=DEV), torch.tensor([5, 3], device=DEV)
+
+    def step(cache):
+        natten_amd.cache_append(cache, k, k, tables, lens)
+        return natten_amd.cache_attention(q, cache, tables, lens).clone()
+
+    outside = natten_amd.paged_cache(2, 2, 32, 16)
+    outs = [step(outside)]
+    with torch.inference_mode():
+        outs.append(step(outside))
+        outs.append(step(natten_amd.paged_cache(2, 2, 32, 16)))
+        with fused.python_autograd():
+            outs.append(step(outside))
+            outs.append(step(natten_amd.paged_cache(2, 2, 32, 16)))
+        inside = natten_amd.paged_cache(2, 2, 32, 16)
+        outs.append(torch.compile(step, backend="eager")(inside))
+    outs.append(step(inside))
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
+@pytest.mark.gpu
+def test_fused_layer_with_unlike_norms():
+    """Weights of two types, which one pass does not take, run as without qk_fused."""
+    kw = dict(embed_dim=64, num_heads=2, kernel_size=7, qk_norm=True, rotary=True)
+    two, one = (_layer(2, BF16, qk_fused=f, **kw).to(DEV) for f in (False, True))
+    x = randn((2, 16, 14, 64), BF16, 1).to(DEV)
+    for m in (two, one):
+        m.q_norm.float()  # (the other's weights stay bfloat16)
+    assert torch.equal(one(x), two(x))

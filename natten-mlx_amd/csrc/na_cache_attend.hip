@@ -1020,8 +1020,16 @@ __global__ void __launch_bounds__(64 * cache_whole(D).waves) k_cache_whole(Cache
   cache_narrow<T, D, 1, cache_whole(D).waves>(P, A, w, uniform(g), w.k0, w.hi, -1, smem);
 }
 
+// Waves that a SIMD holds of a wide workgroup's.  Eight waves of 16 bf16 rows of 64
+// channels have few enough registers for four (8 x 8 heads, 512 rows: 118 us, four waves
+// of 32 rows, two a SIMD: 125; 128 rows: 45 and 47).
+template <typename T, int D, int NW>
+constexpr int cache_wide_waves() {
+  return D > 128 ? 1 : std::is_same<T, bf16_t>::value && D <= 64 && NW == 8 ? 4 : 2;
+}
+
 template <typename T, int D, int NQ, int NW>
-__global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_wide(CacheProb P, CacheArgs A) {
+__global__ void __launch_bounds__(64 * NW, (cache_wide_waves<T, D, NW>())) k_cache_wide(CacheProb P, CacheArgs A) {
   extern __shared__ __align__(16) char smem[];
   cache_parts_of(P, A, [&](const CacheItem &w, int g, int ka, int kb, int part) {
     cache_wide<T, D, NQ, NW>(P, A, w, g, ka, kb, part, smem);
@@ -1121,13 +1129,13 @@ CacheShape cache_shape(int dtype, int D, int64_t rows) {
   // grids of two 750; bf16 439, of one 629)
   if (D > 128) return {64, 4, dtype == NA_F16 ? 256 : 512, 1};
   // (16 x 8 heads, 48 rows of 128: 87, three narrow tiles 128; 64 rows: 85, in a tile of
-  // 128 159; of 64 channels 49 and 64)
+  // 128 159; of 64 channels 52 and 66)
   if (rows <= 64) return {64, 4, 512, 1};
   // (8 x 8 heads, 256 rows of 128: fp16 135, in tiles of 64 156; bf16 89, in tiles of 64 or
   // 128 130; 2 x 8 heads, 4096 rows: 267, 449 and 386)
   if (dtype == NA_F16) return {128, 8, 256, 1};
   if (D > 64) return {256, 8, 256, 1};
-  return {128, 4, 512, 1};  // (8 x 8 heads, 512 rows: 118, in tiles of 64 145)
+  return {128, 8, 512, 1};  // (8 x 8 heads, 512 rows: 118, in tiles of 64 145)
 }
 
 // The most keys that an item's rows see, where tables are full.
@@ -1231,12 +1239,10 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
         if (P.rows == 32) return cache_launch<T, D, 2, 4, false>(P, A, st);
       }
       if constexpr (D <= 128) {
-        if constexpr (std::is_same<T, f16_t>::value) {
-          if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
-        } else if constexpr (D > 64) {
+        if constexpr (std::is_same<T, bf16_t>::value && D > 64) {
           if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
         } else {
-          if (P.rows == 128) return cache_launch<T, D, 2, 4, true>(P, A, st);
+          if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
         }
       }
     }

@@ -88,11 +88,15 @@ struct CacheItem {
   int units;
 };
 
-__device__ __forceinline__ CacheItem cache_item(const CacheProb &P, int i) {
+__device__ __forceinline__ int cache_len(const CacheProb &P, int i) {
+  return min(max(P.lens[fdiv((uint32_t)i, P.frt)], 0), P.M << P.lgT);
+}
+
+__device__ __forceinline__ CacheItem cache_item(const CacheProb &P, int i, int len) {
   CacheItem w;
   w.b = (int)fdiv((uint32_t)i, P.frt);
   const int r = i - w.b * P.rt;
-  w.len = min(max(P.lens[w.b], 0), P.M << P.lgT);
+  w.len = len;
   w.row0 = r * P.rows;
   w.row1 = min(w.row0 + P.rows, P.Mo);
   const int first = w.len - P.Lq + (int)fdiv((uint32_t)w.row0, P.frep);
@@ -127,20 +131,25 @@ __device__ __forceinline__ void cache_uniform(CacheItem &w) {
 
 // The items of a head in order, 64 at a time, their chunks of `size` units added up.
 struct CacheScan {
-  int i0 = -1, size = 0, units = 0;  // first item, the lane's units
+  int i0 = -64, size = 0, units = 0, len = 0;  // first item, the lane's units
   int mine = 0, sum = 0, all = 0;    // the lane's chunks, up to it, of all 64
   __device__ __forceinline__ void load(const CacheProb &P, int first, int chunk) {
     if (first != i0) {
       i0 = first;
       size = 0;
       const int i = i0 + (threadIdx.x & 63);
-      units = i < P.items ? cache_item(P, i).units : 0;
+      len = i < P.items ? cache_len(P, i) : 0;
+      units = i < P.items ? cache_item(P, i, len).units : 0;
     }
     if (chunk == size) return;
     size = chunk;
     mine = (int)((unsigned)(units + size - 1) / (unsigned)size);
     sum = wave_scan(mine);
     all = __builtin_amdgcn_readlane(sum, 63);
+  }
+  __device__ __forceinline__ CacheItem item(const CacheProb &P, int i) const {
+    return cache_item(P, i, (uint32_t)(i - i0) < 64u ? __builtin_amdgcn_readlane(len, i - i0)
+                                                     : cache_len(P, i));
   }
   // Chunks of all items.
   __device__ __forceinline__ int total(const CacheProb &P, int chunk) {
@@ -166,25 +175,43 @@ struct CacheScan {
   }
 };
 
-// Entry i of a sample's table: the page or -1, and the bytes of its scales, of keys and
-// above of values.
-__device__ __forceinline__ int2 cache_entry(const CacheProb &P, int sample, int g, int i) {
-  int page = i < P.M ? P.tables[sample * P.ts + i] : -1;
-  if ((uint32_t)page >= (uint32_t)P.pages) return make_int2(-1, 0);
-  const int a = P.k.scale[page * P.k.sc[0] + g * P.k.sc[1]];
-  const int b = P.v.scale[page * P.v.sc[0] + g * P.v.sc[1]];
-  // (bytes past the largest scale, as unwritten pages hold them, stay finite)
-  return make_int2(page, min(a, kScaleBias + kScaleHigh) | min(b, kScaleBias + kScaleHigh) << 8);
+// Entry i of a sample's table: the page or -1, and the bytes of its scales.
+struct CacheEntry {
+  int page, k, v;
+  __device__ __forceinline__ CacheEntry(const CacheProb &P, int sample, int g, int i) {
+    page = i < P.M ? P.tables[sample * P.ts + i] : -1;
+    k = v = 0;
+    if ((uint32_t)page >= (uint32_t)P.pages) {
+      page = -1;
+    } else {
+      k = P.k.scale[page * P.k.sc[0] + g * P.k.sc[1]];
+      v = P.v.scale[page * P.v.sc[0] + g * P.v.sc[1]];
+    }
+  }
+};
+
+// Both scales' bytes, of keys and above of values.  (Bytes past the largest scale, as
+// unwritten pages hold them, stay finite.)
+__device__ __forceinline__ int cache_scales(int k, int v) {
+  return min(k, kScaleBias + kScaleHigh) | min(v, kScaleBias + kScaleHigh) << 8;
 }
 
-// 64 entries of a sample's table, one a lane.
+// As the wide workgroups' table holds it.
+__device__ __forceinline__ int2 cache_entry(const CacheProb &P, int sample, int g, int i) {
+  const CacheEntry e(P, sample, g, i);
+  return make_int2(e.page, cache_scales(e.k, e.v));
+}
+
+// 64 entries of a sample's table, one a lane.  The scales' bytes stay as they are loaded,
+// so that the first keys' loads do not wait for them.
 struct PageWindow {
-  int base, page, sc;
+  int base, page, k, v;
   __device__ __forceinline__ void load(const CacheProb &P, int sample, int g, int first) {
     base = first;
-    const int2 x = cache_entry(P, sample, g, first + (threadIdx.x & 63));
-    page = x.x;
-    sc = x.y;
+    const CacheEntry e(P, sample, g, first + (threadIdx.x & 63));
+    page = e.page;
+    k = e.k;
+    v = e.v;
   }
   // Whether it holds table entry i (uniform).
   __device__ __forceinline__ bool holds(int i) const { return (uint32_t)(i - base) < 64u; }
@@ -192,7 +219,7 @@ struct PageWindow {
     return __builtin_amdgcn_readlane(page, i - base);
   }
   __device__ __forceinline__ int scales_of(int i) const {
-    return __builtin_amdgcn_readlane(sc, i - base);
+    return cache_scales(__builtin_amdgcn_readlane(k, i - base), __builtin_amdgcn_readlane(v, i - base));
   }
 };
 
@@ -393,7 +420,7 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   __bf16 *const vs = reinterpret_cast<__bf16 *>(smem) + wv * (kTile * RS);  // the wave's own
   uint16_t *const nan = reinterpret_cast<uint16_t *>(smem + sizeof(__bf16) * NW * kTile * RS) +
                         wv * (kTile * UPR);
-  bf8 qf[NQ][2 * NS][NP];
+  Query8<T> qr[NQ][2 * NS];
   int lo[NQ], cnt[NQ];
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) {
@@ -403,11 +430,10 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
 #pragma unroll
     for (int s = 0; s < 2 * NS; ++s) {
       const int c = 64 * (s / 2) + 16 * gq + 8 * (s & 1);
-      Query8<T> x;
-      x.load(row.q + c, c < P.D);
-      x.template parts<NP>(qf[qi][s]);
+      qr[qi][s].load(row.q + c, c < P.D);
     }
   }
+  bf8 qf[NQ][2 * NS][NP];
   const int vc = lane % UPR, vr = lane / UPR;
   u4 kr[2][NS], vr8[NU];
   int entry[2];  // of the table, of the loaded tile's halves
@@ -564,6 +590,10 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
   };
   int t0 = ka + wv * kTile;
   if (t0 < kb) load(t0);
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+    for (int s = 0; s < 2 * NS; ++s) qr[qi][s].template parts<NP>(qf[qi][s]);  // beside those loads
   for (; t0 < kb; t0 += NW * kTile) {
     if (t0 >= all0 && t0 + kTile <= all1 && !bad) run_tile(t0, std::false_type{});
     else run_tile(t0, std::true_type{});
@@ -977,7 +1007,7 @@ __device__ __forceinline__ void cache_parts_of(const CacheProb &P, const CacheAr
   int i = uniform(scan.find(P, off, chunk));
   off = uniform(off);
   while (u < end) {
-    CacheItem w = cache_item(P, i);
+    CacheItem w = scan.item(P, i);
     cache_uniform(w);
     if (w.units > 0) {
       const int chunks = uniform((w.units + chunk - 1) / chunk);
@@ -1015,7 +1045,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(64 * cache_whole(D).waves) k_cache_whole(CacheProb P, CacheArgs A) {
   extern __shared__ __align__(16) char smem[];
   const int g = (int)(blockIdx.x / (uint32_t)P.items);
-  CacheItem w = cache_item(P, (int)blockIdx.x - g * P.items);
+  const int i = (int)blockIdx.x - g * P.items;
+  CacheItem w = cache_item(P, i, cache_len(P, i));
   cache_uniform(w);
   cache_narrow<T, D, 1, cache_whole(D).waves>(P, A, w, uniform(g), w.k0, w.hi, -1, smem);
 }
@@ -1049,8 +1080,8 @@ __global__ void __launch_bounds__(256) k_cache_join(CacheProb P, CacheArgs A, in
   const int64_t at = min(mine, rows - 1), bg = at / P.Mo;
   const int row = (int)(at - bg * P.Mo), b = (int)(bg / P.Hkv), g = (int)(bg - (int64_t)b * P.Hkv);
   const int tile = row / P.rows, item = b * P.rt + tile, r = row - tile * P.rows;
-  int2 span = make_int2(0, -1);
-  if (cache_item(P, item).units > 0) span = A.span[(int64_t)g * P.items + item];
+  int2 span = A.span[(int64_t)g * P.items + item];  // beside the length
+  if (cache_item(P, item, cache_len(P, item)).units == 0) span = make_int2(0, -1);  // (not written)
   float m = -INFINITY, l = 0.f;
   f32x4 acc = zero4();
   if (span.x != span.y) {  // (else its workgroup has written it)

@@ -67,16 +67,18 @@ struct CacheArgs {
 };
 
 // Keys, of full tables or a window, up to which each item of narrow tiles has a workgroup
-// of its own, and its waves: what a second launch costs weighs more than what idle CUs
-// would do.  One token, up to so many keys, us (shared out and joined): 4 x 2 heads of 64:
-// 512 6.7 (11.7), 1280 9.5 (12.0), 2048 12.7 (12.2); 1 x 8 of 128: 512 8.1 (12.0), 1280
-// 12.6 (12.4), 2048 17.0 (12.5); 64 x 8 of 128: 512 18.6 (21.2), 1280 29.9 (33.5); 4 x 4
-// of 256: 256 10.2 (14.3), 512 15.0 (14.7).
+// of its own: what a second launch costs weighs more than what idle CUs would do.  `many`
+// where there are items for half of the CUs.  One token, up to so many keys, us (shared
+// out and joined): 4 x 2 heads of 64: 512 6.7 (11.7), 1280 9.5 (12.0), 2048 12.7 (12.2);
+// 1 x 8 of 128: 512 8.1 (12.0), 1280 12.6 (12.4), 2048 17.0 (12.5); 16 x 8 of 128: 1536
+// 16.6 (21.0), 2048 20.3 (22.9), 2560 22.9 (25.2), of lengths from 1 on 15.9 (16.4), 18.9
+// (20.1), 21.3 (22.0), in float32 19.3 (18.7), 23.4 (22.6), 26.4 (24.5); 4 x 4 of 256: 256
+// 10.2 (14.3), 512 15.0 (14.7).
 struct CacheWhole {
-  int keys, waves;
+  int keys, many, waves;
 };
 constexpr CacheWhole cache_whole(int D) {
-  return D > 128 ? CacheWhole{384, 4} : CacheWhole{1280, 8};
+  return D > 128 ? CacheWhole{384, 384, 4} : CacheWhole{1280, 2048, 8};
 }
 
 // The keys that an item's rows see, and units over them.
@@ -1193,8 +1195,10 @@ CacheProb cache_prob(const na_cache_params *p, const na_cache *c) {
   P.W = p->window > 0 ? std::min(p->window, 1 << 30) : 1 << 30;
   P.least = shape.least;
   const CacheWhole whole = cache_whole(cache_width(P.D));
-  const bool one_launch = (int64_t)P.items * P.Hkv * 64 * whole.waves < ((int64_t)1 << 32);
-  P.wgs = P.rows == 16 && cache_keys(P) <= whole.keys && one_launch ? 0 : shape.wgs;
+  const int64_t items = (int64_t)P.items * P.Hkv;
+  const bool is_whole = P.rows == 16 && cache_keys(P) <= (items < 128 ? whole.keys : whole.many) &&
+                        items * 64 * whole.waves < ((int64_t)1 << 32);
+  P.wgs = is_whole ? 0 : shape.wgs;
   P.sl2 = p->scale * kLog2e;
   P.frep = make_fastdiv((uint32_t)P.rep);
   P.frt = make_fastdiv((uint32_t)P.rt);

@@ -1026,6 +1026,15 @@ def test_on_both_sides_of_the_division(pages, dim, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("samples, pages", [(63, 128), (64, 128), (64, 129)])
+def test_on_both_sides_of_the_division_of_many(samples, pages, dtype):
+    """Half a chip's items, tables of up to 2048 keys and one page more."""
+    lens = [16 * pages, 1, 777, 0, 1300, 16 * pages - 30]
+    _check(_make((samples, 1, 4, 2, 64, 16, lens, None), dtype, pages))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_a_long_sequence_with_a_short_window(dtype):
     """Keys from 60000 on, windows on either side of the division."""
     for window in (1, 300, 1264, 1265, 3000):

@@ -36,9 +36,10 @@ namespace {
 
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
-// Units of an even share up to which each workgroup takes one chunk of one item: 8 x 128
-// tokens of 4 heads of 64, a window of 4095: 37 us (46 with 0), 4 tokens against 1000 7.8
-// (10.2); at 80, 32 tokens of 8 heads of 128 against 16384 102 us (98).
+// Units of an even share up to which each workgroup takes one chunk of one item.  Ragged
+// lengths, us (with 0): 8 x 128 tokens of 4 heads of 64, a window of 4095: 36 (39); a token
+// each of 8 samples of up to 4096, 8 heads of 128: 17.5 (19.2).  At 80, 32 samples of up to
+// 16384: 122, at 24 111.
 constexpr int kAligned = 24;
 constexpr int kEntries = 512;  // of a sample's table at a time, 4 KB of a wide workgroup's LDS
 constexpr int kJoin = 8;    // parts that a thread of the join loads at once

@@ -35,8 +35,8 @@ namespace na {
 namespace {
 
 // Most workgroups of a backward, four on a CU, and units per thread of a run: 25088
-// tokens of 8 + 8 heads of 32 bf16 channels, backward: 30 us, 37 with 2048 workgroups;
-// 131072 of 8 + 8 heads of 64, forward: 139, 146 with 8 units and 171 with 4.
+// tokens of 8 + 8 heads of 32 bf16 channels, backward: 27 us, 34 with 2048 workgroups;
+// 131072 of 8 + 8 heads of 64, forward: 126, 135 with 8 units and 162 with 4.
 constexpr int kNrBlocks = 1024;
 constexpr int kNrUnits = 16;
 constexpr int kNrTable = 2048;  // entries of a run's table, 16 KB

@@ -6,10 +6,10 @@
 // softmax's sum.  Token i lies in slot i mod T of page tables[b][i / T]; keys and values
 // are e4m3 codes times their page's and head's power of two, which every bf16 holds
 // exactly: they become bf16 as they are read, and products run on the bf16 matrix
-// cores.  Queries and probabilities meet them in parts of 8 bits each: bf16 in one,
-// fp16 in two (16 bits; its queries exactly), float32 in three (24 bits).  Scores, sums
-// and outputs are float32, probabilities lose half a step of their parts, out is
-// rounded once.
+// cores.  Queries and probabilities meet them in parts of 8 bits each: bf16 queries in
+// one and fp16 ones in two (both exactly), float32 in three (24 bits); probabilities of
+// 16-bit queries in two (16 bits), of float32 in three.  Scores, sums and outputs are
+// float32, probabilities lose half a step of their parts, out is rounded once.
 //
 // The rows of a sample and key/value head (its query heads of all its new tokens)
 // are cut into tiles; a tile and the keys its rows see are an item, cut into units of
@@ -20,9 +20,10 @@
 // online softmax, float32 -- per workgroup, and k_cache_join adds those of a row.
 // Where tables are short, each item has a workgroup of its own and nothing is joined.
 //
-// A token each of 32 samples of 8192 tokens, 8 heads of 128, 537 MB: 103 us with the
-// join, 5.2 TB/s (memory); 2 x 1024 tokens of 32 heads at 8192 tokens: 267 us, 0.97
-// PFLOP/s (the matrix cores; a large bf16 product reaches 1.15).
+// A token each of 32 samples of 8192 tokens, 8 heads of 128, 537 MB: 101 us with the
+// join, 5.3 TB/s (memory); 2 x 1024 tokens of 32 heads at 8192 tokens: 352 us, 0.73
+// PFLOP/s in 1.5 products for one, 1.10 of the matrix cores, which bound it (a large
+// bf16 product reaches 1.09 to 1.15; probabilities of 8 bits: 265 us).
 #include "na_cache.h"
 #include "na_chunk.h"
 #include "na_launch.h"
@@ -37,9 +38,9 @@ namespace {
 constexpr int kUnit = 64;   // keys
 constexpr int kTile = 32;   // keys of a narrow wave's tile
 // Units of an even share up to which each workgroup takes one chunk of one item.  Ragged
-// lengths, us (with 0): 8 x 128 tokens of 4 heads of 64, a window of 4095: 36 (39); a token
-// each of 8 samples of up to 4096, 8 heads of 128: 17.5 (19.2).  At 80, 32 samples of up to
-// 16384: 122, at 24 111.
+// lengths, us (with 0): 8 x 128 tokens of 4 heads of 64, a window of 4095: 48.0 (50.5); a
+// token each of 8 samples of up to 4096, 8 heads of 128: 16.9 (18.9).  At 80, 32 samples of
+// up to 16384: 119, at 24 110.
 constexpr int kAligned = 24;
 constexpr int kEntries = 512;  // of a sample's table at a time, 4 KB of a wide workgroup's LDS
 constexpr int kJoin = 8;    // parts that a thread of the join loads at once
@@ -247,9 +248,16 @@ __device__ __forceinline__ bf8 decode8(uint32_t a, uint32_t b, float s) {
   return o.v;
 }
 
+// Parts of a query, and of a probability: one of 8 bits is off by up to half a step of
+// bf16 outputs themselves (0.0023 of the outputs against 64 bits, with two 0.0017, which is
+// their own rounding).
 template <typename T>
 constexpr int cache_parts() {
   return std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3;
+}
+template <typename T>
+constexpr int cache_prob_parts() {
+  return sizeof(T) == 2 ? 2 : 3;
 }
 
 // Eight numbers as sums of parts.
@@ -416,7 +424,8 @@ template <typename T, int D, int NQ, int NW>
 __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs &A,
                                              const CacheItem &w, int g, int ka, int kb, int part,
                                              char *smem) {
-  constexpr int NP = cache_parts<T>(), NS = D / 64, NDB = D / 16, RS = D + 8;
+  constexpr int NP = cache_parts<T>(), PP = cache_prob_parts<T>();
+  constexpr int NS = D / 64, NDB = D / 16, RS = D + 8;
   constexpr int UPR = D / 16, RPP = 64 / UPR, NU = kTile / RPP;  // V: units per row, rows per pass
   const int tid = threadIdx.x, wv = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 15, gq = lane >> 4;
@@ -571,9 +580,9 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    bf8 bp[NQ][NP];
+    bf8 bp[NQ][PP];
 #pragma unroll
-    for (int qi = 0; qi < NQ; ++qi) split8<NP>(p[qi], bp[qi]);
+    for (int qi = 0; qi < NQ; ++qi) split8<PP>(p[qi], bp[qi]);
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const bf4 lo4 = M16::tr(vs + tr_off + 16 * db);
@@ -582,7 +591,7 @@ __device__ __forceinline__ void cache_narrow(const CacheProb &P, const CacheArgs
 #pragma unroll
       for (int qi = 0; qi < NQ; ++qi)
 #pragma unroll
-        for (int x = NP - 1; x >= 0; --x) o[qi][db] = M16::mma(va, bp[qi][x], o[qi][db]);
+        for (int x = PP - 1; x >= 0; --x) o[qi][db] = M16::mma(va, bp[qi][x], o[qi][db]);
     }
     if (EDGE && odd) {
 #pragma unroll
@@ -654,7 +663,7 @@ template <typename T, int D, int NQ, int NW>
 __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &A,
                                            const CacheItem &w, int g, int ka, int kb, int part,
                                            char *smem) {
-  constexpr int NP = cache_parts<T>();
+  constexpr int NP = cache_parts<T>(), PP = cache_prob_parts<T>();
   constexpr int TK = cache_tile<D>(), CH = TK / 16;
   constexpr int NT = D / 32, NDB = D / 16, RSE = lds_row(D);
   constexpr int UPR = D / 16, RPW = 64 / UPR, RPP = RPW * NW / 2, NU = TK / RPP;
@@ -711,9 +720,9 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
     const bf4 lo4 = M16::tr(ca), hi4 = M16::tr(ca + 16 * RSE);
     return (bf8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto product = [&](bf8 a, const bf8 (&b)[NP], f32x4 c) {
+  auto product = [&](bf8 a, const auto &b, f32x4 c) {
 #pragma unroll
-    for (int p = NP - 1; p >= 0; --p) c = M16::mma(a, b[p], c);
+    for (int p = (int)(sizeof(b) / sizeof(bf8)) - 1; p >= 0; --p) c = M16::mma(a, b[p], c);
     return c;
   };
   typedef f32x4 Scores[NQ][CH];
@@ -854,11 +863,11 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
       p = __builtin_amdgcn_exp2f(fmaf(p, sl2, -mu[qi]));
       l[qi] += p;
     };
-    auto rounded = [&](int qi, int jj, bf8 (&b)[NP]) {
+    auto rounded = [&](int qi, int jj, bf8 (&b)[PP]) {
       float p[8];
 #pragma unroll
       for (int x = 0; x < 8; ++x) p[x] = s[qi][2 * jj + x / 4][x % 4];
-      split8<NP>(p, b);
+      split8<PP>(p, b);
     };
     constexpr int ALL = CH * 4, FIRST = CH > 2 ? ALL / 2 : ALL;  // a lane's scores, beside QK
     constexpr int QS = CH * NT, OS = CH / 2 * NDB;  // steps of the two products
@@ -881,7 +890,7 @@ __device__ __forceinline__ void cache_wide(const CacheProb &P, const CacheArgs &
       }
       __builtin_amdgcn_sched_barrier(0x124);
     }
-    bf8 bp[NQ][NP];
+    bf8 bp[NQ][PP];
 #pragma unroll
     for (int qi = 0; qi < NQ; ++qi) rounded(qi, 0, bp[qi]);
     bf8 va[2];
@@ -1043,9 +1052,11 @@ __global__ void __launch_bounds__(64 * NW, D > 128 ? 1 : 2) k_cache_narrow(Cache
   });
 }
 
-// An item a workgroup.
+// An item a workgroup.  Two of 64 bf16 channels share a CU (64 x 8 heads, 2048 keys: 24.4
+// us, one 26.9).
 template <typename T, int D>
-__global__ void __launch_bounds__(64 * cache_whole(D).waves) k_cache_whole(CacheProb P, CacheArgs A) {
+__global__ void __launch_bounds__(64 * cache_whole(D).waves, (std::is_same<T, bf16_t>::value && D <= 64 ? 4 : 1))
+    k_cache_whole(CacheProb P, CacheArgs A) {
   extern __shared__ __align__(16) char smem[];
   const int g = (int)(blockIdx.x / (uint32_t)P.items);
   const int i = (int)blockIdx.x - g * P.items;
@@ -1055,8 +1066,9 @@ __global__ void __launch_bounds__(64 * cache_whole(D).waves) k_cache_whole(Cache
 }
 
 // Waves that a SIMD holds of a wide workgroup's.  Eight waves of 16 bf16 rows of 64
-// channels have few enough registers for four (8 x 8 heads, 512 rows: 118 us, four waves
-// of 32 rows, two a SIMD: 125; 128 rows: 45 and 47).
+// channels run as four, which spills 5 registers (8 x 8 heads, 512 rows: 138 us, as three
+// 167, as two 164; 128 rows: 50, 60 and 61).  Of 128 channels eight waves of 32 rows spill
+// 22, and are faster than 16 rows, which spill none (cache_shape's figures).
 template <typename T, int D, int NW>
 constexpr int cache_wide_waves() {
   return D > 128 ? 1 : std::is_same<T, bf16_t>::value && D <= 64 && NW == 8 ? 4 : 2;
@@ -1153,23 +1165,24 @@ struct CacheShape {
 };
 // Times in us, 8192 keys, bf16 but where said; heads: samples x key/value heads.
 CacheShape cache_shape(int dtype, int D, int64_t rows) {
-  // Float32's three parts leave registers for 16 rows; so do 32 of more than 64 channels
-  // (16 x 8 heads, 32 rows of 128: 76, narrow tiles of 32 rows 106, a wide one of 64 83;
-  // 8 x 4 heads, 24 of 256: 50 and the wide one 52).  More than 128 channels: one
-  // workgroup a CU (16 x 1 heads, 16 rows: 27, two of them 36).
+  // Float32's three parts leave registers for 16 rows; so do more than 64 channels (16 x 8
+  // heads, 32 rows of 128: 72 to 75, a wide tile of 64 84 to 86; 8 x 4 heads, 24 of 256: 49
+  // and the wide one 52).  More than 128 channels: one workgroup a CU (16 x 1 heads, 16
+  // rows: 26, two of them 35).
   if (dtype == NA_F32 || rows <= (D > 64 ? 32 : 16)) return {16, 4, D > 128 ? 256 : 512, 2};
-  if (rows <= 32) return {32, 4, 512, 2};  // (37; 16 rows 47, a wide tile 48)
+  if (rows <= 32) return {32, 4, 512, 2};  // (8 x 4 heads: 21; 16 rows 23, a wide tile 27)
   // fp16's two parts leave registers for one workgroup a CU (2 x 8 heads, 2048 rows: 735,
-  // grids of two 750; bf16 439, of one 629)
+  // grids of two 750; bf16 481, of one 690)
   if (D > 128) return {64, 4, dtype == NA_F16 ? 256 : 512, 1};
-  // (16 x 8 heads, 48 rows of 128: 87, three narrow tiles 128; 64 rows: 85, in a tile of
-  // 128 159; of 64 channels 52 and 66)
+  // (16 x 8 heads, 48 rows of 128: 86, three narrow tiles 125; 64 rows: 87, in a tile of
+  // 128 118; of 64 channels 59 and 80)
   if (rows <= 64) return {64, 4, 512, 1};
-  // (8 x 8 heads, 256 rows of 128: fp16 135, in tiles of 64 156; bf16 89, in tiles of 64 or
-  // 128 130; 2 x 8 heads, 4096 rows: 267, 449 and 386)
-  if (dtype == NA_F16) return {128, 8, 256, 1};
+  // (8 x 8 heads, 256 rows of 128: fp16 135, in tiles of 64 156; bf16 114, in tiles of 64
+  // 142, of 128 119; 2 x 8 heads, 4096 rows: 352, 503 and 410; 16 x 8 heads, 128 rows: in a
+  // tile of 256 194, of 128 122)
+  if (dtype == NA_F16 || (D > 64 && rows <= 128)) return {128, 8, 256, 1};
   if (D > 64) return {256, 8, 256, 1};
-  return {128, 8, 512, 1};  // (8 x 8 heads, 512 rows: 118, in tiles of 64 145)
+  return {128, 8, 512, 1};  // (8 x 8 heads, 512 rows: 138, in tiles of 64 170)
 }
 
 // The most keys that an item's rows see, where tables are full.
@@ -1277,9 +1290,8 @@ void cache_run(const CacheProb &P, const CacheArgs &A, hipStream_t st) {
       if constexpr (D <= 128) {
         if constexpr (std::is_same<T, bf16_t>::value && D > 64) {
           if (P.rows == 256) return cache_launch<T, D, 2, 8, true>(P, A, st);
-        } else {
-          if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
         }
+        if (P.rows == 128) return cache_launch<T, D, 1, 8, true>(P, A, st);
       }
     }
     cache_launch<T, D, 1, 4, false>(P, A, st);

@@ -198,9 +198,10 @@ def cache_attention(query: torch.Tensor, cache: PagedCache, tables: torch.Tensor
 
     float32, float16 or bfloat16 queries; query heads share key/value heads as in
     ``na1d``.  The cache's elements are taken exactly, products and sums are float32;
-    probabilities are rounded to 8 bits for bfloat16 queries (their own), 16 for float16
-    and 24 for float32; sums may be divided differently, and differ in their last bits,
-    for tables of another width or batches of other lengths.  The output has query's type; the LSE (``return_lse``) is float32
+    probabilities are rounded to 16 bits for bfloat16 and float16 queries and to 24 for
+    float32; sums may be divided differently, and differ in their last bits, for tables of
+    another width or batches of other lengths.  The output has query's type; the LSE
+    (``return_lse``) is float32
     ``[B, L, H]``, ready for ``merge_attentions``, as with ``prefix_attention`` over tokens
     that the batch shares.  ``tables`` and ``seq_lens`` as ``cache_append`` takes them.
     There is no derivative: inputs that require grad are refused outside

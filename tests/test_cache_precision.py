@@ -1,0 +1,36 @@
+"""cache_attention's rounding of probabilities, by every kernel that bfloat16 queries take:
+an output is off by half a step of its own type, the products' and sums' float32, and
+no more than 2^-16 of the mean of |v| by the probabilities (test_cache gives the bounds;
+there a bfloat16 row may be off by 2^-8 of it)."""
+
+import pytest
+import torch
+
+import test_cache as C
+
+BF16 = torch.bfloat16
+
+# B, tokens, heads, kv heads, dim, page, lengths, window: rows of a tile, channels
+TILES = {
+    "a workgroup an item, 64": (2, 1, 8, 2, 64, 16, [700, 90], None),
+    "a workgroup an item, 128": (2, 1, 8, 2, 128, 64, [700, 90], None),
+    "a workgroup an item, 256": (2, 1, 6, 2, 256, 32, [350, 90], None),
+    "shared out, 64": (1, 1, 4, 1, 64, 16, [3100], None),
+    "shared out, 128": (1, 1, 4, 1, 128, 16, [3100], None),
+    "shared out, 256": (1, 1, 4, 1, 256, 32, [1500], None),
+    "32 rows of 64": (2, 7, 4, 1, 64, 16, [900, 300], None),
+    "64 rows of 64": (2, 9, 4, 1, 64, 32, [900, 300], None),
+    "64 rows of 128": (2, 12, 4, 1, 128, 64, [900, 300], None),
+    "64 rows of 256": (1, 12, 4, 1, 256, 64, [700], None),
+    "128 rows of 64": (1, 70, 4, 2, 64, 16, [900], 600),
+    "128 rows of 128": (1, 30, 4, 1, 128, 64, [900], None),
+    "256 rows of 128": (1, 70, 4, 1, 128, 64, [900], None),
+    "256 rows of 96": (1, 70, 4, 1, 96, 16, [400], 300),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", list(TILES))
+def test_probabilities_of_bfloat16_queries(case, monkeypatch):
+    monkeypatch.setitem(C.PARTS, BF16, 2.0 ** -16)
+    C._check(C._make(TILES[case], BF16, 2), case)

@@ -272,12 +272,13 @@ class _NeighborhoodAttention(_nn.Module):
     def _fuses_norms(self) -> bool:
         """Whether the norms are the layer's plain ones, alike: a replaced or hooked module
         is called itself."""
-        return (self.q_norm.eps == self.k_norm.eps
-                and self.q_norm.weight.dtype == self.k_norm.weight.dtype
-                and not torch.nn.modules.module._has_any_global_hook()
-                and all(type(m) is LayerNorm and "forward" not in m.__dict__
-                        and not any(getattr(m, h) for h in _HOOKS)
-                        for m in (self.q_norm, self.k_norm)))
+        norms = (self.q_norm, self.k_norm)
+        if torch.nn.modules.module._has_any_global_hook() or any(
+                type(m) is not LayerNorm or "forward" in m.__dict__
+                or any(getattr(m, h) for h in _HOOKS) for m in norms):
+            return False
+        dtypes = {t.dtype for m in norms for t in (m.weight, m.bias) if t is not None}
+        return norms[0].eps == norms[1].eps and len(dtypes) <= 1
 
     def _attend(self, x: torch.Tensor, sizes: Optional[torch.Tensor]) -> torch.Tensor:
         r = self.rank

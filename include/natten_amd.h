@@ -627,7 +627,8 @@ size_t na_cache_attend_workspace_bytes(const na_cache_params *p);
  * tokens up to t (the last `window` of them where window > 0).  out and lse
  * (float32 [batch, tokens, heads], natural log, or NULL) as na_prefix_fwd writes them;
  * a query that sees no key gets zeros and -infinity.  What lies behind a length, in
- * front of every window or in no page is not read.
+ * front of every window or in no page is not read; tables may be NULL where table_pages
+ * is 0.
  */
 int na_cache_attend(const na_cache_params *p, const na_cache *cache, const void *q,
                     const int32_t *tables, const int32_t *seq_lens, void *out, float *lse,

@@ -1151,7 +1151,7 @@ int na_cache_attend(const na_cache_params *p, const na_cache *cache, const void 
   const bool keys = p->pages > 0 && p->table_pages > 0;
   if (keys && (rc = check_pages(cache)) != NA_OK) return rc;
   if (cache == nullptr || q == nullptr || out == nullptr || seq_lens == nullptr ||
-      (keys && tables == nullptr))
+      (p->table_pages > 0 && tables == nullptr))  // (read up to a length, whatever they name)
     return fail(NA_ERR_INVALID, "cache/q/tables/seq_lens/out must be non-NULL");
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(NA_ERR_WORKSPACE, "na_cache_attend needs a %zu-byte workspace (got %zu)", need,

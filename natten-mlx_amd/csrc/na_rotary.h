@@ -123,7 +123,7 @@ __device__ __forceinline__ void rot_table(const RotProb &P, const void *pos, con
 // What a call's sizes and axes say; returns how its rows split into units.
 inline RotMode rot_prob(const na_rotary_params *p, RotProb &P) {
   const int n = p->dtype == NA_F32 ? 4 : 8;
-  int64_t per_sample = 1;
+  int64_t per_sample = p->batch > 0 ? 1 : 0;  // (without samples extents are not bounded)
   for (int a = 0; a < 3; ++a) per_sample *= p->extent[a];
   P.tokens = (int32_t)(p->batch * per_sample);
   P.H = p->heads;
@@ -149,9 +149,10 @@ inline RotMode rot_prob(const na_rotary_params *p, RotProb &P) {
     P.qs[i] = p->q_stride[i];
     P.ks[i] = p->k_stride[i];
   }
-  P.fS = make_fastdiv((uint32_t)per_sample);
-  P.fE1 = make_fastdiv((uint32_t)p->extent[1]);
-  P.fE2 = make_fastdiv((uint32_t)p->extent[2]);
+  // (an extent may be 0: a backward without tokens still writes the weights' gradients)
+  P.fS = make_fastdiv((uint32_t)std::max<int64_t>(per_sample, 1));
+  P.fE1 = make_fastdiv((uint32_t)std::max<int64_t>(p->extent[1], 1));
+  P.fE2 = make_fastdiv((uint32_t)std::max<int64_t>(p->extent[2], 1));
   P.fupr = make_fastdiv((uint32_t)P.upr);
   P.fpairs = make_fastdiv((uint32_t)P.pairs);
   return mode;

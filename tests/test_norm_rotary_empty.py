@@ -1,0 +1,55 @@
+"""norm_rotary without tokens or without heads: gradients are zeros, and no call ends the
+process."""
+
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from _helpers import DEV
+
+PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "natten-mlx_amd")
+
+SIZES = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from natten_amd._core import _lib
+r = _lib.NaRotaryParams(batch=int(sys.argv[5]), heads=4, kv_heads=1, head_dim=16, dtype=2, n_axes=1, theta=1e4)
+r.extent[:] = [int(x) for x in sys.argv[2:5]]
+r.axis_dim[0] = 16
+p = _lib.NaNormRotaryParams(rotary=r, weight_dtype=0, eps=1e-5)
+print(_lib.load().na_norm_rotary_bwd_workspace_bytes(p))
+"""
+
+
+@pytest.mark.parametrize("extent, batch", [((1, 1, 0), 2), ((1, 0, 3), 2), ((0, 1, 5), 2), ((0, 0, 0), 2),
+                                           ((1, 1 << 16, 1 << 16), 0), ((1, 0, 0), 0)], ids=str)
+def test_sizes_of_an_empty_grid(extent, batch):
+    """In a process of its own, which a division by an extent of zero would end."""
+    run = subprocess.run([sys.executable, "-c", SIZES, PKG, *map(str, extent), str(batch)],
+                         capture_output=True, text=True)
+    assert run.returncode == 0, (run.returncode, run.stderr)
+    assert run.stdout.split()[-1] == "0"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(2, 0), (2, 3, 0), (2, 0, 3), (0, 5), (1, 2, 0, 4), (0, 0),
+                                  (0, 1 << 16, 1 << 16)], ids=str)
+@pytest.mark.parametrize("twin", [False, True])
+def test_gradients_without_tokens(lead, twin):
+    import natten_amd
+    import natten_amd.autograd.fused as AF
+
+    q, k = (torch.empty((*lead, h, 16), device=DEV, requires_grad=True) for h in (4, 1))
+    w = [torch.ones(16, device=DEV, requires_grad=True) for _ in range(4)]
+    with AF.python_autograd(twin):
+        out = natten_amd.norm_rotary(q, k, *w)
+        assert out[0].shape == q.shape and out[1].shape == k.shape
+        grads = torch.autograd.grad(out[0].sum() + out[1].sum(), (q, k, *w), retain_graph=True)
+        alone, = torch.autograd.grad(out[0].sum(), q)
+    assert grads[0].shape == q.shape and grads[1].shape == k.shape and alone.shape == q.shape
+    for g in grads[2:]:
+        assert g.shape == (16,) and not g.any()

@@ -994,7 +994,7 @@ int na_norm_rotary_bwd(const na_norm_rotary_params *p, const void *q, const void
   if (rc != NA_OK) return rc;
   const na_rotary_params &r = p->rotary;
   const bool sums = dwq != nullptr || dbq != nullptr || dwk != nullptr || dbk != nullptr;
-  if (r.heads + r.kv_heads == 0 || (dq == nullptr && dk == nullptr && !sums)) return NA_OK;
+  if (!sums && (r.heads + r.kv_heads == 0 || (dq == nullptr && dk == nullptr))) return NA_OK;
   if (tokens > 0 && ((r.heads > 0 && (q == nullptr || gq == nullptr)) ||
                      (r.kv_heads > 0 && (k == nullptr || gk == nullptr)) ||
                      (r.pos_type != NA_POS_GRID && positions == nullptr)))

@@ -587,7 +587,7 @@ void nr_bwd_plan(NrProb &Q, int dtype, RotMode mode) {
   RotProb &P = Q.R;
   const int entries = nr_entries(P, dtype, mode);
   auto part = [&](int heads, int32_t *per, int32_t *blocks) {
-    const int most = std::max(1, (int)((int64_t)kNrBlocks * heads / (P.H + P.Hk)));
+    const int most = std::max(1, (int)((int64_t)kNrBlocks * heads / std::max(P.H + P.Hk, 1)));
     *per = nr_run(P, entries, heads, most);
     *blocks = heads == 0 ? 0 : (int)std::min<int64_t>(most, ((int64_t)P.tokens + *per - 1) / *per);
   };

@@ -53,3 +53,25 @@ def test_gradients_without_tokens(lead, twin):
     assert grads[0].shape == q.shape and grads[1].shape == k.shape and alone.shape == q.shape
     for g in grads[2:]:
         assert g.shape == (16,) and not g.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("twin", [False, True])
+@pytest.mark.parametrize("key", [False, True])
+def test_gradients_without_heads(key, twin, dtype):
+    """Not what the memory held before: blocks of NaN of every size are there to be taken."""
+    import natten_amd
+    import natten_amd.autograd.fused as AF
+
+    q = torch.empty((2, 3, 0, 16), device=DEV, dtype=dtype, requires_grad=True)
+    k = q.detach().clone().requires_grad_(True) if key else None
+    w = [torch.ones(16, device=DEV, dtype=dtype, requires_grad=True) for _ in range(4 if key else 2)]
+    dirty = [torch.full((16,), float("nan"), device=DEV, dtype=dtype) for _ in range(64)]
+    torch.cuda.synchronize()
+    del dirty
+    with AF.python_autograd(twin):
+        out = natten_amd.norm_rotary(q, k, *w)
+        grads = torch.autograd.grad(sum(o.sum() for o in (out if key else (out,))), w)
+    for g in grads:
+        assert g.shape == (16,) and g.isfinite().all() and not g.any()

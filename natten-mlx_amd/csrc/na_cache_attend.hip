@@ -260,7 +260,7 @@ constexpr int cache_prob_parts() {
   return sizeof(T) == 2 ? 2 : 3;
 }
 
-// Eight numbers as sums of parts.
+// Eight probabilities as sums of parts.
 template <int NP>
 __device__ __forceinline__ void split8(const float (&x)[8], bf8 (&o)[NP]) {
   float r[8];
@@ -268,6 +268,27 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf8 (&o)[NP]) {
   for (int i = 0; i < 8; ++i) r[i] = x[i];
 #pragma unroll
   for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[p][i] = (__bf16)r[i];
+      if (p + 1 < NP) r[i] -= (float)o[p][i];
+    }
+}
+
+// Eight channels of a query: the first part of what would round to an infinity is the
+// largest bf16, and what is not finite has no further parts.
+template <int NP>
+__device__ __forceinline__ void split_query8(const float (&x)[8], bf8 (&o)[NP]) {
+  constexpr float kMost = 0x1.fep127f;
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool finite = fabsf(x[i]) < INFINITY;
+    o[0][i] = (__bf16)(finite ? fminf(fmaxf(x[i], -kMost), kMost) : x[i]);
+    r[i] = finite ? x[i] - (float)o[0][i] : 0.f;
+  }
+#pragma unroll
+  for (int p = 1; p < NP; ++p)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       o[p][i] = (__bf16)r[i];
@@ -297,7 +318,7 @@ struct Query8 {
       for (int i = 0; i < 8; ++i)
         x[i] = sizeof(T) == 4 ? __uint_as_float(r[i / 4 % (sizeof(T) / 2)][i % 4])
                               : (float)__builtin_bit_cast(f16_t, (uint16_t)(r[0][i / 2] >> (16 * (i & 1))));
-      split8<NP>(x, o);
+      split_query8<NP>(x, o);
     }
   }
 };

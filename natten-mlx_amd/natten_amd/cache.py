@@ -194,10 +194,12 @@ def cache_attention(query: torch.Tensor, cache: PagedCache, tables: torch.Tensor
     ``tables[b, i // page_size]``; tokens of an entry outside ``[0, pages)``, such as -1
     for pages that have left every window, are not seen.  What lies behind a length or
     in front of every window is not read.  A query that sees no key, such as one before
-    the sequence's start (t < 0), gets zeros and an LSE of -inf.
+    the sequence's start (t < 0), or whose scores are all -inf, gets zeros and an LSE of
+    -inf.
 
     float32, float16 or bfloat16 queries; query heads share key/value heads as in
-    ``na1d``.  The cache's elements are taken exactly, products and sums are float32;
+    ``na1d``.  The cache's elements are taken exactly, and so are queries (in float32 to 24
+    bits, to 2^-126 where they are smaller); products and sums are float32;
     probabilities are rounded to 16 bits for bfloat16 and float16 queries and to 24 for
     float32; sums may be divided differently, and differ in their last bits, for tables of
     another width or batches of other lengths.  The output has query's type; the LSE

@@ -27,3 +27,68 @@ def test_tables_are_needed_where_they_have_entries(pages):
     assert b"tables" in lib.na_last_error()
     lib, p, c = _entry(pages=pages, table_pages=0)  # none to read: as far as the workspace
     assert lib.na_cache_attend(p, c, 1, None, 1, 1, None, None, 0, None) == 4
+
+
+# ---- queries at the ends of their types ----------------------------------------
+
+# B, tokens, heads, kv heads, dim, page, lengths, window: every kind of tile
+TILES = {
+    "a workgroup an item": (2, 1, 8, 2, 64, 16, [131, 40], None),
+    "a workgroup an item, 128": (2, 1, 8, 2, 128, 64, [131, 40], None),
+    "shared out, 256": (1, 1, 4, 1, 256, 32, [700], None),
+    "32 rows": (2, 7, 4, 1, 64, 16, [90, 33], None),
+    "64 rows": (2, 12, 4, 1, 128, 64, [200, 70], None),
+    "128 rows": (1, 70, 4, 2, 64, 16, [300], 200),
+    "256 rows": (1, 70, 4, 1, 96, 16, [300], None),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", list(TILES))
+def test_queries_next_to_the_largest_float32(case):
+    """They round to no infinity as they are split.  Keys are some 2^-110, so that scores
+    are finite, and `scale` brings them back to some units."""
+    import test_cache as C
+
+    t = C._make(TILES[case], F32, 5)
+    t["cache"].key_scale.view(torch.uint8).fill_(10)
+    g = torch.Generator().manual_seed(1)
+    most = torch.finfo(F32).max
+    near = torch.rand(t["q"].shape, generator=g) * 2.0 ** -7
+    big = torch.where(t["q"] < 0, -1.0, 1.0) * (most * (1 - near))
+    big[..., 0] = most
+    some = torch.rand(t["q"].shape, generator=g) < 0.25
+    t["q"] = torch.where(some, big, t["q"] * 2.0 ** 120)
+    assert t["q"].isfinite().all()
+    C._check(t, case, scale=2.0 ** -20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", list(TILES))
+def test_infinite_queries(case, dtype):
+    """Scores of -inf weigh nothing, a row of them alone sees nothing; a row with one of
+    +inf, or with infinities of both signs, is NaN, its LSE too."""
+    import test_cache as C
+
+    t = C._make(TILES[case], dtype, 6)
+    codes = t["cache"].key.view(torch.uint8)
+    low = codes[..., 3] & 0x7f
+    codes[..., 3] = torch.where(low == 0, 0x38, low) | 0x80  # channel 3: negative, none 0
+    codes[..., 5] = torch.where(codes[..., 5] & 0x7f == 0, 0x38, codes[..., 5] & 0x7f)  # 5: positive
+    want, want_lse = C._run(t)
+    q = t["q"]
+    t["q"] = q.clone()
+    t["q"][:, -1, 0, 3] = float("inf")   # every score -inf
+    t["q"][:, -1, 1, 5] = float("-inf")
+    t["q"][:, -1, 2, 5] = float("inf")   # every score +inf
+    t["q"][:, -1, 3, [3, 5]] = float("inf")  # -inf + inf
+    out, lse = C._run(t)
+    for h, kind in ((0, "none"), (1, "none"), (2, "nan"), (3, "nan")):
+        if kind == "none":
+            assert not out[:, -1, h].any() and (lse[:, -1, h] == -float("inf")).all(), h
+        else:
+            assert out[:, -1, h].isnan().all() and lse[:, -1, h].isnan().all(), h
+    rest = torch.ones(out.shape[:3], dtype=torch.bool, device=out.device)
+    rest[:, -1, :4] = False
+    assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])

@@ -570,9 +570,9 @@ int na_prefix_fwd(const na_prefix_params *p, const void *q, const void *prefix_k
  * Token i of sample b lies in slot i % page_size of page tables[b][i / page_size].
  * An element of a page and head is its e4m3 code (4 exponent bits, 3 of mantissa,
  * largest 448) times 2^(s - 127), s the scale byte of that page and head (e8m0), in
- * [10, 246] as na_cache_append writes it.  A table's entry outside [0, pages) is no
- * page: what would lie there is not written and not seen.  No counterpart in the
- * reference.
+ * [10, 246] as na_cache_append writes it; other bytes, 255 (NaN) among them, are taken
+ * as the nearer end.  A table's entry outside [0, pages) is no page: what would lie
+ * there is not written and not seen.  No counterpart in the reference.
  */
 typedef struct na_cache {
   void *key;                     /* codes of [pages, kv_heads, page_size, head_dim] */

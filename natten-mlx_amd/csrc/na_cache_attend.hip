@@ -194,10 +194,11 @@ struct CacheEntry {
   }
 };
 
-// Both scales' bytes, of keys and above of values.  (Bytes past the largest scale, as
-// unwritten pages hold them, stay finite.)
+// Both scales' bytes, of keys and above of values, in the range that the append keeps to,
+// where the append takes them for held ones too.  (Unwritten pages may hold others.)
 __device__ __forceinline__ int cache_scales(int k, int v) {
-  return min(k, kScaleBias + kScaleHigh) | min(v, kScaleBias + kScaleHigh) << 8;
+  constexpr int low = kScaleBias + kScaleLow, high = kScaleBias + kScaleHigh;
+  return min(max(k, low), high) | min(max(v, low), high) << 8;
 }
 
 // As the wide workgroups' table holds it.

@@ -23,7 +23,9 @@ from .prefix import _host_lens
 class PagedCache(NamedTuple):
     """Keys and values ``[pages, H_kv, page_size, D]`` in float8_e4m3fn and the scales of
     each page and head ``[pages, H_kv]`` in float8_e8m0fnu (a power of two): an element
-    stands for its value times its page's and head's scale.
+    stands for its value times its page's and head's scale.  Scales lie in ``[2^-117,
+    2^119]``, as ``cache_append`` writes them; smaller ones are taken as 2^-117, larger
+    ones and NaN as 2^119.
 
     Which page holds which tokens is the caller's: a table ``[B, M]`` says that token i
     of sample b lies in slot ``i % page_size`` of page ``tables[b, i // page_size]``.

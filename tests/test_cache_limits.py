@@ -92,3 +92,58 @@ def test_infinite_queries(case, dtype):
     rest = torch.ones(out.shape[:3], dtype=torch.bool, device=out.device)
     rest[:, -1, :4] = False
     assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])
+
+
+# ---- scales outside the append's range -----------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", list(TILES))
+def test_scales_outside_the_range_are_its_ends(case, dtype):
+    import test_cache as C
+
+    t = C._make(TILES[case], dtype, 7)
+    outs = []
+    for byte in (0, 1, 9, 10):
+        for i in (2, 3):
+            t["cache"][i].view(torch.uint8).fill_(byte)
+        outs.append(C._run(t, scale=2.0 ** 100))
+    assert outs[-1][0].abs().max() > 0 or dtype == F16  # (float16 ends at 2^-24)
+    for out, lse in outs[:-1]:
+        assert torch.equal(out, outs[-1][0]) and torch.equal(lse, outs[-1][1])
+    outs = []
+    # (256 products of up to 8 * 448 * 2^119 would pass 2^128, and so would the sums of 700
+    # values of 448 * 2^119 before their division: codes of 7 * 2^-9 at most, sums below 2^127)
+    t["q"] = t["q"] * 2.0 ** -20
+    t["cache"].value.view(torch.uint8).bitwise_and_(0x87)
+    for byte in (247, 255, 246):
+        for i in (2, 3):
+            t["cache"][i].view(torch.uint8).fill_(byte)
+        outs.append(C._run(t, scale=2.0 ** -110))
+    assert outs[-1][1].isfinite().all() and not outs[-1][0].isnan().any()
+    for out, lse in outs[:-1]:
+        assert torch.equal(out, outs[-1][0]) and torch.equal(lse, outs[-1][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("byte, taken", [(0, 10), (9, 10), (247, 246), (255, 246)])
+def test_appending_to_a_page_with_such_a_scale(byte, taken):
+    """Tokens in front keep their codes' values by the scale that they were taken by."""
+    import natten_amd
+    from _helpers import DEV, randn
+
+    caches = []
+    for b in (byte, taken):
+        cache = natten_amd.paged_cache(2, 2, 32, 16)
+        x = randn((1, 5, 2, 32), F32, 1).to(DEV)
+        tables = torch.tensor([[1, 0]], device=DEV)
+        natten_amd.cache_append(cache, x, x, tables, torch.tensor([5], device=DEV))
+        for s in cache[2:]:
+            s.view(torch.uint8).fill_(b)
+        y = randn((1, 3, 2, 32), F32, 2).to(DEV) * 2.0 ** -116
+        natten_amd.cache_append(cache, y, y, tables, torch.tensor([8], device=DEV))
+        caches.append(cache)
+    used = caches[0].key_scale.view(torch.uint8)[1]
+    assert ((used >= 10) & (used <= 246)).all()
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8)[1], b.view(torch.uint8)[1])

@@ -596,7 +596,7 @@ typedef struct na_cache_params {
   int32_t page_size;    /* 16, 32, 64 or 128 */
   int32_t table_pages;  /* entries of a sample's table */
   int32_t window;       /* attention: 0 for all tokens; any width */
-  float scale;          /* attention: positive and finite */
+  float scale;          /* attention: positive, at most 2e38 */
   int64_t table_stride; /* elements from sample to sample */
   int64_t q_stride[3];  /* attention: sample, token, head; channels adjacent */
   int64_t k_stride[3];  /* append: of the new keys and values */

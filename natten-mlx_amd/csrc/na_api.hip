@@ -1090,8 +1090,8 @@ int check_cache_attend(const na_cache_params *p, size_t *need) {
     return fail(NA_ERR_INVALID, "heads (%d) must be divisible by kv_heads (%d)", p->heads,
                 p->kv_heads);
   if (p->window < 0) return fail(NA_ERR_INVALID, "window is negative");
-  if (!(p->scale > 0.f) || p->scale > 3e38f)
-    return fail(NA_ERR_INVALID, "scale must be positive and finite, got %g", (double)p->scale);
+  if (!(p->scale > 0.f) || p->scale > 2e38f)  // (times log2 e a float32 too)
+    return fail(NA_ERR_INVALID, "scale must be positive and at most 2e38, got %g", (double)p->scale);
   if ((int64_t)p->batch * p->tokens >= ((int64_t)1 << 30) ||
       (int64_t)p->batch * p->tokens * p->heads >= ((int64_t)1 << 30))
     return fail(NA_ERR_UNSUPPORTED, "batch * tokens * heads is 2^30 or more");

@@ -9,7 +9,6 @@ cache at half the bytes of 16-bit ones (``csrc/na_cache.hip``,
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -221,8 +220,8 @@ def cache_attention(query: torch.Tensor, cache: PagedCache, tables: torch.Tensor
     _check_lens("seq_lens", seq_lens, b)
     if kernel_size is not None and (not isinstance(kernel_size, int) or kernel_size < 1):
         raise ValueError(f"kernel_size must be a positive int or None, got {kernel_size!r}.")
-    if scale is not None and not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite, got {scale}.")
+    if scale is not None and not 2.0 ** -149 <= scale <= 2e38:  # (times log2 e a float32)
+        raise ValueError(f"scale must be positive and at most 2e38, got {scale}.")
     capacity = tables.shape[1] * shape[2]
     scale = d ** -0.5 if scale is None else float(scale)
     if not seq_lens.is_cuda and query.is_cuda:

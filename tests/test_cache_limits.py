@@ -29,6 +29,21 @@ def test_tables_are_needed_where_they_have_entries(pages):
     assert lib.na_cache_attend(p, c, 1, None, 1, 1, None, None, 0, None) == 4
 
 
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38])
+def test_scales_whose_product_with_log2_e_is_infinite(scale):
+    import natten_amd
+
+    lib, p, c = _entry(scale=scale)
+    assert lib.na_cache_attend(p, c, 1, 1, 1, 1, None, None, 0, None) == 1 and b"scale" in lib.na_last_error()
+    lib, p, c = _entry(scale=1.9e38)
+    assert lib.na_cache_attend(p, c, 1, 1, 1, 1, None, None, 0, None) == 4  # as far as the workspace
+    cache = natten_amd.paged_cache(4, 2, 32, 16, device="cpu")
+    args = torch.zeros(2, 1, 4, 32), cache, torch.zeros(2, 2, dtype=torch.int32), torch.tensor([3, 1])
+    for bad in (scale, 1e-46):  # (float32 holds nothing as small)
+        with pytest.raises(ValueError, match="scale"):
+            natten_amd.cache_attention(*args, scale=bad)
+
+
 # ---- queries at the ends of their types ----------------------------------------
 
 # B, tokens, heads, kv heads, dim, page, lengths, window: every kind of tile

@@ -162,3 +162,71 @@ def test_appending_to_a_page_with_such_a_scale(byte, taken):
     assert ((used >= 10) & (used <= 246)).all()
     for a, b in zip(*caches):
         assert torch.equal(a.view(torch.uint8)[1], b.view(torch.uint8)[1])
+
+
+# ---- refusals and bounds that other tests pass by -------------------------------
+
+def test_caches_whose_channels_are_not_adjacent():
+    import natten_amd
+
+    cache = natten_amd.paged_cache(5, 2, 32, 16, device="cpu")
+    apart = (cache.key.view(torch.uint8).transpose(2, 3).contiguous().transpose(2, 3)
+             .view(torch.float8_e4m3fn))
+    assert apart.shape == cache.key.shape and apart.stride(3) == 16
+    k, q = torch.randn(2, 3, 2, 32), torch.randn(2, 3, 4, 32)
+    tables, lens = torch.zeros(2, 4, dtype=torch.int32), torch.tensor([5, 7])
+    for name in ("key", "value"):
+        bad = cache._replace(**{name: apart})
+        with pytest.raises(ValueError, match="adjacent channels"):
+            natten_amd.cache_append(bad, k, k, tables, lens)
+        with pytest.raises(ValueError, match="adjacent channels"):
+            natten_amd.cache_attention(q, bad, tables, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", list(TILES))
+def test_float16_outputs_around_their_largest(case):
+    """Values around 65520, halfway from 65504 to what would come next: an output past it
+    by more than its tolerance is an infinity of its sign, one before it finite and within
+    the tolerance and half a step of 32; between them it is one of the two, and never NaN."""
+    import test_cache as C
+
+    t = C._make(TILES[case], F16, 8)
+    g = torch.Generator().manual_seed(3)
+    codes = t["cache"].value.view(torch.uint8)
+    # 1.75, 1.875, 2 and 2.25, times 2^15: 57344, 61440, 65536 and 73728
+    codes.copy_(torch.tensor([0x3e, 0x3f, 0x40, 0x41], dtype=torch.uint8)[
+        torch.randint(0, 4, codes.shape, generator=g)])
+    codes[..., 1::2] |= 0x80
+    t["cache"].value_scale.view(torch.uint8).fill_(127 + 15)
+    out, _ = C._run(t)
+    (v, tol), _ = C._reference(t)
+    tol = tol - v.abs() * torch.finfo(F16).eps / 2  # without the output's own rounding
+    o = out.cpu().double()
+    assert not o.isnan().any() and ((o.sign() == v.sign()) | (v == 0)).all()
+    past, before = v.abs() - tol > 65520, v.abs() + tol < 65520
+    assert past.any() and before.any()
+    assert o[past].isinf().all() and o[before].isfinite().all()
+    fin = o.isfinite()
+    assert ((o - v).abs()[fin] <= (tol + 16)[fin]).all()
+    assert (v.abs()[o.isinf()] >= (65520 - tol)[o.isinf()]).all()
+
+
+@pytest.mark.gpu
+def test_rows_that_see_nothing_and_masked_values_of_every_kind():
+    """Codes of NaN behind the lengths, in rows that see nothing and in pages of no one."""
+    import natten_amd
+    from _helpers import DEV
+
+    for dim in (64, 128, 256):
+        cache = natten_amd.paged_cache(8, 2, dim, 16)
+        for t in cache[:2]:
+            t.view(torch.uint8).fill_(0x7f)
+        for t in cache[2:]:
+            t.view(torch.uint8).fill_(255)
+        tables = torch.tensor([[0, 1, -1, 7], [2, 3, 4, 5]], dtype=torch.int32, device=DEV)
+        for n in (1, 5, 40):
+            q = torch.randn(2, n, 8, dim, device=DEV, dtype=BF16)
+            out, lse = natten_amd.cache_attention(q, cache, tables, torch.zeros(2, dtype=torch.int32, device=DEV),
+                                                  return_lse=True)
+            assert not out.any() and (lse == -float("inf")).all()

@@ -612,8 +612,8 @@ typedef struct na_cache_params {
  * power of two that puts the new tokens' largest finite magnitude at 448 at most, and
  * at least the held one where tokens of the page lie in front of the new ones, whose
  * codes are rescaled where it grows.  Codes are rounded to the nearest, ties to even;
- * what is not finite becomes NaN.  Pages that one call writes belong to one sample
- * each.  seq_lens, new_lens and tables: int32 on the device.
+ * what is not finite becomes NaN.  Every entry that one call writes to names a page of
+ * its own.  seq_lens, new_lens and tables: int32 on the device.
  */
 int na_cache_append(const na_cache_params *p, const na_cache *cache, const void *key,
                     const void *value, const int32_t *tables, const int32_t *seq_lens,

@@ -139,8 +139,10 @@ def cache_append(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, tabl
     written, nor, with ``new_lens``, any but the last ``new_lens[b]`` of the L: a batch of
     unlike numbers of new tokens is padded in front.  Token t goes to slot
     ``t % page_size`` of page ``tables[b, t // page_size]``; an entry outside
-    ``[0, pages)``, such as -1, is no page and takes nothing.  Two samples must not write
-    to one page in a call.
+    ``[0, pages)``, such as -1, is no page and takes nothing.  The entries that a call
+    writes to, of all samples, must name different pages (a table may name a page again
+    where its tokens have left every window).  Cache tensors whose elements share memory,
+    such as expanded ones, are refused.
 
     A page's and head's scale is the smallest power of two that brings the new tokens
     of the page to 448 at most, e4m3's largest value; where tokens of the page lie in
@@ -155,6 +157,10 @@ def cache_append(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, tabl
     ``torch.no_grad()``.
     """
     shape = _check_cache(cache)
+    for t in cache:
+        if not t.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+            raise ValueError("cache_append cannot write to a cache whose elements share memory, got "
+                             f"strides {[c.stride() for c in cache]}.")
     new = tuple(key.shape)
     if len(new) != 4 or value.shape != new or new[2:] != (shape[1], shape[3]):
         raise ValueError(f"key and value must be [B, L, {shape[1]}, {shape[3]}], got "

@@ -183,6 +183,51 @@ def test_caches_whose_channels_are_not_adjacent():
             natten_amd.cache_attention(q, bad, tables, lens)
 
 
+def test_appending_to_shared_elements_is_refused():
+    import natten_amd
+
+    cache = natten_amd.paged_cache(5, 2, 32, 16, device="cpu")
+    one = natten_amd.paged_cache(1, 1, 32, 16, device="cpu")
+    k, q = torch.randn(2, 3, 2, 32), torch.randn(2, 3, 4, 32)
+    tables, lens = torch.zeros(2, 4, dtype=torch.int32), torch.tensor([5, 7])
+    for name, t in zip(cache._fields, one):
+        shared = t.view(torch.uint8).expand(getattr(cache, name).shape).view(t.dtype)
+        with pytest.raises(ValueError, match="share memory"):
+            natten_amd.cache_append(cache._replace(**{name: shared}), k, k, tables, lens)
+        with pytest.raises(RuntimeError, match="HIP"):  # (reading them is no mistake)
+            natten_amd.cache_attention(q, cache._replace(**{name: shared}), tables, lens)
+    with pytest.raises(RuntimeError, match="HIP"):  # one page and head: nothing is shared
+        natten_amd.cache_append(one, k[:, :, :1], k[:, :, :1], tables, lens)
+
+
+@pytest.mark.gpu
+def test_a_table_that_names_pages_again():
+    """A ring of four pages under a window of 20: tokens one at a time and in steps of up
+    to 16, against a table of as many pages as the sequence has."""
+    import natten_amd
+    from _helpers import DEV, randn
+
+    n, window = 400, 20
+    ring, flat = natten_amd.paged_cache(4, 2, 64, 16), natten_amd.paged_cache(25, 2, 64, 16)
+    tables = torch.arange(25, dtype=torch.int32, device=DEV).view(1, 25)
+    k, v = (randn((1, n, 2, 64), BF16, s).to(DEV) for s in (1, 2))
+    at = 0
+    for step in [1] * 70 + [16, 3, 11, 16, 1, 7, 16, 16, 16, 5] * 3:
+        if at + step > n:
+            break
+        at += step
+        lens = torch.tensor([at], device=DEV)
+        q = randn((1, step, 8, 64), BF16, at).to(DEV)
+        outs = []
+        for cache, t in ((ring, tables % 4), (flat, tables)):
+            natten_amd.cache_append(cache, k[:, at - step:at], v[:, at - step:at], t, lens)
+            # (pages that have left every window are no longer the ring's)
+            gone = torch.arange(25, device=DEV) * 16 + 16 <= at - step - window + 1
+            outs.append(natten_amd.cache_attention(q, cache, t.masked_fill(gone, -1), lens, kernel_size=window))
+        assert torch.equal(*outs), at
+    assert at > 300
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("case", list(TILES))
 def test_float16_outputs_around_their_largest(case):

@@ -565,7 +565,9 @@ int nr_entries(const RotProb &P, int dtype, RotMode mode) {
   return n;
 }
 
-// Whether rows of runs of up to `per` tokens are and lie as NrProb::fast says.
+// Whether rows of runs of up to `per` tokens are and lie as NrProb::fast says.  (A slice in
+// time of 131072 tokens of 8 + 8 heads of 64, whose samples lie apart: bf16 119 -> 130 us,
+// backward 173 -> 202; float32 220 -> 221 and 330 -> 333.)
 bool nr_fast(const RotProb &P, int dtype, const int64_t *st, int heads, int per) {
   if (P.D % (dtype == NA_F32 ? 4 : 8) != 0) return false;
   if (P.fS.d > 1 && (uint32_t)P.tokens > P.fS.d && st[0] != st[1] * (int64_t)P.fS.d) return false;

@@ -34,3 +34,24 @@ TILES = {
 def test_probabilities_of_bfloat16_queries(case, monkeypatch):
     monkeypatch.setitem(C.PARTS, BF16, 2.0 ** -16)
     C._check(C._make(TILES[case], BF16, 2), case)
+
+
+# 65 to 128 rows of 65 to 128 channels: a bfloat16 tile of its own, through test_cache's
+# tests of what a row sees
+ROWS = {
+    "100 rows of 128": (2, 25, 8, 2, 128, 64, [200, 33], None),
+    "128 rows of 96": (2, 32, 4, 1, 96, 16, [330, 101], None),
+    "window, 66 rows of 80": (2, 33, 4, 2, 80, 32, [300, 60], 37),
+    "window, 120 rows of 128": (1, 40, 3, 1, 128, 128, [390], 100),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("test", [
+    C.test_attention_against_the_definition, C.test_what_no_row_sees_is_not_read,
+    C.test_entries_that_are_no_page_are_not_seen, C.test_tokens_that_a_row_does_not_see,
+    C.test_long_tables_of_short_sequences], ids=lambda t: t.__name__)
+@pytest.mark.parametrize("case", list(ROWS))
+def test_tiles_of_128_rows(case, test, monkeypatch):
+    monkeypatch.setitem(C.CASES, case, ROWS[case])
+    test(case, BF16)

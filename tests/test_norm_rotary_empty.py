@@ -75,3 +75,27 @@ def test_gradients_without_heads(key, twin, dtype):
         grads = torch.autograd.grad(sum(o.sum() for o in (out if key else (out,))), w)
     for g in grads:
         assert g.shape == (16,) and g.isfinite().all() and not g.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads", [(0, 3), (3, 0)])
+@pytest.mark.parametrize("twin", [False, True])
+def test_heads_of_one_tensor_alone(heads, kv_heads, twin):
+    """The other's weights get zeros, and what has heads what it gets by itself."""
+    import natten_amd
+    import natten_amd.autograd.fused as AF
+    from _helpers import randn
+
+    q, k = (randn((2, 5, h, 16), seed=s).to(DEV).requires_grad_(True) for s, h in ((1, heads), (2, kv_heads)))
+    w = [randn((16,), seed=3 + i).to(DEV).requires_grad_(True) for i in range(4)]
+    some, ws, none = (q, w[:2], w[2:]) if heads else (k, w[2:], w[:2])
+    with AF.python_autograd(twin):
+        out = natten_amd.norm_rotary(q, k, *w)
+        part = out[0] if heads else out[1]
+        g = torch.autograd.grad(out[0].square().sum() + out[1].square().sum(), (some, *ws, *none))
+        alone = natten_amd.norm_rotary(some, q_weight=ws[0], q_bias=ws[1])
+        want = torch.autograd.grad(alone.square().sum(), (some, *ws))
+    assert torch.equal(part, alone)
+    for a, b in zip(g, want):
+        assert torch.equal(a, b)
+    assert not g[3].any() and not g[4].any()

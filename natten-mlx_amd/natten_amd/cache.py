@@ -209,8 +209,9 @@ def cache_attention(query: torch.Tensor, cache: PagedCache, tables: torch.Tensor
     bits, to 2^-126 where they are smaller); products and sums are float32;
     probabilities are rounded to 16 bits for bfloat16 and float16 queries and to 24 for
     float32; sums may be divided differently, and differ in their last bits, for tables of
-    another width or batches of other lengths.  The output has query's type; the LSE
-    (``return_lse``) is float32
+    another width or batches of other lengths.  Values are summed before the division, by
+    weights of up to 2^8: 2^8 times a row's tokens times their largest value has to stay
+    below 2^128.  The output has query's type; the LSE (``return_lse``) is float32
     ``[B, L, H]``, ready for ``merge_attentions``, as with ``prefix_attention`` over tokens
     that the batch shares.  ``tables`` and ``seq_lens`` as ``cache_append`` takes them.
     There is no derivative: inputs that require grad are refused outside
